@@ -230,6 +230,81 @@ int tx_flash_attn_fwd_noalloc(const void* qk, const void* vt, int64_t ldvt, void
                               int64_t batch, int64_t seq, int64_t heads, int64_t head_dim,
                               float scale, int causal, int softmax_mode, int dt, void* stream);
 
+/*
+ * Sequences of different lengths, packed: token rows [T][heads][head_dim], row strides in elements
+ * {token, head} with head_dim contiguous; sequence b holds the rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1
+ * (int32 [batch + 1], ascending from 0 or more).  Rows outside every sequence are neither read nor written.
+ * A paged cache: k_cache / v_cache element (page, kv_head, slot, d) at strides {page, head, slot}
+ * (head_dim contiguous); sequence b's key j is in page block_table[b * table_ld + j / page_size] at slot
+ * j % page_size.  Of kv_lens[b] keys (int32, the new ones included) the last ones belong to the sequence's rows
+ * cu_seqlens[b] ..: row i of n is key kv_lens[b] - n + i.  None of these arrays is read on the host, so one
+ * captured graph serves any lengths of the same totals.  Values that do not fit stay in bounds: cu_seqlens are
+ * cut to [0, T]; what a page index outside [0, num_pages), or a kv_lens above max_pages * page_size, would
+ * have to read makes the rows that need it NaN, and what it would have to write is dropped.
+ * All of it 16 bit (TX_F16, TX_BF16); pointers 16-byte aligned, strides multiples of 8; page_size a power of
+ * two of 8 .. 2^15, max_pages * page_size <= 2^30; T <= 2^24, batch <= 2^20, q_heads <= 65535 and
+ * T * q_heads <= 2^27.  These entry points have no counterpart in the reference, which has no cache, no positions and pads its batches (TTB:4380-4396).
+ */
+
+/*
+ * Rotary positions, and the write of new keys and values into a paged cache, in one pass over q, k and v:
+ *   (x1, x2) -> amplitude * (x1 cos t - x2 sin t, x2 cos t + x1 sin t),   t = 2 pi * 2^-64 * (p * steps[i]),
+ * for pairs i < rotary_dim / 2 of a head of q and k: elements (i, i + rotary_dim / 2), or (2i, 2i + 1) when
+ * interleaved != 0; elements from rotary_dim on and all of v pass unchanged.  steps[i] is the pair's turn per
+ * position in units of 2^-64 (int64; taken mod 2^64, so the angle of any position is exact to 2^-65 * |p|
+ * turns); computed in fp32, rounded once.  p = positions[t] (int64 [T]); NULL: the row's key index
+ * kv_lens[b] - n + i, or i when kv_lens is NULL too.
+ * q_out / k_out (nullable: k_out, or q with q_out) receive the turned rows; either may be its input itself (same
+ * pointer and strides) and may share no other memory with an input.  k_cache (NULL: no cache; then v,
+ * v_cache, block_table are unused) receives the turned k, v_cache the v, at the rows' key indices; rows whose
+ * index is negative are not cached.  Slots written by one call must be distinct.  head_dim a multiple of
+ * 8 up to 256, rotary_dim even, 2 .. head_dim.
+ */
+int tx_rotary_append(const void* q, const int64_t q_strides[2], void* q_out, const int64_t q_out_strides[2],
+                     const void* k, const int64_t k_strides[2], void* k_out, const int64_t k_out_strides[2],
+                     const void* v, const int64_t v_strides[2],
+                     void* k_cache, const int64_t k_cache_strides[3],
+                     void* v_cache, const int64_t v_cache_strides[3],
+                     const int64_t* steps, const int64_t* positions,
+                     const int32_t* cu_seqlens, const int32_t* kv_lens,
+                     const int32_t* block_table, int64_t table_ld,
+                     int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                     int64_t rotary_dim, int64_t num_pages, int64_t page_size, int64_t max_pages,
+                     float amplitude, int interleaved, int dt, void* stream);
+
+/*
+ * Attention over packed sequences with grouped heads:
+ *   o[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h / (q_heads / kv_heads)]) v[j, ..]
+ * over the keys j of t's own sequence (causal != 0: up to t itself).  fp32 scores and sums, one pass with a
+ * running maximum; the weights are rounded to dt as operands of the second product only.  A key outside a
+ * row's mask has no influence on it, whatever it holds (NaN and infinities included).  head_dim 64 or 128,
+ * kv_heads divides q_heads.  o may not share memory with q, k or v.
+ */
+int tx_flash_attn_packed(const void* q, const int64_t q_strides[2], const void* k, const int64_t k_strides[2],
+                         const void* v, const int64_t v_strides[2], void* o, const int64_t o_strides[2],
+                         const int32_t* cu_seqlens, int64_t tokens, int64_t batch, int64_t q_heads,
+                         int64_t kv_heads, int64_t head_dim, float scale, int causal, int dt, void* stream);
+
+/*
+ * The same for new tokens over a paged cache: row i of a sequence's n sees the keys j < kv_lens[b], when
+ * causal those up to its own, j <= kv_lens[b] - n + i.  A row that sees no key gets 0.  max_q_len bounds the
+ * rows of a sequence (<= 0: T); a call with a bound that is too small is still in bounds and right, only slower.
+ * workspace: at least the floats that tx_flash_attn_paged_workspace gives for the same sizes (scratch; 16-byte
+ * aligned, NULL when that is 0); calls that overlap in time need one each.
+ */
+int tx_flash_attn_paged(const void* q, const int64_t q_strides[2],
+                        const void* k_cache, const int64_t k_cache_strides[3],
+                        const void* v_cache, const int64_t v_cache_strides[3],
+                        void* o, const int64_t o_strides[2],
+                        const int32_t* cu_seqlens, const int32_t* kv_lens,
+                        const int32_t* block_table, int64_t table_ld,
+                        int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                        int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t max_q_len,
+                        float scale, int causal, float* workspace, int64_t workspace_floats, int dt, void* stream);
+int tx_flash_attn_paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                  int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t max_q_len,
+                                  int64_t* floats);
+
 /* tx_select_kernel: for tests and timing, the kernel that the calling thread's
  * later calls of `op` take where several give the result; no counterpart in
  * the reference.  variant < 0 restores the process's choice: the dispatcher's

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
 import os
 import threading
 from pathlib import Path
@@ -51,6 +52,10 @@ EXPORTED_SYMBOLS = (
     "tx_flash_attn_fwd",
     "tx_flash_attn_fwd_strided",
     "tx_flash_attn_fwd_noalloc",
+    "tx_rotary_append",
+    "tx_flash_attn_packed",
+    "tx_flash_attn_paged",
+    "tx_flash_attn_paged_workspace",
     "tx_select_kernel",
 )
 
@@ -129,6 +134,32 @@ def _declare(lib: ctypes.CDLL) -> None:
         _i64, _i64, _i64, _i64,             # batch seq heads head_dim
         _f32, _i32, _i32, _i32, _vp,        # scale causal softmax_mode dt stream
     ]
+    lib.tx_rotary_append.restype = _i32
+    lib.tx_rotary_append.argtypes = [
+        _vp, _vp, _vp, _vp,                 # q strides q_out strides
+        _vp, _vp, _vp, _vp, _vp, _vp,       # k strides k_out strides v strides
+        _vp, _vp, _vp, _vp,                 # k_cache strides v_cache strides
+        _vp, _vp, _vp, _vp, _vp, _i64,      # steps positions cu_seqlens kv_lens block_table table_ld
+        _i64, _i64, _i64, _i64, _i64, _i64,  # tokens batch q_heads kv_heads head_dim rotary_dim
+        _i64, _i64, _i64,                   # num_pages page_size max_pages
+        _f32, _i32, _i32, _vp,              # amplitude interleaved dt stream
+    ]
+    lib.tx_flash_attn_packed.restype = _i32
+    lib.tx_flash_attn_packed.argtypes = [
+        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,  # q k v o, each with its strides
+        _vp, _i64, _i64, _i64, _i64, _i64,  # cu_seqlens tokens batch q_heads kv_heads head_dim
+        _f32, _i32, _i32, _vp,              # scale causal dt stream
+    ]
+    lib.tx_flash_attn_paged.restype = _i32
+    lib.tx_flash_attn_paged.argtypes = [
+        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,  # q k_cache v_cache o, each with its strides
+        _vp, _vp, _vp, _i64,                # cu_seqlens kv_lens block_table table_ld
+        _i64, _i64, _i64, _i64, _i64,       # tokens batch q_heads kv_heads head_dim
+        _i64, _i64, _i64, _i64,             # num_pages page_size max_pages max_q_len
+        _f32, _i32, _vp, _i64, _i32, _vp,   # scale causal workspace workspace_floats dt stream
+    ]
+    lib.tx_flash_attn_paged_workspace.restype = _i32
+    lib.tx_flash_attn_paged_workspace.argtypes = [_i64] * 8 + [_vp]
 
 
 def _hip_runtime_mappings() -> set:
@@ -577,4 +608,307 @@ def flash_attn_noalloc(
     info = {"op": "flash_attn", "batch": batch, "seq": seq, "heads": heads, "head_dim": head_dim,
             "causal": bool(causal), "softmax": softmax, "noalloc": True}
     _launch("tx_flash_attn_fwd_noalloc", args, (qk, vt, out, kv), info)
+    return out
+
+
+# ------------------------------------------- packed sequences, paged cache
+ROTARY_SCALINGS = ("none", "linear", "base", "ramp")
+
+
+def rotary_steps(
+    rotary_dim: int,
+    base: float = 10000.0,
+    *,
+    scaling: str = "none",
+    factor: float = 1.0,
+    original_len: int = 0,
+    low_turns: float = 1.0,
+    high_turns: float = 32.0,
+    device: Optional[torch.device] = None,
+) -> Tuple[torch.Tensor, float]:
+    """``(steps, amplitude)`` of :func:`rotary_append`, made once per model.
+
+    ``steps`` (int64 ``[rotary_dim / 2]``) holds each pair's turn per position in units of 2^-64 turn:
+    ``f_i / (2 pi)`` with ``f_i = base^(-2i / rotary_dim)``, scaled for contexts ``factor`` times as long as the
+    model was trained on (``original_len`` positions):
+
+    * ``"linear"``: ``f_i / factor`` (positions interpolated);
+    * ``"base"``: ``base * factor^(r / (r - 2))``, which divides the lowest frequency by ``factor`` and keeps the
+      highest;
+    * ``"ramp"``: by parts: pairs that turn more than ``high_turns`` times within ``original_len`` keep their
+      frequency, those below ``low_turns`` turns are divided by ``factor``, a linear ramp between; the turned
+      values grow by ``0.1 ln(factor) + 1``, the amplitude.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be positive and even")
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"scaling must be one of {ROTARY_SCALINGS}")
+    if not (math.isfinite(base) and base > 0.0) or not (math.isfinite(factor) and factor > 0.0):
+        raise ValueError("base and factor must be positive and finite")
+    if scaling == "ramp" and (original_len <= 0 or not low_turns < high_turns):
+        raise ValueError("ramp scaling needs original_len > 0 and low_turns < high_turns")
+    if scaling == "base":
+        if rotary_dim <= 2:
+            raise ValueError("base scaling needs a rotary_dim above 2")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    amplitude = 1.0
+    steps = []
+    for i in range(rotary_dim // 2):
+        f = base ** (-2.0 * i / rotary_dim)
+        if scaling == "linear":
+            f /= factor
+        elif scaling == "ramp":
+            keep = (original_len * f / (2.0 * math.pi) - low_turns) / (high_turns - low_turns)
+            keep = min(1.0, max(0.0, keep))
+            f = f * keep + f / factor * (1.0 - keep)
+        # Whole turns fall away; the fraction as a signed 64-bit integer.
+        turn = math.ldexp(math.fmod(f / (2.0 * math.pi), 1.0), 64)
+        step = int(round(turn)) % (1 << 64)
+        steps.append(step - (1 << 64) if step >= 1 << 63 else step)
+    if scaling == "ramp" and factor > 1.0:
+        amplitude = 0.1 * math.log(factor) + 1.0
+    return torch.tensor(steps, dtype=torch.int64, device=device), amplitude
+
+
+def _heads3(name: str, t: torch.Tensor, rows: int, heads: Optional[int], hd: int, dtype: torch.dtype) -> None:
+    if t.dim() != 3 or t.shape[0] != rows or (heads is not None and t.shape[1] != heads) or t.shape[2] != hd:
+        raise ValueError(f"{name} must be [{rows}, {'heads' if heads is None else heads}, {hd}], got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must share q's dtype")
+    if hd > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name} must be contiguous in head_dim")
+
+
+def _int_vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype = torch.int32) -> None:
+    if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {str(dtype).replace('torch.', '')} [{n}] tensor")
+
+
+def _check_cache(k_cache, v_cache, block_table, batch: int, hd: int, dtype: torch.dtype) -> None:
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != hd:
+        raise ValueError(f"k_cache and v_cache must be [pages, kv_heads, page_size, {hd}] of one shape")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise ValueError("the caches must share q's dtype")
+    if hd > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        raise ValueError("the caches must be contiguous in head_dim")
+    if block_table.dim() != 2 or block_table.shape[0] != batch or block_table.dtype != torch.int32:
+        raise ValueError("block_table must be an int32 [batch, max_pages] tensor")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError("block_table rows must be contiguous")
+
+
+def _starts(cu_seqlens: torch.Tensor) -> int:
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must be an int32 [batch + 1] tensor")
+    _int_vector("cu_seqlens", cu_seqlens, cu_seqlens.shape[0])
+    return cu_seqlens.shape[0] - 1
+
+
+def _sv(t: Optional[torch.Tensor], n: int):
+    return None if t is None else (ctypes.c_int64 * n)(*t.stride()[:n])
+
+
+def _addr(a) -> Optional[int]:
+    return None if a is None else ctypes.addressof(a)
+
+
+def _one_device(*ts: Optional[torch.Tensor]) -> torch.device:
+    _require_cuda(*ts)
+    dev = None
+    for t in ts:
+        if t is not None:
+            if dev is not None and t.device != dev:
+                raise ValueError(f"tensors on two devices ({dev} and {t.device})")
+            dev = t.device
+    return dev
+
+
+def rotary_append(
+    q: Optional[torch.Tensor],
+    k: torch.Tensor,
+    v: Optional[torch.Tensor],
+    steps: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    *,
+    kv_lens: Optional[torch.Tensor] = None,
+    positions: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    k_cache: Optional[torch.Tensor] = None,
+    v_cache: Optional[torch.Tensor] = None,
+    q_out: Optional[torch.Tensor] = None,
+    k_out: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    amplitude: float = 1.0,
+) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """Rotary positions on packed q ``[T, heads, hd]`` and k ``[T, kv_heads, hd]``, and with a cache the
+    turned k and v written into its pages (``tx_rotary_append``).  Returns ``(q_out, k_out)``.
+
+    ``steps``, ``amplitude``: from :func:`rotary_steps`; its length is half the rotary dim.  A row's position is
+    ``positions[t]`` (int64), by default its key index ``kv_lens[b] - n + i`` (``i`` without ``kv_lens``).  The
+    caches are ``[pages, kv_heads, page_size, hd]`` views of any strides (a cache kept token by token passes
+    ``.transpose(1, 2)``); ``kv_lens`` counts the new tokens already.  q_out and k_out may be q and k
+    themselves; k_out is made when omitted only where there is no cache (else it is None).  Rows outside every
+    sequence are left as they were (in a tensor made here: undefined)."""
+    t, kvh, hd = k.shape if k.dim() == 3 else (-1, -1, -1)
+    _heads3("k", k, t, None, hd, k.dtype)
+    batch = _starts(cu_seqlens)
+    if steps.dim() != 1 or not 0 < 2 * steps.shape[0] <= hd:
+        raise ValueError(f"steps must be an int64 [rotary_dim / 2] tensor with rotary_dim <= {hd}")
+    _int_vector("steps", steps, steps.shape[0], torch.int64)
+    heads = kvh
+    if q is not None:
+        heads = q.shape[1] if q.dim() == 3 else 0
+        _heads3("q", q, t, None, hd, k.dtype)
+        if q_out is not None:
+            _heads3("q_out", q_out, t, heads, hd, k.dtype)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if k_out is not None:
+        _heads3("k_out", k_out, t, kvh, hd, k.dtype)
+    if kv_lens is not None:
+        _int_vector("kv_lens", kv_lens, batch)
+    if positions is not None:
+        _int_vector("positions", positions, t, torch.int64)
+    pages = page_size = max_pages = table_ld = 0
+    if k_cache is not None or v_cache is not None:
+        if k_cache is None or v_cache is None or block_table is None or kv_lens is None or v is None:
+            raise ValueError("a cache needs k_cache, v_cache, block_table, kv_lens and v")
+        _heads3("v", v, t, kvh, hd, k.dtype)
+        _check_cache(k_cache, v_cache, block_table, batch, hd, k.dtype)
+        if k_cache.shape[1] != kvh:
+            raise ValueError("the caches must hold k's heads")
+        pages, _, page_size, _ = k_cache.shape
+        max_pages, table_ld = block_table.shape[1], block_table.stride(0)
+    else:
+        block_table = v = None
+    dev = _one_device(q, k, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache, v_cache, q_out, k_out)
+    load_library()
+    if q is not None and q_out is None:
+        q_out = torch.empty((t, heads, hd), dtype=k.dtype, device=dev)
+    if k_cache is None and k_out is None:
+        k_out = torch.empty((t, kvh, hd), dtype=k.dtype, device=dev)
+    if t == 0 or batch == 0:
+        return q_out, k_out
+    st = tuple(_sv(x, n) for x, n in ((q, 2), (q_out, 2), (k, 2), (k_out, 2), (v, 2), (k_cache, 3), (v_cache, 3)))
+    ad = [_addr(x) for x in st]
+    args = (_ptr(q), ad[0], _ptr(q_out), ad[1], _ptr(k), ad[2], _ptr(k_out), ad[3], _ptr(v), ad[4],
+            _ptr(k_cache), ad[5], _ptr(v_cache), ad[6], _ptr(steps), _ptr(positions), _ptr(cu_seqlens),
+            _ptr(kv_lens), _ptr(block_table), table_ld, t, batch, heads, kvh, hd, 2 * steps.shape[0], pages,
+            page_size, max_pages, float(amplitude), 1 if interleaved else 0, _dt(k))
+    info = {"op": "rotary_append", "tokens": t, "heads": heads, "kv_heads": kvh, "head_dim": hd,
+            "cache": k_cache is not None}
+    with torch.cuda.device(dev):
+        _launch("tx_rotary_append", args, (q, k, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache,
+                                           v_cache, q_out, k_out, st), info)
+    return q_out, k_out
+
+
+def flash_attn_packed(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    scale: float,
+    causal: bool,
+    *,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of packed sequences: q ``[T, heads, hd]``, k and v ``[T, kv_heads, hd]`` (strided views, e.g.
+    columns of one projection), sequence b in rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` (int32, on the
+    device; not read by the host).  Query head h reads K/V head ``h // (heads // kv_heads)``.  Returns out
+    ``[T, heads, hd]``; rows outside every sequence are left as they were (``tx_flash_attn_packed``)."""
+    t, heads, hd = q.shape if q.dim() == 3 else (-1, -1, -1)
+    _heads3("q", q, t, heads, hd, q.dtype)
+    kvh = k.shape[1] if k.dim() == 3 else 0
+    _heads3("k", k, t, None, hd, q.dtype)
+    _heads3("v", v, t, kvh, hd, q.dtype)
+    if kvh <= 0 or heads % kvh:
+        raise ValueError(f"{kvh} K/V heads do not divide {heads} query heads")
+    batch = _starts(cu_seqlens)
+    if out is not None:
+        _heads3("out", out, t, heads, hd, q.dtype)
+    dev = _one_device(q, k, v, cu_seqlens, out)
+    load_library()
+    if out is None:
+        out = torch.empty((t, heads, hd), dtype=q.dtype, device=dev)
+    if t == 0 or batch == 0:
+        return out
+    st = tuple(_sv(x, 2) for x in (q, k, v, out))
+    ad = [_addr(x) for x in st]
+    args = (_ptr(q), ad[0], _ptr(k), ad[1], _ptr(v), ad[2], _ptr(out), ad[3], _ptr(cu_seqlens), t, batch, heads, kvh,
+            hd, float(scale), 1 if causal else 0, _dt(q))
+    info = {"op": "flash_attn_packed", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh, "head_dim": hd,
+            "causal": bool(causal)}
+    with torch.cuda.device(dev):
+        _launch("tx_flash_attn_packed", args, (q, k, v, out, cu_seqlens, st), info)
+    return out
+
+
+def flash_attn_paged_workspace(tokens: int, batch: int, heads: int, kv_heads: int, head_dim: int, page_size: int,
+                               max_pages: int, max_q_len: int = 0) -> int:
+    """fp32 values of workspace that :func:`flash_attn_paged` needs for these sizes (0: none)."""
+    n = ctypes.c_int64(0)
+    _check("tx_flash_attn_paged_workspace",
+           load_library().tx_flash_attn_paged_workspace(tokens, batch, heads, kv_heads, head_dim, page_size, max_pages,
+                                                        max_q_len, ctypes.addressof(n)))
+    return n.value
+
+
+def flash_attn_paged(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    kv_lens: torch.Tensor,
+    scale: float,
+    causal: bool = True,
+    *,
+    max_q_len: int = 0,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of each sequence's new tokens over its paged cache (``tx_flash_attn_paged``): one token per
+    sequence when decoding, a chunk of a prompt, or any mixture.  q ``[T, heads, hd]`` packed by ``cu_seqlens``;
+    caches ``[pages, kv_heads, page_size, hd]`` (any strides) that already hold the new tokens; ``kv_lens``
+    counts them.  Row i of n sees the keys up to its own, ``kv_lens[b] - n + i``, when causal, else all of them.
+    A page index outside ``[0, pages)`` makes the rows that need it NaN.
+
+    ``max_q_len``: a bound on the rows of one sequence that the caller knows (0: T), to choose the kernel by.
+    ``workspace``: fp32, at least :func:`flash_attn_paged_workspace` values, made here when omitted; calls that
+    overlap in time need one each."""
+    t, heads, hd = q.shape if q.dim() == 3 else (-1, -1, -1)
+    _heads3("q", q, t, heads, hd, q.dtype)
+    batch = _starts(cu_seqlens)
+    _int_vector("kv_lens", kv_lens, batch)
+    _check_cache(k_cache, v_cache, block_table, batch, hd, q.dtype)
+    pages, kvh, page_size, _ = k_cache.shape
+    if kvh <= 0 or heads % kvh:
+        raise ValueError(f"{kvh} K/V heads do not divide {heads} query heads")
+    if out is not None:
+        _heads3("out", out, t, heads, hd, q.dtype)
+    dev = _one_device(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, out, workspace)
+    load_library()
+    if out is None:
+        out = torch.empty((t, heads, hd), dtype=q.dtype, device=dev)
+    if t == 0 or batch == 0:
+        return out
+    max_pages = block_table.shape[1]
+    need = flash_attn_paged_workspace(t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+    if workspace is None and need > 0:
+        workspace = torch.empty(need, dtype=torch.float32, device=dev)
+    if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous()
+                                  or workspace.numel() < need):
+        raise ValueError(f"workspace must be contiguous fp32 with at least {need} elements")
+    st = (_sv(q, 2), _sv(k_cache, 3), _sv(v_cache, 3), _sv(out, 2))
+    ad = [_addr(x) for x in st]
+    args = (_ptr(q), ad[0], _ptr(k_cache), ad[1], _ptr(v_cache), ad[2], _ptr(out), ad[3], _ptr(cu_seqlens),
+            _ptr(kv_lens), _ptr(block_table), block_table.stride(0), t, batch, heads, kvh, hd, pages, page_size,
+            max_pages, int(max_q_len), float(scale), 1 if causal else 0, _ptr(workspace),
+            0 if workspace is None else workspace.numel(), _dt(q))
+    info = {"op": "flash_attn_paged", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh, "head_dim": hd,
+            "causal": bool(causal), "page_size": page_size}
+    with torch.cuda.device(dev):
+        _launch("tx_flash_attn_paged", args, (q, k_cache, v_cache, out, cu_seqlens, kv_lens, block_table, workspace, st),
+                info)
     return out

@@ -338,4 +338,295 @@ int tx_flash_attn_fwd_strided(const void* q, const void* k, const void* v, void*
   return launch_attention(at, dt, (hipStream_t)stream);
 }
 
+// ---- packed sequences and the paged cache ------------------------------------
+// A [rows][heads][head_dim] view: 16-byte rows, heads that do not overlap, and
+// (outputs) rows that do not either.
+static int check_rows(const void* p, const int64_t* st, int64_t rows, int64_t heads, int64_t hd, bool out) {
+  if (!p || !st) return TX_EINVAL;
+  if (st[0] < 0 || st[1] < 0) return TX_EINVAL;
+  if (!aligned16(p) || st[0] % 8 || st[1] % 8) return TX_EUNSUPPORTED;
+  if (st[0] > (int64_t)1 << 40 || st[1] > (int64_t)1 << 40) return TX_EUNSUPPORTED;
+  const int64_t st3[3] = {st[0], st[1], 0};
+  if (out && !view_is_nonoverlapping(st3, rows, heads, 1, hd)) return TX_EINVAL;
+  return TX_OK;
+}
+// A [pages][heads][slots][head_dim] cache view.
+static int check_cache(const void* p, const int64_t* st, int64_t pages, int64_t heads, int64_t slots, int64_t hd) {
+  if (!p || !st) return TX_EINVAL;
+  for (int i = 0; i < 3; ++i) {
+    if (st[i] < 0) return TX_EINVAL;
+    if (st[i] % 8 || st[i] > (int64_t)1 << 40) return TX_EUNSUPPORTED;
+  }
+  if (!aligned16(p)) return TX_EUNSUPPORTED;
+  // The tile loaders form offsets within a page's run of slots in 32 bits.
+  if (st[2] >= 1 << 24) return TX_EUNSUPPORTED;
+  return view_is_nonoverlapping(st, pages, heads, slots, hd) ? TX_OK : TX_EINVAL;
+}
+static bool rows_disjoint(const void* a, const int64_t* as, int64_t ah, const void* b, const int64_t* bs,
+                          int64_t bh, int64_t rows, int64_t hd) {
+  return blocks_disjoint((uintptr_t)a, as[0], (ah - 1) * as[1] + hd, rows, (uintptr_t)b, bs[0],
+                         (bh - 1) * bs[1] + hd, rows);
+}
+static int64_t page_extent(const int64_t* st, int64_t heads, int64_t slots, int64_t hd) {
+  return (heads - 1) * st[1] + (slots - 1) * st[2] + hd;
+}
+static bool same_rows(const void* a, const int64_t* as, const void* b, const int64_t* bs) {
+  return a == b && as[0] == bs[0] && as[1] == bs[1];
+}
+// Totals every entry point of this group shares.
+static int check_seqs(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t hd, int dt,
+                      const int32_t* cu) {
+  if (!cu || tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || hd <= 0) return TX_EINVAL;
+  if (!is16(dt)) return TX_EUNSUPPORTED;
+  if (heads % kv_heads) return TX_EINVAL;
+  // Grids of 256 threads per 16 rows, per 4 tokens and per sequence stay below 2^32 threads.
+  if (tokens > 1 << 24 || batch > 1 << 20 || heads > 65535 || tokens * heads > 1 << 27) return TX_EUNSUPPORTED;
+  if (((uintptr_t)cu & 3u)) return TX_EUNSUPPORTED;
+  return TX_OK;
+}
+static int check_pages(const int32_t* table, int64_t table_ld, int64_t batch, int64_t num_pages, int64_t page_size,
+                       int64_t max_pages) {
+  if (!table || num_pages <= 0 || page_size <= 0 || max_pages <= 0) return TX_EINVAL;
+  if (batch > 1 && table_ld < max_pages) return TX_EINVAL;
+  if (((uintptr_t)table & 3u) || table_ld < 0 || table_ld > (int64_t)1 << 40) return TX_EUNSUPPORTED;
+  if (page_size < 8 || page_size > 1 << 15 || (page_size & (page_size - 1))) return TX_EUNSUPPORTED;
+  if (num_pages > 0x7fffffff || max_pages > (int64_t)1 << 30 || max_pages * page_size > (int64_t)1 << 30)
+    return TX_EUNSUPPORTED;
+  return TX_OK;
+}
+static int page_log2(int64_t page_size) {
+  int n = 0;
+  while (((int64_t)1 << n) < page_size) ++n;
+  return n;
+}
+
+int tx_rotary_append(const void* q, const int64_t q_strides[2], void* q_out, const int64_t q_out_strides[2],
+                     const void* k, const int64_t k_strides[2], void* k_out, const int64_t k_out_strides[2],
+                     const void* v, const int64_t v_strides[2], void* k_cache,
+                     const int64_t k_cache_strides[3], void* v_cache, const int64_t v_cache_strides[3],
+                     const int64_t* steps, const int64_t* positions, const int32_t* cu_seqlens,
+                     const int32_t* kv_lens, const int32_t* block_table, int64_t table_ld, int64_t tokens,
+                     int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim,
+                     int64_t num_pages, int64_t page_size, int64_t max_pages, float amplitude, int interleaved,
+                     int dt, void* stream) {
+  if (!k || !steps || (!q) != (!q_out) || (!k_cache) != (!v_cache)) return TX_EINVAL;
+  if (!k_out && !k_cache) return TX_EINVAL;
+  if (!(amplitude > 0.f) || !(amplitude < 3.0e38f)) return TX_EINVAL;
+  int rc = check_seqs(tokens, batch, q_heads, kv_heads, head_dim, dt, cu_seqlens);
+  if (rc != TX_OK) return rc;
+  if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > head_dim) return TX_EINVAL;
+  if (head_dim % 8 || head_dim > 256) return TX_EUNSUPPORTED;
+  if (((uintptr_t)steps & 7u) || ((uintptr_t)positions & 7u) || ((uintptr_t)kv_lens & 3u)) return TX_EUNSUPPORTED;
+  // Work units of one workgroup's tokens are counted in 32 bits.
+  if ((q_heads + 2 * kv_heads) * head_dim > (int64_t)1 << 26) return TX_EUNSUPPORTED;
+  if (q && (rc = check_rows(q, q_strides, tokens, q_heads, head_dim, false)) != TX_OK) return rc;
+  if (q && (rc = check_rows(q_out, q_out_strides, tokens, q_heads, head_dim, true)) != TX_OK) return rc;
+  if ((rc = check_rows(k, k_strides, tokens, kv_heads, head_dim, false)) != TX_OK) return rc;
+  if (k_out && (rc = check_rows(k_out, k_out_strides, tokens, kv_heads, head_dim, true)) != TX_OK) return rc;
+  if (k_cache) {
+    if (!kv_lens) return TX_EINVAL;
+    if ((rc = check_rows(v, v_strides, tokens, kv_heads, head_dim, false)) != TX_OK) return rc;
+    if ((rc = check_pages(block_table, table_ld, batch, num_pages, page_size, max_pages)) != TX_OK) return rc;
+    if ((rc = check_cache(k_cache, k_cache_strides, num_pages, kv_heads, page_size, head_dim)) != TX_OK) return rc;
+    if ((rc = check_cache(v_cache, v_cache_strides, num_pages, kv_heads, page_size, head_dim)) != TX_OK) return rc;
+  }
+  // Outputs: an input itself, or memory that no input and no other output uses.
+  struct View {
+    const void* p;
+    const int64_t* st;
+    int64_t extent, count;
+    int in_place;  // the input (index) that it may be
+  } in[3], out[4];
+  int n_in = 0, n_out = 0;
+  const int64_t qx = q ? (q_heads - 1) * q_strides[1] + head_dim : 0;
+  const int64_t kx = (kv_heads - 1) * k_strides[1] + head_dim;
+  in[n_in++] = {k, k_strides, kx, tokens, -1};
+  if (q) in[n_in++] = {q, q_strides, qx, tokens, -1};
+  if (k_cache) in[n_in++] = {v, v_strides, (kv_heads - 1) * v_strides[1] + head_dim, tokens, -1};
+  if (k_out) out[n_out++] = {k_out, k_out_strides, (kv_heads - 1) * k_out_strides[1] + head_dim, tokens, 0};
+  if (q) out[n_out++] = {q_out, q_out_strides, (q_heads - 1) * q_out_strides[1] + head_dim, tokens, 1};
+  if (k_cache) {
+    out[n_out++] = {k_cache, k_cache_strides, page_extent(k_cache_strides, kv_heads, page_size, head_dim), num_pages, -1};
+    out[n_out++] = {v_cache, v_cache_strides, page_extent(v_cache_strides, kv_heads, page_size, head_dim), num_pages, -1};
+  }
+  for (int o = 0; o < n_out; ++o) {
+    for (int i = 0; i < n_in; ++i) {
+      if (out[o].in_place == i && same_rows(out[o].p, out[o].st, in[i].p, in[i].st)) continue;
+      if (!blocks_disjoint((uintptr_t)out[o].p, out[o].st[0], out[o].extent, out[o].count, (uintptr_t)in[i].p,
+                           in[i].st[0], in[i].extent, in[i].count))
+        return TX_EINVAL;
+    }
+    for (int i = 0; i < o; ++i)
+      if (!blocks_disjoint((uintptr_t)out[o].p, out[o].st[0], out[o].extent, out[o].count, (uintptr_t)out[i].p,
+                           out[i].st[0], out[i].extent, out[i].count))
+        return TX_EINVAL;
+  }
+  RotaryArgs a{};
+  a.s = {cu_seqlens, kv_lens, block_table, table_ld, (int)tokens, (int)batch, 0, 0, 0};
+  a.k = k;
+  a.k_st = k_strides[0];
+  a.k_sh = k_strides[1];
+  if (q) {
+    a.q = q;
+    a.q_st = q_strides[0];
+    a.q_sh = q_strides[1];
+    a.q_out = q_out;
+    a.qo_st = q_out_strides[0];
+    a.qo_sh = q_out_strides[1];
+  }
+  if (k_out) {
+    a.k_out = k_out;
+    a.ko_st = k_out_strides[0];
+    a.ko_sh = k_out_strides[1];
+  }
+  if (k_cache) {
+    a.s.num_pages = (int)num_pages;
+    a.s.page_log2 = page_log2(page_size);
+    a.s.max_pages = (int)max_pages;
+    a.v = v;
+    a.v_st = v_strides[0];
+    a.v_sh = v_strides[1];
+    a.k_cache = k_cache;
+    a.kc_sp = k_cache_strides[0];
+    a.kc_sh = k_cache_strides[1];
+    a.kc_st = k_cache_strides[2];
+    a.v_cache = v_cache;
+    a.vc_sp = v_cache_strides[0];
+    a.vc_sh = v_cache_strides[1];
+    a.vc_st = v_cache_strides[2];
+  }
+  a.steps = (const uint64_t*)steps;
+  a.positions = positions;
+  a.heads = (int)q_heads;
+  a.kv_heads = (int)kv_heads;
+  a.head_dim = (int)head_dim;
+  a.rotary = (int)rotary_dim;
+  a.amplitude = amplitude;
+  a.interleaved = interleaved ? 1 : 0;
+  return launch_rotary_append(a, dt, (hipStream_t)stream);
+}
+
+int tx_flash_attn_packed(const void* q, const int64_t q_strides[2], const void* k, const int64_t k_strides[2],
+                         const void* v, const int64_t v_strides[2], void* o, const int64_t o_strides[2],
+                         const int32_t* cu_seqlens, int64_t tokens, int64_t batch, int64_t q_heads,
+                         int64_t kv_heads, int64_t head_dim, float scale, int causal, int dt, void* stream) {
+  int rc = check_seqs(tokens, batch, q_heads, kv_heads, head_dim, dt, cu_seqlens);
+  if (rc != TX_OK) return rc;
+  if (!(scale > 0.f) || !(scale < 3.0e38f)) return TX_EINVAL;
+  if (head_dim != 64 && head_dim != 128) return TX_EUNSUPPORTED;
+  if ((rc = check_rows(q, q_strides, tokens, q_heads, head_dim, false)) != TX_OK) return rc;
+  if ((rc = check_rows(k, k_strides, tokens, kv_heads, head_dim, false)) != TX_OK) return rc;
+  if ((rc = check_rows(v, v_strides, tokens, kv_heads, head_dim, false)) != TX_OK) return rc;
+  if ((rc = check_rows(o, o_strides, tokens, q_heads, head_dim, true)) != TX_OK) return rc;
+  // The tile loaders form 32-bit byte offsets within a tile of key rows.
+  if (k_strides[0] >= 1 << 24 || v_strides[0] >= 1 << 24) return TX_EUNSUPPORTED;
+  if (!rows_disjoint(o, o_strides, q_heads, q, q_strides, q_heads, tokens, head_dim) ||
+      !rows_disjoint(o, o_strides, q_heads, k, k_strides, kv_heads, tokens, head_dim) ||
+      !rows_disjoint(o, o_strides, q_heads, v, v_strides, kv_heads, tokens, head_dim))
+    return TX_EINVAL;
+  SeqAttnArgs a{};
+  a.s = {cu_seqlens, nullptr, nullptr, 0, (int)tokens, (int)batch, 0, 0, 0};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.o = o;
+  a.q_st = q_strides[0];
+  a.q_sh = q_strides[1];
+  a.k_st = k_strides[0];
+  a.k_sh = k_strides[1];
+  a.v_st = v_strides[0];
+  a.v_sh = v_strides[1];
+  a.o_st = o_strides[0];
+  a.o_sh = o_strides[1];
+  a.heads = (int)q_heads;
+  a.kv_heads = (int)kv_heads;
+  a.group = (int)(q_heads / kv_heads);
+  a.head_dim = (int)head_dim;
+  a.scale = scale;
+  a.causal = causal ? 1 : 0;
+  return launch_seq_attention(a, dt, (hipStream_t)stream);
+}
+
+int tx_flash_attn_paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                  int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t max_q_len,
+                                  int64_t* floats) {
+  const int32_t some = 0;
+  int rc = check_seqs(tokens, batch, q_heads, kv_heads, head_dim, TX_BF16, &some);
+  if (rc != TX_OK) return rc;
+  if (!floats) return TX_EINVAL;
+  if (head_dim != 64 && head_dim != 128) return TX_EUNSUPPORTED;
+  if ((rc = check_pages(&some, max_pages, batch, 1, page_size, max_pages)) != TX_OK) return rc;
+  SeqAttnArgs a{};
+  a.s.tokens = (int)tokens;
+  a.s.batch = (int)batch;
+  a.s.page_log2 = page_log2(page_size);
+  a.s.max_pages = (int)max_pages;
+  a.heads = (int)q_heads;
+  a.kv_heads = (int)kv_heads;
+  a.group = (int)(q_heads / kv_heads);
+  a.head_dim = (int)head_dim;
+  a.paged = 1;
+  a.max_q_len = max_q_len <= 0 || max_q_len > tokens ? tokens : max_q_len;
+  *floats = seq_attention_workspace(a);
+  return TX_OK;
+}
+
+int tx_flash_attn_paged(const void* q, const int64_t q_strides[2], const void* k_cache,
+                        const int64_t k_cache_strides[3], const void* v_cache,
+                        const int64_t v_cache_strides[3], void* o, const int64_t o_strides[2],
+                        const int32_t* cu_seqlens, const int32_t* kv_lens, const int32_t* block_table,
+                        int64_t table_ld, int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                        int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages,
+                        int64_t max_q_len, float scale, int causal, float* workspace, int64_t workspace_floats,
+                        int dt, void* stream) {
+  int rc = check_seqs(tokens, batch, q_heads, kv_heads, head_dim, dt, cu_seqlens);
+  if (rc != TX_OK) return rc;
+  if (!kv_lens || !(scale > 0.f) || !(scale < 3.0e38f)) return TX_EINVAL;
+  if ((uintptr_t)kv_lens & 3u) return TX_EUNSUPPORTED;
+  if (head_dim != 64 && head_dim != 128) return TX_EUNSUPPORTED;
+  if ((rc = check_rows(q, q_strides, tokens, q_heads, head_dim, false)) != TX_OK) return rc;
+  if ((rc = check_rows(o, o_strides, tokens, q_heads, head_dim, true)) != TX_OK) return rc;
+  if ((rc = check_pages(block_table, table_ld, batch, num_pages, page_size, max_pages)) != TX_OK) return rc;
+  if ((rc = check_cache(k_cache, k_cache_strides, num_pages, kv_heads, page_size, head_dim)) != TX_OK) return rc;
+  if ((rc = check_cache(v_cache, v_cache_strides, num_pages, kv_heads, page_size, head_dim)) != TX_OK) return rc;
+  const int64_t ox = (q_heads - 1) * o_strides[1] + head_dim;
+  if (!rows_disjoint(o, o_strides, q_heads, q, q_strides, q_heads, tokens, head_dim) ||
+      !blocks_disjoint((uintptr_t)o, o_strides[0], ox, tokens, (uintptr_t)k_cache, k_cache_strides[0],
+                       page_extent(k_cache_strides, kv_heads, page_size, head_dim), num_pages) ||
+      !blocks_disjoint((uintptr_t)o, o_strides[0], ox, tokens, (uintptr_t)v_cache, v_cache_strides[0],
+                       page_extent(v_cache_strides, kv_heads, page_size, head_dim), num_pages))
+    return TX_EINVAL;
+  SeqAttnArgs a{};
+  a.s = {cu_seqlens, kv_lens, block_table, table_ld, (int)tokens, (int)batch, (int)num_pages,
+         page_log2(page_size), (int)max_pages};
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.o = o;
+  a.q_st = q_strides[0];
+  a.q_sh = q_strides[1];
+  a.o_st = o_strides[0];
+  a.o_sh = o_strides[1];
+  a.k_sp = k_cache_strides[0];
+  a.k_sh = k_cache_strides[1];
+  a.k_st = k_cache_strides[2];
+  a.v_sp = v_cache_strides[0];
+  a.v_sh = v_cache_strides[1];
+  a.v_st = v_cache_strides[2];
+  a.heads = (int)q_heads;
+  a.kv_heads = (int)kv_heads;
+  a.group = (int)(q_heads / kv_heads);
+  a.head_dim = (int)head_dim;
+  a.scale = scale;
+  a.causal = causal ? 1 : 0;
+  a.paged = 1;
+  a.max_q_len = max_q_len <= 0 || max_q_len > tokens ? tokens : max_q_len;
+  a.ws = workspace;
+  const int64_t need = seq_attention_workspace(a);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_floats < need)) return TX_EINVAL;
+  if (need > 0 && spans_overlap((uintptr_t)workspace, need * 4, (uintptr_t)o, ((tokens - 1) * o_strides[0] + ox) * 2))
+    return TX_EINVAL;
+  return launch_seq_attention(a, dt, (hipStream_t)stream);
+}
+
 }  // extern "C"

@@ -62,6 +62,22 @@ inline bool spans_overlap(uintptr_t a, int64_t a_len, uintptr_t b, int64_t b_len
   return a < b + (uintptr_t)b_len && b < a + (uintptr_t)a_len;
 }
 
+// Whether two strided views share no byte.  Each is `count` blocks of
+// `extent` elements at distance `stride` (16-bit elements).  Either their
+// spans do not meet, or they have one stride in common and, within it, blocks
+// that lie side by side (column views of one projection, K and V of one page).
+inline bool blocks_disjoint(uintptr_t a, int64_t a_stride, int64_t a_extent, int64_t a_count,
+                            uintptr_t b, int64_t b_stride, int64_t b_extent, int64_t b_count) {
+  const __int128 a_len = ((__int128)(a_count - 1) * a_stride + a_extent) * 2;
+  const __int128 b_len = ((__int128)(b_count - 1) * b_stride + b_extent) * 2;
+  if ((__int128)a + a_len <= (__int128)b || (__int128)b + b_len <= (__int128)a) return true;
+  if (a_stride != b_stride || a_stride <= 0) return false;
+  const __int128 row = (__int128)a_stride * 2;
+  __int128 at = ((__int128)b - (__int128)a) % row;  // b's blocks start here within a's
+  if (at < 0) at += row;
+  return at >= (__int128)a_extent * 2 && at + (__int128)b_extent * 2 <= row;
+}
+
 }  // namespace tx
 
 namespace tx {

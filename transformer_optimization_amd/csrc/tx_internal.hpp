@@ -74,6 +74,56 @@ struct AttnArgs {
   float* row_stats;   // eager mode: [B*H*S][2] (max, sum) workspace
 };
 
+// Packed sequences and a paged cache (tx_api.h).  Strides in elements: st per
+// token (or slot), sh per head, sp per page.
+struct SeqArgs {
+  const int32_t* cu;        // [batch + 1]
+  const int32_t* kv_lens;   // [batch] or nullptr (as many keys as rows)
+  const int32_t* table;     // [batch][table_ld] page indices (paged only)
+  int64_t table_ld;
+  int tokens, batch;
+  int num_pages, page_log2, max_pages;
+};
+
+struct RotaryArgs {
+  SeqArgs s;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_out;
+  void* k_cache;
+  void* v_cache;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh, ko_st, ko_sh;
+  int64_t kc_sp, kc_sh, kc_st, vc_sp, vc_sh, vc_st;
+  const uint64_t* steps;
+  const int64_t* positions;
+  int heads, kv_heads, head_dim, rotary;
+  float amplitude;
+  int interleaved;
+};
+
+struct SeqAttnArgs {
+  SeqArgs s;
+  const void* q;
+  const void* k;  // [T][kv_heads][hd], or the cache
+  const void* v;
+  void* o;
+  int64_t q_st, q_sh, o_st, o_sh;
+  int64_t k_sp, k_sh, k_st, v_sp, v_sh, v_st;
+  int heads, kv_heads, group, head_dim;
+  float scale;
+  int causal;
+  int paged;
+  int64_t max_q_len;
+  float* ws;
+};
+
+int launch_rotary_append(const RotaryArgs& a, int dt, hipStream_t st);
+int launch_seq_attention(const SeqAttnArgs& a, int dt, hipStream_t st);
+// Floats of workspace a paged call of these sizes needs.
+int64_t seq_attention_workspace(const SeqAttnArgs& a);
+
 int launch_layernorm(const LayerNormArgs& a, hipStream_t st);
 int launch_gemm(const GemmArgs& g, int ab_dt, int c_dt, int bias_dt, int res_dt, bool qkv,
                 hipStream_t st);
