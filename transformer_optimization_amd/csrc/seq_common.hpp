@@ -44,11 +44,11 @@ __device__ __forceinline__ SeqTile seq_find(const SeqArgs& s, int group, int r, 
   }
   SeqTile t;
   t.b = __builtin_amdgcn_readfirstlane(lo);
-  const int q0 = seq_cut(s.cu[t.b], 0, s.tokens);
-  const int q1 = seq_cut(s.cu[t.b + 1], q0, s.tokens);
+  const int q0 = __builtin_amdgcn_readfirstlane(seq_cut(s.cu[t.b], 0, s.tokens));
+  const int q1 = __builtin_amdgcn_readfirstlane(seq_cut(s.cu[t.b + 1], q0, s.tokens));
   t.q0 = q0;
   t.qn = q1 - q0;
-  t.kvn = s.kv_lens ? s.kv_lens[t.b] : t.qn;
+  t.kvn = s.kv_lens ? __builtin_amdgcn_readfirstlane(s.kv_lens[t.b]) : t.qn;
   t.kvn = t.kvn < 0 ? 0 : t.kvn;
   const int64_t d = w - ((int64_t)q0 * group / r + t.b);
   t.tile = (int)d;
