@@ -618,6 +618,30 @@ def test_paged_attention_cache_beyond_32_bit_offsets(cuda):
     _same(got, ref, tol, "paged")
 
 
+@gpu
+@pytest.mark.parametrize("starts", [[0, 9, 2, 20, 11, 30], [0, 40, 40, -5, 10**9, 30], [7, 3, 1, 0, 0, 0]])
+def test_starts_that_do_not_ascend_stay_in_bounds(cuda, starts):
+    """No result is promised for such starts but that nothing outside the rows and the slots named is written."""
+    dtype, hd, h, hk, batch = torch.bfloat16, 64, 4, 2, 5
+    _, _, kc, vc, table = _paged([600] * batch, hk, 16, hd, dtype, cuda, 150, fill=0.0)
+    whole = torch.full((40, h, hd), 3.0, dtype=dtype, device=cuda)
+    out, cu, kvl = whole[5:35], _i32(starts, cuda), _i32([600] * batch, cuda)
+    x = _randn((30, h + 2 * hk, hd), dtype, cuda, 151)
+    for max_q in (0, 1):
+        ws = torch.full((_C.flash_attn_paged_workspace(30, batch, h, hk, hd, 16, table.shape[1], max_q) + 64,), 2.0,
+                        device=cuda)
+        _C.flash_attn_paged(x[:, :h], kc, vc, table, cu, kvl, 0.1, max_q_len=max_q, out=out, workspace=ws[:-64])
+        assert bool((ws[-64:] == 2).all())
+    _C.flash_attn_packed(x[:, :h], x[:, h:h + hk], x[:, h + hk:], cu, 0.1, True, out=out)
+    steps, _ = _C.rotary_steps(hd, device=cuda)
+    spare = [p for p in range(kc.shape[0]) if not bool((table == p).any())]
+    _C.rotary_append(x[:, :h], x[:, h:h + hk], x[:, h + hk:], steps, cu, kv_lens=kvl, block_table=table, k_cache=kc,
+                     v_cache=vc, q_out=out)
+    torch.cuda.synchronize()
+    assert bool((whole[:5] == 3).all()) and bool((whole[35:] == 3).all())
+    assert bool((kc[spare] == 0).all()) and bool((vc[spare] == 0).all())
+
+
 # ---------------------------------------------------------------- together
 @gpu
 @pytest.mark.parametrize("dtype,hd,h,hk,page", [(torch.bfloat16, 128, 8, 2, 16), (torch.float16, 64, 8, 8, 32)])

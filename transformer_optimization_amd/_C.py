@@ -894,7 +894,8 @@ def flash_attn_paged(
     if t == 0 or batch == 0:
         return out
     max_pages = block_table.shape[1]
-    need = flash_attn_paged_workspace(t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+    with torch.cuda.device(dev):
+        need = flash_attn_paged_workspace(t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
     if workspace is None and need > 0:
         workspace = torch.empty(need, dtype=torch.float32, device=dev)
     if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous()

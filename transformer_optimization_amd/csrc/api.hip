@@ -358,8 +358,9 @@ static int check_cache(const void* p, const int64_t* st, int64_t pages, int64_t 
     if (st[i] % 8 || st[i] > (int64_t)1 << 40) return TX_EUNSUPPORTED;
   }
   if (!aligned16(p)) return TX_EUNSUPPORTED;
-  // The tile loaders form offsets within a page's run of slots in 32 bits.
-  if (st[2] >= 1 << 24) return TX_EUNSUPPORTED;
+  // Byte strides of a page, and byte offsets within one K/V head's part of it, are 32-bit.
+  if (st[2] >= 1 << 24 || st[0] >= (int64_t)1 << 31 || (slots - 1) * st[2] + hd >= (int64_t)1 << 31)
+    return TX_EUNSUPPORTED;
   return view_is_nonoverlapping(st, pages, heads, slots, hd) ? TX_OK : TX_EINVAL;
 }
 static bool rows_disjoint(const void* a, const int64_t* as, int64_t ah, const void* b, const int64_t* bs,
@@ -379,8 +380,9 @@ static int check_seqs(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_h
   if (!cu || tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || hd <= 0) return TX_EINVAL;
   if (!is16(dt)) return TX_EUNSUPPORTED;
   if (heads % kv_heads) return TX_EINVAL;
-  // Grids of 256 threads per 16 rows, per 4 tokens and per sequence stay below 2^32 threads.
-  if (tokens > 1 << 24 || batch > 1 << 20 || heads > 65535 || tokens * heads > 1 << 27) return TX_EUNSUPPORTED;
+  // Grids (256 threads per 128 rows, per 4 tokens and per sequence) stay below 2^32 threads, and the items of
+  // a paged call (per 16 rows and per sequence, up to 256 parts of the keys) below 2^31.
+  if (tokens > 1 << 24 || batch > 1 << 20 || heads > 65535 || tokens * heads > 1 << 26) return TX_EUNSUPPORTED;
   if (((uintptr_t)cu & 3u)) return TX_EUNSUPPORTED;
   return TX_OK;
 }

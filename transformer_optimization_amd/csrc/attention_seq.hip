@@ -15,10 +15,10 @@ struct SeqHead {
   const T* k;  // row 0 of the sequence, or page 0 of the cache
   const T* v;
   int b;
-  __device__ __forceinline__ void init(const SeqAttnArgs& a, const SeqTile& t, int hk) {
-    k = (const T*)a.k + hk * a.k_sh + (PAGED ? 0 : (int64_t)t.q0 * a.k_st);
-    v = (const T*)a.v + hk * a.v_sh + (PAGED ? 0 : (int64_t)t.q0 * a.v_st);
-    b = t.b;
+  __device__ __forceinline__ void init(const SeqAttnArgs& a, int b_, int q0, int hk) {
+    k = (const T*)a.k + hk * a.k_sh + (PAGED ? 0 : (int64_t)q0 * a.k_st);
+    v = (const T*)a.v + hk * a.v_sh + (PAGED ? 0 : (int64_t)q0 * a.v_st);
+    b = b_;
   }
   // Offset of key j's row in units of (page, slot); false: it has no page.
   __device__ __forceinline__ bool at(const SeqAttnArgs& a, int j, const T*& kr, const T*& vr) const {
@@ -50,6 +50,7 @@ __device__ void seq_row(const SeqAttnArgs& a, const SeqHead<T, PAGED>& hp, const
     const T* kr;
     if (!hp.at(a, j, kr, vr)) return NAN_;  // a key that has no page
     float s = 0.f;
+#pragma unroll 1  // this path is never hot: few registers
     for (int d = 0; d < HD; d += 8) {
       const u32x4 x = ld128(qrow + d), y = ld128(kr + d);
 #pragma unroll
@@ -62,6 +63,7 @@ __device__ void seq_row(const SeqAttnArgs& a, const SeqHead<T, PAGED>& hp, const
   l = 0.f;
   if (j1 <= j0) return;
   const T* vr;
+#pragma unroll 1
   for (int j = j0 + lane; j < j1; j += 64) {
     const float s = score(j, vr), mn = fmaxf(m, s);
     l = (m == NEG_INF ? l : l * expf(m - mn)) + (mn == NEG_INF ? 0.f : expf(s - mn));
@@ -73,11 +75,13 @@ __device__ void seq_row(const SeqAttnArgs& a, const SeqHead<T, PAGED>& hp, const
   l = wave_sum(m == NEG_INF ? l : l * expf(m - mw));
   m = mw;
   const float inv = 1.0f / l;  // l = 0 (every score -inf): 0 * inf below is NaN, as softmax gives
+#pragma unroll 1
   for (int b0 = j0; b0 < j1; b0 += 64) {
     const int j = b0 + lane;
     float p = 0.f;
     if (j < j1) p = (m == NEG_INF ? 0.f : expf(score(j, vr) - m)) * inv;
     const int n = j1 - b0 < 64 ? j1 - b0 : 64;
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       const float pi = __shfl(p, i, 64);
       const T* kr;
@@ -96,7 +100,7 @@ __device__ void seq_row(const SeqAttnArgs& a, const SeqHead<T, PAGED>& hp, const
 // v_mfma_f32_32x32x16, from the key-permuted K operand, so that a lane's
 // scores are, in order, the P operand of the second product; V keeps its
 // natural layout and is transposed by its LDS reads (attention_tiles.hpp).
-constexpr int SQ_ROWS = 128;
+constexpr int SQ_ROWS = SEQ_TILE;
 constexpr int SQ_THREADS = 256;
 constexpr float SQ_LOG2E = 1.4426950408889634f;
 
@@ -328,53 +332,75 @@ __device__ __forceinline__ int sq_bad_from(int mine, int* slot, int wave, int la
   return min(min(slot[0], slot[1]), min(slot[2], slot[3]));
 }
 
+// Partial results of unit_rows rows over one part of their keys: o (fp32,
+// normalised) [unit_rows][HD], then the rows' maxima m (log2 units) and sums l.
+__host__ __device__ constexpr int64_t sq_unit_floats(int rows, int hd) { return (int64_t)((rows * (hd + 2) + 3) & ~3); }
+
+// One row again, key by key, into the output or its partial result.
 template <typename T, int HD, bool PAGED>
-__global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_tile_kernel(SeqAttnArgs a, int tiles) {
+__device__ __forceinline__ void sq_row_again(const SeqAttnArgs& a, const SeqHead<T, PAGED>& hp, int64_t tok, int h,
+                                             int j0, int j1, float* po, float* pml, int unit_rows) {
+  const int lane = threadIdx.x & 63;
+  float o[HD / 64], m, l;
+  seq_row<T, HD, PAGED>(a, hp, (const T*)a.q + tok * a.q_st + h * a.q_sh, j0, j1, o, m, l);
+  T* orow = (T*)a.o + tok * a.o_st + h * a.o_sh;
+#pragma unroll
+  for (int e = 0; e < HD / 64; ++e) {
+    if (po) po[lane + 64 * e] = o[e];
+    else orow[lane + 64 * e] = from_f32<T>(o[e]);
+  }
+  if (po && lane == 0) {
+    pml[0] = m * SQ_LOG2E;
+    pml[unit_rows] = l;
+  }
+}
+
+// Rows [r0, r0 + 128) of a sequence over the keys [j0, j1) (j0 and, but for
+// the last part, j1 multiples of 64).  part: where their partial results go, or
+// nullptr for the output.
+template <typename T, int HD, bool PAGED>
+__device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0, int qn, int kvn, int hk, int r0,
+                                             int j0, int j1, float* part, T* lds, int* bad, int lane, int wave) {
   typedef SqTile<T, HD, PAGED> Tile;
-  __shared__ __attribute__((aligned(16))) T lds[Tile::LDS_ELEMS];
-  __shared__ int bad[4];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  // The last tiles of a sequence, which see the most keys, start first.
-  const int hk = blockIdx.x % a.kv_heads;
-  const SeqTile t = seq_find(a.s, a.group, SQ_ROWS, tiles - 1 - (int)(blockIdx.x / a.kv_heads));
-  const int rows = t.qn * a.group, r0 = t.tile * SQ_ROWS;
-  if (r0 >= rows) return;
-  const int G = a.group, n = min(rows - r0, SQ_ROWS);
-  const int cap = PAGED ? a.s.max_pages << a.s.page_log2 : t.kvn;
+  const int G = a.group, n = min(qn * G - r0, SQ_ROWS);
+  const int cap = PAGED ? a.s.max_pages << a.s.page_log2 : kvn;
   auto keys_of = [&](int r) {  // keys that row r sees
-    return max(a.causal ? t.kvn - t.qn + r / G + 1 : t.kvn, 0);
+    return max(a.causal ? kvn - qn + r / G + 1 : kvn, 0);
   };
-  const int lim = min(keys_of(r0 + n - 1), cap);
+  const int lim = seq_uni(min(min(keys_of(r0 + n - 1), cap), j1));
   const int w0 = r0 + 32 * wave, wn = min(n - 32 * wave, 32);
-  const int wlim_max = wn > 0 ? min(keys_of(w0 + wn - 1), cap) : 0;
-  const int wlim_min = wn > 0 ? min(keys_of(w0), cap) : 0;
+  const int wlim_max = seq_uni(wn > 0 ? min(keys_of(w0 + wn - 1), lim) : 0);
+  const int wlim_min = seq_uni(wn > 0 ? min(keys_of(w0), lim) : 0);
   const int r = min(w0 + (lane & 31), r0 + n - 1);
   const bool active = (lane & 31) < wn;
-  const int64_t tok = t.q0 + r / G;
+  const int64_t tok = q0 + r / G;
   const int h = hk * G + r - (r / G) * G;
-  const int sees = keys_of(r), mylim = min(sees, cap);
-  const T* qrow = (const T*)a.q + tok * a.q_st + h * a.q_sh;
+  const int sees = keys_of(r);
 
   SeqHead<T, PAGED> hp;
-  hp.init(a, t, hk);
+  hp.init(a, b, q0, hk);
   typename Tile::L ld;
   ld.init(a, hp, wave, lane);
   ld.last = lim - 1;
   ld.bad_from = cap;
   Tile tile;
   tile.lsum = f32x4{0.f, 0.f, 0.f, 0.f};
+  tile.m_run = -__builtin_inff();
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) tile.o[d][e] = 0.f;
-  if (lim > 0) tile.run(ld, qrow, a.scale, mylim, wlim_min, wlim_max, 0, (lim + AX_BN - 1) / AX_BN, lds, lane);
+  if (lim > j0)
+    tile.run(ld, (const T*)a.q + tok * a.q_st + h * a.q_sh, a.scale, min(sees, cap), wlim_min, wlim_max, j0 / AX_BN,
+             (lim + AX_BN - 1) / AX_BN, lds, lane);
   const int bad_from = PAGED ? sq_bad_from(ld.bad_from, bad, wave, lane) : 0x7fffffff;
 
-  const float l = tile.lsum[0];
-  const bool lost = PAGED && sees > bad_from;
   // Rows without keys are 0; without a page for a key, or when every score is
-  // -inf, NaN.
-  const float inv = l != 0.f ? 1.0f / l : (sees > 0 ? __builtin_nanf("") : 0.f);
+  // -inf, NaN.  (Of a part, l = 0 says nothing yet: the join decides.)
+  const float l = tile.lsum[0];
+  const bool lost = PAGED && sees > bad_from && bad_from < j1;
+  const float none = part || sees <= 0 ? 0.f : __builtin_nanf("");
+  const float inv = l != 0.f ? 1.0f / l : none;
   float odd = 0.f;  // NaN if any value of the row is not finite
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d)
@@ -386,9 +412,15 @@ __global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_tile_kernel(SeqAttnArg
   // A value that is not finite may come from a key that the row does not see
   // (its weight of 0 times a NaN or an infinity).  Such rows run again key by
   // key; they are rare enough that nothing above pays for them.
-  const uint64_t odd_lanes = __ballot(active && !lost && sees > 0 && !(odd == 0.f));
+  const uint64_t odd_lanes = __ballot(active && !lost && sees > j0 && !(odd == 0.f));
   uint32_t todo = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
-  if (active && !((todo >> (lane & 31)) & 1u)) {
+  const bool mine = active && !((todo >> (lane & 31)) & 1u);
+  auto unit_of = [&](int rt, float*& po, float*& pml) {  // rt: row of the tile
+    float* u = part + (rt / SEQ_FEW) * sq_unit_floats(SEQ_FEW, HD);
+    po = u + (rt % SEQ_FEW) * HD;
+    pml = u + SEQ_FEW * HD + rt % SEQ_FEW;
+  };
+  if (mine && !part) {
     T* orow = (T*)a.o + tok * a.o_st + h * a.o_sh + 4 * (lane >> 5);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
@@ -396,36 +428,486 @@ __global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_tile_kernel(SeqAttnArg
       for (int q4 = 0; q4 < 4; ++q4)
         st64(orow + 32 * d + 8 * q4, u32x2{pack2<T>(tile.o[d][4 * q4], tile.o[d][4 * q4 + 1]),
                                            pack2<T>(tile.o[d][4 * q4 + 2], tile.o[d][4 * q4 + 3])});
+  } else if (mine) {
+    float *po, *pml;
+    unit_of(r - r0, po, pml);
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        store4<float>(po + 32 * d + 8 * q4 + 4 * (lane >> 5), (const float*)&tile.o[d] + 4 * q4);
+    if (lane < 32) {
+      pml[0] = lost ? __builtin_nanf("") : tile.m_run;
+      pml[SEQ_FEW] = l * exp2f(-Tile::BIAS);
+    }
   }
   while (todo != 0) {
-    const int i = __builtin_ctz(todo);
+    const int i = __builtin_ctz(todo), ri = w0 + i;
     todo &= todo - 1;
-    const int ri = w0 + i;
-    const int64_t ti = t.q0 + ri / G;
-    const int hi = hk * G + ri - (ri / G) * G;
-    float o[HD / 64], m, l1;
-    seq_row<T, HD, PAGED>(a, hp, (const T*)a.q + ti * a.q_st + hi * a.q_sh, 0, min(keys_of(ri), cap), o, m, l1);
-    T* orow = (T*)a.o + ti * a.o_st + hi * a.o_sh;
-#pragma unroll
-    for (int e = 0; e < HD / 64; ++e) orow[lane + 64 * e] = from_f32<T>(o[e]);
+    float *po = nullptr, *pml = nullptr;
+    if (part) unit_of(ri - r0, po, pml);
+    sq_row_again<T, HD, PAGED>(a, hp, q0 + ri / G, hk * G + ri - (ri / G) * G, j0, min(keys_of(ri), lim), po, pml, SEQ_FEW);
   }
 }
 
+// ------------------------------------------------------------- packed prompts
 template <typename T, int HD>
-static int launch_hd(const SeqAttnArgs& a, hipStream_t st) {
-  const int tiles = (int)seq_tiles(a.s, a.group, SQ_ROWS);
-  const dim3 grid((unsigned)tiles * (unsigned)a.kv_heads), block(SQ_THREADS);
-  if (a.paged) seq_attn_tile_kernel<T, HD, true><<<grid, block, 0, st>>>(a, tiles);
-  else seq_attn_tile_kernel<T, HD, false><<<grid, block, 0, st>>>(a, tiles);
-  return hipGetLastError() == hipSuccess ? TX_OK : TX_EHIP;
+__global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_packed_kernel(SeqAttnArgs a, int tiles) {
+  __shared__ __attribute__((aligned(16))) T lds[SqTile<T, HD, false>::LDS_ELEMS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  // The last tiles of a sequence, which see the most keys, start first.
+  const int hk = blockIdx.x % a.kv_heads;
+  const SeqTile t = seq_find(a.s, a.group, SQ_ROWS, tiles - 1 - (int)(blockIdx.x / a.kv_heads));
+  const int r0 = t.tile * SQ_ROWS;
+  if (r0 >= t.qn * a.group) return;
+  sq_tile_item<T, HD, false>(a, t.b, t.q0, t.qn, t.qn, hk, r0, 0, 0x7fffffff, nullptr, lds, nullptr, lane, wave);
+}
+
+// -------------------------------------------------------------- few rows
+// Up to 16 rows (one token's query heads of a K/V head, or a few tokens')
+// against one part of the keys: bound by reading K and V once.  Each of the 4
+// waves takes blocks of 32 keys by itself, no barrier between them: K rows
+// straight into the MFMA A operand (16 keys x 32 dims), V rows into registers
+// and through a wave's own LDS (transposing reads) into the A operand of o^T +=
+// V^T P^T; the loads of the next block are in flight while one is worked on.
+// S^T leaves lane l the keys 4 (l >> 4) .. + 3 of both 16-key halves of row l &
+// 15, which is a P operand as it stands if V's rows are taken in that order.
+// The waves' results meet in LDS at the end.
+template <typename T, int HD>
+struct SqFew {
+  typedef typename Mfma16<T>::vec vec;
+  static constexpr int CH = HD / 8, RPI = 64 / CH, LDV = 32 / RPI;  // V loads per block and lane
+  static constexpr int WAVE_ELEMS = 32 * HD;                        // V block; o of 16 rows in fp32
+  static constexpr float BIAS = SqTile<T, HD, true>::BIAS;
+  // Chunk swizzle of the V block: the 32 lanes of one transposing read cover
+  // 8 keys (4 of each of two 16-lane groups) x 32 bytes.
+  static __device__ __forceinline__ int swz(int key) { return HD == 128 ? (key & 7) << 1 : ((key >> 1) & 3) << 1; }
+};
+
+template <typename T, int HD>
+__device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork& w, int hk, int r0, int j0, int j1,
+                                            float* part, T* lds, float* stat, int* bad, int lane, int wave) {
+  typedef SqFew<T, HD> F;
+  typedef typename F::vec vec;
+  const float NEG_INF = -__builtin_inff();
+  const float c = a.scale * SQ_LOG2E;
+  const int G = a.group, n = min(w.qn * G - r0, w.cut.unit_rows);
+  const int cap = a.s.max_pages << a.s.page_log2, ps1 = (1 << a.s.page_log2) - 1;
+  auto keys_of = [&](int r) { return max(a.causal ? w.kvn - w.qn + r / G + 1 : w.kvn, 0); };
+  const int lim = seq_uni(min(min(keys_of(r0 + n - 1), cap), j1));
+  const int col = lane & 15, g = lane >> 4;
+  const int r = r0 + min(col, n - 1);
+  const int64_t tok = w.q0 + r / G;
+  const int h = hk * G + r - (r / G) * G;
+  const int mylim = min(keys_of(r), lim);
+  SeqHead<T, true> hp;
+  hp.init(a, w.b, w.q0, hk);
+  const int32_t* table = a.s.table + (int64_t)w.b * a.s.table_ld;
+
+  vec qf[HD / 32];
+  {
+    const T* qrow = (const T*)a.q + tok * a.q_st + h * a.q_sh + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < HD / 32; ++ks) qf[ks] = __builtin_bit_cast(vec, ld128(qrow + 32 * ks));
+  }
+  vec ones;
+  {
+    const uint32_t one2 = std::is_same<T, bf16>::value ? 0x3F803F80u : 0x3C003C00u;
+    ones = __builtin_bit_cast(vec, u32x4{one2, one2, one2, one2});
+  }
+  f32x4 o[HD / 16], lsum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = NEG_INF, mc = 0.f;
+  int bad_from = cap;
+
+  // A lane's rows of a block: for K keys col and 16 + col, for V LDV
+  // consecutive ones (of one page: LDV divides 8).  Keys past the last re-read
+  // the last.  Page and slot parts of an address are 32 x 32 -> 64 bit products
+  // (the entry point bounds the strides).
+  const uint32_t k_sp = (uint32_t)(a.k_sp * 2), v_sp = (uint32_t)(a.v_sp * 2);
+  const uint32_t k_st = (uint32_t)(a.k_st * 2), v_st = (uint32_t)(a.v_st * 2);
+  struct Pages {
+    int k[2], v;
+  };
+  auto vrow0 = [&](int kb) { return min(kb + lane / F::CH * F::LDV, (lim - 1) & ~(F::LDV - 1)); };
+  auto lookup = [&](int kb) {
+    Pages p;
+    p.k[0] = table[min(kb + col, lim - 1) >> a.s.page_log2];
+    p.k[1] = table[min(kb + 16 + col, lim - 1) >> a.s.page_log2];
+    p.v = table[vrow0(kb) >> a.s.page_log2];
+    return p;
+  };
+  auto page_of = [&](int p, int key) {  // page 0 in the place of one that is not there
+    if ((uint32_t)p < (uint32_t)a.s.num_pages) return (uint32_t)p;
+    bad_from = min(bad_from, key & ~ps1);
+    return 0u;
+  };
+  u32x4 kr[2][HD / 32], vr[F::LDV];
+  auto load_k = [&](int kb, const Pages& p) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int key = min(kb + 16 * x + col, lim - 1);
+      const char* row = (const char*)hp.k + (uint64_t)page_of(p.k[x], key) * k_sp + ((uint32_t)(key & ps1) * k_st + 16u * g);
+#pragma unroll
+      for (int ks = 0; ks < HD / 32; ++ks) kr[x][ks] = ld128(row + 64 * ks);
+    }
+  };
+  auto load_v = [&](int kb, const Pages& p) {
+    const int key = vrow0(kb), left = lim - 1 - key;
+    const char* row = (const char*)hp.v + (uint64_t)page_of(p.v, key) * v_sp +
+                      ((uint32_t)(key & ps1) * v_st + 16u * (lane % F::CH));
+#pragma unroll
+    for (int x = 0; x < F::LDV; ++x) vr[x] = ld128(row + (uint32_t)min(x, left) * v_st);
+  };
+  T* vs = lds + wave * F::WAVE_ELEMS;
+  const uint32_t vbase = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) T*)vs;
+  // Transposing reads: lane j of a 16-lane group g addresses key 4 g + j / 4
+  // (and + 16) at dims 16 d + 4 (j % 4) and receives dim 16 d + j of 4 keys.
+  const int vkey = 4 * g + (col >> 2);
+  const uint32_t vrow = vbase + (uint32_t)(vkey * HD * 2 + (col & 1) * 8);
+  const int vx = (col & 3) >> 1, vsw = F::swz(vkey);
+  // One block: its V rows move to LDS and its scores are formed, each followed
+  // at once by the loads of the block after it into the same registers.
+  auto compute = [&](int kb, const Pages& pages, bool more) {
+#pragma unroll
+    for (int x = 0; x < F::LDV; ++x) {
+      const int i = lane / F::CH * F::LDV + x;
+      st128(vs + i * HD + (((lane % F::CH) ^ F::swz(i)) << 3), vr[x]);
+    }
+    if (more) load_v(kb + 128, pages);
+    float s[8];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < HD / 32; ++ks) acc = Mfma16<T>::mma(__builtin_bit_cast(vec, kr[x][ks]), qf[ks], acc);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[4 * x + e] = (kb + 16 * x + 4 * g + e < mylim) ? acc[e] : NEG_INF;
+    }
+    if (more) load_k(kb + 128, pages);
+    float mx = NEG_INF;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    mx *= c;
+    if (__any(mx > m_run + 8.f)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float corr = m_run == NEG_INF ? 0.f : exp2f(m_run - m_new);
+      lsum *= corr;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) o[d] *= corr;
+      m_run = m_new;
+      mc = (m_run == NEG_INF ? 0.f : m_run) - F::BIAS;
+    }
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -mc));
+    const vec pf = __builtin_bit_cast(vec, u32x4{pack2_raw<T>(p[0], p[1]), pack2_raw<T>(p[2], p[3]),
+                                                 pack2_raw<T>(p[4], p[5]), pack2_raw<T>(p[6], p[7])});
+    lsum = Mfma16<T>::mma(ones, pf, lsum);
+    // The block's rows are in LDS before the reads (the compiler does not see
+    // that they read it), and the reads are done before the next block's.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int d4 = 0; d4 < HD / 64; ++d4) {
+      u32x4 vop[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t at = vrow + (uint32_t)((((2 * (4 * d4 + i)) ^ vsw) + vx) << 4);
+        u32x2 lo, hi;
+        asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo) : "v"(at));
+        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(hi) : "v"(at), "n"(16 * HD * 2));
+        vop[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+      ax_vnat_wait<4>(vop);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[4 * d4 + i] = Mfma16<T>::mma(__builtin_bit_cast(vec, vop[i]), pf, o[4 * d4 + i]);
+    }
+    asm volatile("" ::: "memory");
+  };
+
+  const int first = j0 + 32 * wave;
+  if (first < lim) {
+    Pages pages = lookup(first), next = lookup(first + 128);
+    load_v(first, pages);
+    load_k(first, pages);
+    for (int kb = first; kb < lim; kb += 128) {
+      pages = next;
+      next = lookup(kb + 256);
+      compute(kb, pages, kb + 128 < lim);
+    }
+  }
+
+  // Join the waves: o in fp32 over each wave's V block, m and l beside it.
+  if (threadIdx.x == 0) *bad = cap;
+  float* ow = (float*)lds + wave * 16 * HD;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  float* sm = stat + wave * 16;
+  float* sl = stat + 64 + wave * 16;
+  int* sagain = (int*)(stat + 128);
+  __syncthreads();
+  if (bad_from < cap) atomicMin(bad, bad_from);
+#pragma unroll
+  for (int d = 0; d < HD / 16; ++d) *reinterpret_cast<f32x4*>(ow + col * HD + 16 * d + 4 * g) = o[d];
+  if (g == 0) {
+    sm[col] = m_run;
+    sl[col] = lsum[0];
+  }
+  if (threadIdx.x < 16) sagain[threadIdx.x] = 0;
+  __syncthreads();
+  const int lost_from = *bad;
+  constexpr int DT = HD / 16;  // dims a thread joins: 16 threads a row
+  const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 4;
+  const float* s0 = stat + row;
+  float M = fmaxf(fmaxf(s0[0], s0[16]), fmaxf(s0[32], s0[48]));
+  const float M0 = M == NEG_INF ? 0.f : M;
+  float wt[4], L = 0.f;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    wt[x] = exp2f(s0[16 * x] - M0);
+    L += wt[x] * s0[64 + 16 * x];
+  }
+  const int rr = r0 + min(row, n - 1);
+  const int sees = keys_of(rr);
+  const bool active = row < n, lost = sees > lost_from && lost_from < j1;
+  const float none = part || sees <= 0 ? 0.f : __builtin_nanf("");
+  const float inv = L != 0.f ? 1.0f / L : none;
+  float res[DT], odd = 0.f;
+#pragma unroll
+  for (int y = 0; y < DT / 4; ++y) {
+    f32x4 ov[4];  // a wave without keys for the row left 0 here, its weight is 0 too
+#pragma unroll
+    for (int x = 0; x < 4; ++x) ov[x] = *reinterpret_cast<const f32x4*>((const float*)lds + (x * 16 + row) * HD + 64 * y + d0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v = 0.f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        v = __builtin_fmaf(wt[x], ov[x][e], v);
+      }
+      v = lost ? __builtin_nanf("") : v * inv;
+      res[4 * y + e] = v;
+      odd += v * 0.f;
+    }
+  }
+  const bool redo = active && !lost && sees > j0 && !(odd == 0.f);
+  if (redo) sagain[row] = 1;
+  __syncthreads();
+  const int64_t tk = w.q0 + rr / G;
+  const int hh = hk * G + rr - (rr / G) * G;
+  if (active && !sagain[row]) {
+    if (part) {
+      float* po = part + row * HD + d0;
+#pragma unroll
+      for (int y = 0; y < DT / 4; ++y) store4<float>(po + 64 * y, res + 4 * y);
+      if ((threadIdx.x & 15) == 0) {
+        part[w.cut.unit_rows * HD + row] = lost ? __builtin_nanf("") : M;
+        part[w.cut.unit_rows * HD + w.cut.unit_rows + row] = L * exp2f(-F::BIAS);
+      }
+    } else {
+      T* orow = (T*)a.o + tk * a.o_st + hh * a.o_sh + d0;
+#pragma unroll
+      for (int y = 0; y < DT / 4; ++y) store4<T>(orow + 64 * y, res + 4 * y);
+    }
+  }
+  for (int i = wave; i < n; i += 4) {
+    if (!sagain[i]) continue;  // wave-uniform
+    const int ri = r0 + i;
+    sq_row_again<T, HD, true>(a, hp, w.q0 + ri / G, hk * G + ri - (ri / G) * G, j0, min(keys_of(ri), lim),
+                              part ? part + i * HD : nullptr, part ? part + w.cut.unit_rows * HD + i : nullptr,
+                              w.cut.unit_rows);
+  }
+}
+
+// ---------------------------------------------------------------- paged calls
+__host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
+  return SeqShape{a.group, a.kv_heads, a.cus, a.few};
+}
+
+// Persistent workgroups over the items of a call (SeqWalk); a grid of at most
+// the items, so every workgroup's loop ends.
+template <typename T, int HD, bool FEW_ONLY>
+__global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_paged_kernel(SeqAttnArgs a) {
+  constexpr int TILE_ELEMS = SqTile<T, HD, true>::LDS_ELEMS, FEW_ELEMS = 4 * SqFew<T, HD>::WAVE_ELEMS;
+  constexpr int ELEMS = FEW_ONLY || FEW_ELEMS > TILE_ELEMS ? FEW_ELEMS : TILE_ELEMS;
+  __shared__ __attribute__((aligned(16))) T lds[ELEMS];
+  __shared__ float stat[144];
+  __shared__ int bad[4];
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const SeqShape sh = sq_shape(a);
+  SeqWalk walk;
+  walk.init(a.s, sh, false);
+  SeqWork w;
+  for (int i = blockIdx.x; walk.find(a.s, sh, false, i, w); i += gridDim.x) {
+    // An item's lane constants are formed within it: held across the items
+    // they cost the registers that its loads need (56 spills).
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    // Item u of a sequence: its (part, K/V head) pairs first, then its tiles:
+    // the tiles that share keys meet on one XCD when the pairs are a multiple
+    // of 8.
+    const int u = i - w.item, np = w.cut.parts * a.kv_heads;
+    const int tile = seq_uni(u / np), pair = u - tile * np;
+    const int p = seq_uni(pair / a.kv_heads), hk = pair - p * a.kv_heads;
+    const int j0 = p * w.cut.part_keys, j1 = p + 1 < w.cut.parts ? j0 + w.cut.part_keys : 0x7fffffff;
+    float* part = nullptr;
+    if (w.cut.parts > 1) part = a.ws + (int64_t)(w.unit + u * w.cut.units) * sq_unit_floats(w.cut.unit_rows, HD);
+    if constexpr (FEW_ONLY) {
+      sq_few_item<T, HD>(a, w, hk, tile * w.cut.unit_rows, j0, j1, part, lds, stat, bad, lane, wave);
+    } else {
+      if (w.cut.few)
+        sq_few_item<T, HD>(a, w, hk, tile * w.cut.unit_rows, j0, j1, part, lds, stat, bad, lane, wave);
+      else
+        sq_tile_item<T, HD, true>(a, w.b, w.q0, w.qn, w.kvn, hk, tile * SQ_ROWS, j0, j1, part, lds, bad, lane, wave);
+    }
+    __syncthreads();  // LDS belongs to the next item
+  }
+}
+
+// Joins the parts of each row: o = sum_p w_p o_p / sum_p w_p, w_p = l_p 2^(m_p
+// - max m).  One workgroup a row; parts are always taken in the same order.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void seq_attn_join_kernel(SeqAttnArgs a) {
+  constexpr int LPR = HD / 4, GRP = 256 / LPR;  // lanes of 4 dims a part, parts at a time
+  __shared__ float wt[256];
+  __shared__ float red[256][4];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const float NEG_INF = -__builtin_inff();
+  const SeqShape sh = sq_shape(a);
+  SeqWalk walk;
+  walk.init(a.s, sh, true);
+  SeqWork w;
+  for (int i = blockIdx.x; walk.find(a.s, sh, true, i, w); i += gridDim.x) {
+    const int u = i - w.item, rows = w.qn * a.group;
+    const int hk = seq_uni(u / rows), r = u - hk * rows;
+    const int tr = w.cut.few ? w.cut.unit_rows : SQ_ROWS, tile = seq_uni(r / tr), rt = r - tile * tr;
+    const int np = w.cut.parts * a.kv_heads;
+    const int64_t uf = sq_unit_floats(w.cut.unit_rows, HD);
+    const float* first = a.ws + ((int64_t)w.unit + (tile * np + hk) * w.cut.units + rt / w.cut.unit_rows) * uf;
+    const int64_t step = (int64_t)a.kv_heads * w.cut.units * uf;  // from part to part
+    const int ru = rt % w.cut.unit_rows;
+    const int sees = max(a.causal ? w.kvn - w.qn + r / a.group + 1 : w.kvn, 0);
+    const int cap = a.s.max_pages << a.s.page_log2;
+    const int parts = min(w.cut.parts, seq_ceil(min(sees, cap), w.cut.part_keys));  // those the row sees
+    // Weights (at most 256 parts: one a thread).
+    float m = NEG_INF, l = 0.f;
+    if (tid < parts) {
+      m = first[tid * step + w.cut.unit_rows * HD + ru];
+      l = first[tid * step + w.cut.unit_rows * HD + w.cut.unit_rows + ru];
+    }
+    float M = m;
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
+    if (lane == 0) red[0][tid >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float wgt = tid < parts ? (m == NEG_INF && M != NEG_INF ? 0.f : l * exp2f(m - M)) : 0.f;
+    wt[tid] = wgt;
+    __syncthreads();  // before red is written again, and wt read
+    const int d0 = (tid % LPR) * 4;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, L = 0.f;
+    for (int p = tid / LPR; p < parts; p += GRP) {
+      float x[4];
+      load4<float>(first + p * step + ru * HD + d0, x);
+      const float f = wt[p];
+      L += f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += f == 0.f ? 0.f : f * x[e];
+    }
+    store4<float>(red[tid], acc);
+    __syncthreads();
+    // Sum of the weights in the same order, by every thread that writes.
+    if (tid < LPR) {
+      L = 0.f;
+      for (int p = 0; p < parts; ++p) L += wt[p];
+      float out[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = 0.f;
+#pragma unroll
+        for (int x = 0; x < GRP; ++x) v += red[x * LPR + tid][e];
+        out[e] = L != 0.f ? v / L : (sees > 0 ? __builtin_nanf("") : 0.f);
+      }
+      const int64_t tok = w.q0 + r / a.group;
+      store4<T>((T*)a.o + tok * a.o_st + (hk * a.group + r % a.group) * a.o_sh + d0, out);
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------- launch
+// Upper bounds, over all lengths that these totals allow, of a call's items
+// and of its units of partial results.
+struct SqBounds {
+  int64_t items, units, join_rows;
+};
+static SqBounds sq_bounds(const SeqAttnArgs& a) {
+  const int64_t rows = (int64_t)a.s.tokens * a.group, cap = (int64_t)a.s.max_pages << a.s.page_log2;
+  const int64_t hk = a.kv_heads, cus = a.cus;
+  auto least = [](int64_t x, int64_t y) { return x < y ? x : y; };
+  const int64_t few_most = cus / hk < 1 ? 1 : cus / hk;
+  const int64_t few_parts = least((cap + SEQ_PART_FEW - 1) / SEQ_PART_FEW, few_most);
+  const int64_t few_tiles = a.few ? rows / a.few + a.s.batch : a.s.batch;
+  SqBounds b;
+  b.items = few_tiles * hk * few_parts;
+  b.units = few_parts > 1 ? b.items : 0;
+  b.join_rows = few_parts > 1 ? rows * hk : 0;
+  if (!a.few) {
+    const int64_t seqs = least(a.s.batch, rows / (SEQ_FEW + 1));
+    const int64_t tiles = (rows / SEQ_TILE + seqs) * hk;
+    int64_t parts = least(cap / SEQ_PART_TILE, (2 * cus + hk - 1) / hk);
+    parts = parts < 1 ? 1 : parts;
+    const int64_t items = least(tiles * parts, tiles + seqs * 2 * cus);
+    b.items += items;
+    b.units += parts > 1 ? items * (SEQ_TILE / SEQ_FEW) : 0;
+    b.join_rows = b.units > 0 ? rows * hk : 0;
+  }
+  return b;
+}
+static void sq_finish(SeqAttnArgs& a) {
+  const int cus = device_cu_count();
+  a.cus = cus > 0 ? cus : 256;
+  if (a.cus > 256) a.cus = 256;  // the join holds one part a thread
+  a.few = 0;
+  const int64_t most = a.max_q_len * a.group;
+  // Calls of few-row sequences only; where their tiles could pass 32-bit
+  // counts (rows beyond what max_q_len promises), the general kernel.
+  if (most <= SEQ_FEW && ((int64_t)a.s.tokens * a.group / most + a.s.batch) * (a.kv_heads + 256) < 1 << 30) a.few = (int)most;
+}
+
+int64_t seq_attention_workspace(const SeqAttnArgs& a0) {
+  SeqAttnArgs a = a0;
+  sq_finish(a);
+  return sq_bounds(a).units * sq_unit_floats(a.few ? a.few : SEQ_FEW, a.head_dim);
+}
+
+template <typename T, int HD>
+static int launch_hd(SeqAttnArgs a, hipStream_t st) {
+  const dim3 block(SQ_THREADS);
+  if (!a.paged) {
+    const int tiles = (int)seq_tiles(a.s, a.group, SQ_ROWS);
+    seq_attn_packed_kernel<T, HD><<<dim3((unsigned)tiles * (unsigned)a.kv_heads), block, 0, st>>>(a, tiles);
+    return hipGetLastError() == hipSuccess ? TX_OK : TX_EHIP;
+  }
+  sq_finish(a);
+  const SqBounds b = sq_bounds(a);
+  auto grid = [](int64_t items, int64_t most) { return dim3((unsigned)(items < most ? items : most)); };
+  if (a.few) seq_attn_paged_kernel<T, HD, true><<<grid(b.items, 2 * a.cus), block, 0, st>>>(a);
+  else seq_attn_paged_kernel<T, HD, false><<<grid(b.items, 2 * a.cus), block, 0, st>>>(a);
+  if (hipGetLastError() != hipSuccess) return TX_EHIP;
+  if (b.units > 0) {
+    seq_attn_join_kernel<T, HD><<<grid(b.join_rows, 16 * a.cus), block, 0, st>>>(a);
+    if (hipGetLastError() != hipSuccess) return TX_EHIP;
+  }
+  return TX_OK;
 }
 
 template <typename T>
 static int launch_typed(const SeqAttnArgs& a, hipStream_t st) {
   return a.head_dim == 64 ? launch_hd<T, 64>(a, st) : launch_hd<T, 128>(a, st);
 }
-
-int64_t seq_attention_workspace(const SeqAttnArgs&) { return 0; }
 
 int launch_seq_attention(const SeqAttnArgs& a, int dt, hipStream_t st) {
   return dt == TX_BF16 ? launch_typed<bf16>(a, st) : launch_typed<f16>(a, st);

@@ -26,6 +26,10 @@ struct SeqTile {
 
 __device__ __forceinline__ int seq_cut(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
+// A wave-uniform value that the compiler holds in vector registers (integer
+// quotients are formed there), moved to a scalar one.
+__device__ __forceinline__ int seq_uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // The sequence and tile with index w: the largest b with first_tile(b) <= w,
 // found by the whole wave, 64 candidates at a time (two rounds of loads up to
 // 4096 sequences).  Wave-uniform; every lane takes part.
@@ -44,17 +48,138 @@ __device__ __forceinline__ SeqTile seq_find(const SeqArgs& s, int group, int r, 
   }
   SeqTile t;
   t.b = __builtin_amdgcn_readfirstlane(lo);
-  const int q0 = __builtin_amdgcn_readfirstlane(seq_cut(s.cu[t.b], 0, s.tokens));
-  const int q1 = __builtin_amdgcn_readfirstlane(seq_cut(s.cu[t.b + 1], q0, s.tokens));
+  const int q0 = seq_uni(seq_cut(s.cu[t.b], 0, s.tokens));
+  const int q1 = seq_uni(seq_cut(s.cu[t.b + 1], q0, s.tokens));
   t.q0 = q0;
   t.qn = q1 - q0;
-  t.kvn = s.kv_lens ? __builtin_amdgcn_readfirstlane(s.kv_lens[t.b]) : t.qn;
+  t.kvn = s.kv_lens ? seq_uni(s.kv_lens[t.b]) : t.qn;
   t.kvn = t.kvn < 0 ? 0 : t.kvn;
   const int64_t d = w - ((int64_t)q0 * group / r + t.b);
   t.tile = (int)d;
   if (d < 0) t.qn = t.tile = 0;  // before the first sequence
   return t;
 }
+
+// ---- how a paged call's work is cut ---------------------------------------
+// A sequence of at most SEQ_FEW rows (query heads of one K/V head x new
+// tokens) is bound by reading its keys: one item per K/V head and part of the
+// keys, every row in it.  More rows: tiles of 128 rows, their keys in parts
+// where the tiles alone leave the card idle.  The cut of a sequence depends on
+// nothing but its own rows, keys and head counts (and the card), so that its
+// result does not change with the batch around it.
+constexpr int SEQ_FEW = 16;
+constexpr int SEQ_TILE = 128;
+constexpr int SEQ_PART_FEW = 128;   // fewest keys of a part: one block of 32 for each of 4 waves
+constexpr int SEQ_PART_TILE = 512;  // fewer are not worth writing and joining partial rows for
+
+struct SeqShape {
+  int group, kv_heads, cus;
+  int few;  // rows of a tile when the call has few-row items only (<= SEQ_FEW), else 0
+};
+struct SeqCut {
+  int tiles, parts, part_keys;
+  int unit_rows, units;  // partial results of one item: units of unit_rows rows (0: one part, none)
+  bool few;
+};
+__host__ __device__ inline int seq_ceil(int x, int y) { return (x + y - 1) / y; }
+__host__ __device__ inline SeqCut seq_cut_of(const SeqShape& s, int rows, int keys) {
+  SeqCut c;
+  c.few = s.few > 0 || rows <= SEQ_FEW;
+  c.unit_rows = s.few > 0 ? s.few : SEQ_FEW;
+  c.tiles = seq_ceil(rows, c.few ? c.unit_rows : SEQ_TILE);
+  int most, step;
+  if (c.few) {
+    most = s.cus / s.kv_heads;
+    step = SEQ_PART_FEW;
+  } else {
+    most = seq_ceil(2 * s.cus, c.tiles * s.kv_heads);
+    step = 64;  // a key tile
+    most = most < keys / SEQ_PART_TILE ? most : keys / SEQ_PART_TILE;
+  }
+  most = most < 1 ? 1 : most;
+  c.part_keys = seq_ceil(seq_ceil(keys, most), step) * step;
+  c.parts = keys > 0 ? seq_ceil(keys, c.part_keys) : 1;
+  c.units = c.parts > 1 ? (c.few ? 1 : SEQ_TILE / SEQ_FEW) : 0;
+  return c;
+}
+
+// A sequence of a paged call: its cut, its first item and its first unit of
+// partial results, both counted over the call.
+struct SeqWork {
+  int b, q0, qn, kvn, keys;  // keys: those the table can hold
+  SeqCut cut;
+  int item, unit;
+};
+
+// Walks the items of a call in ascending order, 64 sequences at a time (lane
+// i: sequence base + i); every lane of the wave takes part.
+struct SeqWalk {
+  int base, items, units;        // before sequence base
+  int row;                       // first row that sequence base may hold
+  int n_items, n_units;          // of this lane's sequence
+  int at_item, at_unit;          // this lane's first item and unit (from base on)
+  int q0, qn, kvn;
+
+  __device__ __forceinline__ void load(const SeqArgs& s, const SeqShape& sh, bool rows_as_items) {
+    const int b = base + (int)(threadIdx.x & 63);
+    const bool in = b < s.batch;
+    // Starts that do not ascend are raised to the largest before them, so that
+    // no row is in two sequences and the host's bounds on items and units hold
+    // whatever the array says.
+    q0 = max(in ? seq_cut(s.cu[b], 0, s.tokens) : 0, row);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) q0 = max(q0, __shfl_up(q0, o, 64));  // (lanes below o see themselves)
+    qn = in ? max(seq_cut(s.cu[b + 1], 0, s.tokens) - q0, 0) : 0;
+    kvn = in ? max(s.kv_lens[b], 0) : 0;
+    n_items = n_units = 0;
+    if (qn > 0) {
+      const SeqCut c = seq_cut_of(sh, qn * sh.group, min(kvn, s.max_pages << s.page_log2));
+      n_items = c.tiles * c.parts * sh.kv_heads;
+      n_units = n_items * c.units;
+      if (rows_as_items) n_items = c.parts > 1 ? qn * sh.group * sh.kv_heads : 0;
+    }
+    at_item = n_items;
+    at_unit = n_units;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(at_item, o, 64), y = __shfl_up(at_unit, o, 64);
+      if ((int)(threadIdx.x & 63) >= o) {
+        at_item += x;
+        at_unit += y;
+      }
+    }
+  }
+  __device__ __forceinline__ void init(const SeqArgs& s, const SeqShape& sh, bool rows_as_items) {
+    base = items = units = row = 0;
+    load(s, sh, rows_as_items);
+  }
+  // The sequence of item w (ascending from call to call); false: past the end.
+  __device__ __forceinline__ bool find(const SeqArgs& s, const SeqShape& sh, bool rows_as_items, int w, SeqWork& r) {
+    for (;;) {
+      const int in_items = seq_uni(__shfl(at_item, 63, 64)), in_units = seq_uni(__shfl(at_unit, 63, 64));
+      if (w - items < in_items) break;
+      if (base + 64 >= s.batch) return false;
+      items += in_items;
+      units += in_units;
+      row = seq_uni(__shfl(q0 + qn, 63, 64));
+      base += 64;
+      load(s, sh, rows_as_items);
+    }
+    const int i = __builtin_popcountll(__ballot(at_item <= w - items));  // lanes that end before w
+    r.b = seq_uni(base + i);
+    r.q0 = seq_uni(__shfl(q0, i, 64));
+    r.qn = seq_uni(__shfl(qn, i, 64));
+    r.kvn = seq_uni(__shfl(kvn, i, 64));
+    r.item = seq_uni(items + __shfl(at_item - n_items, i, 64));
+    r.unit = seq_uni(units + __shfl(at_unit - n_units, i, 64));
+    r.keys = min(r.kvn, s.max_pages << s.page_log2);
+    r.cut = seq_cut_of(sh, r.qn * sh.group, r.keys);
+    r.cut.tiles = seq_uni(r.cut.tiles);
+    r.cut.parts = seq_uni(r.cut.parts);
+    r.cut.part_keys = seq_uni(r.cut.part_keys);
+    return true;
+  }
+};
 
 // The page of key j of sequence b, or -1.
 __device__ __forceinline__ int seq_page(const SeqArgs& s, int b, int j) {

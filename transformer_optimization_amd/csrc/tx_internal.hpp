@@ -116,6 +116,8 @@ struct SeqAttnArgs {
   int causal;
   int paged;
   int64_t max_q_len;
+  int few;   // rows of a tile where every sequence has few rows (seq_common.hpp), else 0
+  int cus;
   float* ws;
 };
 
