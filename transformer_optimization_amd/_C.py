@@ -11,6 +11,7 @@ capturable into a graph.
 
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 import math
@@ -670,57 +671,87 @@ def rotary_steps(
     return torch.tensor(steps, dtype=torch.int64, device=device), amplitude
 
 
-def _heads3(name: str, t: torch.Tensor, rows: int, heads: Optional[int], hd: int, dtype: torch.dtype) -> None:
-    if t.dim() != 3 or t.shape[0] != rows or (heads is not None and t.shape[1] != heads) or t.shape[2] != hd:
-        raise ValueError(f"{name} must be [{rows}, {'heads' if heads is None else heads}, {hd}], got {tuple(t.shape)}")
+# The checks below run on every call of a decoding loop: one comparison each
+# where all is well, the message only when not.
+def _heads3(name: str, t: torch.Tensor, rows: int, heads: int, hd: int, dtype: torch.dtype) -> tuple:
+    if t.shape != (rows, heads, hd):
+        raise ValueError(f"{name} must be [{rows}, {heads}, {hd}], got {tuple(t.shape)}")
     if t.dtype != dtype:
-        raise ValueError(f"{name} must share q's dtype")
-    if hd > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name} must share the other tensors' dtype {dtype}")
+    st = t.stride()
+    if st[2] != 1 and hd > 1:
         raise ValueError(f"{name} must be contiguous in head_dim")
+    return st
+
+
+def _dims3(name: str, t: torch.Tensor) -> Tuple[int, int, int]:
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
+    return t.shape
 
 
 def _int_vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype = torch.int32) -> None:
-    if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype or not t.is_contiguous():
+    if t.shape != (n,) or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {str(dtype).replace('torch.', '')} [{n}] tensor")
 
 
-def _check_cache(k_cache, v_cache, block_table, batch: int, hd: int, dtype: torch.dtype) -> None:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != hd:
+def _check_cache(k_cache, v_cache, block_table, batch: int, hd: int, dtype: torch.dtype) -> tuple:
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape or shape[3] != hd:
         raise ValueError(f"k_cache and v_cache must be [pages, kv_heads, page_size, {hd}] of one shape")
     if k_cache.dtype != dtype or v_cache.dtype != dtype:
-        raise ValueError("the caches must share q's dtype")
-    if hd > 1 and (k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
+        raise ValueError(f"the caches must share the other tensors' dtype {dtype}")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if (ks[3] != 1 or vs[3] != 1) and hd > 1:
         raise ValueError("the caches must be contiguous in head_dim")
-    if block_table.dim() != 2 or block_table.shape[0] != batch or block_table.dtype != torch.int32:
+    table = block_table.shape
+    if len(table) != 2 or table[0] != batch or block_table.dtype != torch.int32:
         raise ValueError("block_table must be an int32 [batch, max_pages] tensor")
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+    ld, unit = block_table.stride()
+    if unit != 1 and table[1] > 1:
         raise ValueError("block_table rows must be contiguous")
+    return ks, vs, (shape[0], shape[1], shape[2], table[1], ld)
 
 
 def _starts(cu_seqlens: torch.Tensor) -> int:
-    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
-        raise ValueError("cu_seqlens must be an int32 [batch + 1] tensor")
-    _int_vector("cu_seqlens", cu_seqlens, cu_seqlens.shape[0])
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype != torch.int32 \
+            or not cu_seqlens.is_contiguous():
+        raise ValueError("cu_seqlens must be a contiguous int32 [batch + 1] tensor")
     return cu_seqlens.shape[0] - 1
 
 
-def _sv(t: Optional[torch.Tensor], n: int):
-    return None if t is None else (ctypes.c_int64 * n)(*t.stride()[:n])
+def _one_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> torch.device:
+    at = first.get_device()  # -1 on the CPU
+    if at < 0:
+        _require_cuda(first)
+    for t in rest:
+        if t is not None and t.get_device() != at:
+            _require_cuda(t)
+            raise ValueError(f"tensors on two devices ({first.device} and {t.device})")
+    return first.device
 
 
-def _addr(a) -> Optional[int]:
-    return None if a is None else ctypes.addressof(a)
+def _launch_on(dev: torch.device, fn: str, args: tuple, keep: tuple, info: dict) -> None:
+    """``_launch`` on the current stream of the tensors' device."""
+    if dev.index == torch.cuda.current_device():
+        _launch(fn, args, keep, info)
+    else:
+        with torch.cuda.device(dev):
+            _launch(fn, args, keep, info)
 
 
-def _one_device(*ts: Optional[torch.Tensor]) -> torch.device:
-    _require_cuda(*ts)
-    dev = None
-    for t in ts:
-        if t is not None:
-            if dev is not None and t.device != dev:
-                raise ValueError(f"tensors on two devices ({dev} and {t.device})")
-            dev = t.device
-    return dev
+def _addresses(views: tuple) -> tuple:
+    """The strides of each view, four places each, in one array (kept by the caller), and the addresses of the
+    views' parts of it."""
+    flat: list = []
+    for st in views:
+        flat += st if len(st) == 4 else (*st, 0)
+    arr = array.array("q", flat)
+    at = arr.buffer_info()[0]
+    return arr, range(at, at + 32 * len(views), 32)
+
+
+_NO_STRIDES = (0, 0, 0)
 
 
 def rotary_append(
@@ -749,22 +780,24 @@ def rotary_append(
     ``.transpose(1, 2)``); ``kv_lens`` counts the new tokens already.  q_out and k_out may be q and k
     themselves; k_out is made when omitted only where there is no cache (else it is None).  Rows outside every
     sequence are left as they were (in a tensor made here: undefined)."""
-    t, kvh, hd = k.shape if k.dim() == 3 else (-1, -1, -1)
-    _heads3("k", k, t, None, hd, k.dtype)
+    t, kvh, hd = _dims3("k", k)
+    dtype = k.dtype
+    ks = _heads3("k", k, t, kvh, hd, dtype)
+    qs = qos = kos = vs = kcs = vcs = _NO_STRIDES
     batch = _starts(cu_seqlens)
-    if steps.dim() != 1 or not 0 < 2 * steps.shape[0] <= hd:
-        raise ValueError(f"steps must be an int64 [rotary_dim / 2] tensor with rotary_dim <= {hd}")
-    _int_vector("steps", steps, steps.shape[0], torch.int64)
+    half = steps.shape[0] if steps.dim() == 1 else 0
+    if not 0 < 2 * half <= hd or steps.dtype != torch.int64 or not steps.is_contiguous():
+        raise ValueError(f"steps must be a contiguous int64 [rotary_dim / 2] tensor with rotary_dim <= {hd}")
     heads = kvh
     if q is not None:
-        heads = q.shape[1] if q.dim() == 3 else 0
-        _heads3("q", q, t, None, hd, k.dtype)
+        heads = _dims3("q", q)[1]
+        qs = _heads3("q", q, t, heads, hd, dtype)
         if q_out is not None:
-            _heads3("q_out", q_out, t, heads, hd, k.dtype)
+            qos = _heads3("q_out", q_out, t, heads, hd, dtype)
     elif q_out is not None:
         raise ValueError("q_out without q")
     if k_out is not None:
-        _heads3("k_out", k_out, t, kvh, hd, k.dtype)
+        kos = _heads3("k_out", k_out, t, kvh, hd, dtype)
     if kv_lens is not None:
         _int_vector("kv_lens", kv_lens, batch)
     if positions is not None:
@@ -773,33 +806,32 @@ def rotary_append(
     if k_cache is not None or v_cache is not None:
         if k_cache is None or v_cache is None or block_table is None or kv_lens is None or v is None:
             raise ValueError("a cache needs k_cache, v_cache, block_table, kv_lens and v")
-        _heads3("v", v, t, kvh, hd, k.dtype)
-        _check_cache(k_cache, v_cache, block_table, batch, hd, k.dtype)
-        if k_cache.shape[1] != kvh:
+        vs = _heads3("v", v, t, kvh, hd, dtype)
+        kcs, vcs, (pages, cache_heads, page_size, max_pages, table_ld) = _check_cache(k_cache, v_cache, block_table, batch,
+                                                                                     hd, dtype)
+        if cache_heads != kvh:
             raise ValueError("the caches must hold k's heads")
-        pages, _, page_size, _ = k_cache.shape
-        max_pages, table_ld = block_table.shape[1], block_table.stride(0)
     else:
         block_table = v = None
-    dev = _one_device(q, k, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache, v_cache, q_out, k_out)
+    dev = _one_device(k, q, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache, v_cache, q_out, k_out)
     load_library()
     if q is not None and q_out is None:
-        q_out = torch.empty((t, heads, hd), dtype=k.dtype, device=dev)
+        q_out = torch.empty((t, heads, hd), dtype=dtype, device=dev)
+        qos = (heads * hd, hd, 1)
     if k_cache is None and k_out is None:
-        k_out = torch.empty((t, kvh, hd), dtype=k.dtype, device=dev)
+        k_out = torch.empty((t, kvh, hd), dtype=dtype, device=dev)
+        kos = (kvh * hd, hd, 1)
     if t == 0 or batch == 0:
         return q_out, k_out
-    st = tuple(_sv(x, n) for x, n in ((q, 2), (q_out, 2), (k, 2), (k_out, 2), (v, 2), (k_cache, 3), (v_cache, 3)))
-    ad = [_addr(x) for x in st]
-    args = (_ptr(q), ad[0], _ptr(q_out), ad[1], _ptr(k), ad[2], _ptr(k_out), ad[3], _ptr(v), ad[4],
-            _ptr(k_cache), ad[5], _ptr(v_cache), ad[6], _ptr(steps), _ptr(positions), _ptr(cu_seqlens),
-            _ptr(kv_lens), _ptr(block_table), table_ld, t, batch, heads, kvh, hd, 2 * steps.shape[0], pages,
-            page_size, max_pages, float(amplitude), 1 if interleaved else 0, _dt(k))
+    st, ad = _addresses((qs, qos, ks, kos, vs, kcs, vcs))
+    args = (_ptr(q), ad[0], _ptr(q_out), ad[1], k.data_ptr(), ad[2], _ptr(k_out), ad[3], _ptr(v), ad[4],
+            _ptr(k_cache), ad[5], _ptr(v_cache), ad[6], steps.data_ptr(), _ptr(positions), cu_seqlens.data_ptr(),
+            _ptr(kv_lens), _ptr(block_table), table_ld, t, batch, heads, kvh, hd, 2 * half, pages,
+            page_size, max_pages, amplitude, 1 if interleaved else 0, _dt(k))
     info = {"op": "rotary_append", "tokens": t, "heads": heads, "kv_heads": kvh, "head_dim": hd,
             "cache": k_cache is not None}
-    with torch.cuda.device(dev):
-        _launch("tx_rotary_append", args, (q, k, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache,
-                                           v_cache, q_out, k_out, st), info)
+    _launch_on(dev, "tx_rotary_append", args, (q, k, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache,
+                                               v_cache, q_out, k_out, st), info)
     return q_out, k_out
 
 
@@ -817,30 +849,30 @@ def flash_attn_packed(
     columns of one projection), sequence b in rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` (int32, on the
     device; not read by the host).  Query head h reads K/V head ``h // (heads // kv_heads)``.  Returns out
     ``[T, heads, hd]``; rows outside every sequence are left as they were (``tx_flash_attn_packed``)."""
-    t, heads, hd = q.shape if q.dim() == 3 else (-1, -1, -1)
-    _heads3("q", q, t, heads, hd, q.dtype)
-    kvh = k.shape[1] if k.dim() == 3 else 0
-    _heads3("k", k, t, None, hd, q.dtype)
-    _heads3("v", v, t, kvh, hd, q.dtype)
+    t, heads, hd = _dims3("q", q)
+    dtype = q.dtype
+    qs = _heads3("q", q, t, heads, hd, dtype)
+    kvh = _dims3("k", k)[1]
+    ks = _heads3("k", k, t, kvh, hd, dtype)
+    vs = _heads3("v", v, t, kvh, hd, dtype)
     if kvh <= 0 or heads % kvh:
         raise ValueError(f"{kvh} K/V heads do not divide {heads} query heads")
     batch = _starts(cu_seqlens)
     if out is not None:
-        _heads3("out", out, t, heads, hd, q.dtype)
+        os_ = _heads3("out", out, t, heads, hd, dtype)
     dev = _one_device(q, k, v, cu_seqlens, out)
     load_library()
     if out is None:
-        out = torch.empty((t, heads, hd), dtype=q.dtype, device=dev)
+        out = torch.empty((t, heads, hd), dtype=dtype, device=dev)
+        os_ = (heads * hd, hd, 1)
     if t == 0 or batch == 0:
         return out
-    st = tuple(_sv(x, 2) for x in (q, k, v, out))
-    ad = [_addr(x) for x in st]
-    args = (_ptr(q), ad[0], _ptr(k), ad[1], _ptr(v), ad[2], _ptr(out), ad[3], _ptr(cu_seqlens), t, batch, heads, kvh,
-            hd, float(scale), 1 if causal else 0, _dt(q))
+    st, ad = _addresses((qs, ks, vs, os_))
+    args = (q.data_ptr(), ad[0], k.data_ptr(), ad[1], v.data_ptr(), ad[2], out.data_ptr(), ad[3], cu_seqlens.data_ptr(),
+            t, batch, heads, kvh, hd, scale, 1 if causal else 0, _dt(q))
     info = {"op": "flash_attn_packed", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh, "head_dim": hd,
             "causal": bool(causal)}
-    with torch.cuda.device(dev):
-        _launch("tx_flash_attn_packed", args, (q, k, v, out, cu_seqlens, st), info)
+    _launch_on(dev, "tx_flash_attn_packed", args, (q, k, v, out, cu_seqlens, st), info)
     return out
 
 
@@ -877,39 +909,38 @@ def flash_attn_paged(
     ``max_q_len``: a bound on the rows of one sequence that the caller knows (0: T), to choose the kernel by.
     ``workspace``: fp32, at least :func:`flash_attn_paged_workspace` values, made here when omitted; calls that
     overlap in time need one each."""
-    t, heads, hd = q.shape if q.dim() == 3 else (-1, -1, -1)
-    _heads3("q", q, t, heads, hd, q.dtype)
+    t, heads, hd = _dims3("q", q)
+    dtype = q.dtype
+    qs = _heads3("q", q, t, heads, hd, dtype)
     batch = _starts(cu_seqlens)
     _int_vector("kv_lens", kv_lens, batch)
-    _check_cache(k_cache, v_cache, block_table, batch, hd, q.dtype)
-    pages, kvh, page_size, _ = k_cache.shape
+    ks, vs, (pages, kvh, page_size, max_pages, table_ld) = _check_cache(k_cache, v_cache, block_table, batch, hd, dtype)
     if kvh <= 0 or heads % kvh:
         raise ValueError(f"{kvh} K/V heads do not divide {heads} query heads")
     if out is not None:
-        _heads3("out", out, t, heads, hd, q.dtype)
+        os_ = _heads3("out", out, t, heads, hd, dtype)
     dev = _one_device(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, out, workspace)
     load_library()
     if out is None:
-        out = torch.empty((t, heads, hd), dtype=q.dtype, device=dev)
+        out = torch.empty((t, heads, hd), dtype=dtype, device=dev)
+        os_ = (heads * hd, hd, 1)
     if t == 0 or batch == 0:
         return out
-    max_pages = block_table.shape[1]
-    with torch.cuda.device(dev):
-        need = flash_attn_paged_workspace(t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
-    if workspace is None and need > 0:
-        workspace = torch.empty(need, dtype=torch.float32, device=dev)
-    if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous()
-                                  or workspace.numel() < need):
-        raise ValueError(f"workspace must be contiguous fp32 with at least {need} elements")
-    st = (_sv(q, 2), _sv(k_cache, 3), _sv(v_cache, 3), _sv(out, 2))
-    ad = [_addr(x) for x in st]
-    args = (_ptr(q), ad[0], _ptr(k_cache), ad[1], _ptr(v_cache), ad[2], _ptr(out), ad[3], _ptr(cu_seqlens),
-            _ptr(kv_lens), _ptr(block_table), block_table.stride(0), t, batch, heads, kvh, hd, pages, page_size,
-            max_pages, int(max_q_len), float(scale), 1 if causal else 0, _ptr(workspace),
+    need = 0
+    if workspace is None or workspace.dtype != torch.float32 or not workspace.is_contiguous():
+        if workspace is not None:
+            raise ValueError("workspace must be contiguous fp32")
+        with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext():
+            need = flash_attn_paged_workspace(t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+        if need > 0:
+            workspace = torch.empty(need, dtype=torch.float32, device=dev)
+    st, ad = _addresses((qs, ks, vs, os_))
+    args = (q.data_ptr(), ad[0], k_cache.data_ptr(), ad[1], v_cache.data_ptr(), ad[2], out.data_ptr(), ad[3],
+            cu_seqlens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), table_ld, t, batch, heads, kvh,
+            hd, pages, page_size, max_pages, max_q_len, scale, 1 if causal else 0, _ptr(workspace),
             0 if workspace is None else workspace.numel(), _dt(q))
     info = {"op": "flash_attn_paged", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh, "head_dim": hd,
             "causal": bool(causal), "page_size": page_size}
-    with torch.cuda.device(dev):
-        _launch("tx_flash_attn_paged", args, (q, k_cache, v_cache, out, cu_seqlens, kv_lens, block_table, workspace, st),
-                info)
+    _launch_on(dev, "tx_flash_attn_paged", args, (q, k_cache, v_cache, out, cu_seqlens, kv_lens, block_table, workspace, st),
+               info)
     return out

@@ -104,8 +104,6 @@ constexpr int SQ_ROWS = SEQ_TILE;
 constexpr int SQ_THREADS = 256;
 constexpr float SQ_LOG2E = 1.4426950408889634f;
 
-typedef const __attribute__((address_space(4))) int32_t* SqConstInt;
-
 // K and V tiles of 64 keys, global -> LDS by DMA.  One wave instruction moves
 // RPI consecutive key rows, which lie in one page (page sizes are powers of
 // two of at least 8): the page and the row's address are wave-uniform (scalar
@@ -118,15 +116,16 @@ struct SqLoader {
   static constexpr int ELEMS = AX_BN * HD;
   const T* k;  // this K/V head's row 0 (packed) or page 0 (paged)
   const T* v;
-  SqConstInt table;
+  const int32_t* table;
   int64_t k_sp, k_st, v_sp, v_st;
   int psl, num_pages;
   int wv, last;        // last key that may be read
   int rl;              // this lane's row within an instruction's rows
   uint32_t kc, vc;     // byte offset of its chunk within a row
   uint32_t ko, vo;     // byte offset of row and chunk
-  int pg[LD];          // pages of the tile that issue() loads next (looked up one tile ahead)
-  int bad_from;        // first key found without a page
+  int pages;           // lane x: page of rows x % LD of tile base + x / LD (one load for 64 / LD tiles)
+  int base;
+  int bad_from;        // first key found without a page (over the lane's lookups)
 
   __device__ __forceinline__ void init(const SeqAttnArgs& a, const SeqHead<T, PAGED>& hp, int wave, int lane) {
     k = hp.k;
@@ -141,7 +140,8 @@ struct SqLoader {
     ko = kc + 2u * (uint32_t)rl * (uint32_t)k_st;
     vo = vc + 2u * (uint32_t)rl * (uint32_t)v_st;
     if constexpr (PAGED) {
-      table = (SqConstInt)(uintptr_t)(a.s.table + (int64_t)hp.b * a.s.table_ld);
+      table = a.s.table + (int64_t)hp.b * a.s.table_ld;
+      base = -(1 << 30);
       k_sp = a.k_sp;
       v_sp = a.v_sp;
       psl = a.s.page_log2;
@@ -152,28 +152,31 @@ struct SqLoader {
     return min(kt * AX_BN + (i * 4 + wv) * RPI, last & ~(RPI - 1));
   }
   __device__ __forceinline__ void lookup(int kt) {
-    if constexpr (PAGED) {
-#pragma unroll
-      for (int i = 0; i < LD; ++i) pg[i] = table[row0(kt, i) >> psl];
+    base = kt;
+    const int x = threadIdx.x & 63, key = row0(kt + x / LD, x % LD);
+    pages = table[key >> psl];
+    if ((uint32_t)pages >= (uint32_t)num_pages) {  // page 0 in its place
+      bad_from = min(bad_from, (key >> psl) << psl);
+      pages = 0;
     }
   }
   // Rows past the last key re-read the last one (their scores are masked).
   __device__ __forceinline__ void issue(int kt, uint32_t ks, uint32_t vs) {
     const bool full = (kt + 1) * AX_BN <= last + 1;
+    if constexpr (PAGED) {
+      if (kt >= base + 64 / LD || kt < base) lookup(kt);
+    }
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const int r0 = row0(kt, i);
       const T* kb;
       const T* vb;
       if constexpr (PAGED) {
-        int p = pg[i];
-        if ((uint32_t)p >= (uint32_t)num_pages) {
-          bad_from = min(bad_from, (r0 >> psl) << psl);
-          p = 0;
-        }
+        const uint32_t p = (uint32_t)__builtin_amdgcn_readlane(pages, (kt - base) * LD + i);
         const int slot = r0 & ((1 << psl) - 1);
-        kb = k + p * k_sp + slot * k_st;
-        vb = v + p * v_sp + slot * v_st;
+        // (32 x 32 -> 64 bits: the entry point bounds the byte strides)
+        kb = (const T*)((const char*)k + (uint64_t)p * (uint32_t)(k_sp * 2) + (uint32_t)slot * (uint32_t)(k_st * 2));
+        vb = (const T*)((const char*)v + (uint64_t)p * (uint32_t)(v_sp * 2) + (uint32_t)slot * (uint32_t)(v_st * 2));
       } else {
         kb = k + r0 * k_st;
         vb = v + r0 * v_st;
@@ -247,9 +250,7 @@ struct SqTile {
     auto issue = [&](int kt) {  // tiles past the end re-read the last one
       const uint32_t s = stage(kt);
       ld.issue(min(kt, kt1 - 1), s, s + L::ELEMS * 2);
-      ld.lookup(min(kt + 1, kt1 - 1));
     };
-    ld.lookup(kt0);
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s) issue(kt0 + s);
 
@@ -327,6 +328,8 @@ struct SqTile {
 
 // First key (of those the row needs) that has no page, over the workgroup.
 __device__ __forceinline__ int sq_bad_from(int mine, int* slot, int wave, int lane) {
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) mine = min(mine, __shfl_xor(mine, x, 64));
   if (lane == 0) slot[wave] = mine;
   __syncthreads();
   return min(min(slot[0], slot[1]), min(slot[2], slot[3]));
@@ -767,73 +770,125 @@ __global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_paged_kernel(SeqAttnAr
 }
 
 // Joins the parts of each row: o = sum_p w_p o_p / sum_p w_p, w_p = l_p 2^(m_p
-// - max m).  One workgroup a row; parts are always taken in the same order.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void seq_attn_join_kernel(SeqAttnArgs a) {
-  constexpr int LPR = HD / 4, GRP = 256 / LPR;  // lanes of 4 dims a part, parts at a time
-  __shared__ float wt[256];
-  __shared__ float red[256][4];
-  const int tid = threadIdx.x, lane = tid & 63;
+// - max m), parts in one order whatever runs first.  Rows of at most
+// SEQ_WAVE_PARTS parts take a wave each, others a workgroup each.  Its time is
+// a chain of loads (sequence, then m and l beside o), so the o of the first
+// parts is asked for before their weights are known.
+template <typename T, int HD, bool WAVE>
+__device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork& w, int hk, int r, int tid,
+                                            float (*red)[4]) {
+  constexpr int LPR = HD / 4;                    // lanes of 4 dims a part
+  constexpr int GRP = (WAVE ? 64 : 256) / LPR;   // parts at a time
+  constexpr int NP = WAVE ? SEQ_WAVE_PARTS / GRP : 8;  // o values asked for at once
+  constexpr int MLS = WAVE ? 1 : 4;              // parts whose m and l a lane holds
+  const int lane = tid & 63;
+  if (WAVE) tid = lane;
   const float NEG_INF = -__builtin_inff();
+  const int tr = w.cut.few ? w.cut.unit_rows : SQ_ROWS, tile = seq_uni(r / tr), rt = r - tile * tr;
+  const int unit = seq_uni(rt / w.cut.unit_rows), ru = rt - unit * w.cut.unit_rows;
+  const int np = w.cut.parts * a.kv_heads;
+  const int64_t uf = sq_unit_floats(w.cut.unit_rows, HD);
+  // Byte offsets from the row's first part: at most (2 CUs + kv_heads) units
+  // of a tile's rows, below 2^32.
+  const char* first = (const char*)(a.ws + ((int64_t)w.unit + (int64_t)(tile * np + hk) * w.cut.units + unit) * uf);
+  const uint32_t step = (uint32_t)(a.kv_heads * w.cut.units) * (uint32_t)(uf * 4);  // from part to part
+  const int i = seq_uni(r / a.group);
+  const int sees = max(a.causal ? w.kvn - w.qn + i + 1 : w.kvn, 0);
+  const int parts = seq_uni(min(w.cut.parts, seq_ceil(min(sees, w.keys), w.cut.part_keys)));  // those the row sees
+  const char* ml = first + (uint32_t)(w.cut.unit_rows * HD + ru) * 4u;
+  const uint32_t lo = (uint32_t)w.cut.unit_rows * 4u, po = (uint32_t)(ru * HD + (tid % LPR) * 4) * 4u;
+  auto f32_at = [](const char* base, uint32_t off) { return *reinterpret_cast<const float*>(base + off); };
+  const int p0 = tid / LPR;
+
+  float m[MLS], l[MLS];
+#pragma unroll
+  for (int x = 0; x < MLS; ++x) {
+    const int p = lane + 64 * x;
+    m[x] = p < parts ? f32_at(ml, p * step) : NEG_INF;
+    l[x] = p < parts ? f32_at(ml, p * step + lo) : 0.f;
+  }
+  f32x4 o[NP];
+  float om[NP], ol[NP];
+  auto fetch = [&](int b) {
+#pragma unroll
+    for (int x = 0; x < NP; ++x) {
+      const int p = b + p0 + GRP * x;
+      o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+      om[x] = NEG_INF;
+      ol[x] = 0.f;
+      if (p < parts) {
+        o[x] = *reinterpret_cast<const f32x4*>(first + (po + p * step));
+        om[x] = f32_at(ml, p * step);
+        ol[x] = f32_at(ml, p * step + lo);
+      }
+    }
+  };
+  fetch(0);
+  float M = m[0];
+#pragma unroll
+  for (int x = 1; x < MLS; ++x) M = fmaxf(M, m[x]);
+#pragma unroll
+  for (int x = WAVE ? SEQ_WAVE_PARTS / 2 : 32; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
+  if (WAVE) M = __shfl(M, 0, 64);
+  // (A part whose m is NaN makes L and the row NaN; M = -inf leaves L = 0.)
+  auto weight = [&](float pm, float pl) { return pm == NEG_INF ? 0.f : pl * exp2f(pm - M); };
+  float L = 0.f;
+#pragma unroll
+  for (int x = 0; x < MLS; ++x) L += weight(m[x], l[x]);
+  L = wave_sum(L);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int b = 0; b < parts; b += GRP * NP) {
+    if (b > 0) fetch(b);
+#pragma unroll
+    for (int x = 0; x < NP; ++x) {
+      const float f = weight(om[x], ol[x]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += f == 0.f ? 0.f : f * o[x][e];
+    }
+  }
+  if constexpr (WAVE) {
+#pragma unroll
+    for (int x = 32; x >= LPR; x >>= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], x, 64);
+  } else {
+    *reinterpret_cast<f32x4*>(red[tid]) = acc;
+    __syncthreads();
+    if (tid < LPR) {
+#pragma unroll
+      for (int x = 1; x < GRP; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += red[x * LPR + tid][e];
+    }
+    __syncthreads();  // before the next row
+  }
+  if (tid < LPR) {
+    float out[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = L != 0.f ? acc[e] / L : (sees > 0 ? __builtin_nanf("") : 0.f);
+    store4<T>((T*)a.o + (int64_t)(w.q0 + i) * a.o_st + (int64_t)(hk * a.group + r - i * a.group) * a.o_sh + 4 * tid, out);
+  }
+}
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256, 4) void seq_attn_join_kernel(SeqAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) float red[256][4];
   const SeqShape sh = sq_shape(a);
   SeqWalk walk;
   walk.init(a.s, sh, true);
   SeqWork w;
   for (int i = blockIdx.x; walk.find(a.s, sh, true, i, w); i += gridDim.x) {
-    const int u = i - w.item, rows = w.qn * a.group;
-    const int hk = seq_uni(u / rows), r = u - hk * rows;
-    const int tr = w.cut.few ? w.cut.unit_rows : SQ_ROWS, tile = seq_uni(r / tr), rt = r - tile * tr;
-    const int np = w.cut.parts * a.kv_heads;
-    const int64_t uf = sq_unit_floats(w.cut.unit_rows, HD);
-    const float* first = a.ws + ((int64_t)w.unit + (tile * np + hk) * w.cut.units + rt / w.cut.unit_rows) * uf;
-    const int64_t step = (int64_t)a.kv_heads * w.cut.units * uf;  // from part to part
-    const int ru = rt % w.cut.unit_rows;
-    const int sees = max(a.causal ? w.kvn - w.qn + r / a.group + 1 : w.kvn, 0);
-    const int cap = a.s.max_pages << a.s.page_log2;
-    const int parts = min(w.cut.parts, seq_ceil(min(sees, cap), w.cut.part_keys));  // those the row sees
-    // Weights (at most 256 parts: one a thread).
-    float m = NEG_INF, l = 0.f;
-    if (tid < parts) {
-      m = first[tid * step + w.cut.unit_rows * HD + ru];
-      l = first[tid * step + w.cut.unit_rows * HD + w.cut.unit_rows + ru];
+    const int rows = w.qn * a.group, all = rows * a.kv_heads;
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // as in seq_attn_paged_kernel
+    if (w.cut.parts <= SEQ_WAVE_PARTS) {
+      const int u = (i - w.item) * 4 + seq_uni((int)(threadIdx.x >> 6));
+      const int hk = seq_uni(u / rows);
+      if (u < all) sq_join_row<T, HD, true>(a, w, hk, u - hk * rows, tid, red);
+    } else {
+      const int u = i - w.item, hk = seq_uni(u / rows);
+      sq_join_row<T, HD, false>(a, w, hk, u - hk * rows, tid, red);
     }
-    float M = m;
-#pragma unroll
-    for (int x = 32; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
-    if (lane == 0) red[0][tid >> 6] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float wgt = tid < parts ? (m == NEG_INF && M != NEG_INF ? 0.f : l * exp2f(m - M)) : 0.f;
-    wt[tid] = wgt;
-    __syncthreads();  // before red is written again, and wt read
-    const int d0 = (tid % LPR) * 4;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, L = 0.f;
-    for (int p = tid / LPR; p < parts; p += GRP) {
-      float x[4];
-      load4<float>(first + p * step + ru * HD + d0, x);
-      const float f = wt[p];
-      L += f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += f == 0.f ? 0.f : f * x[e];
-    }
-    store4<float>(red[tid], acc);
-    __syncthreads();
-    // Sum of the weights in the same order, by every thread that writes.
-    if (tid < LPR) {
-      L = 0.f;
-      for (int p = 0; p < parts; ++p) L += wt[p];
-      float out[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v = 0.f;
-#pragma unroll
-        for (int x = 0; x < GRP; ++x) v += red[x * LPR + tid][e];
-        out[e] = L != 0.f ? v / L : (sees > 0 ? __builtin_nanf("") : 0.f);
-      }
-      const int64_t tok = w.q0 + r / a.group;
-      store4<T>((T*)a.o + tok * a.o_st + (hk * a.group + r % a.group) * a.o_sh + d0, out);
-    }
-    __syncthreads();
   }
 }
 
@@ -894,7 +949,8 @@ static int launch_hd(SeqAttnArgs a, hipStream_t st) {
   sq_finish(a);
   const SqBounds b = sq_bounds(a);
   auto grid = [](int64_t items, int64_t most) { return dim3((unsigned)(items < most ? items : most)); };
-  if (a.few) seq_attn_paged_kernel<T, HD, true><<<grid(b.items, 2 * a.cus), block, 0, st>>>(a);
+  // Resident workgroups: 3 to a CU at head dim 64 (149 registers), 2 at 128.
+  if (a.few) seq_attn_paged_kernel<T, HD, true><<<grid(b.items, (HD == 64 ? 3 : 2) * a.cus), block, 0, st>>>(a);
   else seq_attn_paged_kernel<T, HD, false><<<grid(b.items, 2 * a.cus), block, 0, st>>>(a);
   if (hipGetLastError() != hipSuccess) return TX_EHIP;
   if (b.units > 0) {

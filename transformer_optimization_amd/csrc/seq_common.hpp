@@ -69,8 +69,10 @@ __device__ __forceinline__ SeqTile seq_find(const SeqArgs& s, int group, int r, 
 // result does not change with the batch around it.
 constexpr int SEQ_FEW = 16;
 constexpr int SEQ_TILE = 128;
-constexpr int SEQ_PART_FEW = 128;   // fewest keys of a part: one block of 32 for each of 4 waves
+constexpr int SEQ_PART_FEW = 256;   // fewest keys of a part: two blocks of 32 for each of 4 waves
 constexpr int SEQ_PART_TILE = 512;  // fewer are not worth writing and joining partial rows for
+
+constexpr int SEQ_WAVE_PARTS = 16;  // rows of up to so many parts are joined by one wave
 
 struct SeqShape {
   int group, kv_heads, cus;
@@ -120,15 +122,15 @@ struct SeqWalk {
   int at_item, at_unit;          // this lane's first item and unit (from base on)
   int q0, qn, kvn;
 
-  __device__ __forceinline__ void load(const SeqArgs& s, const SeqShape& sh, bool rows_as_items) {
+  __device__ __forceinline__ void load(const SeqArgs& s, const SeqShape& sh, bool join) {
     const int b = base + (int)(threadIdx.x & 63);
     const bool in = b < s.batch;
     // Starts that do not ascend are raised to the largest before them, so that
     // no row is in two sequences and the host's bounds on items and units hold
     // whatever the array says.
     q0 = max(in ? seq_cut(s.cu[b], 0, s.tokens) : 0, row);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) q0 = max(q0, __shfl_up(q0, o, 64));  // (lanes below o see themselves)
+    const int n = min(s.batch - base, 64);  // the scans need log2(n) steps
+    for (int o = 1; o < n; o <<= 1) q0 = max(q0, __shfl_up(q0, o, 64));  // (lanes below o see themselves)
     qn = in ? max(seq_cut(s.cu[b + 1], 0, s.tokens) - q0, 0) : 0;
     kvn = in ? max(s.kv_lens[b], 0) : 0;
     n_items = n_units = 0;
@@ -136,12 +138,14 @@ struct SeqWalk {
       const SeqCut c = seq_cut_of(sh, qn * sh.group, min(kvn, s.max_pages << s.page_log2));
       n_items = c.tiles * c.parts * sh.kv_heads;
       n_units = n_items * c.units;
-      if (rows_as_items) n_items = c.parts > 1 ? qn * sh.group * sh.kv_heads : 0;
+      if (join) {  // rows, four to an item where a wave joins one
+        const int all = qn * sh.group * sh.kv_heads;
+        n_items = c.parts <= 1 ? 0 : (c.parts <= SEQ_WAVE_PARTS ? seq_ceil(all, 4) : all);
+      }
     }
     at_item = n_items;
     at_unit = n_units;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
+    for (int o = 1; o < n; o <<= 1) {
       const int x = __shfl_up(at_item, o, 64), y = __shfl_up(at_unit, o, 64);
       if ((int)(threadIdx.x & 63) >= o) {
         at_item += x;
@@ -149,23 +153,25 @@ struct SeqWalk {
       }
     }
   }
-  __device__ __forceinline__ void init(const SeqArgs& s, const SeqShape& sh, bool rows_as_items) {
+  __device__ __forceinline__ void init(const SeqArgs& s, const SeqShape& sh, bool join) {
     base = items = units = row = 0;
-    load(s, sh, rows_as_items);
+    load(s, sh, join);
   }
   // The sequence of item w (ascending from call to call); false: past the end.
-  __device__ __forceinline__ bool find(const SeqArgs& s, const SeqShape& sh, bool rows_as_items, int w, SeqWork& r) {
+  __device__ __forceinline__ bool find(const SeqArgs& s, const SeqShape& sh, bool join, int w, SeqWork& r) {
     for (;;) {
-      const int in_items = seq_uni(__shfl(at_item, 63, 64)), in_units = seq_uni(__shfl(at_unit, 63, 64));
+      const int last = min(s.batch - base, 64) - 1;
+      const int in_items = seq_uni(__shfl(at_item, last, 64)), in_units = seq_uni(__shfl(at_unit, last, 64));
       if (w - items < in_items) break;
       if (base + 64 >= s.batch) return false;
       items += in_items;
       units += in_units;
-      row = seq_uni(__shfl(q0 + qn, 63, 64));
+      row = seq_uni(__shfl(q0 + qn, last, 64));
       base += 64;
-      load(s, sh, rows_as_items);
+      load(s, sh, join);
     }
-    const int i = __builtin_popcountll(__ballot(at_item <= w - items));  // lanes that end before w
+    // Lanes that end before w (those past the batch do not count).
+    const int lane = threadIdx.x & 63, i = __builtin_popcountll(__ballot(base + lane < s.batch && at_item <= w - items));
     r.b = seq_uni(base + i);
     r.q0 = seq_uni(__shfl(q0, i, 64));
     r.qn = seq_uni(__shfl(qn, i, 64));
