@@ -720,7 +720,7 @@ def _starts(cu_seqlens: torch.Tensor) -> int:
     return cu_seqlens.shape[0] - 1
 
 
-def _one_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> torch.device:
+def _one_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> int:
     at = first.get_device()  # -1 on the CPU
     if at < 0:
         _require_cuda(first)
@@ -728,16 +728,20 @@ def _one_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> torch.dev
         if t is not None and t.get_device() != at:
             _require_cuda(t)
             raise ValueError(f"tensors on two devices ({first.device} and {t.device})")
-    return first.device
+    return at
 
 
-def _launch_on(dev: torch.device, fn: str, args: tuple, keep: tuple, info: dict) -> None:
-    """``_launch`` on the current stream of the tensors' device."""
-    if dev.index == torch.cuda.current_device():
-        _launch(fn, args, keep, info)
-    else:
-        with torch.cuda.device(dev):
-            _launch(fn, args, keep, info)
+def _launch_on(at: int, fn: str, args: tuple, keep: tuple, info) -> None:
+    """``_launch`` on the current stream of device ``at``; ``info`` is called when a recording is active."""
+    if at != torch.cuda.current_device():
+        with torch.cuda.device(at):
+            _launch_on(at, fn, args, keep, info)
+        return
+    code = getattr(_lib, fn)(*args, torch._C._cuda_getCurrentRawStream(at))
+    if code != TX_OK:
+        _check(fn, code)
+    if _recorder is not None:
+        _recorder.append(Launch(fn, args, keep, info()))
 
 
 def _addresses(views: tuple) -> tuple:
@@ -813,13 +817,13 @@ def rotary_append(
             raise ValueError("the caches must hold k's heads")
     else:
         block_table = v = None
-    dev = _one_device(k, q, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache, v_cache, q_out, k_out)
+    at = _one_device(k, q, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache, v_cache, q_out, k_out)
     load_library()
     if q is not None and q_out is None:
-        q_out = torch.empty((t, heads, hd), dtype=dtype, device=dev)
+        q_out = torch.empty((t, heads, hd), dtype=dtype, device=k.device)
         qos = (heads * hd, hd, 1)
     if k_cache is None and k_out is None:
-        k_out = torch.empty((t, kvh, hd), dtype=dtype, device=dev)
+        k_out = torch.empty((t, kvh, hd), dtype=dtype, device=k.device)
         kos = (kvh * hd, hd, 1)
     if t == 0 or batch == 0:
         return q_out, k_out
@@ -828,10 +832,8 @@ def rotary_append(
             _ptr(k_cache), ad[5], _ptr(v_cache), ad[6], steps.data_ptr(), _ptr(positions), cu_seqlens.data_ptr(),
             _ptr(kv_lens), _ptr(block_table), table_ld, t, batch, heads, kvh, hd, 2 * half, pages,
             page_size, max_pages, amplitude, 1 if interleaved else 0, _dt(k))
-    info = {"op": "rotary_append", "tokens": t, "heads": heads, "kv_heads": kvh, "head_dim": hd,
-            "cache": k_cache is not None}
-    _launch_on(dev, "tx_rotary_append", args, (q, k, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache,
-                                               v_cache, q_out, k_out, st), info)
+    _launch_on(at, "tx_rotary_append", args, (q, k, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache, v_cache, q_out, k_out, st),
+               lambda: {"op": "rotary_append", "tokens": t, "heads": heads, "kv_heads": kvh, "head_dim": hd, "cache": k_cache is not None})
     return q_out, k_out
 
 
@@ -860,19 +862,18 @@ def flash_attn_packed(
     batch = _starts(cu_seqlens)
     if out is not None:
         os_ = _heads3("out", out, t, heads, hd, dtype)
-    dev = _one_device(q, k, v, cu_seqlens, out)
+    at = _one_device(q, k, v, cu_seqlens, out)
     load_library()
     if out is None:
-        out = torch.empty((t, heads, hd), dtype=dtype, device=dev)
+        out = torch.empty((t, heads, hd), dtype=dtype, device=q.device)
         os_ = (heads * hd, hd, 1)
     if t == 0 or batch == 0:
         return out
     st, ad = _addresses((qs, ks, vs, os_))
     args = (q.data_ptr(), ad[0], k.data_ptr(), ad[1], v.data_ptr(), ad[2], out.data_ptr(), ad[3], cu_seqlens.data_ptr(),
             t, batch, heads, kvh, hd, scale, 1 if causal else 0, _dt(q))
-    info = {"op": "flash_attn_packed", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh, "head_dim": hd,
-            "causal": bool(causal)}
-    _launch_on(dev, "tx_flash_attn_packed", args, (q, k, v, out, cu_seqlens, st), info)
+    _launch_on(at, "tx_flash_attn_packed", args, (q, k, v, out, cu_seqlens, st),
+               lambda: {"op": "flash_attn_packed", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh, "head_dim": hd, "causal": bool(causal)})
     return out
 
 
@@ -919,21 +920,23 @@ def flash_attn_paged(
         raise ValueError(f"{kvh} K/V heads do not divide {heads} query heads")
     if out is not None:
         os_ = _heads3("out", out, t, heads, hd, dtype)
-    dev = _one_device(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, out, workspace)
+    at = _one_device(q, k_cache, v_cache, block_table, cu_seqlens, kv_lens, out, workspace)
     load_library()
     if out is None:
-        out = torch.empty((t, heads, hd), dtype=dtype, device=dev)
+        out = torch.empty((t, heads, hd), dtype=dtype, device=q.device)
         os_ = (heads * hd, hd, 1)
     if t == 0 or batch == 0:
         return out
-    need = 0
-    if workspace is None or workspace.dtype != torch.float32 or not workspace.is_contiguous():
-        if workspace is not None:
-            raise ValueError("workspace must be contiguous fp32")
-        with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext():
+    if workspace is None:
+        if at != torch.cuda.current_device():
+            with torch.cuda.device(at):
+                need = flash_attn_paged_workspace(t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+        else:
             need = flash_attn_paged_workspace(t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
         if need > 0:
-            workspace = torch.empty(need, dtype=torch.float32, device=dev)
+            workspace = torch.empty(need, dtype=torch.float32, device=q.device)
+    elif workspace.dtype != torch.float32 or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous fp32")
     st, ad = _addresses((qs, ks, vs, os_))
     args = (q.data_ptr(), ad[0], k_cache.data_ptr(), ad[1], v_cache.data_ptr(), ad[2], out.data_ptr(), ad[3],
             cu_seqlens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), table_ld, t, batch, heads, kvh,
@@ -941,6 +944,6 @@ def flash_attn_paged(
             0 if workspace is None else workspace.numel(), _dt(q))
     info = {"op": "flash_attn_paged", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh, "head_dim": hd,
             "causal": bool(causal), "page_size": page_size}
-    _launch_on(dev, "tx_flash_attn_paged", args, (q, k_cache, v_cache, out, cu_seqlens, kv_lens, block_table, workspace, st),
+    _launch_on(at, "tx_flash_attn_paged", args, (q, k_cache, v_cache, out, cu_seqlens, kv_lens, block_table, workspace, st),
                info)
     return out

@@ -458,9 +458,8 @@ template <typename T, int HD>
 __global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_packed_kernel(SeqAttnArgs a, int tiles) {
   __shared__ __attribute__((aligned(16))) T lds[SqTile<T, HD, false>::LDS_ELEMS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  // The last tiles of a sequence, which see the most keys, start first.
   const int hk = blockIdx.x % a.kv_heads;
-  const SeqTile t = seq_find(a.s, a.group, SQ_ROWS, tiles - 1 - (int)(blockIdx.x / a.kv_heads));
+  const SeqTile t = seq_find_longest_first(a.s, a.group, SQ_ROWS, tiles, (int)(blockIdx.x / a.kv_heads));
   const int r0 = t.tile * SQ_ROWS;
   if (r0 >= t.qn * a.group) return;
   sq_tile_item<T, HD, false>(a, t.b, t.q0, t.qn, t.qn, hk, r0, 0, 0x7fffffff, nullptr, lds, nullptr, lane, wave);

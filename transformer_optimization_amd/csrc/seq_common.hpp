@@ -60,6 +60,53 @@ __device__ __forceinline__ SeqTile seq_find(const SeqArgs& s, int group, int r, 
   return t;
 }
 
+// Sum over the wave (all lanes active), on the vector ALU alone.
+__device__ __forceinline__ int seq_wave_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// The w-th tile of a call of packed prompts in the order of descending tile
+// index over all sequences at once: under a causal mask the tiles with the
+// most keys start first, whichever sequence they belong to.  Up to 64
+// sequences (one a lane, one round of loads); more keep seq_find's order,
+// where the tail of one long sequence weighs little.  qn = 0: no such tile.
+__device__ __forceinline__ SeqTile seq_find_longest_first(const SeqArgs& s, int group, int r, int tiles, int w) {
+  if (s.batch > 64) return seq_find(s, group, r, tiles - 1 - w);
+  const int lane = threadIdx.x & 63;
+  const int i = lane < s.batch ? lane : s.batch - 1;
+  const int q0 = seq_cut(s.cu[i], 0, s.tokens);
+  const int qn = lane < s.batch ? max(seq_cut(s.cu[i + 1], 0, s.tokens) - q0, 0) : 0;
+  const int n = (qn * group + r - 1) / r;
+  // count(t): tiles of index t or more.  count(lo) > w >= count(hi).
+  auto count = [&](int t) { return seq_wave_sum(max(n - t, 0)); };
+  int lo = 0, hi = tiles, after = 0;
+  SeqTile t{};
+  if (count(0) <= w) return t;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, c = count(mid);
+    if (c > w) lo = mid;
+    else {
+      hi = mid;
+      after = c;
+    }
+  }
+  // The (w - count(lo + 1))-th sequence of those with a tile lo.
+  uint64_t has = __ballot(n > lo);
+  for (int k = w - after; k > 0; --k) has &= has - 1;
+  t.b = seq_uni((int)__builtin_ctzll(has));
+  t.tile = lo;
+  t.q0 = __builtin_amdgcn_readlane(q0, t.b);
+  t.qn = __builtin_amdgcn_readlane(qn, t.b);
+  t.kvn = t.qn;
+  return t;
+}
+
 // ---- how a paged call's work is cut ---------------------------------------
 // A sequence of at most SEQ_FEW rows (query heads of one K/V head x new
 // tokens) is bound by reading its keys: one item per K/V head and part of the
