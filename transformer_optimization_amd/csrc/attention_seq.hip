@@ -105,103 +105,133 @@ constexpr int SQ_THREADS = 256;
 constexpr float SQ_LOG2E = 1.4426950408889634f;
 
 // K and V tiles of 64 keys, global -> LDS by DMA.  One wave instruction moves
-// RPI consecutive key rows, which lie in one page (page sizes are powers of
-// two of at least 8): the page and the row's address are wave-uniform (scalar
-// loads and arithmetic), the lane adds one constant offset.
+// RPI consecutive key rows.  Packed: one wave-uniform base a tile, a constant
+// offset per lane and instruction.  Paged: an instruction's rows lie in one
+// page (page sizes are powers of two of at least 8), so its base is uniform
+// too; a lookup fetches the pages of 64 / LD tiles at once, one lane each, and
+// turns them into byte offsets, so that an issue is two lane reads and an add
+// (looked up tile by tile with scalar loads, whose wait is shared with the LDS
+// reads, a chunk of 512 tokens over 32768 keys took 174 us for 151).
 template <typename T, int HD, bool PAGED>
 struct SqLoader {
   static constexpr int CH = HD / 8;         // 16-byte chunks per row
   static constexpr int RPI = 64 / CH;       // rows per wave instruction (8 or 4)
   static constexpr int LD = AX_BN / RPI / 4;  // instructions per wave and tile (2 or 4)
   static constexpr int ELEMS = AX_BN * HD;
-  const T* k;  // this K/V head's row 0 (packed) or page 0 (paged)
-  const T* v;
+  static constexpr int NOFF = PAGED ? 1 : LD;
+  struct Side {
+    const char* head;    // this K/V head's row 0 (packed) or page 0 (paged)
+    uint32_t st;         // bytes per row
+    uint32_t chunk;      // byte offset of this lane's chunk within a row
+    uint32_t off[NOFF];  // of its row and chunk within a tile (paged: within an instruction's rows)
+    uint32_t lo, hi;     // paged: lane x holds the offset of rows x % LD of tile base + x / LD
+  };
+  Side k, v;
   const int32_t* table;
-  int64_t k_sp, k_st, v_sp, v_st;
   int psl, num_pages;
-  int wv, last;        // last key that may be read
-  int rl;              // this lane's row within an instruction's rows
-  uint32_t kc, vc;     // byte offset of its chunk within a row
-  uint32_t ko, vo;     // byte offset of row and chunk
-  int pages;           // lane x: page of rows x % LD of tile base + x / LD (one load for 64 / LD tiles)
+  uint32_t k_sp, v_sp;  // bytes per page
+  int wv, last;         // last key that may be read
+  int rl;               // this lane's row within an instruction's rows
   int base;
-  int bad_from;        // first key found without a page (over the lane's lookups)
+  int bad_from;         // first key found without a page (over the lane's lookups)
 
   __device__ __forceinline__ void init(const SeqAttnArgs& a, const SeqHead<T, PAGED>& hp, int wave, int lane) {
-    k = hp.k;
-    v = hp.v;
-    k_st = a.k_st;
-    v_st = a.v_st;
     wv = wave;
     rl = lane / CH;
     const int row = wave * RPI + rl;  // the swizzles repeat every 4 * RPI rows
-    kc = 16u * (uint32_t)((lane % CH) ^ ax_kswz<HD>(row));
-    vc = 16u * (uint32_t)((lane % CH) ^ ax_vswz<HD>(row));
-    ko = kc + 2u * (uint32_t)rl * (uint32_t)k_st;
-    vo = vc + 2u * (uint32_t)rl * (uint32_t)v_st;
+    auto side = [&](Side& x, const T* head, int64_t st, int swz) {
+      x.head = (const char*)head;
+      x.st = (uint32_t)(st * 2);
+      x.chunk = 16u * (uint32_t)((lane % CH) ^ swz);
+#pragma unroll
+      for (int i = 0; i < NOFF; ++i) x.off[i] = x.chunk + (uint32_t)(PAGED ? rl : i * 4 * RPI + row) * x.st;
+    };
+    side(k, hp.k, a.k_st, ax_kswz<HD>(row));
+    side(v, hp.v, a.v_st, ax_vswz<HD>(row));
     if constexpr (PAGED) {
       table = a.s.table + (int64_t)hp.b * a.s.table_ld;
       base = -(1 << 30);
-      k_sp = a.k_sp;
-      v_sp = a.v_sp;
       psl = a.s.page_log2;
       num_pages = a.s.num_pages;
+      k_sp = (uint32_t)(a.k_sp * 2);
+      v_sp = (uint32_t)(a.v_sp * 2);
     }
   }
   __device__ __forceinline__ int row0(int kt, int i) const {
     return min(kt * AX_BN + (i * 4 + wv) * RPI, last & ~(RPI - 1));
   }
   __device__ __forceinline__ void lookup(int kt) {
-    base = kt;
-    const int x = threadIdx.x & 63, key = row0(kt + x / LD, x % LD);
-    pages = table[key >> psl];
-    if ((uint32_t)pages >= (uint32_t)num_pages) {  // page 0 in its place
+    base = max(kt - 1, 0);  // V follows K by one tile
+    const int x = threadIdx.x & 63, key = row0(base + x / LD, x % LD);
+    uint32_t page = (uint32_t)table[key >> psl];
+    if (page >= (uint32_t)num_pages) {  // page 0 in its place
       bad_from = min(bad_from, (key >> psl) << psl);
-      pages = 0;
+      page = 0;
     }
+    // 32 x 32 -> 64 bits: the entry point bounds the byte strides.
+    const uint32_t slot = (uint32_t)key & ((1u << psl) - 1);
+    const uint64_t ko = (uint64_t)page * k_sp + slot * k.st, vo = (uint64_t)page * v_sp + slot * v.st;
+    k.lo = (uint32_t)ko;
+    k.hi = (uint32_t)(ko >> 32);
+    v.lo = (uint32_t)vo;
+    v.hi = (uint32_t)(vo >> 32);
   }
-  // Rows past the last key re-read the last one (their scores are masked).
-  __device__ __forceinline__ void issue(int kt, uint32_t ks, uint32_t vs) {
+  // One tile of K or V rows to LDS byte address `to`.  Rows past the last key
+  // re-read the last one (their scores are masked).
+  __device__ __forceinline__ void issue(int kt, uint32_t to, const Side& x) {
     const bool full = (kt + 1) * AX_BN <= last + 1;
-    if constexpr (PAGED) {
-      if (kt >= base + 64 / LD || kt < base) lookup(kt);
+    to += (uint32_t)(wv * RPI * HD * 2);
+    if (!PAGED && full) {
+      const char* tile = x.head + (uint64_t)(uint32_t)(kt * AX_BN) * x.st;
+#pragma unroll
+      for (int i = 0; i < LD; ++i) dma16_m0(tile, x.off[i % NOFF], to + (uint32_t)(i * 4 * RPI * HD * 2));
+      return;
     }
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const int r0 = row0(kt, i);
-      const T* kb;
-      const T* vb;
+      uint64_t at;
       if constexpr (PAGED) {
-        const uint32_t p = (uint32_t)__builtin_amdgcn_readlane(pages, (kt - base) * LD + i);
-        const int slot = r0 & ((1 << psl) - 1);
-        // (32 x 32 -> 64 bits: the entry point bounds the byte strides)
-        kb = (const T*)((const char*)k + (uint64_t)p * (uint32_t)(k_sp * 2) + (uint32_t)slot * (uint32_t)(k_st * 2));
-        vb = (const T*)((const char*)v + (uint64_t)p * (uint32_t)(v_sp * 2) + (uint32_t)slot * (uint32_t)(v_st * 2));
+        const int at_lane = (kt - base) * LD + i;
+        at = (uint32_t)__builtin_amdgcn_readlane((int)x.lo, at_lane) |
+             ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x.hi, at_lane) << 32);
       } else {
-        kb = k + r0 * k_st;
-        vb = v + r0 * v_st;
+        at = (uint64_t)(uint32_t)r0 * x.st;
       }
-      uint32_t kof = ko, vof = vo;
-      if (!full) {
-        const uint32_t r = (uint32_t)min(rl, last - r0);
-        kof = kc + 2u * r * (uint32_t)k_st;
-        vof = vc + 2u * r * (uint32_t)v_st;
-      }
-      const uint32_t at = (uint32_t)((i * 4 + wv) * RPI * HD * 2);
-      dma16_m0(kb, kof, ks + at);
-      dma16_m0(vb, vof, vs + at);
+      uint32_t o = x.off[0];
+      if (!PAGED || !full) o = x.chunk + (uint32_t)min(rl, last - r0) * x.st;
+      dma16_m0(x.head + at, o, to + (uint32_t)(i * 4 * RPI * HD * 2));
     }
   }
+  __device__ __forceinline__ void issue_k(int kt, uint32_t to) {
+    if constexpr (PAGED) {
+      if (kt >= base + 64 / LD) lookup(kt);
+    }
+    issue(kt, to, k);
+  }
+  // Of the tile of issue_k's last call or the one before it (looked up by then).
+  __device__ __forceinline__ void issue_v(int kt, uint32_t to) { issue(kt, to, v); }
 };
 
 // The rows [32 wave, + 32) of a tile over the keys of the tiles [kt0, kt1):
 // unnormalised o, the row sum l of its weights and the base mc (log2 units)
 // they were measured from.
+// LEAD = 1: the scores of a tile are formed while the softmax of the one before
+// it runs (its K tile is staged one tile ahead of V, two sets of scores).  At
+// head dim 128, where registers allow two workgroups a CU either way: one
+// prompt of 32768 tokens 3990 -> 3900 us, of 2048 48.5 -> 45 us.  At head dim 64
+// it costs the third workgroup (181 registers for 124): 40.4 -> 45.9 us for
+// 16 prompts of up to 1021 tokens, so LEAD = 0 there.
+// NST, the stages of the K and V rings: two workgroups a CU have the LDS for 2 at
+// head dim 128, three for 3 at 64.  (With 4 and 8 where a call has no more
+// workgroups than CUs, one prompt of 1024 tokens took 29.9 us for 25.9: what
+// a lone workgroup waits for is not its loads.)
 template <typename T, int HD, bool PAGED>
 struct SqTile {
   typedef typename Mfma<T>::vec vec;
   typedef typename Mfma16<T>::vec vec16;
   typedef SqLoader<T, HD, PAGED> L;
+  static constexpr int LEAD = HD == 128 ? 1 : 0;
   static constexpr int NST = HD == 128 ? 2 : 3;
   static constexpr int LDS_ELEMS = NST * 2 * L::ELEMS;
   static constexpr int LPW = 2 * L::LD;
@@ -246,37 +276,66 @@ struct SqTile {
     m_run = NEG_INF;
     mc = 0.f;
     const uint32_t base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) T*)lds;
-    auto stage = [&](int kt) { return base + (uint32_t)((kt % NST) * 2 * L::ELEMS * 2); };
-    auto issue = [&](int kt) {  // tiles past the end re-read the last one
-      const uint32_t s = stage(kt);
-      ld.issue(min(kt, kt1 - 1), s, s + L::ELEMS * 2);
-    };
+    auto k_at = [&](int kt) { return base + (uint32_t)((kt % NST) * L::ELEMS * 2); };
+    auto v_at = [&](int kt) { return base + (uint32_t)((NST + kt % NST) * L::ELEMS * 2); };
+    // Tiles past the end re-read the last one.
+    auto issue_k = [&](int kt) { ld.issue_k(min(kt, kt1 - 1), k_at(kt)); };
+    auto issue_v = [&](int kt) { ld.issue_v(min(kt, kt1 - 1), v_at(kt)); };
+    if constexpr (LEAD) issue_k(kt0);
 #pragma unroll
-    for (int s = 0; s < NST - 1; ++s) issue(kt0 + s);
-
-    for (int kt = kt0; kt < kt1; ++kt) {
+    for (int s = 0; s < NST - 1; ++s) {
+      issue_k(kt0 + LEAD + s);
+      issue_v(kt0 + s);
+    }
+    // Scores of one 16-wide step of the head dim, both 32-key halves.
+    auto qk = [&](const T* Ks, int ks, f32x16* s) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const vec kf = *reinterpret_cast<const vec*>(Ks + 32 * t * HD + ko.off[ks]);
+        s[t] = Mfma<T>::mma32(kf, qf[ks], s[t]);
+      }
+    };
+    auto zero = [&](f32x16* s) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+    };
+    // One tile: the weights and P V of tile kt from its scores sc (formed here
+    // without LEAD), and with LEAD the scores sn of tile kt + 1, whose matrix
+    // instructions run beside the vector work of tile kt's softmax.
+    auto step = [&](int kt, f32x16* sc, f32x16* sn) {
       const int j0 = kt * AX_BN;
-      ring_barrier<LPW * (NST - 2)>();
-      issue(kt + NST - 1);
-      if (j0 >= wlim_max) continue;  // no row of this wave sees these keys
-      const T* Ks = lds + (kt % NST) * 2 * L::ELEMS;
+      ring_barrier<LPW * (NST - 2)>();  // K of tile kt + LEAD, V of tile kt
+      issue_k(kt + LEAD + NST - 1);
+      issue_v(kt + NST - 1);
+      if (j0 >= wlim_max) return;  // no row of this wave sees these keys, nor later ones
+      const T* Kn = lds + ((kt + LEAD) % NST) * L::ELEMS;
       uint32_t va[HD / 32];
 #pragma unroll
-      for (int dt = 0; dt < HD / 32; ++dt) va[dt] = stage(kt) + L::ELEMS * 2 + 2u * (uint32_t)vn.off[dt];
-      f32x16 s[2];
-      ax_scores<T, HD>(Ks, qf, ko, s);
+      for (int dt = 0; dt < HD / 32; ++dt) va[dt] = v_at(kt) + 2u * (uint32_t)vn.off[dt];
+      if constexpr (!LEAD) {
+        zero(sc);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) qk(Kn, ks, sc);
+      }
       if (j0 + AX_BN > wlim_min) {
         const int d = mylim - j0 - 8 * half;  // slot of key j0 + 8 half + x is seen if x < d
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[t][r] = (32 * t + ((r >> 3) << 4) + (r & 7) < d) ? s[t][r] : NEG_INF;
+          for (int r = 0; r < 16; ++r) sc[t][r] = (32 * t + ((r >> 3) << 4) + (r & 7) < d) ? sc[t][r] : NEG_INF;
+      }
+      if constexpr (LEAD) {  // (after the last tile: scores that nothing uses)
+        zero(sn);
+#pragma unroll
+        for (int ks = 0; ks < HD / 64; ++ks) qk(Kn, ks, sn);
       }
       float mx = NEG_INF;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[t][r]);
       {
         const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
                                                          __builtin_bit_cast(uint32_t, mx), false, false);
@@ -296,9 +355,24 @@ struct SqTile {
         m_run = m_new;
         mc = (m_run == NEG_INF ? 0.f : m_run) - BIAS;
       }
+      u32x4 pk[4];
+      auto weights = [&](int u) {
+        const int t = u >> 1, hh = u & 1;
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][8 * hh + e], c, -mc));
+        pk[u] = u32x4{pack2_raw<T>(p[0], p[1]), pack2_raw<T>(p[2], p[3]), pack2_raw<T>(p[4], p[5]),
+                      pack2_raw<T>(p[6], p[7])};
+      };
+      if constexpr (LEAD) {
+#pragma unroll
+        for (int ks = HD / 64; ks < HD / 16; ++ks) qk(Kn, ks, sn);
+        weights(0);
+        weights(1);
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int t = u >> 1, hh = u & 1;
         u32x4 vop[HD / 32];
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt) {
@@ -309,18 +383,28 @@ struct SqTile {
             default: vop[dt] = ax_vnat_issue<HD, 3>(va[dt]); break;
           }
         }
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][8 * hh + e], c, -mc));
-        const u32x4 pk = u32x4{pack2_raw<T>(p[0], p[1]), pack2_raw<T>(p[2], p[3]), pack2_raw<T>(p[4], p[5]),
-                               pack2_raw<T>(p[6], p[7])};
-        const vec pf = __builtin_bit_cast(vec, pk);
-        lsum = Mfma16<T>::mma(sel, __builtin_bit_cast(vec16, pk), lsum);
+        if constexpr (!LEAD) weights(u);
+        lsum = Mfma16<T>::mma(sel, __builtin_bit_cast(vec16, pk[u]), lsum);
+        if (LEAD && u < 2) weights(u + 2);
         ax_vnat_wait<HD / 32>(vop);
 #pragma unroll
-        for (int dt = 0; dt < HD / 32; ++dt) o[dt] = Mfma<T>::mma32(__builtin_bit_cast(vec, vop[dt]), pf, o[dt]);
+        for (int dt = 0; dt < HD / 32; ++dt)
+          o[dt] = Mfma<T>::mma32(__builtin_bit_cast(vec, vop[dt]), __builtin_bit_cast(vec, pk[u]), o[dt]);
       }
+    };
+    f32x16 sa[2];
+    if constexpr (LEAD) {
+      f32x16 sb[2];
+      ring_barrier<LPW * (NST - 1)>();  // K of the first tile
+      zero(sa);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) qk(lds + (kt0 % NST) * L::ELEMS, ks, sa);
+      for (int kt = kt0; kt < kt1; kt += 2) {
+        step(kt, sa, sb);
+        if (kt + 1 < kt1) step(kt + 1, sb, sa);
+      }
+    } else {
+      for (int kt = kt0; kt < kt1; ++kt) step(kt, sa, sa);
     }
     ring_drain();
   }
@@ -739,8 +823,9 @@ __global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_paged_kernel(SeqAttnAr
   __shared__ int bad[4];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const SeqShape sh = sq_shape(a);
+  __shared__ int seqs[4][SeqWalk::LDS_INTS];
   SeqWalk walk;
-  walk.init(a.s, sh, false);
+  walk.init(a.s, sh, false, seqs[wave]);
   SeqWork w;
   for (int i = blockIdx.x; walk.find(a.s, sh, false, i, w); i += gridDim.x) {
     // An item's lane constants are formed within it: held across the items
@@ -873,8 +958,9 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256, 4) void seq_attn_join_kernel(SeqAttnArgs a) {
   __shared__ __attribute__((aligned(16))) float red[256][4];
   const SeqShape sh = sq_shape(a);
+  __shared__ int seqs[4][SeqWalk::LDS_INTS];
   SeqWalk walk;
-  walk.init(a.s, sh, true);
+  walk.init(a.s, sh, true, seqs[seq_uni((int)(threadIdx.x >> 6))]);
   SeqWork w;
   for (int i = blockIdx.x; walk.find(a.s, sh, true, i, w); i += gridDim.x) {
     const int rows = w.qn * a.group, all = rows * a.kv_heads;
@@ -942,7 +1028,8 @@ static int launch_hd(SeqAttnArgs a, hipStream_t st) {
   const dim3 block(SQ_THREADS);
   if (!a.paged) {
     const int tiles = (int)seq_tiles(a.s, a.group, SQ_ROWS);
-    seq_attn_packed_kernel<T, HD><<<dim3((unsigned)tiles * (unsigned)a.kv_heads), block, 0, st>>>(a, tiles);
+    const dim3 grid((unsigned)tiles * (unsigned)a.kv_heads);
+    seq_attn_packed_kernel<T, HD><<<grid, block, 0, st>>>(a, tiles);
     return hipGetLastError() == hipSuccess ? TX_OK : TX_EHIP;
   }
   sq_finish(a);

@@ -161,70 +161,85 @@ struct SeqWork {
 };
 
 // Walks the items of a call in ascending order, 64 sequences at a time (lane
-// i: sequence base + i); every lane of the wave takes part.
+// i: sequence base + i); every lane of the wave takes part.  What the lanes
+// hold of their sequences stays in LDS between the items, whose own work needs
+// the registers.
 struct SeqWalk {
-  int base, items, units;        // before sequence base
-  int row;                       // first row that sequence base may hold
-  int n_items, n_units;          // of this lane's sequence
-  int at_item, at_unit;          // this lane's first item and unit (from base on)
-  int q0, qn, kvn;
+  struct Lane {
+    int n_items, n_units;    // of this lane's sequence
+    int at_item, at_unit;    // behind its last item and unit (from base on)
+    int q0, qn, kvn;
+  };
+  static constexpr int LDS_INTS = 64 * 7;  // per wave
+  int base, items, units;  // before sequence base
+  int row;                 // first row that sequence base may hold
+  int* lds;                // this wave's LDS_INTS
 
   __device__ __forceinline__ void load(const SeqArgs& s, const SeqShape& sh, bool join) {
-    const int b = base + (int)(threadIdx.x & 63);
+    const int lane = threadIdx.x & 63, b = base + lane;
     const bool in = b < s.batch;
+    Lane x;
     // Starts that do not ascend are raised to the largest before them, so that
     // no row is in two sequences and the host's bounds on items and units hold
     // whatever the array says.
-    q0 = max(in ? seq_cut(s.cu[b], 0, s.tokens) : 0, row);
+    x.q0 = max(in ? seq_cut(s.cu[b], 0, s.tokens) : 0, row);
+    const int end = in ? seq_cut(s.cu[b + 1], 0, s.tokens) : 0;
+    x.kvn = in ? max(s.kv_lens[b], 0) : 0;
     const int n = min(s.batch - base, 64);  // the scans need log2(n) steps
-    for (int o = 1; o < n; o <<= 1) q0 = max(q0, __shfl_up(q0, o, 64));  // (lanes below o see themselves)
-    qn = in ? max(seq_cut(s.cu[b + 1], 0, s.tokens) - q0, 0) : 0;
-    kvn = in ? max(s.kv_lens[b], 0) : 0;
-    n_items = n_units = 0;
-    if (qn > 0) {
-      const SeqCut c = seq_cut_of(sh, qn * sh.group, min(kvn, s.max_pages << s.page_log2));
-      n_items = c.tiles * c.parts * sh.kv_heads;
-      n_units = n_items * c.units;
+    for (int o = 1; o < n; o <<= 1) x.q0 = max(x.q0, __shfl_up(x.q0, o, 64));  // (lanes below o see themselves)
+    x.qn = max(end - x.q0, 0);
+    x.n_items = x.n_units = 0;
+    if (x.qn > 0) {
+      const SeqCut c = seq_cut_of(sh, x.qn * sh.group, min(x.kvn, s.max_pages << s.page_log2));
+      x.n_items = c.tiles * c.parts * sh.kv_heads;
+      x.n_units = x.n_items * c.units;
       if (join) {  // rows, four to an item where a wave joins one
-        const int all = qn * sh.group * sh.kv_heads;
-        n_items = c.parts <= 1 ? 0 : (c.parts <= SEQ_WAVE_PARTS ? seq_ceil(all, 4) : all);
+        const int all = x.qn * sh.group * sh.kv_heads;
+        x.n_items = c.parts <= 1 ? 0 : (c.parts <= SEQ_WAVE_PARTS ? seq_ceil(all, 4) : all);
       }
     }
-    at_item = n_items;
-    at_unit = n_units;
+    x.at_item = x.n_items;
+    x.at_unit = x.n_units;
     for (int o = 1; o < n; o <<= 1) {
-      const int x = __shfl_up(at_item, o, 64), y = __shfl_up(at_unit, o, 64);
-      if ((int)(threadIdx.x & 63) >= o) {
-        at_item += x;
-        at_unit += y;
+      const int i = __shfl_up(x.at_item, o, 64), u = __shfl_up(x.at_unit, o, 64);
+      if (lane >= o) {
+        x.at_item += i;
+        x.at_unit += u;
       }
     }
+    const int f[7] = {x.n_items, x.n_units, x.at_item, x.at_unit, x.q0, x.qn, x.kvn};
+#pragma unroll
+    for (int i = 0; i < 7; ++i) lds[64 * i + lane] = f[i];
   }
-  __device__ __forceinline__ void init(const SeqArgs& s, const SeqShape& sh, bool join) {
+  __device__ __forceinline__ void init(const SeqArgs& s, const SeqShape& sh, bool join, int* lds_) {
     base = items = units = row = 0;
+    lds = lds_;
     load(s, sh, join);
   }
+  // Field f of the Lane of sequence base + i (one wave's own LDS: in order).
+  __device__ __forceinline__ int field(int f, int i) const { return seq_uni(lds[64 * f + i]); }
   // The sequence of item w (ascending from call to call); false: past the end.
   __device__ __forceinline__ bool find(const SeqArgs& s, const SeqShape& sh, bool join, int w, SeqWork& r) {
     for (;;) {
       const int last = min(s.batch - base, 64) - 1;
-      const int in_items = seq_uni(__shfl(at_item, last, 64)), in_units = seq_uni(__shfl(at_unit, last, 64));
+      const int in_items = field(2, last);
       if (w - items < in_items) break;
       if (base + 64 >= s.batch) return false;
       items += in_items;
-      units += in_units;
-      row = seq_uni(__shfl(q0 + qn, last, 64));
+      units += field(3, last);
+      row = field(4, last) + field(5, last);
       base += 64;
       load(s, sh, join);
     }
     // Lanes that end before w (those past the batch do not count).
-    const int lane = threadIdx.x & 63, i = __builtin_popcountll(__ballot(base + lane < s.batch && at_item <= w - items));
-    r.b = seq_uni(base + i);
-    r.q0 = seq_uni(__shfl(q0, i, 64));
-    r.qn = seq_uni(__shfl(qn, i, 64));
-    r.kvn = seq_uni(__shfl(kvn, i, 64));
-    r.item = seq_uni(items + __shfl(at_item - n_items, i, 64));
-    r.unit = seq_uni(units + __shfl(at_unit - n_units, i, 64));
+    const int lane = threadIdx.x & 63;
+    const int i = __builtin_popcountll(__ballot(base + lane < s.batch && lds[64 * 2 + lane] <= w - items));
+    r.b = base + i;
+    r.q0 = field(4, i);
+    r.qn = field(5, i);
+    r.kvn = field(6, i);
+    r.item = items + field(2, i) - field(0, i);
+    r.unit = units + field(3, i) - field(1, i);
     r.keys = min(r.kvn, s.max_pages << s.page_log2);
     r.cut = seq_cut_of(sh, r.qn * sh.group, r.keys);
     r.cut.tiles = seq_uni(r.cut.tiles);
