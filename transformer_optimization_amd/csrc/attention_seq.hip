@@ -539,11 +539,11 @@ __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0
 
 // ------------------------------------------------------------- packed prompts
 template <typename T, int HD>
-__global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_packed_kernel(SeqAttnArgs a, int tiles) {
+__global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_packed_kernel(SeqAttnArgs a, SeqOrder order) {
   __shared__ __attribute__((aligned(16))) T lds[SqTile<T, HD, false>::LDS_ELEMS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int hk = blockIdx.x % a.kv_heads;
-  const SeqTile t = seq_find_longest_first(a.s, a.group, SQ_ROWS, tiles, (int)(blockIdx.x / a.kv_heads));
+  int hk;
+  const SeqTile t = seq_ordered(a.s, a.group, SQ_ROWS, order, a.kv_heads, (int)blockIdx.x, hk);
   const int r0 = t.tile * SQ_ROWS;
   if (r0 >= t.qn * a.group) return;
   sq_tile_item<T, HD, false>(a, t.b, t.q0, t.qn, t.qn, hk, r0, 0, 0x7fffffff, nullptr, lds, nullptr, lane, wave);
@@ -1027,9 +1027,8 @@ template <typename T, int HD>
 static int launch_hd(SeqAttnArgs a, hipStream_t st) {
   const dim3 block(SQ_THREADS);
   if (!a.paged) {
-    const int tiles = (int)seq_tiles(a.s, a.group, SQ_ROWS);
-    const dim3 grid((unsigned)tiles * (unsigned)a.kv_heads);
-    seq_attn_packed_kernel<T, HD><<<grid, block, 0, st>>>(a, tiles);
+    const SeqOrder o = seq_order(a.s, a.group, SQ_ROWS, (int64_t)a.s.tokens * a.kv_heads * HD * 4);
+    seq_attn_packed_kernel<T, HD><<<dim3((unsigned)seq_order_grid(o, a.kv_heads)), block, 0, st>>>(a, o);
     return hipGetLastError() == hipSuccess ? TX_OK : TX_EHIP;
   }
   sq_finish(a);

@@ -71,22 +71,49 @@ __device__ __forceinline__ int seq_wave_sum(int x) {
   return __builtin_amdgcn_readlane(x, 63);
 }
 
-// The w-th tile of a call of packed prompts in the order of descending tile
-// index over all sequences at once: under a causal mask the tiles with the
-// most keys start first, whichever sequence they belong to.  Up to 64
-// sequences (one a lane, one round of loads); more keep seq_find's order,
-// where the tail of one long sequence weighs little.  qn = 0: no such tile.
-__device__ __forceinline__ SeqTile seq_find_longest_first(const SeqArgs& s, int group, int r, int tiles, int w) {
-  if (s.batch > 64) return seq_find(s, group, r, tiles - 1 - w);
-  const int lane = threadIdx.x & 63;
-  const int i = lane < s.batch ? lane : s.batch - 1;
-  const int q0 = seq_cut(s.cu[i], 0, s.tokens);
-  const int qn = lane < s.batch ? max(seq_cut(s.cu[i + 1], 0, s.tokens) - q0, 0) : 0;
-  const int n = (qn * group + r - 1) / r;
-  // count(t): tiles of index t or more.  count(lo) > w >= count(hi).
-  auto count = [&](int t) { return seq_wave_sum(max(n - t, 0)); };
-  int lo = 0, hi = tiles, after = 0;
+// Order of a call of packed prompts: the tiles of all sequences and heads in
+// descending order of their index, so that under a causal mask those with the
+// most keys start first, whichever sequence they belong to (16 prompts of up
+// to 1021 tokens 47 -> 40 us).  Where the keys and values are more than the memory-side
+// cache holds, bands of 16 neighbouring tiles of one (sequence, K/V head), which read the
+// same keys in step, are ordered instead, each on one XCD (workgroup i runs on
+// XCD i % 8), whose L2 then serves them: 8 x 16384 tokens, 16 heads with keys
+// of their own, 10.1 -> 8.2 ms, 8 x 8192 2.50 -> 2.18; below that size the
+// coarser order costs more than it saves (8 x 2048 156 -> 164 us).
+struct SeqOrder {
+  int band;   // log2 tiles of a band
+  int bands;  // bound on a head's bands over all sequences
+};
+// More than 64 sequences keep seq_find's order (reversed), where the tail of
+// one long sequence weighs little.
+inline SeqOrder seq_order(const SeqArgs& s, int group, int r, int64_t kv_bytes) {
+  const int64_t tiles = seq_tiles(s, group, r);
+  SeqOrder o;
+  o.band = s.batch <= 64 && kv_bytes >= (int64_t)1 << 28 && tiles / s.batch >= 16 ? 4 : 0;
+  o.bands = (int)(s.batch > 64 ? tiles : (tiles >> o.band) + s.batch);
+  return o;
+}
+inline int64_t seq_order_grid(const SeqOrder& o, int kv_heads) {
+  return (((int64_t)o.bands * kv_heads + 7) / 8 * 8) << o.band;
+}
+// The tile and K/V head of workgroup wg; qn = 0: none.
+__device__ __forceinline__ SeqTile seq_ordered(const SeqArgs& s, int group, int r, SeqOrder o, int kv_heads, int wg,
+                                               int& hk) {
+  const int i = wg >> 3, sub = i & ((1 << o.band) - 1);
+  const int slot = (i >> o.band) * 8 + (wg & 7);
+  const int w = seq_uni(slot / kv_heads);
+  hk = slot - w * kv_heads;
   SeqTile t{};
+  if (s.batch > 64) return w < o.bands ? seq_find(s, group, r, o.bands - 1 - w) : t;
+  // One lane a sequence, one round of loads.
+  const int lane = threadIdx.x & 63;
+  const int b = lane < s.batch ? lane : s.batch - 1;
+  const int q0 = seq_cut(s.cu[b], 0, s.tokens);
+  const int qn = lane < s.batch ? max(seq_cut(s.cu[b + 1], 0, s.tokens) - q0, 0) : 0;
+  const int n = (qn * group + r - 1) / r, nb = (n + (1 << o.band) - 1) >> o.band;
+  // count(x): bands of index x or more.  count(lo) > w >= count(hi).
+  auto count = [&](int x) { return seq_wave_sum(max(nb - x, 0)); };
+  int lo = 0, hi = o.bands, after = 0;
   if (count(0) <= w) return t;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1, c = count(mid);
@@ -96,13 +123,13 @@ __device__ __forceinline__ SeqTile seq_find_longest_first(const SeqArgs& s, int 
       after = c;
     }
   }
-  // The (w - count(lo + 1))-th sequence of those with a tile lo.
-  uint64_t has = __ballot(n > lo);
+  // The (w - count(lo + 1))-th sequence of those with a band lo.
+  uint64_t has = __ballot(nb > lo);
   for (int k = w - after; k > 0; --k) has &= has - 1;
   t.b = seq_uni((int)__builtin_ctzll(has));
-  t.tile = lo;
+  t.tile = (lo << o.band) + (1 << o.band) - 1 - sub;
   t.q0 = __builtin_amdgcn_readlane(q0, t.b);
-  t.qn = __builtin_amdgcn_readlane(qn, t.b);
+  t.qn = t.tile < __builtin_amdgcn_readlane(n, t.b) ? __builtin_amdgcn_readlane(qn, t.b) : 0;
   t.kvn = t.qn;
   return t;
 }
