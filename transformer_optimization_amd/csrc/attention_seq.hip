@@ -222,17 +222,18 @@ struct SqLoader {
 // prompt of 32768 tokens 3990 -> 3900 us, of 2048 48.5 -> 45 us.  At head dim 64
 // it costs the third workgroup (181 registers for 124): 40.4 -> 45.9 us for
 // 16 prompts of up to 1021 tokens, so LEAD = 0 there.
-// NST, the stages of the K and V rings: two workgroups a CU have the LDS for 2 at
-// head dim 128, three for 3 at 64.  (With 4 and 8 where a call has no more
-// workgroups than CUs, one prompt of 1024 tokens took 29.9 us for 25.9: what
-// a lone workgroup waits for is not its loads.)
+// NST, the stages of the K and V rings: 2, for two workgroups a CU at head dim
+// 128 and four at 64 (126 registers): a third stage there leaves three, 2 x 8192
+// tokens 300 us for 285, 16 prompts of up to 1021 42.9 for 38.4.  (With 4 and 8
+// where a call has no more workgroups than CUs, one prompt of 1024 tokens
+// took 29.9 us for 25.9: what a lone workgroup waits for is not its loads.)
 template <typename T, int HD, bool PAGED>
 struct SqTile {
   typedef typename Mfma<T>::vec vec;
   typedef typename Mfma16<T>::vec vec16;
   typedef SqLoader<T, HD, PAGED> L;
   static constexpr int LEAD = HD == 128 ? 1 : 0;
-  static constexpr int NST = HD == 128 ? 2 : 3;
+  static constexpr int NST = 2;
   static constexpr int LDS_ELEMS = NST * 2 * L::ELEMS;
   static constexpr int LPW = 2 * L::LD;
   // fp16 weights reach 2^15 at most instead of 2^8, so that the small ones
@@ -1034,9 +1035,10 @@ static int launch_hd(SeqAttnArgs a, hipStream_t st) {
   sq_finish(a);
   const SqBounds b = sq_bounds(a);
   auto grid = [](int64_t items, int64_t most) { return dim3((unsigned)(items < most ? items : most)); };
-  // Resident workgroups: 3 to a CU at head dim 64 (149 registers), 2 at 128.
-  if (a.few) seq_attn_paged_kernel<T, HD, true><<<grid(b.items, (HD == 64 ? 3 : 2) * a.cus), block, 0, st>>>(a);
-  else seq_attn_paged_kernel<T, HD, false><<<grid(b.items, 2 * a.cus), block, 0, st>>>(a);
+  // Resident workgroups: 3 to a CU at head dim 64 (133 and 157 registers), 2 at 128.
+  const int64_t resident = (HD == 64 ? 3 : 2) * a.cus;
+  if (a.few) seq_attn_paged_kernel<T, HD, true><<<grid(b.items, resident), block, 0, st>>>(a);
+  else seq_attn_paged_kernel<T, HD, false><<<grid(b.items, resident), block, 0, st>>>(a);
   if (hipGetLastError() != hipSuccess) return TX_EHIP;
   if (b.units > 0) {
     seq_attn_join_kernel<T, HD><<<grid(b.join_rows, 16 * a.cus), block, 0, st>>>(a);
