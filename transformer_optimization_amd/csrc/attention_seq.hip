@@ -453,7 +453,7 @@ __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0
   const int G = a.group, n = min(qn * G - r0, SQ_ROWS);
   const int cap = PAGED ? a.s.max_pages << a.s.page_log2 : kvn;
   auto keys_of = [&](int r) {  // keys that row r sees
-    return max(a.causal ? kvn - qn + r / G + 1 : kvn, 0);
+    return max(a.causal ? kvn - qn + seq_div(r, a.by_group) + 1 : kvn, 0);
   };
   const int lim = seq_uni(min(min(keys_of(r0 + n - 1), cap), j1));
   const int w0 = r0 + 32 * wave, wn = min(n - 32 * wave, 32);
@@ -461,8 +461,9 @@ __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0
   const int wlim_min = seq_uni(wn > 0 ? min(keys_of(w0), lim) : 0);
   const int r = min(w0 + (lane & 31), r0 + n - 1);
   const bool active = (lane & 31) < wn;
-  const int64_t tok = q0 + r / G;
-  const int h = hk * G + r - (r / G) * G;
+  const int i0 = seq_div(r, a.by_group);
+  const int64_t tok = q0 + i0;
+  const int h = hk * G + r - i0 * G;
   const int sees = keys_of(r);
 
   SeqHead<T, PAGED> hp;
@@ -534,7 +535,8 @@ __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0
     todo &= todo - 1;
     float *po = nullptr, *pml = nullptr;
     if (part) unit_of(ri - r0, po, pml);
-    sq_row_again<T, HD, PAGED>(a, hp, q0 + ri / G, hk * G + ri - (ri / G) * G, j0, min(keys_of(ri), lim), po, pml, SEQ_FEW);
+    const int ti = seq_div(ri, a.by_group);
+    sq_row_again<T, HD, PAGED>(a, hp, q0 + ti, hk * G + ri - ti * G, j0, min(keys_of(ri), lim), po, pml, SEQ_FEW);
   }
 }
 
@@ -580,12 +582,13 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   const float c = a.scale * SQ_LOG2E;
   const int G = a.group, n = min(w.qn * G - r0, w.cut.unit_rows);
   const int cap = a.s.max_pages << a.s.page_log2, ps1 = (1 << a.s.page_log2) - 1;
-  auto keys_of = [&](int r) { return max(a.causal ? w.kvn - w.qn + r / G + 1 : w.kvn, 0); };
+  auto keys_of = [&](int r) { return max(a.causal ? w.kvn - w.qn + seq_div(r, a.by_group) + 1 : w.kvn, 0); };
   const int lim = seq_uni(min(min(keys_of(r0 + n - 1), cap), j1));
   const int col = lane & 15, g = lane >> 4;
   const int r = r0 + min(col, n - 1);
-  const int64_t tok = w.q0 + r / G;
-  const int h = hk * G + r - (r / G) * G;
+  const int i0 = seq_div(r, a.by_group);
+  const int64_t tok = w.q0 + i0;
+  const int h = hk * G + r - i0 * G;
   const int mylim = min(keys_of(r), lim);
   SeqHead<T, true> hp;
   hp.init(a, w.b, w.q0, hk);
@@ -782,8 +785,9 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   const bool redo = active && !lost && sees > j0 && !(odd == 0.f);
   if (redo) sagain[row] = 1;
   __syncthreads();
-  const int64_t tk = w.q0 + rr / G;
-  const int hh = hk * G + rr - (rr / G) * G;
+  const int ir = seq_div(rr, a.by_group);
+  const int64_t tk = w.q0 + ir;
+  const int hh = hk * G + rr - ir * G;
   if (active && !sagain[row]) {
     if (part) {
       float* po = part + row * HD + d0;
@@ -802,7 +806,8 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   for (int i = wave; i < n; i += 4) {
     if (!sagain[i]) continue;  // wave-uniform
     const int ri = r0 + i;
-    sq_row_again<T, HD, true>(a, hp, w.q0 + ri / G, hk * G + ri - (ri / G) * G, j0, min(keys_of(ri), lim),
+    const int ti = seq_div(ri, a.by_group);
+    sq_row_again<T, HD, true>(a, hp, w.q0 + ti, hk * G + ri - ti * G, j0, min(keys_of(ri), lim),
                               part ? part + i * HD : nullptr, part ? part + w.cut.unit_rows * HD + i : nullptr,
                               w.cut.unit_rows);
   }
@@ -810,7 +815,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
 
 // ---------------------------------------------------------------- paged calls
 __host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
-  return SeqShape{a.group, a.kv_heads, a.cus, a.few};
+  return SeqShape{a.group, a.kv_heads, a.cus, a.few_parts, a.few};
 }
 
 // Persistent workgroups over the items of a call (SeqWalk); a grid of at most
@@ -837,8 +842,8 @@ __global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_paged_kernel(SeqAttnAr
     // the tiles that share keys meet on one XCD when the pairs are a multiple
     // of 8.
     const int u = i - w.item, np = w.cut.parts * a.kv_heads;
-    const int tile = seq_uni(u / np), pair = u - tile * np;
-    const int p = seq_uni(pair / a.kv_heads), hk = pair - p * a.kv_heads;
+    const int tile = w.cut.tiles > 1 ? seq_uni(u / np) : 0, pair = u - tile * np;
+    const int p = seq_uni(seq_div(pair, a.by_kv_heads)), hk = pair - p * a.kv_heads;
     const int j0 = p * w.cut.part_keys, j1 = p + 1 < w.cut.parts ? j0 + w.cut.part_keys : 0x7fffffff;
     float* part = nullptr;
     if (w.cut.parts > 1) part = a.ws + (int64_t)(w.unit + u * w.cut.units) * sq_unit_floats(w.cut.unit_rows, HD);
@@ -869,17 +874,19 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
   const int lane = tid & 63;
   if (WAVE) tid = lane;
   const float NEG_INF = -__builtin_inff();
-  const int tr = w.cut.few ? w.cut.unit_rows : SQ_ROWS, tile = seq_uni(r / tr), rt = r - tile * tr;
-  const int unit = seq_uni(rt / w.cut.unit_rows), ru = rt - unit * w.cut.unit_rows;
+  const int tr = w.cut.few ? w.cut.unit_rows : SQ_ROWS;
+  const int tile = w.cut.tiles == 1 ? 0 : (w.cut.few ? seq_uni(r / tr) : r / SQ_ROWS), rt = r - tile * tr;
+  const int unit = w.cut.few ? 0 : rt / SEQ_FEW, ru = rt - unit * SEQ_FEW;
   const int np = w.cut.parts * a.kv_heads;
   const int64_t uf = sq_unit_floats(w.cut.unit_rows, HD);
   // Byte offsets from the row's first part: at most (2 CUs + kv_heads) units
   // of a tile's rows, below 2^32.
   const char* first = (const char*)(a.ws + ((int64_t)w.unit + (int64_t)(tile * np + hk) * w.cut.units + unit) * uf);
   const uint32_t step = (uint32_t)(a.kv_heads * w.cut.units) * (uint32_t)(uf * 4);  // from part to part
-  const int i = seq_uni(r / a.group);
+  const int i = seq_uni(seq_div(r, a.by_group));
   const int sees = max(a.causal ? w.kvn - w.qn + i + 1 : w.kvn, 0);
-  const int parts = seq_uni(min(w.cut.parts, seq_ceil(min(sees, w.keys), w.cut.part_keys)));  // those the row sees
+  int parts = w.cut.parts;  // those the row sees
+  while (parts > 0 && (parts - 1) * w.cut.part_keys >= sees) --parts;
   const char* ml = first + (uint32_t)(w.cut.unit_rows * HD + ru) * 4u;
   const uint32_t lo = (uint32_t)w.cut.unit_rows * 4u, po = (uint32_t)(ru * HD + (tid % LPR) * 4) * 4u;
   auto f32_at = [](const char* base, uint32_t off) { return *reinterpret_cast<const float*>(base + off); };
@@ -964,16 +971,16 @@ __global__ __launch_bounds__(256, 4) void seq_attn_join_kernel(SeqAttnArgs a) {
   walk.init(a.s, sh, true, seqs[seq_uni((int)(threadIdx.x >> 6))]);
   SeqWork w;
   for (int i = blockIdx.x; walk.find(a.s, sh, true, i, w); i += gridDim.x) {
-    const int rows = w.qn * a.group, all = rows * a.kv_heads;
+    const int all = w.qn * a.heads;
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // as in seq_attn_paged_kernel
     if (w.cut.parts <= SEQ_WAVE_PARTS) {
       const int u = (i - w.item) * 4 + seq_uni((int)(threadIdx.x >> 6));
-      const int hk = seq_uni(u / rows);
-      if (u < all) sq_join_row<T, HD, true>(a, w, hk, u - hk * rows, tid, red);
+      const int r = seq_uni(seq_div(u, a.by_kv_heads));
+      if (u < all) sq_join_row<T, HD, true>(a, w, u - r * a.kv_heads, r, tid, red);
     } else {
-      const int u = i - w.item, hk = seq_uni(u / rows);
-      sq_join_row<T, HD, false>(a, w, hk, u - hk * rows, tid, red);
+      const int u = i - w.item, r = seq_uni(seq_div(u, a.by_kv_heads));
+      sq_join_row<T, HD, false>(a, w, u - r * a.kv_heads, r, tid, red);
     }
   }
 }
@@ -988,8 +995,7 @@ static SqBounds sq_bounds(const SeqAttnArgs& a) {
   const int64_t rows = (int64_t)a.s.tokens * a.group, cap = (int64_t)a.s.max_pages << a.s.page_log2;
   const int64_t hk = a.kv_heads, cus = a.cus;
   auto least = [](int64_t x, int64_t y) { return x < y ? x : y; };
-  const int64_t few_most = cus / hk < 1 ? 1 : cus / hk;
-  const int64_t few_parts = least((cap + SEQ_PART_FEW - 1) / SEQ_PART_FEW, few_most);
+  const int64_t few_parts = least((cap + SEQ_PART_FEW - 1) / SEQ_PART_FEW, a.few_parts);
   const int64_t few_tiles = a.few ? rows / a.few + a.s.batch : a.s.batch;
   SqBounds b;
   b.items = few_tiles * hk * few_parts;
@@ -1011,6 +1017,7 @@ static void sq_finish(SeqAttnArgs& a) {
   const int cus = device_cu_count();
   a.cus = cus > 0 ? cus : 256;
   if (a.cus > 256) a.cus = 256;  // the join holds one part a thread
+  a.few_parts = a.cus / a.kv_heads < 1 ? 1 : a.cus / a.kv_heads;
   a.few = 0;
   const int64_t most = a.max_q_len * a.group;
   // Calls of few-row sequences only; where their tiles could pass 32-bit
@@ -1027,6 +1034,8 @@ int64_t seq_attention_workspace(const SeqAttnArgs& a0) {
 template <typename T, int HD>
 static int launch_hd(SeqAttnArgs a, hipStream_t st) {
   const dim3 block(SQ_THREADS);
+  a.by_group = seq_div_by(a.group);
+  a.by_kv_heads = seq_div_by(a.kv_heads);
   if (!a.paged) {
     const SeqOrder o = seq_order(a.s, a.group, SQ_ROWS, (int64_t)a.s.tokens * a.kv_heads * HD * 4);
     seq_attn_packed_kernel<T, HD><<<dim3((unsigned)seq_order_grid(o, a.kv_heads)), block, 0, st>>>(a, o);
@@ -1041,7 +1050,7 @@ static int launch_hd(SeqAttnArgs a, hipStream_t st) {
   else seq_attn_paged_kernel<T, HD, false><<<grid(b.items, resident), block, 0, st>>>(a);
   if (hipGetLastError() != hipSuccess) return TX_EHIP;
   if (b.units > 0) {
-    seq_attn_join_kernel<T, HD><<<grid(b.join_rows, 16 * a.cus), block, 0, st>>>(a);
+    seq_attn_join_kernel<T, HD><<<grid(b.join_rows, 4 * a.cus), block, 0, st>>>(a);
     if (hipGetLastError() != hipSuccess) return TX_EHIP;
   }
   return TX_OK;

@@ -30,6 +30,10 @@ __device__ __forceinline__ int seq_cut(int x, int lo, int hi) { return x < lo ? 
 // quotients are formed there), moved to a scalar one.
 __device__ __forceinline__ int seq_uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+__device__ __forceinline__ int seq_div(int x, const SeqDiv& d) {
+  return (int)((__umulhi((uint32_t)x, d.m) + (uint32_t)x) >> d.s);
+}
+
 // The sequence and tile with index w: the largest b with first_tile(b) <= w,
 // found by the whole wave, 64 candidates at a time (two rounds of loads up to
 // 4096 sequences).  Wave-uniform; every lane takes part.
@@ -150,6 +154,7 @@ constexpr int SEQ_WAVE_PARTS = 16;  // rows of up to so many parts are joined by
 
 struct SeqShape {
   int group, kv_heads, cus;
+  int few_parts;  // most parts of few-row items
   int few;  // rows of a tile when the call has few-row items only (<= SEQ_FEW), else 0
 };
 struct SeqCut {
@@ -162,10 +167,10 @@ __host__ __device__ inline SeqCut seq_cut_of(const SeqShape& s, int rows, int ke
   SeqCut c;
   c.few = s.few > 0 || rows <= SEQ_FEW;
   c.unit_rows = s.few > 0 ? s.few : SEQ_FEW;
-  c.tiles = seq_ceil(rows, c.few ? c.unit_rows : SEQ_TILE);
+  c.tiles = rows <= c.unit_rows ? 1 : (c.few ? seq_ceil(rows, c.unit_rows) : seq_ceil(rows, SEQ_TILE));
   int most, step;
   if (c.few) {
-    most = s.cus / s.kv_heads;
+    most = s.few_parts;
     step = SEQ_PART_FEW;
   } else {
     most = seq_ceil(2 * s.cus, c.tiles * s.kv_heads);
@@ -196,8 +201,9 @@ struct SeqWalk {
     int n_items, n_units;    // of this lane's sequence
     int at_item, at_unit;    // behind its last item and unit (from base on)
     int q0, qn, kvn;
+    int tiles, parts, part_keys;
   };
-  static constexpr int LDS_INTS = 64 * 7;  // per wave
+  static constexpr int LDS_INTS = 64 * 10;  // per wave
   int base, items, units;  // before sequence base
   int row;                 // first row that sequence base may hold
   int* lds;                // this wave's LDS_INTS
@@ -215,11 +221,14 @@ struct SeqWalk {
     const int n = min(s.batch - base, 64);  // the scans need log2(n) steps
     for (int o = 1; o < n; o <<= 1) x.q0 = max(x.q0, __shfl_up(x.q0, o, 64));  // (lanes below o see themselves)
     x.qn = max(end - x.q0, 0);
-    x.n_items = x.n_units = 0;
+    x.n_items = x.n_units = x.tiles = x.parts = x.part_keys = 0;
     if (x.qn > 0) {
       const SeqCut c = seq_cut_of(sh, x.qn * sh.group, min(x.kvn, s.max_pages << s.page_log2));
       x.n_items = c.tiles * c.parts * sh.kv_heads;
       x.n_units = x.n_items * c.units;
+      x.tiles = c.tiles;
+      x.parts = c.parts;
+      x.part_keys = c.part_keys;
       if (join) {  // rows, four to an item where a wave joins one
         const int all = x.qn * sh.group * sh.kv_heads;
         x.n_items = c.parts <= 1 ? 0 : (c.parts <= SEQ_WAVE_PARTS ? seq_ceil(all, 4) : all);
@@ -234,9 +243,9 @@ struct SeqWalk {
         x.at_unit += u;
       }
     }
-    const int f[7] = {x.n_items, x.n_units, x.at_item, x.at_unit, x.q0, x.qn, x.kvn};
+    const int f[10] = {x.n_items, x.n_units, x.at_item, x.at_unit, x.q0, x.qn, x.kvn, x.tiles, x.parts, x.part_keys};
 #pragma unroll
-    for (int i = 0; i < 7; ++i) lds[64 * i + lane] = f[i];
+    for (int i = 0; i < 10; ++i) lds[64 * i + lane] = f[i];
   }
   __device__ __forceinline__ void init(const SeqArgs& s, const SeqShape& sh, bool join, int* lds_) {
     base = items = units = row = 0;
@@ -268,10 +277,12 @@ struct SeqWalk {
     r.item = items + field(2, i) - field(0, i);
     r.unit = units + field(3, i) - field(1, i);
     r.keys = min(r.kvn, s.max_pages << s.page_log2);
-    r.cut = seq_cut_of(sh, r.qn * sh.group, r.keys);
-    r.cut.tiles = seq_uni(r.cut.tiles);
-    r.cut.parts = seq_uni(r.cut.parts);
-    r.cut.part_keys = seq_uni(r.cut.part_keys);
+    r.cut.few = sh.few > 0 || r.qn * sh.group <= SEQ_FEW;
+    r.cut.unit_rows = sh.few > 0 ? sh.few : SEQ_FEW;
+    r.cut.tiles = field(7, i);
+    r.cut.parts = field(8, i);
+    r.cut.part_keys = field(9, i);
+    r.cut.units = r.cut.parts > 1 ? (r.cut.few ? 1 : SEQ_TILE / SEQ_FEW) : 0;
     return true;
   }
 };

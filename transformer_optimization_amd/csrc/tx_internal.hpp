@@ -74,6 +74,18 @@ struct AttnArgs {
   float* row_stats;   // eager mode: [B*H*S][2] (max, sum) workspace
 };
 
+// x / d for 0 <= x < 2^31 and a d that only the call knows: (mulhi(x, m) + x)
+// >> s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1.
+struct SeqDiv {
+  uint32_t d, m, s;
+};
+inline SeqDiv seq_div_by(int d) {
+  SeqDiv v{(uint32_t)d, 0, 0};
+  while (((uint64_t)1 << v.s) < (uint64_t)d) ++v.s;
+  v.m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << v.s) - (uint64_t)d)) / (uint64_t)d + 1);
+  return v;
+}
+
 // Packed sequences and a paged cache (tx_api.h).  Strides in elements: st per
 // token (or slot), sh per head, sp per page.
 struct SeqArgs {
@@ -112,11 +124,13 @@ struct SeqAttnArgs {
   int64_t q_st, q_sh, o_st, o_sh;
   int64_t k_sp, k_sh, k_st, v_sp, v_sh, v_st;
   int heads, kv_heads, group, head_dim;
+  SeqDiv by_group, by_kv_heads;
   float scale;
   int causal;
   int paged;
   int64_t max_q_len;
   int few;   // rows of a tile where every sequence has few rows (seq_common.hpp), else 0
+  int few_parts;  // most parts of the keys of such rows
   int cus;
   float* ws;
 };
