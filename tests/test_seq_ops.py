@@ -726,6 +726,27 @@ def test_one_captured_step_serves_other_lengths(cuda):
 
 
 @gpu
+def test_recorded_launches_run_again(cuda):
+    dtype, hd, h, hk = torch.bfloat16, 64, 4, 2
+    ks, vs, kc, vc, table = _paged([900, 30], hk, 16, hd, dtype, cuda, 160)
+    cu, kvl = _cu([2, 5], cuda), _i32([900, 30], cuda)
+    x = _randn((7, h + 2 * hk, hd), dtype, cuda, 161)
+    q, k, v = x[:, :h], x[:, h:h + hk], x[:, h + hk:]
+    steps, _ = _C.rotary_steps(hd, device=cuda)
+    with _C.record_launches() as calls:
+        outs = [_C.rotary_append(q, k, None, steps, cu)[0], _C.flash_attn_packed(q, k, v, cu, 0.1, True),
+                _C.flash_attn_paged(q, kc, vc, table, cu, kvl, 0.1)]
+    assert [c.info["op"] for c in calls] == ["rotary_append", "flash_attn_packed", "flash_attn_paged"]
+    want = [o.clone() for o in outs]
+    for o in outs:
+        o.zero_()
+    for c in calls:
+        c()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+@gpu
 def test_calls_on_two_streams_at_once(cuda):
     dtype, hd, h, hk = torch.float16, 64, 8, 2
     ks, vs, kc, vc, table = _paged([5000, 400], hk, 32, hd, dtype, cuda, 130)
