@@ -640,7 +640,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
       const int key = min(kb + 16 * x + col, lim - 1);
       const char* row = (const char*)hp.k + (uint64_t)page_of(p.k[x], key) * k_sp + ((uint32_t)(key & ps1) * k_st + 16u * g);
 #pragma unroll
-      for (int ks = 0; ks < HD / 32; ++ks) kr[x][ks] = ld128(row + 64 * ks);
+      for (int ks = 0; ks < HD / 32; ++ks) kr[x][ks] = ld128_once(row + 64 * ks);
     }
   };
   auto load_v = [&](int kb, const Pages& p) {
@@ -648,7 +648,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
     const char* row = (const char*)hp.v + (uint64_t)page_of(p.v, key) * v_sp +
                       ((uint32_t)(key & ps1) * v_st + 16u * (lane % F::CH));
 #pragma unroll
-    for (int x = 0; x < F::LDV; ++x) vr[x] = ld128(row + (uint32_t)min(x, left) * v_st);
+    for (int x = 0; x < F::LDV; ++x) vr[x] = ld128_once(row + (uint32_t)min(x, left) * v_st);
   };
   T* vs = lds + wave * F::WAVE_ELEMS;
   const uint32_t vbase = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) T*)vs;
@@ -740,7 +740,8 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   __syncthreads();
   if (bad_from < cap) atomicMin(bad, bad_from);
 #pragma unroll
-  for (int d = 0; d < HD / 16; ++d) *reinterpret_cast<f32x4*>(ow + col * HD + 16 * d + 4 * g) = o[d];
+  // (4-value chunks xor the row: 16 rows at one chunk would share 4 banks)
+  for (int d = 0; d < HD / 16; ++d) *reinterpret_cast<f32x4*>(ow + col * HD + 4 * ((4 * d + g) ^ col)) = o[d];
   if (g == 0) {
     sm[col] = m_run;
     sl[col] = lsum[0];
@@ -769,7 +770,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   for (int y = 0; y < DT / 4; ++y) {
     f32x4 ov[4];  // a wave without keys for the row left 0 here, its weight is 0 too
 #pragma unroll
-    for (int x = 0; x < 4; ++x) ov[x] = *reinterpret_cast<const f32x4*>((const float*)lds + (x * 16 + row) * HD + 64 * y + d0);
+    for (int x = 0; x < 4; ++x) ov[x] = *reinterpret_cast<const f32x4*>((const float*)lds + (x * 16 + row) * HD + 64 * y + (d0 ^ 4 * row));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float v = 0.f;

