@@ -555,22 +555,33 @@ __global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_packed_kernel(SeqAttnA
 // -------------------------------------------------------------- few rows
 // Up to 16 rows (one token's query heads of a K/V head, or a few tokens')
 // against one part of the keys: bound by reading K and V once.  Each of the 4
-// waves takes blocks of 32 keys by itself, no barrier between them: K rows
-// straight into the MFMA A operand (16 keys x 32 dims), V rows into registers
-// and through a wave's own LDS (transposing reads) into the A operand of o^T +=
-// V^T P^T; the loads of the next block are in flight while one is worked on.
-// S^T leaves lane l the keys 4 (l >> 4) .. + 3 of both 16-key halves of row l &
-// 15, which is a P operand as it stands if V's rows are taken in that order.
-// The waves' results meet in LDS at the end.
+// waves takes blocks of 32 keys by itself, no barrier between them.  Its K and
+// V rows come by DMA, whole rows a wave instruction (loads in the order of the
+// MFMA operand, 16 rows x 64 bytes, reach 5.9 TB/s where whole rows reach 6.8),
+// into the wave's own LDS; K is read as the A operand of S^T = K Q^T (16 keys
+// x 32 dims), V transposed as that of o^T += V^T P^T.  K's rows are replaced by
+// the next block's once its scores are formed, V's once it is used, so that a
+// block's 2 x 64 HD bytes are in flight nearly all the time in each of the 8
+// waves of a CU (16 at head dim 64).  S^T leaves lane l the keys 4 (l >> 4)
+// .. + 3 of both 16-key halves of row l & 15, which is a P operand as it stands
+// if V's rows are taken in that order.  The waves' results meet in LDS at the
+// end.
 template <typename T, int HD>
 struct SqFew {
   typedef typename Mfma16<T>::vec vec;
-  static constexpr int CH = HD / 8, RPI = 64 / CH, LDV = 32 / RPI;  // V loads per block and lane
-  static constexpr int WAVE_ELEMS = 32 * HD;                        // V block; o of 16 rows in fp32
+  static constexpr int CH = HD / 8, RPI = 64 / CH, LDB = 32 / RPI;  // rows per instruction, instructions per block
+  static constexpr int ELEMS = 32 * HD;                             // a block of K or V; o of 16 rows in fp32
+  static constexpr int WAVE_ELEMS = 2 * ELEMS;
   static constexpr float BIAS = SqTile<T, HD, true>::BIAS;
-  // Chunk swizzle of the V block: the 32 lanes of one transposing read cover
-  // 8 keys (4 of each of two 16-lane groups) x 32 bytes.
-  static __device__ __forceinline__ int swz(int key) { return HD == 128 ? (key & 7) << 1 : ((key >> 1) & 3) << 1; }
+  // Instruction x moves the keys LDB (lane / CH) + x, so that a lane's keys lie
+  // in one page (LDB divides 8); they land at LDS row x RPI + lane / CH.  The
+  // 16-byte chunks of a key are xor-ed for the reads: 16 keys at one chunk (K),
+  // 8 keys x 32 bytes (V) fall on different banks.
+  static __device__ __forceinline__ int lds_row(int key) { return key % LDB * RPI + key / LDB; }
+  static __device__ __forceinline__ int kswz(int key) {
+    return HD == 128 ? key & 15 : (key & 3) | ((key >> 1) & 4);
+  }
+  static __device__ __forceinline__ int vswz(int key) { return HD == 128 ? (key & 7) << 1 : (key & 3) << 1; }
 };
 
 template <typename T, int HD>
@@ -611,71 +622,54 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   float m_run = NEG_INF, mc = 0.f;
   int bad_from = cap;
 
-  // A lane's rows of a block: for K keys col and 16 + col, for V LDV
-  // consecutive ones (of one page: LDV divides 8).  Keys past the last re-read
-  // the last.  Page and slot parts of an address are 32 x 32 -> 64 bit products
-  // (the entry point bounds the strides).
-  const uint32_t k_sp = (uint32_t)(a.k_sp * 2), v_sp = (uint32_t)(a.v_sp * 2);
-  const uint32_t k_st = (uint32_t)(a.k_st * 2), v_st = (uint32_t)(a.v_st * 2);
-  struct Pages {
-    int k[2], v;
-  };
-  auto vrow0 = [&](int kb) { return min(kb + lane / F::CH * F::LDV, (lim - 1) & ~(F::LDV - 1)); };
-  auto lookup = [&](int kb) {
-    Pages p;
-    p.k[0] = table[min(kb + col, lim - 1) >> a.s.page_log2];
-    p.k[1] = table[min(kb + 16 + col, lim - 1) >> a.s.page_log2];
-    p.v = table[vrow0(kb) >> a.s.page_log2];
-    return p;
-  };
-  auto page_of = [&](int p, int key) {  // page 0 in the place of one that is not there
-    if ((uint32_t)p < (uint32_t)a.s.num_pages) return (uint32_t)p;
-    bad_from = min(bad_from, key & ~ps1);
-    return 0u;
-  };
-  u32x4 kr[2][HD / 32], vr[F::LDV];
-  auto load_k = [&](int kb, const Pages& p) {
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int key = min(kb + 16 * x + col, lim - 1);
-      const char* row = (const char*)hp.k + (uint64_t)page_of(p.k[x], key) * k_sp + ((uint32_t)(key & ps1) * k_st + 16u * g);
-#pragma unroll
-      for (int ks = 0; ks < HD / 32; ++ks) kr[x][ks] = ld128_once(row + 64 * ks);
+  // A lane's keys of a block.  Keys past the last re-read the last.  Page and
+  // slot parts of an address are 32 x 32 -> 64 bit products (the entry point
+  // bounds the strides).
+  auto key0 = [&](int kb) { return min(kb + lane / F::CH * F::LDB, (lim - 1) & ~(F::LDB - 1)); };
+  auto lookup = [&](int kb) { return (uint32_t)table[key0(kb) >> a.s.page_log2]; };
+  T* ks = lds + wave * F::WAVE_ELEMS;
+  T* vs = ks + F::ELEMS;
+  auto load = [&](int kb, uint32_t page, T* to, const T* head, int64_t sp, int64_t st, auto swz) {
+    const int key = key0(kb), left = lim - 1 - key;
+    if (page >= (uint32_t)a.s.num_pages) {  // page 0 in the place of one that is not there
+      bad_from = min(bad_from, key & ~ps1);
+      page = 0;
     }
-  };
-  auto load_v = [&](int kb, const Pages& p) {
-    const int key = vrow0(kb), left = lim - 1 - key;
-    const char* row = (const char*)hp.v + (uint64_t)page_of(p.v, key) * v_sp +
-                      ((uint32_t)(key & ps1) * v_st + 16u * (lane % F::CH));
+    const uint32_t row_bytes = (uint32_t)(st * 2);
+    const char* row = (const char*)head + (uint64_t)page * (uint32_t)(sp * 2) + (uint32_t)(key & ps1) * row_bytes;
 #pragma unroll
-    for (int x = 0; x < F::LDV; ++x) vr[x] = ld128_once(row + (uint32_t)min(x, left) * v_st);
+    for (int x = 0; x < F::LDB; ++x)
+      dma16_once(row + (uint32_t)min(x, left) * row_bytes + 16u * ((lane % F::CH) ^ swz(lane / F::CH * F::LDB + x)),
+                 to + x * F::RPI * HD);
   };
-  T* vs = lds + wave * F::WAVE_ELEMS;
+  auto load_k = [&](int kb, uint32_t page) { load(kb, page, ks, hp.k, a.k_sp, a.k_st, F::kswz); };
+  auto load_v = [&](int kb, uint32_t page) { load(kb, page, vs, hp.v, a.v_sp, a.v_st, F::vswz); };
   const uint32_t vbase = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) T*)vs;
   // Transposing reads: lane j of a 16-lane group g addresses key 4 g + j / 4
   // (and + 16) at dims 16 d + 4 (j % 4) and receives dim 16 d + j of 4 keys.
   const int vkey = 4 * g + (col >> 2);
-  const uint32_t vrow = vbase + (uint32_t)(vkey * HD * 2 + (col & 1) * 8);
-  const int vx = (col & 3) >> 1, vsw = F::swz(vkey);
-  // One block: its V rows move to LDS and its scores are formed, each followed
-  // at once by the loads of the block after it into the same registers.
-  auto compute = [&](int kb, const Pages& pages, bool more) {
-#pragma unroll
-    for (int x = 0; x < F::LDV; ++x) {
-      const int i = lane / F::CH * F::LDV + x;
-      st128(vs + i * HD + (((lane % F::CH) ^ F::swz(i)) << 3), vr[x]);
-    }
-    if (more) load_v(kb + 128, pages);
+  const uint32_t vrow = vbase + (uint32_t)(F::lds_row(vkey) * HD * 2 + (col & 1) * 8);
+  const int vx = (col & 3) >> 1, vsw = F::vswz(vkey);
+  const T* krow = ks + F::lds_row(col) * HD;
+  const int ksw = F::kswz(col);
+  auto compute = [&](int kb, uint32_t page, bool more) {
+    // This block's K rows are there: only its V rows may still be on the way
+    // (a page lookup among them makes the wait stricter).
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(F::LDB) : "memory");
     float s[8];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ks = 0; ks < HD / 32; ++ks) acc = Mfma16<T>::mma(__builtin_bit_cast(vec, kr[x][ks]), qf[ks], acc);
+      for (int i = 0; i < HD / 32; ++i)
+        acc = Mfma16<T>::mma(__builtin_bit_cast(vec, ld128(krow + 16 / F::LDB * x * HD + (((4 * i + g) ^ ksw) << 3))), qf[i], acc);
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[4 * x + e] = (kb + 16 * x + 4 * g + e < mylim) ? acc[e] : NEG_INF;
     }
-    if (more) load_k(kb + 128, pages);
+    if (more) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read
+      load_k(kb + 128, page);
+    }
     float mx = NEG_INF;
 #pragma unroll
     for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e]);
@@ -697,9 +691,9 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
     const vec pf = __builtin_bit_cast(vec, u32x4{pack2_raw<T>(p[0], p[1]), pack2_raw<T>(p[2], p[3]),
                                                  pack2_raw<T>(p[4], p[5]), pack2_raw<T>(p[6], p[7])});
     lsum = Mfma16<T>::mma(ones, pf, lsum);
-    // The block's rows are in LDS before the reads (the compiler does not see
-    // that they read it), and the reads are done before the next block's.
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // This block's V rows: only the next one's K may still be on the way.
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(F::LDB) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int d4 = 0; d4 < HD / 64; ++d4) {
       u32x4 vop[4];
@@ -708,31 +702,31 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
         const uint32_t at = vrow + (uint32_t)((((2 * (4 * d4 + i)) ^ vsw) + vx) << 4);
         u32x2 lo, hi;
         asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo) : "v"(at));
-        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(hi) : "v"(at), "n"(16 * HD * 2));
+        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(hi) : "v"(at), "n"(16 / F::LDB * HD * 2));
         vop[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
       ax_vnat_wait<4>(vop);
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[4 * d4 + i] = Mfma16<T>::mma(__builtin_bit_cast(vec, vop[i]), pf, o[4 * d4 + i]);
     }
-    asm volatile("" ::: "memory");
+    if (more) load_v(kb + 128, page);  // (every read above has been waited for)
   };
 
   const int first = j0 + 32 * wave;
   if (first < lim) {
-    Pages pages = lookup(first), next = lookup(first + 128);
-    load_v(first, pages);
-    load_k(first, pages);
+    uint32_t page = lookup(first), next = lookup(first + 128);
+    load_k(first, page);
+    load_v(first, page);
     for (int kb = first; kb < lim; kb += 128) {
-      pages = next;
+      page = next;
       next = lookup(kb + 256);
-      compute(kb, pages, kb + 128 < lim);
+      compute(kb, page, kb + 128 < lim);
     }
   }
 
-  // Join the waves: o in fp32 over each wave's V block, m and l beside it.
+  // Join the waves: o in fp32 over each wave's K block, m and l beside it.
   if (threadIdx.x == 0) *bad = cap;
-  float* ow = (float*)lds + wave * 16 * HD;
+  float* ow = (float*)ks;
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   float* sm = stat + wave * 16;
   float* sl = stat + 64 + wave * 16;
@@ -770,7 +764,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   for (int y = 0; y < DT / 4; ++y) {
     f32x4 ov[4];  // a wave without keys for the row left 0 here, its weight is 0 too
 #pragma unroll
-    for (int x = 0; x < 4; ++x) ov[x] = *reinterpret_cast<const f32x4*>((const float*)lds + (x * 16 + row) * HD + 64 * y + (d0 ^ 4 * row));
+    for (int x = 0; x < 4; ++x) ov[x] = *reinterpret_cast<const f32x4*>((const float*)(lds + x * F::WAVE_ELEMS) + row * HD + 64 * y + (d0 ^ 4 * row));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float v = 0.f;
@@ -822,7 +816,7 @@ __host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
 // Persistent workgroups over the items of a call (SeqWalk); a grid of at most
 // the items, so every workgroup's loop ends.
 template <typename T, int HD, bool FEW_ONLY>
-__global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_paged_kernel(SeqAttnArgs a) {
+__global__ __launch_bounds__(SQ_THREADS, FEW_ONLY && HD == 64 ? 4 : 2) void seq_attn_paged_kernel(SeqAttnArgs a) {
   constexpr int TILE_ELEMS = SqTile<T, HD, true>::LDS_ELEMS, FEW_ELEMS = 4 * SqFew<T, HD>::WAVE_ELEMS;
   constexpr int ELEMS = FEW_ONLY || FEW_ELEMS > TILE_ELEMS ? FEW_ELEMS : TILE_ELEMS;
   __shared__ __attribute__((aligned(16))) T lds[ELEMS];
@@ -830,9 +824,9 @@ __global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_paged_kernel(SeqAttnAr
   __shared__ int bad[4];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const SeqShape sh = sq_shape(a);
-  __shared__ int seqs[4][SeqWalk::LDS_INTS];
+  __shared__ int seqs[SeqWalk::LDS_INTS];
   SeqWalk walk;
-  walk.init(a.s, sh, false, seqs[wave]);
+  walk.init(a.s, sh, false, seqs);
   SeqWork w;
   for (int i = blockIdx.x; walk.find(a.s, sh, false, i, w); i += gridDim.x) {
     // An item's lane constants are formed within it: held across the items
@@ -967,9 +961,9 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256, 4) void seq_attn_join_kernel(SeqAttnArgs a) {
   __shared__ __attribute__((aligned(16))) float red[256][4];
   const SeqShape sh = sq_shape(a);
-  __shared__ int seqs[4][SeqWalk::LDS_INTS];
+  __shared__ int seqs[SeqWalk::LDS_INTS];
   SeqWalk walk;
-  walk.init(a.s, sh, true, seqs[seq_uni((int)(threadIdx.x >> 6))]);
+  walk.init(a.s, sh, true, seqs);
   SeqWork w;
   for (int i = blockIdx.x; walk.find(a.s, sh, true, i, w); i += gridDim.x) {
     const int all = w.qn * a.heads;
@@ -1045,10 +1039,10 @@ static int launch_hd(SeqAttnArgs a, hipStream_t st) {
   sq_finish(a);
   const SqBounds b = sq_bounds(a);
   auto grid = [](int64_t items, int64_t most) { return dim3((unsigned)(items < most ? items : most)); };
-  // Resident workgroups: 3 to a CU at head dim 64 (133 and 157 registers), 2 at 128.
-  const int64_t resident = (HD == 64 ? 3 : 2) * a.cus;
-  if (a.few) seq_attn_paged_kernel<T, HD, true><<<grid(b.items, resident), block, 0, st>>>(a);
-  else seq_attn_paged_kernel<T, HD, false><<<grid(b.items, resident), block, 0, st>>>(a);
+  // As many workgroups as are resident: few rows 4 a CU at head dim 64 and 2 at
+  // 128, tiles 3 and 2.
+  if (a.few) seq_attn_paged_kernel<T, HD, true><<<grid(b.items, (HD == 64 ? 4 : 2) * a.cus), block, 0, st>>>(a);
+  else seq_attn_paged_kernel<T, HD, false><<<grid(b.items, (HD == 64 ? 3 : 2) * a.cus), block, 0, st>>>(a);
   if (hipGetLastError() != hipSuccess) return TX_EHIP;
   if (b.units > 0) {
     seq_attn_join_kernel<T, HD><<<grid(b.join_rows, 4 * a.cus), block, 0, st>>>(a);

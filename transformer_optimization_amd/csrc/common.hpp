@@ -101,11 +101,6 @@ __device__ __forceinline__ int mfma32_row(int r, int lane) {
 __device__ __forceinline__ u32x4 ld128(const void* p) {
   return *reinterpret_cast<const u32x4*>(p);
 }
-// The same for data that this kernel reads once (not kept in the caches on its
-// way): a large read runs at 7.1 instead of 6.3 TB/s.
-__device__ __forceinline__ u32x4 ld128_once(const void* p) {
-  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-}
 __device__ __forceinline__ void st128(void* p, u32x4 v) { *reinterpret_cast<u32x4*>(p) = v; }
 __device__ __forceinline__ u32x2 ld64(const void* p) {
   return *reinterpret_cast<const u32x2*>(p);
@@ -187,6 +182,14 @@ __device__ __forceinline__ void dma16(const void* g, const void* lds) {
       (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
   // M0 holds the LDS address; the nop covers the M0-write -> LDS-DMA hazard.
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(g), "{m0}"(l) : "memory");
+}
+
+// The same for data that is read once (not kept in the caches on its way): a
+// large read runs at 7.1 instead of 6.3 TB/s.
+__device__ __forceinline__ void dma16_once(const void* g, const void* lds) {
+  const uint32_t l = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(g), "{m0}"(l) : "memory");
 }
 
 // The same with a wave-uniform base address (SGPR pair) and a 32-bit byte

@@ -193,9 +193,10 @@ struct SeqWork {
 };
 
 // Walks the items of a call in ascending order, 64 sequences at a time (lane
-// i: sequence base + i); every lane of the wave takes part.  What the lanes
-// hold of their sequences stays in LDS between the items, whose own work needs
-// the registers.
+// i: sequence base + i).  Every wave of the workgroup walks the same items and
+// every lane takes part.  What the lanes hold of their sequences stays in LDS
+// between the items, whose own work needs the registers: one copy, which each
+// wave writes alike between two barriers.
 struct SeqWalk {
   struct Lane {
     int n_items, n_units;    // of this lane's sequence
@@ -203,10 +204,10 @@ struct SeqWalk {
     int q0, qn, kvn;
     int tiles, parts, part_keys;
   };
-  static constexpr int LDS_INTS = 64 * 10;  // per wave
+  static constexpr int LDS_INTS = 64 * 10;
   int base, items, units;  // before sequence base
   int row;                 // first row that sequence base may hold
-  int* lds;                // this wave's LDS_INTS
+  int* lds;                // LDS_INTS of the workgroup
 
   __device__ __forceinline__ void load(const SeqArgs& s, const SeqShape& sh, bool join) {
     const int lane = threadIdx.x & 63, b = base + lane;
@@ -243,16 +244,18 @@ struct SeqWalk {
         x.at_unit += u;
       }
     }
+    __syncthreads();  // nobody reads the sequences before these any more
     const int f[10] = {x.n_items, x.n_units, x.at_item, x.at_unit, x.q0, x.qn, x.kvn, x.tiles, x.parts, x.part_keys};
 #pragma unroll
     for (int i = 0; i < 10; ++i) lds[64 * i + lane] = f[i];
+    __syncthreads();
   }
   __device__ __forceinline__ void init(const SeqArgs& s, const SeqShape& sh, bool join, int* lds_) {
     base = items = units = row = 0;
     lds = lds_;
     load(s, sh, join);
   }
-  // Field f of the Lane of sequence base + i (one wave's own LDS: in order).
+  // Field f of the Lane of sequence base + i.
   __device__ __forceinline__ int field(int f, int i) const { return seq_uni(lds[64 * f + i]); }
   // The sequence of item w (ascending from call to call); false: past the end.
   __device__ __forceinline__ bool find(const SeqArgs& s, const SeqShape& sh, bool join, int w, SeqWork& r) {
