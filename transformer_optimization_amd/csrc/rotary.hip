@@ -48,8 +48,8 @@ __device__ __forceinline__ void ra_turn_half(u32x4& x1, u32x4& x2, const float2*
 }
 
 // VEC: the rotated part splits into whole 16-byte chunks (rotary % 16 == 0 in
-// the half layout, % 8 == 0 interleaved); otherwise one pair or one element
-// per thread.
+// the half layout, % 8 == 0 interleaved); otherwise it is turned pair by pair,
+// and only what follows the next multiple of 8 moves in chunks.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(RA_THREADS) void rotary_append_kernel(RotaryArgs a) {
   __shared__ float2 cs[RA_TOKENS][128];
@@ -71,15 +71,14 @@ __global__ __launch_bounds__(RA_THREADS) void rotary_append_kernel(RotaryArgs a)
   }
   __syncthreads();
 
-  // Units of one head: pairs of chunks (half layout), chunks (interleaved and
-  // the rest of a head), or pairs and elements when not VEC.
-  const int turn_units = VEC ? (a.interleaved ? a.rotary >> 3 : a.rotary >> 4) : half;
-  const int rest_units = VEC ? (hd - a.rotary) >> 3 : hd - a.rotary;
-  const int units = turn_units + rest_units, v_units = VEC ? hd >> 3 : hd;
-  const int qh = a.q ? H : 0, kh = HK, vh = a.k_cache ? HK : 0;
-  const int per_token = (qh + kh) * units + vh * v_units;
+  // Units of a head of q and k: turn_units turns (a pair of chunks in the half
+  // layout, a chunk interleaved, a pair of elements when not VEC), single_units
+  // elements up to the next whole chunk, then chunks; of v: chunks.
+  const int units = a.units, v_units = hd >> 3;
+  const int qh = a.q ? H : 0;
+  const int qk_units = (qh + HK) * units, per_token = (int)a.by_token.d;
   for (int i = tid; i < n * per_token; i += RA_THREADS) {
-    const int tt = i / per_token;
+    const int tt = seq_div(i, a.by_token);
     int u = i - tt * per_token;
     const int64_t row = t.q0 + r0 + tt;
     const int key = key0 + tt;
@@ -87,19 +86,15 @@ __global__ __launch_bounds__(RA_THREADS) void rotary_append_kernel(RotaryArgs a)
     const T* src;
     T* dst0 = nullptr;
     T* dst1 = nullptr;
-    bool is_v = false;
-    if (u < qh * units) {
-      const int h = u / units;
-      u -= h * units;
+    const bool is_v = u >= qk_units;
+    if (is_v) u -= qk_units;
+    int h = seq_div(u, is_v ? a.by_v_units : a.by_units);
+    u -= h * (is_v ? v_units : units);
+    if (!is_v && h < qh) {
       src = (const T*)a.q + row * a.q_st + h * a.q_sh;
       dst0 = (T*)a.q_out + row * a.qo_st + h * a.qo_sh;
     } else {
-      u -= qh * units;
-      is_v = u >= kh * units;
-      if (is_v) u -= kh * units;
-      const int per = is_v ? v_units : units;
-      const int h = u / per;
-      u -= h * per;
+      if (!is_v) h -= qh;
       src = is_v ? (const T*)a.v + row * a.v_st + h * a.v_sh : (const T*)a.k + row * a.k_st + h * a.k_sh;
       if (!is_v && a.k_out) dst0 = (T*)a.k_out + row * a.ko_st + h * a.ko_sh;
       if (a.k_cache) {
@@ -110,13 +105,15 @@ __global__ __launch_bounds__(RA_THREADS) void rotary_append_kernel(RotaryArgs a)
       }
       if (!dst0 && !dst1) continue;
     }
+    if (is_v || u >= a.turn_units + (VEC ? 0 : a.single_units)) {
+      const int d = is_v ? u * 8 : a.rotary + (VEC ? 0 : a.single_units) + (u - a.turn_units - (VEC ? 0 : a.single_units)) * 8;
+      const u32x4 x = ld128(src + d);
+      if (dst0) st128(dst0 + d, x);
+      if (dst1) st128(dst1 + d, x);
+      continue;
+    }
     if constexpr (VEC) {
-      if (is_v || u >= turn_units) {
-        const int d = is_v ? u * 8 : a.rotary + (u - turn_units) * 8;
-        const u32x4 x = ld128(src + d);
-        if (dst0) st128(dst0 + d, x);
-        if (dst1) st128(dst1 + d, x);
-      } else if (a.interleaved) {
+      if (a.interleaved) {
         const u32x4 x = ra_turn_interleaved<T>(ld128(src + u * 8), &cs[tt][u * 4]);
         if (dst0) st128(dst0 + u * 8, x);
         if (dst1) st128(dst1 + u * 8, x);
@@ -132,8 +129,8 @@ __global__ __launch_bounds__(RA_THREADS) void rotary_append_kernel(RotaryArgs a)
           st128(dst1 + half + u * 8, x2);
         }
       }
-    } else if (is_v || u >= turn_units) {
-      const int d = is_v ? u : a.rotary + (u - turn_units);
+    } else if (u >= a.turn_units) {
+      const int d = a.rotary + u - a.turn_units;
       const T x = src[d];
       if (dst0) dst0[d] = x;
       if (dst1) dst1[d] = x;
@@ -155,8 +152,15 @@ __global__ __launch_bounds__(RA_THREADS) void rotary_append_kernel(RotaryArgs a)
 }
 
 template <typename T>
-static int launch_typed(const RotaryArgs& a, hipStream_t st) {
+static int launch_typed(RotaryArgs a, hipStream_t st) {
   const bool vec = a.rotary % (a.interleaved ? 8 : 16) == 0;
+  a.single_units = vec ? 0 : (8 - a.rotary % 8) % 8;
+  a.turn_units = vec ? (a.interleaved ? a.rotary >> 3 : a.rotary >> 4) : a.rotary >> 1;
+  a.units = a.turn_units + a.single_units + ((a.head_dim - a.rotary - a.single_units) >> 3);
+  const int v_units = a.head_dim >> 3;
+  a.by_units = seq_div_by(a.units);
+  a.by_v_units = seq_div_by(v_units);
+  a.by_token = seq_div_by(((a.q ? a.heads : 0) + a.kv_heads) * a.units + (a.k_cache ? a.kv_heads * v_units : 0));
   const dim3 grid((unsigned)seq_tiles(a.s, 1, RA_TOKENS)), block(RA_THREADS);
   if (vec) rotary_append_kernel<T, true><<<grid, block, 0, st>>>(a);
   else rotary_append_kernel<T, false><<<grid, block, 0, st>>>(a);

@@ -113,6 +113,9 @@ struct RotaryArgs {
   int heads, kv_heads, head_dim, rotary;
   float amplitude;
   int interleaved;
+  // Work units (rotary.hip): of a head of q or k, of a token; and division by them.
+  int turn_units, single_units, units;
+  SeqDiv by_units, by_v_units, by_token;
 };
 
 struct SeqAttnArgs {
