@@ -242,8 +242,9 @@ int tx_flash_attn_fwd_noalloc(const void* qk, const void* vt, int64_t ldvt, void
  * cut to [0, T]; what a page index outside [0, num_pages), or a kv_lens above max_pages * page_size, would
  * have to read makes the rows that need it NaN, and what it would have to write is dropped.
  * All of it 16 bit (TX_F16, TX_BF16); pointers 16-byte aligned, strides multiples of 8; page_size a power of
- * two of 8 .. 2^15, max_pages * page_size <= 2^30; T <= 2^24, batch <= 2^20, q_heads <= 65535 and
- * T * q_heads <= 2^26.  These entry points have no counterpart in the reference, which has no cache, no positions and pads its batches (TTB:4380-4396).
+ * two of 8 .. 2^15, max_pages * page_size <= 2^30, a cache's page stride below 2^31; T <= 2^24, batch <=
+ * 2^20, q_heads <= 65535, T * q_heads <= 2^26, batch * kv_heads <= 2^23.  These entry points have no
+ * counterpart in the reference, which has no cache and no positions and pads its batches (TTB:4380-4396).
  */
 
 /*

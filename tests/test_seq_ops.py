@@ -211,12 +211,12 @@ SEQ_REFUSALS = [  # of every entry point
     (dict(q=None), E), (dict(cu=None), E), (dict(t=0), E), (dict(b=0), E), (dict(h=0), E), (dict(hk=0), E),
     (dict(hk=3), E), (dict(hd=0), E), (dict(dt=_C.TX_F32), U), (dict(q=FAKE + 2), U), (dict(qs=(516, 64)), U),
     (dict(qs=(512, -64)), E), (dict(t=1 << 25), U), (dict(h=1 << 16, hk=1 << 15), U), (dict(t=1 << 24, h=16), U),
-    (dict(b=1 << 21), U), (dict(cu=FAKE + 1), U),
+    (dict(b=1 << 21), U), (dict(cu=FAKE + 1), U), (dict(t=64, h=1 << 14, hk=1 << 14, b=1 << 10), U),
 ]
 PAGE_REFUSALS = [
     (dict(table=None), E), (dict(kvl=None), E), (dict(np=0), E), (dict(mp=0), E), (dict(ps=0), E), (dict(ps=4), U),
     (dict(ps=24), U), (dict(ps=1 << 16), U), (dict(ld=7), E), (dict(mp=1 << 27, ld=1 << 27), U), (dict(table=FAKE + 2), U),
-    (dict(kcs=(2048, 1024, 60)), U), (dict(kcs=(2048, 1024, -64)), E), (dict(vcs=(2048, 512, 64)), E),
+    (dict(kcs=(2048, 1024, 60)), U), (dict(kcs=(1 << 31, 1024, 64)), U), (dict(vcs=(1 << 30, 1024, 1 << 24)), U), (dict(kcs=(2048, 1024, -64)), E), (dict(vcs=(2048, 512, 64)), E),
     (dict(kcs=(1024, 1024, 64)), E), (dict(kc=(1 << 33) + 8), U), (dict(vc=None), E),
 ]
 
@@ -556,6 +556,83 @@ def test_paged_attention_long_rows(cuda, hd, h, hk, new, keys):
     for b, s in ((0, slice(0, new)), (1, slice(new, new + 1))):
         want, tol = _attend(q[s], ks[b], vs[b], hd**-0.5, True, dtype)
         _same(got[s], want, tol, f"sequence {b}")
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,h,hk", [(1, 8, 2), (3, 4, 4), (60, 8, 2)])
+def test_a_part_of_the_keys_without_a_finite_score_makes_the_row_nan(cuda, hd, new, h, hk):
+    """Keys shared out over the card: one part's keys are all NaN (its largest score is no number), another's
+    scores are all -inf (they weigh nothing)."""
+    dtype, keys = torch.bfloat16, 4096 + new
+    ks, vs, kc, vc, table = _paged([keys], hk, 256, hd, dtype, cuda, 65)
+    q = _randn((new, h, hd), dtype, cuda, 66).abs()
+    args = (table, _cu([new], cuda), _i32([keys], cuda), hd**-0.5)
+    clean_k = kc.clone()
+    kc[int(table[0, 2])] = -3.0e38  # 256 keys: q > 0, so every score is -inf
+    ks[0][512:768] = -3.0e38
+    got = _C.flash_attn_paged(q, kc, vc, *args)
+    keep = [j for j in range(keys) if not 512 <= j < 768]
+    want, tol = _attend(q, ks[0][keep], vs[0][keep], hd**-0.5, True, dtype)
+    _same(got, want, tol, "a part that weighs nothing")
+    for page in (0, 7, 15):
+        kc = clean_k.clone()
+        kc[int(table[0, page])] = math.nan
+        assert bool(torch.isnan(_C.flash_attn_paged(q, kc, vc, *args)).all()), page
+    kc = clean_k.clone()
+    kc[int(table[0, 16]), :, new - 1] = math.nan  # the last key, of the last row alone
+    got = _C.flash_attn_paged(q, kc, vc, *args)
+    assert bool(torch.isnan(got[-1]).all()) and not bool(torch.isnan(got[:-1]).any())
+
+
+@gpu
+@pytest.mark.parametrize("hint", [1, 2, 3])
+def test_paged_attention_with_a_bound_that_is_too_small(cuda, hint):
+    """Slower, but right and within its workspace."""
+    dtype, hd, h, hk = torch.float16, 64, 6, 2
+    new, lens = [40, 1, 7, 200], [900, 300, 7, 1500]
+    ks, vs, kc, vc, table = _paged(lens, hk, 16, hd, dtype, cuda, 68)
+    q = _randn((sum(new), h, hd), dtype, cuda, 69)
+    need = _C.flash_attn_paged_workspace(sum(new), len(new), h, hk, hd, 16, table.shape[1], hint)
+    ws = torch.full((need + 64,), 2.0, device=cuda)
+    got = _C.flash_attn_paged(q, kc, vc, table, _cu(new, cuda), _i32(lens, cuda), 0.125, max_q_len=hint, workspace=ws[:need])
+    assert bool((ws[need:] == 2).all())
+    at = 0
+    for b, n in enumerate(new):
+        want, tol = _attend(q[at:at + n], ks[b], vs[b], 0.125, True, dtype)
+        _same(got[at:at + n], want, tol, f"sequence {b}")
+        at += n
+
+
+@gpu
+@pytest.mark.parametrize("batch", [64, 65, 130])
+def test_many_sequences(cuda, batch):
+    """More than a wave holds at a time, in every operator."""
+    dtype, hd, h, hk, page = torch.bfloat16, 64, 4, 2, 16
+    new = [(7 * b) % 5 if b % 3 else 1 for b in range(batch)]
+    new[batch // 2] = 150
+    lens = [n + (37 * b) % 700 for b, n in enumerate(new)]
+    ks, vs, kc, vc, table = _paged(lens, hk, page, hd, dtype, cuda, 170)
+    x = _randn((sum(new), h + 2 * hk, hd), dtype, cuda, 171)
+    q, k, v = x[:, :h], x[:, h:h + hk], x[:, h + hk:]
+    cu, kvl = _cu(new, cuda), _i32(lens, cuda)
+    packed = _C.flash_attn_packed(q, k, v, cu, 0.125, True)
+    paged = _C.flash_attn_paged(q, kc, vc, table, cu, kvl, 0.125, max_q_len=150)
+    steps, _ = _C.rotary_steps(hd, device=cuda)
+    turned, _ = _C.rotary_append(q, k, v, steps, cu, kv_lens=kvl, block_table=table, k_cache=kc, v_cache=vc)
+    at = 0
+    for b, n in enumerate(new):
+        s = slice(at, at + n)
+        if n:
+            want, tol = _attend(q[s], k[s], v[s], 0.125, True, dtype)
+            _same(packed[s], want, tol, f"packed {b}")
+            want, tol = _attend(q[s], ks[b], vs[b], 0.125, True, dtype)
+            _same(paged[s], want, tol, f"paged {b}")
+            want, tol = _rotate(q[s], list(range(lens[b] - n, lens[b])), steps.cpu(), 1.0, False, dtype)
+            _same(turned[s], want, tol, f"turned {b}")
+            last = lens[b] - 1
+            assert torch.equal(vc[int(table[b, last // page]), :, last % page], v[at + n - 1])
+        at += n
 
 
 @gpu

@@ -831,7 +831,7 @@ def rotary_append(
     args = (_ptr(q), ad[0], _ptr(q_out), ad[1], k.data_ptr(), ad[2], _ptr(k_out), ad[3], _ptr(v), ad[4],
             _ptr(k_cache), ad[5], _ptr(v_cache), ad[6], steps.data_ptr(), _ptr(positions), cu_seqlens.data_ptr(),
             _ptr(kv_lens), _ptr(block_table), table_ld, t, batch, heads, kvh, hd, 2 * half, pages,
-            page_size, max_pages, amplitude, 1 if interleaved else 0, _dt(k))
+            page_size, max_pages, float(amplitude), 1 if interleaved else 0, _dt(k))
     _launch_on(at, "tx_rotary_append", args,
                (q, k, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache, v_cache, q_out, k_out, st),
                lambda: {"op": "rotary_append", "tokens": t, "heads": heads, "kv_heads": kvh, "head_dim": hd,
@@ -873,7 +873,7 @@ def flash_attn_packed(
         return out
     st, ad = _addresses((qs, ks, vs, os_))
     args = (q.data_ptr(), ad[0], k.data_ptr(), ad[1], v.data_ptr(), ad[2], out.data_ptr(), ad[3], cu_seqlens.data_ptr(),
-            t, batch, heads, kvh, hd, scale, 1 if causal else 0, _dt(q))
+            t, batch, heads, kvh, hd, float(scale), 1 if causal else 0, _dt(q))
     _launch_on(at, "tx_flash_attn_packed", args, (q, k, v, out, cu_seqlens, st),
                lambda: {"op": "flash_attn_packed", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh,
                         "head_dim": hd, "causal": bool(causal)})
@@ -943,7 +943,8 @@ def flash_attn_paged(
     st, ad = _addresses((qs, ks, vs, os_))
     args = (q.data_ptr(), ad[0], k_cache.data_ptr(), ad[1], v_cache.data_ptr(), ad[2], out.data_ptr(), ad[3],
             cu_seqlens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), table_ld, t, batch, heads, kvh,
-            hd, pages, page_size, max_pages, max_q_len, scale, 1 if causal else 0, _ptr(workspace),
+            hd, pages, page_size, max_pages, max_q_len, float(scale), 1 if causal else 0,
+            _ptr(workspace),
             0 if workspace is None else workspace.numel(), _dt(q))
     _launch_on(at, "tx_flash_attn_paged", args,
                (q, k_cache, v_cache, out, cu_seqlens, kv_lens, block_table, workspace, st),

@@ -382,7 +382,9 @@ static int check_seqs(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_h
   if (heads % kv_heads) return TX_EINVAL;
   // Grids (256 threads per 128 rows, per 4 tokens and per sequence) stay below 2^32 threads, and the items of
   // a paged call (per 16 rows and per sequence, up to 256 parts of the keys) below 2^31.
-  if (tokens > 1 << 24 || batch > 1 << 20 || heads > 65535 || tokens * heads > 1 << 26) return TX_EUNSUPPORTED;
+  if (tokens > 1 << 24 || batch > 1 << 20 || heads > 65535 || tokens * heads > 1 << 26 ||
+      batch * kv_heads > 1 << 23)
+    return TX_EUNSUPPORTED;
   if (((uintptr_t)cu & 3u)) return TX_EUNSUPPORTED;
   return TX_OK;
 }

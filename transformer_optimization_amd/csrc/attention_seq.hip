@@ -220,10 +220,10 @@ struct SqLoader {
 // it runs (its K tile is staged one tile ahead of V, two sets of scores).  At
 // head dim 128, where registers allow two workgroups a CU either way: one
 // prompt of 32768 tokens 3990 -> 3900 us, of 2048 48.5 -> 45 us.  At head dim 64
-// it costs the third workgroup (181 registers for 124): 40.4 -> 45.9 us for
-// 16 prompts of up to 1021 tokens, so LEAD = 0 there.
+// its registers (181 for 125) cost workgroups: 40.4 -> 45.9 us for 16 prompts
+// of up to 1021 tokens, so LEAD = 0 there.
 // NST, the stages of the K and V rings: 2, for two workgroups a CU at head dim
-// 128 and four at 64 (126 registers): a third stage there leaves three, 2 x 8192
+// 128 and four at 64 (125 registers): a third stage there leaves three, 2 x 8192
 // tokens 300 us for 285, 16 prompts of up to 1021 42.9 for 38.4.  (With 4 and 8
 // where a call has no more workgroups than CUs, one prompt of 1024 tokens
 // took 29.9 us for 25.9: what a lone workgroup waits for is not its loads.)
@@ -438,7 +438,8 @@ __device__ __forceinline__ void sq_row_again(const SeqAttnArgs& a, const SeqHead
     else orow[lane + 64 * e] = from_f32<T>(o[e]);
   }
   if (po && lane == 0) {
-    pml[0] = m * SQ_LOG2E;
+    // (scores that are no number leave m = -inf, which would weigh nothing)
+    pml[0] = l == l ? m * SQ_LOG2E : __builtin_nanf("");
     pml[unit_rows] = l;
   }
 }

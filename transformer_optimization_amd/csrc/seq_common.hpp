@@ -36,7 +36,8 @@ __device__ __forceinline__ int seq_div(int x, const SeqDiv& d) {
 
 // The sequence and tile with index w: the largest b with first_tile(b) <= w,
 // found by the whole wave, 64 candidates at a time (two rounds of loads up to
-// 4096 sequences).  Wave-uniform; every lane takes part.
+// 4096 sequences).  Wave-uniform; every lane takes part.  Starts that do not
+// ascend give some sequence, whose bounds are cut to the tensors all the same.
 __device__ __forceinline__ SeqTile seq_find(const SeqArgs& s, int group, int r, int64_t w) {
   const int lane = threadIdx.x & 63;
   int lo = 0, n = s.batch;
@@ -45,7 +46,7 @@ __device__ __forceinline__ SeqTile seq_find(const SeqArgs& s, int group, int r, 
     const int i = lo + lane * step;
     bool below = false;
     if (lane * step < n) below = (int64_t)seq_cut(s.cu[i], 0, s.tokens) * group / r + i <= w;
-    const int c = __builtin_popcountll(__ballot(below));  // 0: not found before lo (cannot be for lo = 0)
+    const int c = __builtin_popcountll(__ballot(below));
     const int skip = c > 0 ? (c - 1) * step : 0;
     lo += skip;
     n = n - skip < step ? n - skip : step;
@@ -78,12 +79,13 @@ __device__ __forceinline__ int seq_wave_sum(int x) {
 // Order of a call of packed prompts: the tiles of all sequences and heads in
 // descending order of their index, so that under a causal mask those with the
 // most keys start first, whichever sequence they belong to (16 prompts of up
-// to 1021 tokens 47 -> 40 us).  Where the keys and values are more than the memory-side
-// cache holds, bands of 16 neighbouring tiles of one (sequence, K/V head), which read the
-// same keys in step, are ordered instead, each on one XCD (workgroup i runs on
-// XCD i % 8), whose L2 then serves them: 8 x 16384 tokens, 16 heads with keys
-// of their own, 10.1 -> 8.2 ms, 8 x 8192 2.50 -> 2.18; below that size the
-// coarser order costs more than it saves (8 x 2048 156 -> 164 us).
+// to 1021 tokens 47 -> 40 us).  Where the keys and values are more than the
+// 256 MB of the memory-side cache, bands of 16 neighbouring tiles of one
+// (sequence, K/V head), which read the same keys in step, are ordered instead,
+// each on one XCD (workgroup i runs on XCD i % 8), whose L2 then serves them: 8
+// x 16384 tokens, 16 heads with keys of their own, 10.1 -> 8.2 ms, 8 x 8192
+// 2.50 -> 2.18; below that size the coarser order costs more than it saves (8 x
+// 2048 156 -> 164 us).
 struct SeqOrder {
   int band;   // log2 tiles of a band
   int bands;  // bound on a head's bands over all sequences
@@ -147,9 +149,11 @@ __device__ __forceinline__ SeqTile seq_ordered(const SeqArgs& s, int group, int 
 // result does not change with the batch around it.
 constexpr int SEQ_FEW = 16;
 constexpr int SEQ_TILE = 128;
-constexpr int SEQ_PART_FEW = 256;   // fewest keys of a part: two blocks of 32 for each of 4 waves
+// Keys of a part of few rows are a multiple of 256, two blocks of 32 for each of
+// 4 waves (128: 32 streams of up to 2047 keys 24.5 us for 18.4; 512: 64 streams
+// of 8192 keys 131 us for 141, but one of them 15.5 for 13.6).
+constexpr int SEQ_PART_FEW = 256;
 constexpr int SEQ_PART_TILE = 512;  // fewer are not worth writing and joining partial rows for
-
 constexpr int SEQ_WAVE_PARTS = 16;  // rows of up to so many parts are joined by one wave
 
 struct SeqShape {
@@ -187,7 +191,7 @@ __host__ __device__ inline SeqCut seq_cut_of(const SeqShape& s, int rows, int ke
 // A sequence of a paged call: its cut, its first item and its first unit of
 // partial results, both counted over the call.
 struct SeqWork {
-  int b, q0, qn, kvn, keys;  // keys: those the table can hold
+  int b, q0, qn, kvn;
   SeqCut cut;
   int item, unit;
 };
@@ -279,7 +283,6 @@ struct SeqWalk {
     r.kvn = field(6, i);
     r.item = items + field(2, i) - field(0, i);
     r.unit = units + field(3, i) - field(1, i);
-    r.keys = min(r.kvn, s.max_pages << s.page_log2);
     r.cut.few = sh.few > 0 || r.qn * sh.group <= SEQ_FEW;
     r.cut.unit_rows = sh.few > 0 ? sh.few : SEQ_FEW;
     r.cut.tiles = field(7, i);
