@@ -685,9 +685,10 @@ def _heads3(name: str, t: torch.Tensor, rows: int, heads: int, hd: int, dtype: t
 
 
 def _dims3(name: str, t: torch.Tensor) -> Tuple[int, int, int]:
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
-    return t.shape
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(shape)}")
+    return shape
 
 
 def _int_vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype = torch.int32) -> None:
@@ -714,10 +715,10 @@ def _check_cache(k_cache, v_cache, block_table, batch: int, hd: int, dtype: torc
 
 
 def _starts(cu_seqlens: torch.Tensor) -> int:
-    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype != torch.int32 \
-            or not cu_seqlens.is_contiguous():
+    shape = cu_seqlens.shape
+    if len(shape) != 1 or shape[0] < 1 or cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous():
         raise ValueError("cu_seqlens must be a contiguous int32 [batch + 1] tensor")
-    return cu_seqlens.shape[0] - 1
+    return shape[0] - 1
 
 
 def _one_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> int:
@@ -742,17 +743,6 @@ def _launch_on(at: int, fn: str, args: tuple, keep: tuple, info) -> None:
         _check(fn, code)
     if _recorder is not None:
         _recorder.append(Launch(fn, args, keep, info()))
-
-
-def _addresses(views: tuple) -> tuple:
-    """The strides of each view, four places each, in one array (kept by the caller), and the addresses of the
-    views' parts of it."""
-    flat: list = []
-    for st in views:
-        flat += st if len(st) == 4 else (*st, 0)
-    arr = array.array("q", flat)
-    at = arr.buffer_info()[0]
-    return arr, range(at, at + 32 * len(views), 32)
 
 
 _NO_STRIDES = (0, 0, 0)
@@ -827,11 +817,18 @@ def rotary_append(
         kos = (kvh * hd, hd, 1)
     if t == 0 or batch == 0:
         return q_out, k_out
-    st, ad = _addresses((qs, qos, ks, kos, vs, kcs, vcs))
-    args = (_ptr(q), ad[0], _ptr(q_out), ad[1], k.data_ptr(), ad[2], _ptr(k_out), ad[3], _ptr(v), ad[4],
-            _ptr(k_cache), ad[5], _ptr(v_cache), ad[6], steps.data_ptr(), _ptr(positions), cu_seqlens.data_ptr(),
-            _ptr(kv_lens), _ptr(block_table), table_ld, t, batch, heads, kvh, hd, 2 * half, pages,
-            page_size, max_pages, float(amplitude), 1 if interleaved else 0, _dt(k))
+    # The strides in one array, kept with the launch, and their addresses in it.
+    st = array.array("q", (*qs, *qos, *ks, *kos, *vs, *kcs, *vcs))
+    sa = st.buffer_info()[0]
+    cached = k_cache is not None
+    args = (q.data_ptr() if q is not None else None, sa, q_out.data_ptr() if q_out is not None else None, sa + 24,
+            k.data_ptr(), sa + 48, k_out.data_ptr() if k_out is not None else None, sa + 72,
+            v.data_ptr() if cached else None, sa + 96, k_cache.data_ptr() if cached else None, sa + 120,
+            v_cache.data_ptr() if cached else None, sa + 120 + 8 * len(kcs), steps.data_ptr(),
+            positions.data_ptr() if positions is not None else None, cu_seqlens.data_ptr(),
+            kv_lens.data_ptr() if kv_lens is not None else None, block_table.data_ptr() if cached else None, table_ld,
+            t, batch, heads, kvh, hd, 2 * half, pages, page_size, max_pages, float(amplitude), 1 if interleaved else 0,
+            _DT.get(dtype, -1))
     _launch_on(at, "tx_rotary_append", args,
                (q, k, v, steps, cu_seqlens, kv_lens, positions, block_table, k_cache, v_cache, q_out, k_out, st),
                lambda: {"op": "rotary_append", "tokens": t, "heads": heads, "kv_heads": kvh, "head_dim": hd,
@@ -871,9 +868,10 @@ def flash_attn_packed(
         os_ = (heads * hd, hd, 1)
     if t == 0 or batch == 0:
         return out
-    st, ad = _addresses((qs, ks, vs, os_))
-    args = (q.data_ptr(), ad[0], k.data_ptr(), ad[1], v.data_ptr(), ad[2], out.data_ptr(), ad[3], cu_seqlens.data_ptr(),
-            t, batch, heads, kvh, hd, float(scale), 1 if causal else 0, _dt(q))
+    st = array.array("q", (*qs, *ks, *vs, *os_))
+    sa = st.buffer_info()[0]
+    args = (q.data_ptr(), sa, k.data_ptr(), sa + 24, v.data_ptr(), sa + 48, out.data_ptr(), sa + 72,
+            cu_seqlens.data_ptr(), t, batch, heads, kvh, hd, float(scale), 1 if causal else 0, _DT.get(dtype, -1))
     _launch_on(at, "tx_flash_attn_packed", args, (q, k, v, out, cu_seqlens, st),
                lambda: {"op": "flash_attn_packed", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh,
                         "head_dim": hd, "causal": bool(causal)})
@@ -940,12 +938,13 @@ def flash_attn_paged(
             workspace = torch.empty(need, dtype=torch.float32, device=q.device)
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous fp32")
-    st, ad = _addresses((qs, ks, vs, os_))
-    args = (q.data_ptr(), ad[0], k_cache.data_ptr(), ad[1], v_cache.data_ptr(), ad[2], out.data_ptr(), ad[3],
+    st = array.array("q", (*qs, *ks, *vs, *os_))
+    sa = st.buffer_info()[0]
+    args = (q.data_ptr(), sa, k_cache.data_ptr(), sa + 24, v_cache.data_ptr(), sa + 56, out.data_ptr(), sa + 88,
             cu_seqlens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), table_ld, t, batch, heads, kvh,
             hd, pages, page_size, max_pages, max_q_len, float(scale), 1 if causal else 0,
-            _ptr(workspace),
-            0 if workspace is None else workspace.numel(), _dt(q))
+            workspace.data_ptr() if workspace is not None else None, 0 if workspace is None else workspace.numel(),
+            _DT.get(dtype, -1))
     _launch_on(at, "tx_flash_attn_paged", args,
                (q, k_cache, v_cache, out, cu_seqlens, kv_lens, block_table, workspace, st),
                lambda: {"op": "flash_attn_paged", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh,
