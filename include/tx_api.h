@@ -258,8 +258,8 @@ int tx_flash_attn_fwd_noalloc(const void* qk, const void* vt, int64_t ldvt, void
  * q_out / k_out (nullable: k_out, or q with q_out) receive the turned rows; either may be its input itself (same
  * pointer and strides) and may share no other memory with an input.  k_cache (NULL: no cache; then v,
  * v_cache, block_table are unused) receives the turned k, v_cache the v, at the rows' key indices; rows whose
- * index is negative are not cached.  Slots written by one call must be distinct.  head_dim a multiple of
- * 8 up to 256, rotary_dim even, 2 .. head_dim.
+ * index is negative are not cached.  Slots written by one call must be distinct.  kv_heads divides q_heads,
+ * head_dim a multiple of 8 up to 256, rotary_dim even, 2 .. head_dim.
  */
 int tx_rotary_append(const void* q, const int64_t q_strides[2], void* q_out, const int64_t q_out_strides[2],
                      const void* k, const int64_t k_strides[2], void* k_out, const int64_t k_out_strides[2],
