@@ -1,0 +1,42 @@
+"""Edges of attention over packed sequences and over a paged cache: rows without keys, values that are not
+finite, very long caches, workspaces.  Oracle and tolerances of finite elements are test_seq_ops's."""
+
+import math
+
+import shutil
+
+import pytest
+import torch
+
+from transformer_optimization_amd import _C
+from _util import log
+from test_limits import _run_check
+from test_seq_ops import _attend, _cu, _i32, _paged, _randn, _same
+
+DTYPES = [torch.bfloat16, torch.float16]
+gpu = pytest.mark.gpu
+
+
+# -------------------------------------------------- as many parts as there are
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs the host C++ compiler")
+def test_cut_of_a_paged_call(tmp_path):
+    _run_check(tmp_path, "seq_cut_check")
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("h,new,keys", [(16, 2, 200000), (24, 1, 200000), (8, 4, 262144), (64, 2, 131584), (16, 1, 300001),
+                                        (16, 9, 270000)])
+def test_one_kv_head_over_a_very_long_cache(cuda, hd, h, new, keys):
+    """One K/V head alone on the card: its keys go out in as many parts as the join takes, whatever their
+    number; most of the weight lies on a key of a late part."""
+    dtype, page = torch.bfloat16, 256
+    ks, vs, kc, vc, table = _paged([keys], 1, page, hd, dtype, cuda, 210)
+    q = _randn((new, h, hd), dtype, cuda, 211)
+    for j in (0, keys * 3 // 4, keys - new - 3):
+        x = q[:1, j % h] * 1.5
+        ks[0][j] = x[0]
+        kc[int(table[0, j // page]), :, j % page] = x[0]
+    got = _C.flash_attn_paged(q, kc, vc, table, _cu([new], cuda), _i32([keys], cuda), hd**-0.5, max_q_len=new)
+    want, tol = _attend(q, ks[0], vs[0], hd**-0.5, True, dtype)
+    _same(got, want, tol, f"{new} tokens, {h}/1 heads, {keys} keys, hd{hd}")

@@ -867,6 +867,7 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
   constexpr int GRP = (WAVE ? 64 : 256) / LPR;   // parts at a time
   constexpr int NP = WAVE ? SEQ_WAVE_PARTS / GRP : 8;  // o values asked for at once
   constexpr int MLS = WAVE ? 1 : 4;              // parts whose m and l a lane holds
+  static_assert((WAVE ? SEQ_WAVE_PARTS : SEQ_JOIN_PARTS) <= 64 * MLS, "a row's parts are held one a lane");
   const int lane = tid & 63;
   if (WAVE) tid = lane;
   const float NEG_INF = -__builtin_inff();
@@ -982,43 +983,15 @@ __global__ __launch_bounds__(256, 4) void seq_attn_join_kernel(SeqAttnArgs a) {
 }
 
 // ------------------------------------------------------------------- launch
-// Upper bounds, over all lengths that these totals allow, of a call's items
-// and of its units of partial results.
-struct SqBounds {
-  int64_t items, units, join_rows;
-};
-static SqBounds sq_bounds(const SeqAttnArgs& a) {
-  const int64_t rows = (int64_t)a.s.tokens * a.group, cap = (int64_t)a.s.max_pages << a.s.page_log2;
-  const int64_t hk = a.kv_heads, cus = a.cus;
-  auto least = [](int64_t x, int64_t y) { return x < y ? x : y; };
-  const int64_t few_parts = least((cap + SEQ_PART_FEW - 1) / SEQ_PART_FEW, a.few_parts);
-  const int64_t few_tiles = a.few ? rows / a.few + a.s.batch : a.s.batch;
-  SqBounds b;
-  b.items = few_tiles * hk * few_parts;
-  b.units = few_parts > 1 ? b.items : 0;
-  b.join_rows = few_parts > 1 ? rows * hk : 0;
-  if (!a.few) {
-    const int64_t seqs = least(a.s.batch, rows / (SEQ_FEW + 1));
-    const int64_t tiles = (rows / SEQ_TILE + seqs) * hk;
-    int64_t parts = least(cap / SEQ_PART_TILE, (2 * cus + hk - 1) / hk);
-    parts = parts < 1 ? 1 : parts;
-    const int64_t items = least(tiles * parts, tiles + seqs * 2 * cus);
-    b.items += items;
-    b.units += parts > 1 ? items * (SEQ_TILE / SEQ_FEW) : 0;
-    b.join_rows = b.units > 0 ? rows * hk : 0;
-  }
-  return b;
+static SeqBounds sq_bounds(const SeqAttnArgs& a) {
+  return seq_bounds(sq_shape(a), a.s.tokens, a.s.batch, (int64_t)a.s.max_pages << a.s.page_log2);
 }
 static void sq_finish(SeqAttnArgs& a) {
   const int cus = device_cu_count();
-  a.cus = cus > 0 ? cus : 256;
-  if (a.cus > 256) a.cus = 256;  // the join holds one part a thread
-  a.few_parts = a.cus / a.kv_heads < 1 ? 1 : a.cus / a.kv_heads;
-  a.few = 0;
-  const int64_t most = a.max_q_len * a.group;
-  // Calls of few-row sequences only; where their tiles could pass 32-bit
-  // counts (rows beyond what max_q_len promises), the general kernel.
-  if (most <= SEQ_FEW && ((int64_t)a.s.tokens * a.group / most + a.s.batch) * (a.kv_heads + 256) < 1 << 30) a.few = (int)most;
+  const SeqShape s = seq_shape(a.s.tokens, a.s.batch, a.group, a.kv_heads, a.max_q_len, cus > 0 ? cus : 256);
+  a.cus = s.cus;
+  a.few_parts = s.few_parts;
+  a.few = s.few;
 }
 
 int64_t seq_attention_workspace(const SeqAttnArgs& a0) {
@@ -1038,7 +1011,7 @@ static int launch_hd(SeqAttnArgs a, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? TX_OK : TX_EHIP;
   }
   sq_finish(a);
-  const SqBounds b = sq_bounds(a);
+  const SeqBounds b = sq_bounds(a);
   auto grid = [](int64_t items, int64_t most) { return dim3((unsigned)(items < most ? items : most)); };
   // As many workgroups as are resident: few rows 4 a CU at head dim 64 and 2 at
   // 128, tiles 3 and 2.

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.hpp"
+#include "seq_cut.hpp"
 #include "tx_internal.hpp"
 
 namespace tx {
@@ -140,54 +141,7 @@ __device__ __forceinline__ SeqTile seq_ordered(const SeqArgs& s, int group, int 
   return t;
 }
 
-// ---- how a paged call's work is cut ---------------------------------------
-// A sequence of at most SEQ_FEW rows (query heads of one K/V head x new
-// tokens) is bound by reading its keys: one item per K/V head and part of the
-// keys, every row in it.  More rows: tiles of 128 rows, their keys in parts
-// where the tiles alone leave the card idle.  The cut of a sequence depends on
-// nothing but its own rows, keys and head counts (and the card), so that its
-// result does not change with the batch around it.
-constexpr int SEQ_FEW = 16;
-constexpr int SEQ_TILE = 128;
-// Keys of a part of few rows are a multiple of 256, two blocks of 32 for each of
-// 4 waves (128: 32 streams of up to 2047 keys 24.5 us for 18.4; 512: 64 streams
-// of 8192 keys 131 us for 141, but one of them 15.5 for 13.6).
-constexpr int SEQ_PART_FEW = 256;
-constexpr int SEQ_PART_TILE = 512;  // fewer are not worth writing and joining partial rows for
-constexpr int SEQ_WAVE_PARTS = 16;  // rows of up to so many parts are joined by one wave
-
-struct SeqShape {
-  int group, kv_heads, cus;
-  int few_parts;  // most parts of few-row items
-  int few;  // rows of a tile when the call has few-row items only (<= SEQ_FEW), else 0
-};
-struct SeqCut {
-  int tiles, parts, part_keys;
-  int unit_rows, units;  // partial results of one item: units of unit_rows rows (0: one part, none)
-  bool few;
-};
-__host__ __device__ inline int seq_ceil(int x, int y) { return (x + y - 1) / y; }
-__host__ __device__ inline SeqCut seq_cut_of(const SeqShape& s, int rows, int keys) {
-  SeqCut c;
-  c.few = s.few > 0 || rows <= SEQ_FEW;
-  c.unit_rows = s.few > 0 ? s.few : SEQ_FEW;
-  c.tiles = rows <= c.unit_rows ? 1 : (c.few ? seq_ceil(rows, c.unit_rows) : seq_ceil(rows, SEQ_TILE));
-  int most, step;
-  if (c.few) {
-    most = s.few_parts;
-    step = SEQ_PART_FEW;
-  } else {
-    most = seq_ceil(2 * s.cus, c.tiles * s.kv_heads);
-    step = 64;  // a key tile
-    most = most < keys / SEQ_PART_TILE ? most : keys / SEQ_PART_TILE;
-  }
-  most = most < 1 ? 1 : most;
-  c.part_keys = seq_ceil(seq_ceil(keys, most), step) * step;
-  c.parts = keys > 0 ? seq_ceil(keys, c.part_keys) : 1;
-  c.units = c.parts > 1 ? (c.few ? 1 : SEQ_TILE / SEQ_FEW) : 0;
-  return c;
-}
-
+// ---- the items of a paged call (seq_cut.hpp) ------------------------------
 // A sequence of a paged call: its cut, its first item and its first unit of
 // partial results, both counted over the call.
 struct SeqWork {
