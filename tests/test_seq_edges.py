@@ -17,6 +17,30 @@ DTYPES = [torch.bfloat16, torch.float16]
 gpu = pytest.mark.gpu
 
 
+# -------------------------------------------------------- rows without keys
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("h,hk,new,keys", [(2, 2, 4, 1), (4, 4, 9, 3), (8, 2, 40, 25), (6, 2, 150, 70), (4, 1, 1100, 1030)])
+def test_a_row_that_sees_no_key_is_zero_whatever_the_keys_hold(cuda, dtype, hd, h, hk, new, keys):
+    """Fewer keys than new tokens: the first rows see none.  Keys and values of the later rows are not finite;
+    the last shape's keys are shared out over the card."""
+    ks, vs, kc, vc, table = _paged([keys], hk, 16, hd, dtype, cuda, 200)
+    q = _randn((new, h, hd), dtype, cuda, 201)
+    args = (table, _cu([new], cuda), _i32([keys], cuda), hd**-0.5)
+    clean = _C.flash_attn_paged(q, kc, vc, *args)
+    for cache, what in ((vc, math.nan), (vc, math.inf), (kc, math.nan)):
+        good = cache.clone()
+        for j in {0, keys // 2, keys - 1}:
+            cache[int(table[0, j // 16]), :, j % 16] = what
+        got = _C.flash_attn_paged(q, kc, vc, *args)
+        log(f"no keys: {new} rows over {keys}, {h}/{hk} hd{hd} {dtype} {what}")
+        assert bool((got[:new - keys] == 0).all())
+        assert not bool(torch.isfinite(got[new - keys:]).any())
+        cache.copy_(good)
+    assert torch.equal(_C.flash_attn_paged(q, kc, vc, *args), clean)
+
+
 # -------------------------------------------------- as many parts as there are
 @pytest.mark.skipif(shutil.which("g++") is None, reason="needs the host C++ compiler")
 def test_cut_of_a_paged_call(tmp_path):

@@ -497,6 +497,8 @@ __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       tile.o[d][e] = lost ? __builtin_nanf("") : tile.o[d][e] * inv;
+      // (0 weights times a value that is not finite are not 0)
+      if (PAGED) tile.o[d][e] = sees > 0 ? tile.o[d][e] : 0.f;
       odd += tile.o[d][e] * 0.f;
     }
   // A value that is not finite may come from a key that the row does not see
@@ -773,7 +775,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
       for (int x = 0; x < 4; ++x) {
         v = __builtin_fmaf(wt[x], ov[x][e], v);
       }
-      v = lost ? __builtin_nanf("") : v * inv;
+      v = lost ? __builtin_nanf("") : (sees > 0 ? v * inv : 0.f);  // (0 times what is not finite is not 0)
       res[4 * y + e] = v;
       odd += v * 0.f;
     }
