@@ -41,6 +41,172 @@ def test_a_row_that_sees_no_key_is_zero_whatever_the_keys_hold(cuda, dtype, hd, 
     assert torch.equal(_C.flash_attn_paged(q, kc, vc, *args), clean)
 
 
+# ------------------------------------------------ values that are not finite
+def _ieee(q, k, v, scale, causal, dtype):
+    """The formula in 64 bits with IEEE arithmetic over the keys that a row sees: an infinity stays one unless it meets
+    its opposite, a weight of 0 (a score of -inf) or a NaN.  The tolerance of finite elements as _attend's, over the
+    finite products."""
+    n, h, d = q.shape
+    m, hk = k.shape[:2]
+    out = torch.zeros(n, h, d, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    eps = torch.finfo(dtype).eps
+    seen = torch.ones(n, m, dtype=torch.bool, device=q.device)
+    if causal:
+        seen = seen.tril(m - n)
+    for x in range(h):
+        qx, kx, vx = q[:, x].double(), k[:, x // (h // hk)].double(), v[:, x // (h // hk)].double()
+        products = torch.stack([(qx[i] * kx).sum(1) for i in range(n)]) if n * m < 1 << 16 else qx @ kx.T
+        s = torch.where(seen, products * scale, torch.full_like(products, -math.inf))
+        top = s.amax(1, keepdim=True)  # NaN where any is
+        p = torch.where(seen, torch.exp(s - top), torch.zeros_like(s))
+        total = torch.where(seen.any(1), p.sum(1), torch.ones_like(p[:, 0]))[:, None]
+        finite = torch.isfinite(vx)
+        clean = vx.masked_fill(~finite, 0.0)
+        o = (p / total) @ clean
+        # what each bad key adds, key by key
+        for j in (~finite).any(1).nonzero().flatten().tolist():
+            o = o + torch.where(seen[:, j, None], p[:, j, None] * vx[j].masked_fill(finite[j], 0.0), torch.zeros_like(o))
+        o = torch.where(seen.any(1)[:, None], o, torch.zeros_like(o))
+        size = torch.where(seen, (qx.abs() @ kx.abs().nan_to_num(0.0, 0.0, 0.0).T) * scale, torch.zeros_like(s))
+        big = size.nan_to_num(0.0, 0.0, 0.0).amax(1, keepdim=True)
+        a = (p / total).nan_to_num(0.0) @ clean.abs()
+        if dtype == torch.float16:
+            a = a + 2.0**-25 / eps * (seen.double() @ clean.abs()) / total.nan_to_num(1.0)
+        out[:, x] = o
+        tol[:, x] = eps / 2 * o.abs() + a * (eps + 2 * (d + 8) * 2.0**-24 * big + 2 * m * 2.0**-24) + 2.0**-25
+    return out, tol
+
+
+def _strictly_same(got, want, tol, what):
+    """NaN where the formula gives NaN, the same infinities, and finite elements within their tolerance."""
+    got = got.double()
+    for name, f in (("NaN", torch.isnan), ("+inf", torch.isposinf), ("-inf", torch.isneginf)):
+        g, w = f(got), f(want)
+        assert torch.equal(g, w), f"{what}: {name} at {int((g & ~w).sum())} more and {int((w & ~g).sum())} fewer elements"
+    ok = torch.isfinite(want)
+    over = ((got - want).abs() - tol)[ok]
+    log(f"  {what}: {int((~ok).sum())} of {ok.numel()} not finite, largest excess {float(over.max()) if over.numel() else 0:.3e}")
+    assert not over.numel() or float(over.max()) <= 0, what
+
+
+def _spoil(x, seed, count, values):
+    """`count` elements of x [n, heads, hd] at random places, and one in each of the first and last row."""
+    n, h, d = x.shape
+    at = torch.randint(0, n * h * d, (count,), generator=torch.Generator("cpu").manual_seed(seed)).tolist()
+    at += [3, n * h * d - 1]
+    for i, j in enumerate(at):
+        x.view(-1)[j] = values[i % len(values)]
+
+
+SPOILS = [  # bad elements of v, of k, whether of q
+    ((1, [math.nan]), None, False), ((3, [math.inf]), None, False), ((40, [math.inf, -math.inf, math.nan, math.inf]), None, False),
+    (None, (2, [math.nan]), False), (None, (3, [math.inf, -math.inf]), False),
+    ((6, [-math.inf, math.inf]), (2, [-math.inf]), False), (None, None, True), ((2, [math.inf]), None, True),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("h,hk", [(4, 4), (4, 1), (6, 2)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_attention_of_values_that_are_not_finite(cuda, dtype, hd, h, hk, causal):
+    for i, (vs, ks, in_q) in enumerate(SPOILS):
+        for lens in ([150], [5, 1, 90], [333]):
+            t = sum(lens)
+            q, k, v = (_randn((t, x, hd), dtype, cuda, 220 + i) for i, x in enumerate((h, hk, hk)))
+            if vs:
+                _spoil(v, i, *vs)
+            if ks:
+                _spoil(k, i + 50, *ks)
+            if in_q:
+                q[t // 2, 0, 1], q[t - 1, h - 1, 0] = math.nan, math.inf
+            got = _C.flash_attn_packed(q, k, v, _cu(lens, cuda), hd**-0.5, causal)
+            at = 0
+            for n in lens:
+                r = slice(at, at + n)
+                want, tol = _ieee(q[r], k[r], v[r], hd**-0.5, causal, dtype)
+                _strictly_same(got[r], want, tol, f"{i}: {n} of {lens}, {h}/{hk} hd{hd} {dtype}")
+                at += n
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("h,hk,new,keys", [(4, 2, 1, 90), (4, 2, 3, 400), (4, 2, 7, 5000), (4, 1, 1, 9000), (4, 2, 40, 300),
+                                           (4, 1, 60, 5000), (2, 2, 150, 150), (6, 2, 5, 3)])
+def test_paged_attention_of_values_that_are_not_finite(cuda, dtype, hd, h, hk, new, keys):
+    """Few rows and tiles, keys whole and in parts, fewer keys than tokens."""
+    for i, (vs, ks, in_q) in enumerate(SPOILS):
+        k, v, kc, vc, table = _paged([keys], hk, 16, hd, dtype, cuda, 230 + i)
+        k, v = k[0], v[0]
+        q = _randn((new, h, hd), dtype, cuda, 231)
+        if vs:
+            _spoil(v, i, *vs)
+        if ks:
+            _spoil(k, i + 50, *ks)
+        if in_q:
+            q[new // 2, 0, 1], q[new - 1, h - 1, 0] = math.nan, math.inf
+        j = torch.arange(keys, device=cuda)
+        for c, x in ((kc, k), (vc, v)):
+            c[table[0, j // 16].long(), :, j % 16] = x
+        for causal in (True, False):
+            got = _C.flash_attn_paged(q, kc, vc, table, _cu([new], cuda), _i32([keys], cuda), hd**-0.5, causal)
+            want, tol = _ieee(q, k, v, hd**-0.5, causal, dtype)
+            _strictly_same(got, want, tol, f"{i}: {new} over {keys}, {h}/{hk} hd{hd} causal={causal} {dtype}")
+
+
+def _time_us(fn):
+    for _ in range(3):
+        fn()
+    times = []
+    for _ in range(7):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        fn()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3)
+    return min(times)
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("where", ["v first", "k first", "v last", "k last", "q"])
+def test_rows_that_are_not_finite_take_about_the_time_of_others(cuda, hd, where):
+    """One bad element: of the first token, which most rows see (twice a clean call's time at most, and 50 us for what
+    launches of these sizes vary by), or of the last one's.  That is hidden from rows of a few waves, each of which goes
+    through all keys by itself, for two groups of rows, in looks at 64 and then steps of 32 keys: 2 (n / 64 + n / 32)
+    rounds of a few dependent loads, 2 us each at most."""
+    dtype, n, h, hk = torch.float16, 4096, 8, 2
+    q, k, v = (_randn((n, x, hd), dtype, cuda, 250 + i) for i, x in enumerate((h, hk, hk)))
+    _, _, kc, vc, table = _paged([n], hk, 16, hd, dtype, cuda, 253)
+    j = torch.arange(n, device=cuda)
+
+    def fill():
+        for c, x in ((kc, k), (vc, v)):
+            c[table[0, j // 16].long(), :, j % 16] = x
+
+    fill()
+    cu, kvl = _cu([n], cuda), _i32([n], cuda)
+    calls = {"packed": lambda: _C.flash_attn_packed(q, k, v, cu, hd**-0.5, True),
+             "packed, all visible": lambda: _C.flash_attn_packed(q, k, v, cu, hd**-0.5, False),
+             "chunk": lambda: _C.flash_attn_paged(q[-300:], kc, vc, table, _cu300, kvl, hd**-0.5),
+             "token": lambda: _C.flash_attn_paged(q[-1:], kc, vc, table, _cu1, kvl, hd**-0.5, max_q_len=1)}
+    _cu300, _cu1 = _cu([300], cuda), _cu([1], cuda)
+    clean = {name: _time_us(f) for name, f in calls.items()}
+    x = {"v": v, "k": k, "q": q}[where[0]]
+    x[0 if where.endswith("first") else n - 1, 0, 5] = math.nan if x is q else math.inf
+    fill()
+    rounds = 2 * (n // 64 + n // 32)
+    took = {name: _time_us(f) for name, f in calls.items()}
+    for name in calls:
+        log(f"  {where} hd{hd} {name}: {clean[name]:.1f} us clean, {took[name]:.1f} us")
+    for name in calls:
+        assert took[name] <= (2 * clean[name] + 50 if where.endswith("first") else clean[name] + 2 * rounds), name
+
+
 # -------------------------------------------------- as many parts as there are
 @pytest.mark.skipif(shutil.which("g++") is None, reason="needs the host C++ compiler")
 def test_cut_of_a_paged_call(tmp_path):

@@ -36,62 +36,6 @@ struct SeqHead {
   }
 };
 
-// One query row over the keys [j0, j1), by one wave, on the vector ALU: the
-// maximum and sum of the softmax first, then the weighted values, key by key.
-// lane: dims lane, lane + 64, ... of o (fp32, normalised; 0 without keys).
-// Every masked key is skipped, never multiplied by 0.
-template <typename T, int HD, bool PAGED>
-__device__ void seq_row(const SeqAttnArgs& a, const SeqHead<T, PAGED>& hp, const T* qrow, int j0, int j1,
-                        float* o, float& m, float& l) {
-  constexpr int DPL = HD / 64;
-  const int lane = threadIdx.x & 63;
-  const float NEG_INF = -__builtin_inff(), NAN_ = __builtin_nanf("");
-  auto score = [&](int j, const T*& vr) {
-    const T* kr;
-    if (!hp.at(a, j, kr, vr)) return NAN_;  // a key that has no page
-    float s = 0.f;
-#pragma unroll 1  // this path is never hot: few registers
-    for (int d = 0; d < HD; d += 8) {
-      const u32x4 x = ld128(qrow + d), y = ld128(kr + d);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s += unpack8<T>(x, e) * unpack8<T>(y, e);
-    }
-    return s * a.scale;
-  };
-  for (int i = 0; i < DPL; ++i) o[i] = 0.f;
-  m = NEG_INF;
-  l = 0.f;
-  if (j1 <= j0) return;
-  const T* vr;
-#pragma unroll 1
-  for (int j = j0 + lane; j < j1; j += 64) {
-    const float s = score(j, vr), mn = fmaxf(m, s);
-    l = (m == NEG_INF ? l : l * expf(m - mn)) + (mn == NEG_INF ? 0.f : expf(s - mn));
-    m = mn;
-    if (!(s == s)) l = NAN_;
-  }
-  float mw = m;
-  for (int x = 32; x > 0; x >>= 1) mw = fmaxf(mw, __shfl_xor(mw, x, 64));
-  l = wave_sum(m == NEG_INF ? l : l * expf(m - mw));
-  m = mw;
-  const float inv = 1.0f / l;  // l = 0 (every score -inf): 0 * inf below is NaN, as softmax gives
-#pragma unroll 1
-  for (int b0 = j0; b0 < j1; b0 += 64) {
-    const int j = b0 + lane;
-    float p = 0.f;
-    if (j < j1) p = (m == NEG_INF ? 0.f : expf(score(j, vr) - m)) * inv;
-    const int n = j1 - b0 < 64 ? j1 - b0 : 64;
-#pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      const float pi = __shfl(p, i, 64);
-      const T* kr;
-      const T* vi;
-      hp.at(a, b0 + i, kr, vi);
-      for (int e = 0; e < DPL; ++e) o[e] += pi * to_f32(vi[lane + 64 * e]);
-    }
-  }
-}
-
 // ------------------------------------------------------------ tiles of rows
 // A workgroup of 4 waves owns 128 rows of one (sequence, K/V head), 32 per
 // wave.  Row r is (token r / group, query head r % group of the K/V head), so
@@ -332,19 +276,36 @@ struct SqTile {
 #pragma unroll
         for (int ks = 0; ks < HD / 64; ++ks) qk(Kn, ks, sn);
       }
+      // The largest score, NaN if any is (v_maximum3_f32).
       float mx = NEG_INF;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[t][r]);
+        for (int r = 0; r < 16; ++r) mx = __builtin_elementwise_maximum(mx, sc[t][r]);
       {
         const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
                                                          __builtin_bit_cast(uint32_t, mx), false, false);
-        mx = fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]));
+        mx = __builtin_elementwise_maximum(__builtin_bit_cast(float, (uint32_t)sw[0]),
+                                           __builtin_bit_cast(float, (uint32_t)sw[1]));
       }
       mx *= c;
-      // Re-base when a row's maximum grows past m_run + 8.
-      if (__any(mx > m_run + 8.f)) {
+      // Re-base when a row's maximum grows past m_run + 8, or is no number.
+      if (__any(!(mx <= m_run + 8.f))) {
+        // A score that is NaN or +inf makes its row NaN: the row sum says so, and
+        // the row sees nothing from here on (a NaN weight would make the sum of
+        // the row 16 lanes away NaN too).
+        const bool lost = !(mx < -NEG_INF);
+        if (__any(lost)) {
+          mylim = lost ? 0 : mylim;
+          wlim_min = 0;
+          mx = lost ? NEG_INF : mx;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) lsum[j] = lost ? __builtin_nanf("") : lsum[j];
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[t][r] = lost ? NEG_INF : sc[t][r];
+        }
         const float m_new = fmaxf(m_run, mx);
         const float corr = m_run == NEG_INF ? 0.f : exp2f(m_run - m_new);
 #pragma unroll
@@ -424,23 +385,203 @@ __device__ __forceinline__ int sq_bad_from(int mine, int* slot, int wave, int la
 // normalised) [unit_rows][HD], then the rows' maxima m (log2 units) and sums l.
 __host__ __device__ constexpr int64_t sq_unit_floats(int rows, int hd) { return (int64_t)((rows * (hd + 2) + 3) & ~3); }
 
-// One row again, key by key, into the output or its partial result.
+// The kernel's first argument, read where this is called and not before.
+__device__ __forceinline__ const SeqAttnArgs& sq_args_again() {
+  uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const SeqAttnArgs*)(const __attribute__((address_space(4))) SeqAttnArgs*)p;
+}
+
+// Rows whose result is not finite though the sum of their weights is, up to 16
+// by one wave (lane: row lane & 15, r of the sequence's; `need`), after they are
+// stored.  What a row must come to:
+// sum_j w_j v_j over the keys it sees, w_j its fp32 weight, in IEEE arithmetic.
+// The first pass also adds 0 x v of the keys that the mask hides (NaN where v
+// is not finite), and its unnormalised sums pass fp32's range where values near
+// the end of it are added up.  So:
+//  * Look through the keys for values that are not finite.  Of 32 keys with
+//    any, note per element which infinities the row sees (a NaN counts as
+//    both): MFMAs of 0/1 operands, (weight > 0) x (value is that infinity).
+//    This ends where it explains every infinity and NaN that is stored, at the
+//    first bad key as a rule: they are right then.
+//  * Rows with something unexplained run again with normalised weights over
+//    values whose infinities and NaN are replaced by 0, the noted ones added.
+// 4096 causal tokens, 8 / 2 heads of 64, an infinity in v of the first token: 67
+// us for 61 of a clean call, of the last one 570 (one row after another, key by
+// key: 15 and 16 ms).
+// Loads go straight to registers: no other wave need take part.  16 rows, and
+// the call's arguments read again here, so that the kernels around this keep
+// their registers (32 rows and arguments held across put 58 to 90 of them in
+// scratch memory: 32 short streams took 32 us for 21).
+// po: not nullptr: the row's partial result.
 template <typename T, int HD, bool PAGED>
-__device__ __forceinline__ void sq_row_again(const SeqAttnArgs& a, const SeqHead<T, PAGED>& hp, int64_t tok, int h,
-                                             int j0, int j1, float* po, float* pml, int unit_rows) {
-  const int lane = threadIdx.x & 63;
-  float o[HD / 64], m, l;
-  seq_row<T, HD, PAGED>(a, hp, (const T*)a.q + tok * a.q_st + h * a.q_sh, j0, j1, o, m, l);
-  T* orow = (T*)a.o + tok * a.o_st + h * a.o_sh;
+__device__ __forceinline__ void sq_odd_rows(int b, int q0, int hk, int r, bool need, int sees, int j0, float m, float l,
+                                            float bias, float* po, int lane) {
+  typedef typename Mfma16<T>::vec vec;
+  constexpr uint32_t EXP = std::is_same<T, bf16>::value ? 0x7F80u : 0x7C00u;  // all ones: not finite
+  constexpr uint32_t ONE = std::is_same<T, bf16>::value ? 0x3F80u : 0x3C00u;
+  const float INF = __builtin_inff();
+  const SeqAttnArgs& a = sq_args_again();
+  SeqHead<T, PAGED> hp;
+  hp.init(a, b, q0, hk);
+  const int col = lane & 15, g = lane >> 4;
+  const int i0 = seq_div(r, a.by_group);
+  const int64_t tok = q0 + i0;
+  const int h = hk * a.group + r - i0 * a.group;
+  const T* qrow = (const T*)a.q + tok * a.q_st + h * a.q_sh + 8 * g;
+  T* orow = (T*)a.o + tok * a.o_st + h * a.o_sh + 4 * g;
+  const float c = a.scale * SQ_LOG2E, mc = (m == -INF ? 0.f : m) - bias;
+  sees = need ? sees : 0;
+  int lim = sees;
 #pragma unroll
-  for (int e = 0; e < HD / 64; ++e) {
-    if (po) po[lane + 64 * e] = o[e];
-    else orow[lane + 64 * e] = from_f32<T>(o[e]);
+  for (int x = 8; x > 0; x >>= 1) lim = max(lim, __shfl_xor(lim, x, 64));
+  lim = seq_uni(lim);
+
+  // Weights of the 32 keys from k0 on: w[x][e] is of key k0 + 16 x + 4 g + e, 0
+  // where masked.
+  auto key_of = [&](int k0, int x, int e) { return k0 + 16 * x + 4 * g + e; };
+  auto weights = [&](int k0, f32x4* w) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const T *kr, *vr, *qr = qrow;
+      hp.at(a, min(k0 + 16 * x + col, lim - 1), kr, vr);
+      asm volatile("" : "+v"(qr), "+v"(kr));
+      w[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i)
+        w[x] = Mfma16<T>::mma(__builtin_bit_cast(vec, ld128(kr + 32 * i + 8 * g)),
+                              __builtin_bit_cast(vec, ld128(qr + 32 * i)), w[x]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[x][e] = key_of(k0, x, e) < sees ? exp2f(__builtin_fmaf(w[x][e], c, -mc)) : 0.f;
+    }
+  };
+  // Element 16 d + col of the values of the keys that w's weights are of.
+  auto values = [&](int k0, int d, uint32_t* v) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const T *kr, *vr;
+      const int j = min(k0 + 16 * x + 4 * g, (lim - 1) & ~3);  // four keys lie in one page
+      int left = lim - 1 - j;
+      hp.at(a, j, kr, vr);
+      vr += col + 16 * d;
+      asm volatile("" : "+v"(vr), "+v"(left));
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[4 * x + e] = __builtin_bit_cast(uint16_t, vr[(uint64_t)(uint32_t)min(e, left) * (uint32_t)a.v_st]);
+    }
+  };
+
+  // Bit 4 d + e: element 16 d + 4 g + e of the row.  What is +inf or NaN, what
+  // -inf or NaN, and the infinities seen that explain it.
+  uint32_t odd_p = 0, odd_n = 0, pos = 0, neg = 0;
+#pragma unroll
+  for (int d = 0; d < HD / 16; ++d) {
+    float y[4];
+    if (po) load4<float>(po + 16 * d + 4 * g, y);
+    else load4<T>(orow + 16 * d, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      odd_p |= (need && !(y[e] < INF) ? 1u : 0u) << (4 * d + e);
+      odd_n |= (need && !(y[e] > -INF) ? 1u : 0u) << (4 * d + e);
+    }
   }
-  if (po && lane == 0) {
-    // (scores that are no number leave m = -inf, which would weigh nothing)
-    pml[0] = l == l ? m * SQ_LOG2E : __builtin_nanf("");
-    pml[unit_rows] = l;
+  bool bad = false;
+#pragma unroll 1
+  for (int k0 = j0; k0 < lim; k0 += 32) {
+    if ((k0 - j0) % 64 == 0) {  // look through 64 keys
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) {
+        const T *kr, *vr;
+        const int x = 64 * i + lane;
+        hp.at(a, min(k0 + x / (HD / 8), lim - 1), kr, vr);
+        const u32x4 y = ld128(vr + x % (HD / 8) * 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          any |= (y[e] & EXP) == EXP || (y[e] & (EXP << 16)) == EXP << 16 ? 1u : 0u;
+      }
+      bad = __any(any != 0);
+      if (!bad) k0 += 32;
+    }
+    if (!bad) continue;
+    f32x4 w[2];
+    weights(k0, w);
+    // 0/1 operands: seen with a weight, seen with a weight of 0 (which is NaN
+    // times an infinity).
+    u32x4 some, zero;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t s = w[e >> 2][e & 3] > 0.f ? ONE : 0;
+      const uint32_t z = !s && key_of(k0, e >> 2, e & 3) < sees ? ONE : 0;
+      some[e >> 1] = e & 1 ? some[e >> 1] | s << 16 : s;
+      zero[e >> 1] = e & 1 ? zero[e >> 1] | z << 16 : z;
+    }
+#pragma unroll 1
+    for (int d = 0; d < HD / 16; ++d) {
+      uint32_t v[8];
+      values(k0, d, v);
+      u32x4 vp, vn, vz;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t xp = v[e] == EXP || (v[e] & 0x7FFFu) > EXP ? ONE : 0;
+        const uint32_t xn = v[e] == (EXP | 0x8000u) || (v[e] & 0x7FFFu) > EXP ? ONE : 0;
+        vp[e >> 1] = e & 1 ? vp[e >> 1] | xp << 16 : xp;
+        vn[e >> 1] = e & 1 ? vn[e >> 1] | xn << 16 : xn;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vz[e] = vp[e] | vn[e];
+      const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+      const f32x4 tz = Mfma16<T>::mma(__builtin_bit_cast(vec, vz), __builtin_bit_cast(vec, zero), none);
+      const f32x4 tp = Mfma16<T>::mma(__builtin_bit_cast(vec, vp), __builtin_bit_cast(vec, some), tz);
+      const f32x4 tn = Mfma16<T>::mma(__builtin_bit_cast(vec, vn), __builtin_bit_cast(vec, some), tz);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pos |= (tp[e] > 0.f ? 1u : 0u) << (4 * d + e);
+        neg |= (tn[e] > 0.f ? 1u : 0u) << (4 * d + e);
+      }
+    }
+    if (__all(!(odd_p & ~pos) && !(odd_n & ~neg))) return;
+  }
+  bool again = (odd_p & ~pos) || (odd_n & ~neg);
+  again = __shfl_xor((int)again, 16, 64) || again;
+  again = __shfl_xor((int)again, 32, 64) || again;
+  // fp16 weights stay above its subnormal range.
+  constexpr float UP = std::is_same<T, f16>::value ? 0x1p15f : 1.f;
+  const float f = (l != 0.f ? 1.0f / l : 0.f) * UP;
+  f32x4 o[HD / 16];
+#pragma unroll
+  for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int k0 = j0; k0 < lim; k0 += 32) {
+    uint32_t v[HD / 16][8];  // asked for before the keys, whose loads they overlap
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) values(k0, d, v[d]);
+    f32x4 w[2];
+    weights(k0, w);
+    const u32x4 pw = {pack2<T>(w[0][0] * f, w[0][1] * f), pack2<T>(w[0][2] * f, w[0][3] * f),
+                      pack2<T>(w[1][0] * f, w[1][1] * f), pack2<T>(w[1][2] * f, w[1][3] * f)};
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) {
+      u32x4 vv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t x = (v[d][e] & EXP) == EXP ? 0 : v[d][e];
+        vv[e >> 1] = e & 1 ? vv[e >> 1] | x << 16 : x;
+      }
+      o[d] = Mfma16<T>::mma(__builtin_bit_cast(vec, vv), __builtin_bit_cast(vec, pw), o[d]);
+    }
+  }
+  if (!again) return;
+#pragma unroll
+  for (int d = 0; d < HD / 16; ++d) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = 4 * d + e;
+      y[e] = o[d][e] * (1.f / UP) + ((pos >> at) & 1 ? INF : 0.f) + ((neg >> at) & 1 ? -INF : 0.f);
+    }
+    if (po) store4<float>(po + 16 * d + 4 * g, y);
+    else store4<T>(orow + 16 * d, y);
   }
 }
 
@@ -490,62 +631,63 @@ __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0
   const float l = tile.lsum[0];
   const bool lost = PAGED && sees > bad_from && bad_from < j1;
   const float none = part || sees <= 0 ? 0.f : __builtin_nanf("");
-  const float inv = l != 0.f ? 1.0f / l : none;
+  const float inv = lost ? __builtin_nanf("") : (l != 0.f ? 1.0f / l : none);
+  if (PAGED && __any(sees <= 0)) {  // (0 weights times a value that is not finite are not 0)
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) tile.o[d][e] = sees > 0 ? tile.o[d][e] : 0.f;
+  }
   float odd = 0.f;  // NaN if any value of the row is not finite
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      tile.o[d][e] = lost ? __builtin_nanf("") : tile.o[d][e] * inv;
-      // (0 weights times a value that is not finite are not 0)
-      if (PAGED) tile.o[d][e] = sees > 0 ? tile.o[d][e] : 0.f;
-      odd += tile.o[d][e] * 0.f;
-    }
-  // A value that is not finite may come from a key that the row does not see
-  // (its weight of 0 times a NaN or an infinity).  Such rows run again key by
-  // key; they are rare enough that nothing above pays for them.
-  const uint64_t odd_lanes = __ballot(active && !lost && sees > j0 && !(odd == 0.f));
-  uint32_t todo = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
-  const bool mine = active && !((todo >> (lane & 31)) & 1u);
-  auto unit_of = [&](int rt, float*& po, float*& pml) {  // rt: row of the tile
+    for (int e = 0; e < 16; ++e) odd += tile.o[d][e] * 0.f;
+  auto unit_of = [&](int rt, float*& po, float*& ml) {  // rt: row of the tile
     float* u = part + (rt / SEQ_FEW) * sq_unit_floats(SEQ_FEW, HD);
     po = u + (rt % SEQ_FEW) * HD;
-    pml = u + SEQ_FEW * HD + rt % SEQ_FEW;
+    ml = u + SEQ_FEW * HD + rt % SEQ_FEW;
   };
-  if (mine && !part) {
+  const float by = sees > 0 ? inv : 0.f;
+  if (active && !part) {
     T* orow = (T*)a.o + tok * a.o_st + h * a.o_sh + 4 * (lane >> 5);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4)
-        st64(orow + 32 * d + 8 * q4, u32x2{pack2<T>(tile.o[d][4 * q4], tile.o[d][4 * q4 + 1]),
-                                           pack2<T>(tile.o[d][4 * q4 + 2], tile.o[d][4 * q4 + 3])});
-  } else if (mine) {
-    float *po, *pml;
-    unit_of(r - r0, po, pml);
+        st64(orow + 32 * d + 8 * q4, u32x2{pack2<T>(tile.o[d][4 * q4] * by, tile.o[d][4 * q4 + 1] * by),
+                                           pack2<T>(tile.o[d][4 * q4 + 2] * by, tile.o[d][4 * q4 + 3] * by)});
+  } else if (active) {
+    float *po, *ml;
+    unit_of(r - r0, po, ml);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4)
-        store4<float>(po + 32 * d + 8 * q4 + 4 * (lane >> 5), (const float*)&tile.o[d] + 4 * q4);
-    if (lane < 32) {
-      pml[0] = lost ? __builtin_nanf("") : tile.m_run;
-      pml[SEQ_FEW] = l * exp2f(-Tile::BIAS);
+        *reinterpret_cast<f32x4*>(po + 32 * d + 8 * q4 + 4 * (lane >> 5)) =
+            f32x4{tile.o[d][4 * q4] * by, tile.o[d][4 * q4 + 1] * by, tile.o[d][4 * q4 + 2] * by, tile.o[d][4 * q4 + 3] * by};
+    if (lane < 32) {  // (a sum that is no number: the row is NaN)
+      ml[0] = lost || !(l == l) ? __builtin_nanf("") : tile.m_run;
+      ml[SEQ_FEW] = l * exp2f(-Tile::BIAS);
     }
   }
-  while (todo != 0) {
-    const int i = __builtin_ctz(todo), ri = w0 + i;
-    todo &= todo - 1;
-    float *po = nullptr, *pml = nullptr;
-    if (part) unit_of(ri - r0, po, pml);
-    const int ti = seq_div(ri, a.by_group);
-    sq_row_again<T, HD, PAGED>(a, hp, q0 + ti, hk * G + ri - ti * G, j0, min(keys_of(ri), lim), po, pml, SEQ_FEW);
+  // (l = 0: every score is -inf; of a part, hidden keys are no reason for NaN)
+  const uint64_t odd_lanes = __ballot(active && !lost && sees > j0 && l == l && (l != 0.f || part) && !(odd == 0.f));
+  const uint32_t odd_rows = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
+#pragma unroll 1
+  for (int x = 0; x < 32; x += 16) {
+    if (!(odd_rows & (0xFFFFu << x))) continue;
+    const int row = x + (lane & 15), ri = min(w0 + row, r0 + n - 1);
+    float *po = nullptr, *ml;
+    if (part) unit_of(ri - r0, po, ml);
+    sq_odd_rows<T, HD, PAGED>(b, q0, hk, ri, (odd_rows >> row) & 1u, min(keys_of(ri), lim), j0, __shfl(tile.m_run, row, 64),
+                              __shfl(l, row, 64), Tile::BIAS, po, lane);
   }
 }
 
 // ------------------------------------------------------------- packed prompts
 template <typename T, int HD>
-__global__ __launch_bounds__(SQ_THREADS, 2) void seq_attn_packed_kernel(SeqAttnArgs a, SeqOrder order) {
+__global__ __launch_bounds__(SQ_THREADS, HD == 64 ? 4 : 2) void seq_attn_packed_kernel(SeqAttnArgs a, SeqOrder order) {
   __shared__ __attribute__((aligned(16))) T lds[SqTile<T, HD, false>::LDS_ELEMS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   int hk;
@@ -780,19 +922,20 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
       odd += v * 0.f;
     }
   }
-  const bool redo = active && !lost && sees > j0 && !(odd == 0.f);
+  // (as in a tile)
+  const bool redo = active && !lost && sees > j0 && L == L && (L != 0.f || part) && !(odd == 0.f);
   if (redo) sagain[row] = 1;
   __syncthreads();
   const int ir = seq_div(rr, a.by_group);
   const int64_t tk = w.q0 + ir;
   const int hh = hk * G + rr - ir * G;
-  if (active && !sagain[row]) {
+  if (active) {
     if (part) {
       float* po = part + row * HD + d0;
 #pragma unroll
       for (int y = 0; y < DT / 4; ++y) store4<float>(po + 64 * y, res + 4 * y);
-      if ((threadIdx.x & 15) == 0) {
-        part[w.cut.unit_rows * HD + row] = lost ? __builtin_nanf("") : M;
+      if ((threadIdx.x & 15) == 0) {  // (a sum that is no number: the row is NaN)
+        part[w.cut.unit_rows * HD + row] = lost || !(L == L) ? __builtin_nanf("") : M;
         part[w.cut.unit_rows * HD + w.cut.unit_rows + row] = L * exp2f(-F::BIAS);
       }
     } else {
@@ -801,14 +944,17 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
       for (int y = 0; y < DT / 4; ++y) store4<T>(orow + 64 * y, res + 4 * y);
     }
   }
-  for (int i = wave; i < n; i += 4) {
-    if (!sagain[i]) continue;  // wave-uniform
-    const int ri = r0 + i;
-    const int ti = seq_div(ri, a.by_group);
-    sq_row_again<T, HD, true>(a, hp, w.q0 + ti, hk * G + ri - ti * G, j0, min(keys_of(ri), lim),
-                              part ? part + i * HD : nullptr, part ? part + w.cut.unit_rows * HD + i : nullptr,
-                              w.cut.unit_rows);
+  if (!__any(sagain[col])) return;  // (the same in every wave)
+  // Wave 0 sees to the rows that are not finite, once all are stored.
+  if ((threadIdx.x & 15) == 0) {
+    stat[row] = M;
+    stat[64 + row] = L;
   }
+  __syncthreads();
+  if (wave != 0) return;
+  const int ro = min(col, n - 1);
+  sq_odd_rows<T, HD, true>(w.b, w.q0, hk, r0 + ro, col < n && sagain[col] != 0, min(keys_of(r0 + ro), lim), j0, stat[col],
+                           stat[64 + col], F::BIAS, part ? part + ro * HD : nullptr, lane);
 }
 
 // ---------------------------------------------------------------- paged calls
@@ -819,7 +965,7 @@ __host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
 // Persistent workgroups over the items of a call (SeqWalk); a grid of at most
 // the items, so every workgroup's loop ends.
 template <typename T, int HD, bool FEW_ONLY>
-__global__ __launch_bounds__(SQ_THREADS, FEW_ONLY && HD == 64 ? 4 : 2) void seq_attn_paged_kernel(SeqAttnArgs a) {
+__global__ __launch_bounds__(SQ_THREADS, HD == 64 ? (FEW_ONLY ? 4 : 3) : 2) void seq_attn_paged_kernel(SeqAttnArgs a) {
   constexpr int TILE_ELEMS = SqTile<T, HD, true>::LDS_ELEMS, FEW_ELEMS = 4 * SqFew<T, HD>::WAVE_ELEMS;
   constexpr int ELEMS = FEW_ONLY || FEW_ELEMS > TILE_ELEMS ? FEW_ELEMS : TILE_ELEMS;
   __shared__ __attribute__((aligned(16))) T lds[ELEMS];
