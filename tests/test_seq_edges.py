@@ -157,6 +157,25 @@ def test_paged_attention_of_values_that_are_not_finite(cuda, dtype, hd, h, hk, n
             _strictly_same(got, want, tol, f"{i}: {new} over {keys}, {h}/{hk} hd{hd} causal={causal} {dtype}")
 
 
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,keys", [(1, 40), (3, 5000), (200, 200), (40, 5000)])
+def test_values_near_the_end_of_the_range_do_not_overflow(cuda, hd, new, keys):
+    """bf16 values whose sums, weighted but not yet normalised, pass fp32's range."""
+    dtype, h, hk = torch.bfloat16, 4, 2
+    k, v, kc, vc, table = _paged([keys], hk, 16, hd, dtype, cuda, 240)
+    v[0].copy_((v[0].float().abs().clamp(max=1) * 0.5 + 2.5) * 1e38)
+    j = torch.arange(keys, device=cuda)
+    vc[table[0, j // 16].long(), :, j % 16] = v[0]
+    q = _randn((new, h, hd), dtype, cuda, 241)
+    want, tol = _ieee(q, k[0], v[0], hd**-0.5, True, dtype)
+    got = _C.flash_attn_paged(q, kc, vc, table, _cu([new], cuda), _i32([keys], cuda), hd**-0.5)
+    _strictly_same(got, want, tol, f"paged {new} over {keys} hd{hd}")
+    if new == keys:
+        got = _C.flash_attn_packed(q, k[0], v[0], _cu([new], cuda), hd**-0.5, True)
+        _strictly_same(got, want, tol, f"packed {new} hd{hd}")
+
+
 def _time_us(fn):
     for _ in range(3):
         fn()

@@ -1073,14 +1073,17 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
 #pragma unroll
   for (int x = 0; x < MLS; ++x) L += weight(m[x], l[x]);
   L = wave_sum(L);
+  // Scaled by a power of two to a sum in [1/2, 1): the same bits, and values
+  // near the end of fp32's range add up within it.
+  const int scale = -__builtin_amdgcn_frexp_expf(L);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int b = 0; b < parts; b += GRP * NP) {
     if (b > 0) fetch(b);
 #pragma unroll
     for (int x = 0; x < NP; ++x) {
-      const float f = weight(om[x], ol[x]);
+      const float f = ldexpf(weight(om[x], ol[x]), scale);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += f == 0.f ? 0.f : f * o[x][e];
+      for (int e = 0; e < 4; ++e) acc[e] += f * o[x][e];
     }
   }
   if constexpr (WAVE) {
@@ -1102,7 +1105,7 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
   if (tid < LPR) {
     float out[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = L != 0.f ? acc[e] / L : (sees > 0 ? __builtin_nanf("") : 0.f);
+    for (int e = 0; e < 4; ++e) out[e] = L != 0.f ? acc[e] / ldexpf(L, scale) : (sees > 0 ? __builtin_nanf("") : 0.f);
     store4<T>((T*)a.o + (int64_t)(w.q0 + i) * a.o_st + (int64_t)(hk * a.group + r - i * a.group) * a.o_sh + 4 * tid, out);
   }
 }
