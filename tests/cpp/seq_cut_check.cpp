@@ -1,6 +1,7 @@
 // The cut of a paged attention call (csrc/seq_cut.hpp): every row and key in
 // one item, never more parts than the join holds, and the host's bounds on
-// items, partial results and rows to join kept by every split of the totals.
+// items, partial results and rows to join kept by every split of the totals, and
+// of a reasonable size for ordinary calls.
 // Prints "ok" or what failed.
 #include <stdio.h>
 
@@ -22,7 +23,7 @@ static int64_t below(int64_t n) { return (int64_t)(rng() % (uint64_t)n); }
 
 static void check_cut(const SeqShape& s, int rows, int keys) {
   const SeqCut c = seq_cut_of(s, rows, keys);
-  const int tile = c.few ? c.unit_rows : SEQ_TILE;
+  const int tile = c.tile_rows;
   bool ok = c.parts >= 1 && c.parts <= SEQ_JOIN_PARTS;
   ok = ok && (int64_t)c.tiles * tile >= rows && (int64_t)(c.tiles - 1) * tile < rows;
   if (keys > 0)
@@ -44,8 +45,7 @@ int main() {
       for (int few : {0, 1, 4, 16})
         for (int rows : rows_at)
           for (int keys : keys_at) {
-            const SeqShape s = seq_shape(1 << 20, 1, 1, hk, few ? few : 1 << 20, cus);
-            check_cut(s, rows, keys);
+            for (int hd : {64, 128}) check_cut(seq_shape(1 << 20, 1, 1, hk, hd, few ? few : 1 << 20, cus), rows, keys);
           }
   // Split totals over the sequences at random; the calls' actual work.
   for (int trial = 0; trial < 20000 && fails < 10; ++trial) {
@@ -53,9 +53,9 @@ int main() {
     const int64_t cap = (int64_t)8 << below(20);
     const int64_t tokens = 1 + below(trial % 2 ? 64 : 3000);
     const int64_t max_q = trial % 4 == 0 ? tokens : 1 + below(tokens);  // may be too small
-    const SeqShape s = seq_shape(tokens, batch, group, hk, max_q, 256);
+    const SeqShape s = seq_shape(tokens, batch, group, hk, trial % 7 ? 128 : 64, max_q, 256);
     const SeqBounds b = seq_bounds(s, tokens, batch, cap);
-    int64_t left = tokens, items = 0, units = 0, joins = 0;
+    int64_t left = tokens, items = 0, partials = 0, joins = 0;
     for (int i = 0; i < batch; ++i) {
       const int64_t most = trial % 5 == 0 ? (128 / group > 0 ? 128 / group : 1) : left;
       const int64_t n = i + 1 == batch && trial % 2 ? left : below((most < left ? most : left) + 1);
@@ -65,13 +65,31 @@ int main() {
       check_cut(s, rows, keys);
       const SeqCut c = seq_cut_of(s, rows, keys);
       items += (int64_t)c.tiles * c.parts * hk;
-      units += (int64_t)c.tiles * c.parts * hk * c.units;
+      if (c.parts > 1) partials += (int64_t)rows * hk * c.parts;
       if (c.parts > 1) joins += c.parts <= SEQ_WAVE_PARTS ? (rows * hk + 3) / 4 : rows * hk;
     }
-    if (items > b.items || units > b.units || joins > b.join_rows) {
-      printf("FAIL group %d kv_heads %d batch %d tokens %ld cap %ld max_q %ld: items %ld of %ld, units %ld of %ld, joins "
-             "%ld of %ld\n", group, hk, batch, (long)tokens, (long)cap, (long)max_q, (long)items, (long)b.items, (long)units,
-             (long)b.units, (long)joins, (long)b.join_rows);
+    if (items > b.items || partials > b.partials || joins > b.join_rows) {
+      printf("FAIL group %d kv_heads %d batch %d tokens %ld cap %ld max_q %ld: items %ld of %ld, partials %ld of %ld, joins "
+             "%ld of %ld\n", group, hk, batch, (long)tokens, (long)cap, (long)max_q, (long)items, (long)b.items,
+             (long)partials, (long)b.partials, (long)joins, (long)b.join_rows);
+      ++fails;
+    }
+  }
+  // Partial results of head_dim + 2 floats of calls as servers make them: one
+  // chunk of 512 tokens among single ones, and those alone (without max_q_len).
+  const struct {
+    int64_t tokens, batch;
+    int heads, hk;
+    int64_t cap, max_q, mib;
+  } calls[] = {{768, 257, 16, 4, 131072, 512, 400}, {576, 65, 16, 4, 32768, 512, 300}, {576, 65, 32, 8, 131072, 512, 300},
+               {768, 257, 64, 8, 131072, 512, 800}, {535, 24, 16, 2, 8192, 512, 80},   {64, 64, 16, 4, 32768, 64, 33},
+               {64, 64, 16, 4, 32768, 1, 33},       {512, 1, 16, 4, 32768, 512, 40}};
+  for (const auto& c : calls) {
+    const SeqShape s = seq_shape(c.tokens, c.batch, c.heads / c.hk, c.hk, 128, c.max_q, 256);
+    const int64_t mib = (seq_bounds(s, c.tokens, c.batch, c.cap).partials * 130 * 4) >> 20;
+    if (mib > c.mib) {
+      printf("FAIL %ld tokens of %ld sequences, %d/%d heads, %ld keys: %ld MiB of workspace\n", (long)c.tokens,
+             (long)c.batch, c.heads, c.hk, (long)c.cap, (long)mib);
       ++fails;
     }
   }

@@ -249,3 +249,27 @@ def test_one_kv_head_over_a_very_long_cache(cuda, hd, h, new, keys):
     got = _C.flash_attn_paged(q, kc, vc, table, _cu([new], cuda), _i32([keys], cuda), hd**-0.5, max_q_len=new)
     want, tol = _attend(q, ks[0], vs[0], hd**-0.5, True, dtype)
     _same(got, want, tol, f"{new} tokens, {h}/1 heads, {keys} keys, hd{hd}")
+
+
+# -------------------------------------------------------------- workspaces
+@gpu
+@pytest.mark.parametrize("hd,h,hk,new,lens", [
+    (128, 16, 4, [1] * 20 + [150], [3000] * 21), (64, 8, 8, [1] * 9 + [300, 40], [5000] * 11), (128, 8, 1, [17], [40000]),
+    (64, 16, 1, [2, 1, 9], [30000, 70, 9000]), (128, 4, 4, [1, 1, 1], [9000, 1, 700]), (64, 6, 2, [5, 6, 40], [2000, 2000, 2000]),
+])
+@pytest.mark.parametrize("hint", [False, True])
+def test_a_call_stays_within_the_workspace_it_asks_for(cuda, hd, h, hk, new, lens, hint):
+    dtype, page = torch.bfloat16, 64
+    ks, vs, kc, vc, table = _paged(lens, hk, page, hd, dtype, cuda, 260)
+    q = _randn((sum(new), h, hd), dtype, cuda, 261)
+    most = max(new) if hint else 0
+    need = _C.flash_attn_paged_workspace(sum(new), len(new), h, hk, hd, page, table.shape[1], most)
+    ws = torch.full((need + 4096,), 2.0, device=cuda)
+    got = _C.flash_attn_paged(q, kc, vc, table, _cu(new, cuda), _i32(lens, cuda), hd**-0.5, max_q_len=most,
+                              workspace=ws[:need])
+    assert bool((ws[need:] == 2).all())
+    at = 0
+    for b, n in enumerate(new):
+        want, tol = _attend(q[at:at + n], ks[b], vs[b], hd**-0.5, True, dtype)
+        _same(got[at:at + n], want, tol, f"sequence {b}")
+        at += n

@@ -381,10 +381,6 @@ __device__ __forceinline__ int sq_bad_from(int mine, int* slot, int wave, int la
   return min(min(slot[0], slot[1]), min(slot[2], slot[3]));
 }
 
-// Partial results of unit_rows rows over one part of their keys: o (fp32,
-// normalised) [unit_rows][HD], then the rows' maxima m (log2 units) and sums l.
-__host__ __device__ constexpr int64_t sq_unit_floats(int rows, int hd) { return (int64_t)((rows * (hd + 2) + 3) & ~3); }
-
 // The kernel's first argument, read where this is called and not before.
 __device__ __forceinline__ const SeqAttnArgs& sq_args_again() {
   uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
@@ -586,11 +582,11 @@ __device__ __forceinline__ void sq_odd_rows(int b, int q0, int hk, int r, bool n
 }
 
 // Rows [r0, r0 + 128) of a sequence over the keys [j0, j1) (j0 and, but for
-// the last part, j1 multiples of 64).  part: where their partial results go, or
-// nullptr for the output.
+// the last part, j1 multiples of 64).  part, ml: where the partial results of
+// the tile's rows go, or nullptr for the output.
 template <typename T, int HD, bool PAGED>
 __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0, int qn, int kvn, int hk, int r0,
-                                             int j0, int j1, float* part, T* lds, int* bad, int lane, int wave) {
+                                             int j0, int j1, float* part, float* ml, T* lds, int* bad, int lane, int wave) {
   typedef SqTile<T, HD, PAGED> Tile;
   const int G = a.group, n = min(qn * G - r0, SQ_ROWS);
   const int cap = PAGED ? a.s.max_pages << a.s.page_log2 : kvn;
@@ -643,11 +639,6 @@ __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0
   for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) odd += tile.o[d][e] * 0.f;
-  auto unit_of = [&](int rt, float*& po, float*& ml) {  // rt: row of the tile
-    float* u = part + (rt / SEQ_FEW) * sq_unit_floats(SEQ_FEW, HD);
-    po = u + (rt % SEQ_FEW) * HD;
-    ml = u + SEQ_FEW * HD + rt % SEQ_FEW;
-  };
   const float by = sees > 0 ? inv : 0.f;
   if (active && !part) {
     T* orow = (T*)a.o + tok * a.o_st + h * a.o_sh + 4 * (lane >> 5);
@@ -658,8 +649,7 @@ __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0
         st64(orow + 32 * d + 8 * q4, u32x2{pack2<T>(tile.o[d][4 * q4] * by, tile.o[d][4 * q4 + 1] * by),
                                            pack2<T>(tile.o[d][4 * q4 + 2] * by, tile.o[d][4 * q4 + 3] * by)});
   } else if (active) {
-    float *po, *ml;
-    unit_of(r - r0, po, ml);
+    float* po = part + (r - r0) * HD;
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
@@ -667,21 +657,20 @@ __device__ __forceinline__ void sq_tile_item(const SeqAttnArgs& a, int b, int q0
         *reinterpret_cast<f32x4*>(po + 32 * d + 8 * q4 + 4 * (lane >> 5)) =
             f32x4{tile.o[d][4 * q4] * by, tile.o[d][4 * q4 + 1] * by, tile.o[d][4 * q4 + 2] * by, tile.o[d][4 * q4 + 3] * by};
     if (lane < 32) {  // (a sum that is no number: the row is NaN)
-      ml[0] = lost || !(l == l) ? __builtin_nanf("") : tile.m_run;
-      ml[SEQ_FEW] = l * exp2f(-Tile::BIAS);
+      ml[2 * (r - r0)] = lost || !(l == l) ? __builtin_nanf("") : tile.m_run;
+      ml[2 * (r - r0) + 1] = l * exp2f(-Tile::BIAS);
     }
   }
   // (l = 0: every score is -inf; of a part, hidden keys are no reason for NaN)
   const uint64_t odd_lanes = __ballot(active && !lost && sees > j0 && l == l && (l != 0.f || part) && !(odd == 0.f));
   const uint32_t odd_rows = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
+  if (__builtin_expect(odd_rows == 0, 1)) return;
 #pragma unroll 1
   for (int x = 0; x < 32; x += 16) {
     if (!(odd_rows & (0xFFFFu << x))) continue;
     const int row = x + (lane & 15), ri = min(w0 + row, r0 + n - 1);
-    float *po = nullptr, *ml;
-    if (part) unit_of(ri - r0, po, ml);
     sq_odd_rows<T, HD, PAGED>(b, q0, hk, ri, (odd_rows >> row) & 1u, min(keys_of(ri), lim), j0, __shfl(tile.m_run, row, 64),
-                              __shfl(l, row, 64), Tile::BIAS, po, lane);
+                              __shfl(l, row, 64), Tile::BIAS, part ? part + (ri - r0) * HD : nullptr, lane);
   }
 }
 
@@ -694,7 +683,7 @@ __global__ __launch_bounds__(SQ_THREADS, HD == 64 ? 4 : 2) void seq_attn_packed_
   const SeqTile t = seq_ordered(a.s, a.group, SQ_ROWS, order, a.kv_heads, (int)blockIdx.x, hk);
   const int r0 = t.tile * SQ_ROWS;
   if (r0 >= t.qn * a.group) return;
-  sq_tile_item<T, HD, false>(a, t.b, t.q0, t.qn, t.qn, hk, r0, 0, 0x7fffffff, nullptr, lds, nullptr, lane, wave);
+  sq_tile_item<T, HD, false>(a, t.b, t.q0, t.qn, t.qn, hk, r0, 0, 0x7fffffff, nullptr, nullptr, lds, nullptr, lane, wave);
 }
 
 // -------------------------------------------------------------- few rows
@@ -731,12 +720,13 @@ struct SqFew {
 
 template <typename T, int HD>
 __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork& w, int hk, int r0, int j0, int j1,
-                                            float* part, T* lds, float* stat, int* bad, int lane, int wave) {
+                                            float* part, float* ml, T* lds, float* stat, int* bad, int lane,
+                                            int wave) {
   typedef SqFew<T, HD> F;
   typedef typename F::vec vec;
   const float NEG_INF = -__builtin_inff();
   const float c = a.scale * SQ_LOG2E;
-  const int G = a.group, n = min(w.qn * G - r0, w.cut.unit_rows);
+  const int G = a.group, n = min(w.qn * G - r0, w.cut.tile_rows);
   const int cap = a.s.max_pages << a.s.page_log2, ps1 = (1 << a.s.page_log2) - 1;
   auto keys_of = [&](int r) { return max(a.causal ? w.kvn - w.qn + seq_div(r, a.by_group) + 1 : w.kvn, 0); };
   const int lim = seq_uni(min(min(keys_of(r0 + n - 1), cap), j1));
@@ -935,8 +925,8 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
 #pragma unroll
       for (int y = 0; y < DT / 4; ++y) store4<float>(po + 64 * y, res + 4 * y);
       if ((threadIdx.x & 15) == 0) {  // (a sum that is no number: the row is NaN)
-        part[w.cut.unit_rows * HD + row] = lost || !(L == L) ? __builtin_nanf("") : M;
-        part[w.cut.unit_rows * HD + w.cut.unit_rows + row] = L * exp2f(-F::BIAS);
+        ml[2 * row] = lost || !(L == L) ? __builtin_nanf("") : M;
+        ml[2 * row + 1] = L * exp2f(-F::BIAS);
       }
     } else {
       T* orow = (T*)a.o + tk * a.o_st + hh * a.o_sh + d0;
@@ -944,7 +934,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
       for (int y = 0; y < DT / 4; ++y) store4<T>(orow + 64 * y, res + 4 * y);
     }
   }
-  if (!__any(sagain[col])) return;  // (the same in every wave)
+  if (__builtin_expect(!__any(sagain[col]), 1)) return;  // (the same in every wave)
   // Wave 0 sees to the rows that are not finite, once all are stored.
   if ((threadIdx.x & 15) == 0) {
     stat[row] = M;
@@ -959,7 +949,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
 
 // ---------------------------------------------------------------- paged calls
 __host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
-  return SeqShape{a.group, a.kv_heads, a.cus, a.few_parts, a.few};
+  return SeqShape{a.group, a.kv_heads, a.cus, a.head_dim == 128 ? 2 : 1, a.few_parts, a.few};
 }
 
 // Persistent workgroups over the items of a call (SeqWalk); a grid of at most
@@ -989,15 +979,19 @@ __global__ __launch_bounds__(SQ_THREADS, HD == 64 ? (FEW_ONLY ? 4 : 3) : 2) void
     const int tile = w.cut.tiles > 1 ? seq_uni(u / np) : 0, pair = u - tile * np;
     const int p = seq_uni(seq_div(pair, a.by_kv_heads)), hk = pair - p * a.kv_heads;
     const int j0 = p * w.cut.part_keys, j1 = p + 1 < w.cut.parts ? j0 + w.cut.part_keys : 0x7fffffff;
-    float* part = nullptr;
-    if (w.cut.parts > 1) part = a.ws + (int64_t)(w.unit + u * w.cut.units) * sq_unit_floats(w.cut.unit_rows, HD);
+    // Partial results of a sequence: by tile, part, K/V head, row of the tile.
+    const int r0 = tile * w.cut.tile_rows;
+    float *part = nullptr, *ml = nullptr;
+    if (w.cut.parts > 1) {
+      const int64_t at = w.partial + r0 * np + pair * min(w.qn * a.group - r0, w.cut.tile_rows);
+      part = a.ws + at * HD;
+      ml = a.ws_ml + at * 2;
+    }
     if constexpr (FEW_ONLY) {
-      sq_few_item<T, HD>(a, w, hk, tile * w.cut.unit_rows, j0, j1, part, lds, stat, bad, lane, wave);
+      sq_few_item<T, HD>(a, w, hk, r0, j0, j1, part, ml, lds, stat, bad, lane, wave);
     } else {
-      if (w.cut.few)
-        sq_few_item<T, HD>(a, w, hk, tile * w.cut.unit_rows, j0, j1, part, lds, stat, bad, lane, wave);
-      else
-        sq_tile_item<T, HD, true>(a, w.b, w.q0, w.qn, w.kvn, hk, tile * SQ_ROWS, j0, j1, part, lds, bad, lane, wave);
+      if (w.cut.few) sq_few_item<T, HD>(a, w, hk, r0, j0, j1, part, ml, lds, stat, bad, lane, wave);
+      else sq_tile_item<T, HD, true>(a, w.b, w.q0, w.qn, w.kvn, hk, r0, j0, j1, part, ml, lds, bad, lane, wave);
     }
     __syncthreads();  // LDS belongs to the next item
   }
@@ -1019,30 +1013,33 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
   const int lane = tid & 63;
   if (WAVE) tid = lane;
   const float NEG_INF = -__builtin_inff();
-  const int tr = w.cut.few ? w.cut.unit_rows : SQ_ROWS;
-  const int tile = w.cut.tiles == 1 ? 0 : (w.cut.few ? seq_uni(r / tr) : r / SQ_ROWS), rt = r - tile * tr;
-  const int unit = w.cut.few ? 0 : rt / SEQ_FEW, ru = rt - unit * SEQ_FEW;
-  const int np = w.cut.parts * a.kv_heads;
-  const int64_t uf = sq_unit_floats(w.cut.unit_rows, HD);
-  // Byte offsets from the row's first part: at most (2 CUs + kv_heads) units
-  // of a tile's rows, below 2^32.
-  const char* first = (const char*)(a.ws + ((int64_t)w.unit + (int64_t)(tile * np + hk) * w.cut.units + unit) * uf);
-  const uint32_t step = (uint32_t)(a.kv_heads * w.cut.units) * (uint32_t)(uf * 4);  // from part to part
+  const int tr = w.cut.tile_rows;
+  const int tile = w.cut.tiles == 1 ? 0 : (w.cut.few ? seq_uni(r / tr) : r / SQ_ROWS), r0 = tile * tr;
+  const int n = min(w.qn * a.group - r0, tr);
+  const int64_t at = w.partial + r0 * w.cut.parts * a.kv_heads + hk * n + r - r0;  // of part 0
+  // Byte offsets from there to a part's: at most (2 CUs + kv_heads) times a
+  // tile's rows, below 2^32.
+  const char *first = (const char*)(a.ws + at * HD), *ml = (const char*)(a.ws_ml + at * 2);
+  const uint32_t step = (uint32_t)(a.kv_heads * n) * 8u, step_o = step * (HD / 2);
   const int i = seq_uni(seq_div(r, a.by_group));
   const int sees = max(a.causal ? w.kvn - w.qn + i + 1 : w.kvn, 0);
   int parts = w.cut.parts;  // those the row sees
   while (parts > 0 && (parts - 1) * w.cut.part_keys >= sees) --parts;
-  const char* ml = first + (uint32_t)(w.cut.unit_rows * HD + ru) * 4u;
-  const uint32_t lo = (uint32_t)w.cut.unit_rows * 4u, po = (uint32_t)(ru * HD + (tid % LPR) * 4) * 4u;
-  auto f32_at = [](const char* base, uint32_t off) { return *reinterpret_cast<const float*>(base + off); };
+  const uint32_t po = (uint32_t)(tid % LPR) * 16u;
+  auto ml_at = [&](uint32_t off, float& pm, float& pl) {
+    const u32x2 x = ld64(ml + off);
+    pm = __builtin_bit_cast(float, (uint32_t)x[0]);
+    pl = __builtin_bit_cast(float, (uint32_t)x[1]);
+  };
   const int p0 = tid / LPR;
 
   float m[MLS], l[MLS];
 #pragma unroll
   for (int x = 0; x < MLS; ++x) {
     const int p = lane + 64 * x;
-    m[x] = p < parts ? f32_at(ml, p * step) : NEG_INF;
-    l[x] = p < parts ? f32_at(ml, p * step + lo) : 0.f;
+    m[x] = NEG_INF;
+    l[x] = 0.f;
+    if (p < parts) ml_at(p * step, m[x], l[x]);
   }
   f32x4 o[NP];
   float om[NP], ol[NP];
@@ -1054,9 +1051,8 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
       om[x] = NEG_INF;
       ol[x] = 0.f;
       if (p < parts) {
-        o[x] = *reinterpret_cast<const f32x4*>(first + (po + p * step));
-        om[x] = f32_at(ml, p * step);
-        ol[x] = f32_at(ml, p * step + lo);
+        o[x] = *reinterpret_cast<const f32x4*>(first + (po + p * step_o));
+        ml_at(p * step, om[x], ol[x]);
       }
     }
   };
@@ -1139,7 +1135,7 @@ static SeqBounds sq_bounds(const SeqAttnArgs& a) {
 }
 static void sq_finish(SeqAttnArgs& a) {
   const int cus = device_cu_count();
-  const SeqShape s = seq_shape(a.s.tokens, a.s.batch, a.group, a.kv_heads, a.max_q_len, cus > 0 ? cus : 256);
+  const SeqShape s = seq_shape(a.s.tokens, a.s.batch, a.group, a.kv_heads, a.head_dim, a.max_q_len, cus > 0 ? cus : 256);
   a.cus = s.cus;
   a.few_parts = s.few_parts;
   a.few = s.few;
@@ -1148,7 +1144,7 @@ static void sq_finish(SeqAttnArgs& a) {
 int64_t seq_attention_workspace(const SeqAttnArgs& a0) {
   SeqAttnArgs a = a0;
   sq_finish(a);
-  return sq_bounds(a).units * sq_unit_floats(a.few ? a.few : SEQ_FEW, a.head_dim);
+  return sq_bounds(a).partials * (a.head_dim + 2);
 }
 
 template <typename T, int HD>
@@ -1163,13 +1159,14 @@ static int launch_hd(SeqAttnArgs a, hipStream_t st) {
   }
   sq_finish(a);
   const SeqBounds b = sq_bounds(a);
+  a.ws_ml = a.ws + b.partials * HD;
   auto grid = [](int64_t items, int64_t most) { return dim3((unsigned)(items < most ? items : most)); };
   // As many workgroups as are resident: few rows 4 a CU at head dim 64 and 2 at
   // 128, tiles 3 and 2.
   if (a.few) seq_attn_paged_kernel<T, HD, true><<<grid(b.items, (HD == 64 ? 4 : 2) * a.cus), block, 0, st>>>(a);
   else seq_attn_paged_kernel<T, HD, false><<<grid(b.items, (HD == 64 ? 3 : 2) * a.cus), block, 0, st>>>(a);
   if (hipGetLastError() != hipSuccess) return TX_EHIP;
-  if (b.units > 0) {
+  if (b.partials > 0) {
     seq_attn_join_kernel<T, HD><<<grid(b.join_rows, 4 * a.cus), block, 0, st>>>(a);
     if (hipGetLastError() != hipSuccess) return TX_EHIP;
   }

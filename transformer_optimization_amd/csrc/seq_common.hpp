@@ -142,12 +142,12 @@ __device__ __forceinline__ SeqTile seq_ordered(const SeqArgs& s, int group, int 
 }
 
 // ---- the items of a paged call (seq_cut.hpp) ------------------------------
-// A sequence of a paged call: its cut, its first item and its first unit of
-// partial results, both counted over the call.
+// A sequence of a paged call: its cut, its first item and its first partial
+// result, both counted over the call.
 struct SeqWork {
   int b, q0, qn, kvn;
   SeqCut cut;
-  int item, unit;
+  int item, partial;
 };
 
 // Walks the items of a call in ascending order, 64 sequences at a time (lane
@@ -157,13 +157,13 @@ struct SeqWork {
 // wave writes alike between two barriers.
 struct SeqWalk {
   struct Lane {
-    int n_items, n_units;    // of this lane's sequence
-    int at_item, at_unit;    // behind its last item and unit (from base on)
+    int n_items, n_partials;    // of this lane's sequence
+    int at_item, at_partial;    // behind its last item and partial result (from base on)
     int q0, qn, kvn;
     int tiles, parts, part_keys;
   };
   static constexpr int LDS_INTS = 64 * 10;
-  int base, items, units;  // before sequence base
+  int base, items, partials;  // before sequence base
   int row;                 // first row that sequence base may hold
   int* lds;                // LDS_INTS of the workgroup
 
@@ -180,11 +180,11 @@ struct SeqWalk {
     const int n = min(s.batch - base, 64);  // the scans need log2(n) steps
     for (int o = 1; o < n; o <<= 1) x.q0 = max(x.q0, __shfl_up(x.q0, o, 64));  // (lanes below o see themselves)
     x.qn = max(end - x.q0, 0);
-    x.n_items = x.n_units = x.tiles = x.parts = x.part_keys = 0;
+    x.n_items = x.n_partials = x.tiles = x.parts = x.part_keys = 0;
     if (x.qn > 0) {
       const SeqCut c = seq_cut_of(sh, x.qn * sh.group, min(x.kvn, s.max_pages << s.page_log2));
       x.n_items = c.tiles * c.parts * sh.kv_heads;
-      x.n_units = x.n_items * c.units;
+      x.n_partials = c.parts > 1 ? x.qn * sh.group * sh.kv_heads * c.parts : 0;
       x.tiles = c.tiles;
       x.parts = c.parts;
       x.part_keys = c.part_keys;
@@ -194,22 +194,22 @@ struct SeqWalk {
       }
     }
     x.at_item = x.n_items;
-    x.at_unit = x.n_units;
+    x.at_partial = x.n_partials;
     for (int o = 1; o < n; o <<= 1) {
-      const int i = __shfl_up(x.at_item, o, 64), u = __shfl_up(x.at_unit, o, 64);
+      const int i = __shfl_up(x.at_item, o, 64), u = __shfl_up(x.at_partial, o, 64);
       if (lane >= o) {
         x.at_item += i;
-        x.at_unit += u;
+        x.at_partial += u;
       }
     }
     __syncthreads();  // nobody reads the sequences before these any more
-    const int f[10] = {x.n_items, x.n_units, x.at_item, x.at_unit, x.q0, x.qn, x.kvn, x.tiles, x.parts, x.part_keys};
+    const int f[10] = {x.n_items, x.n_partials, x.at_item, x.at_partial, x.q0, x.qn, x.kvn, x.tiles, x.parts, x.part_keys};
 #pragma unroll
     for (int i = 0; i < 10; ++i) lds[64 * i + lane] = f[i];
     __syncthreads();
   }
   __device__ __forceinline__ void init(const SeqArgs& s, const SeqShape& sh, bool join, int* lds_) {
-    base = items = units = row = 0;
+    base = items = partials = row = 0;
     lds = lds_;
     load(s, sh, join);
   }
@@ -223,7 +223,7 @@ struct SeqWalk {
       if (w - items < in_items) break;
       if (base + 64 >= s.batch) return false;
       items += in_items;
-      units += field(3, last);
+      partials += field(3, last);
       row = field(4, last) + field(5, last);
       base += 64;
       load(s, sh, join);
@@ -236,13 +236,12 @@ struct SeqWalk {
     r.qn = field(5, i);
     r.kvn = field(6, i);
     r.item = items + field(2, i) - field(0, i);
-    r.unit = units + field(3, i) - field(1, i);
+    r.partial = partials + field(3, i) - field(1, i);
     r.cut.few = sh.few > 0 || r.qn * sh.group <= SEQ_FEW;
-    r.cut.unit_rows = sh.few > 0 ? sh.few : SEQ_FEW;
+    r.cut.tile_rows = r.cut.few ? (sh.few > 0 ? sh.few : SEQ_FEW) : SEQ_TILE;
     r.cut.tiles = field(7, i);
     r.cut.parts = field(8, i);
     r.cut.part_keys = field(9, i);
-    r.cut.units = r.cut.parts > 1 ? (r.cut.few ? 1 : SEQ_TILE / SEQ_FEW) : 0;
     return true;
   }
 };

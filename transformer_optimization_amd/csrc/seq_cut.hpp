@@ -27,20 +27,26 @@ constexpr int SEQ_JOIN_PARTS = 256;
 
 struct SeqShape {
   int group, kv_heads, cus;
+  // A single tile's keys are cut as one of so many tiles': of two at head dim
+  // 128, where half as many parts, of twice the keys, are as fast (8192 to
+  // 131072 keys, 1 to 8 K/V heads: -9% to +2%; at head dim 64 up to 35% slower)
+  // and a call's partial results may be half as many.
+  int least_tiles;
   int few_parts;  // most parts of few-row items
   int few;  // rows of a tile when the call has few-row items only (<= SEQ_FEW), else 0
 };
 struct SeqCut {
-  int tiles, parts, part_keys;
-  int unit_rows, units;  // partial results of one item: units of unit_rows rows (0: one part, none)
+  int tiles, tile_rows;
+  int parts, part_keys;  // more than one part: each row has a partial result of each
   bool few;
 };
 constexpr int seq_ceil(int x, int y) { return (x + (y - 1)) / y; }  // (2^30 keys in parts of 2^30 fit)
 constexpr int64_t seq_least(int64_t x, int64_t y) { return x < y ? x : y; }
 
 // max_q_len: at most tokens.
-constexpr SeqShape seq_shape(int64_t tokens, int64_t batch, int group, int kv_heads, int64_t max_q_len, int cus) {
-  SeqShape s{group, kv_heads, cus, 1, 0};
+constexpr SeqShape seq_shape(int64_t tokens, int64_t batch, int group, int kv_heads, int head_dim, int64_t max_q_len,
+                             int cus) {
+  SeqShape s{group, kv_heads, cus, head_dim == 128 ? 2 : 1, 1, 0};
   if (cus / kv_heads > 1) s.few_parts = (int)seq_least(cus / kv_heads, SEQ_JOIN_PARTS);
   const int64_t most = max_q_len * group;
   // Calls of few-row sequences only; where their tiles could pass 32-bit
@@ -52,11 +58,11 @@ constexpr SeqShape seq_shape(int64_t tokens, int64_t batch, int group, int kv_he
 constexpr SeqCut seq_cut_of(const SeqShape& s, int rows, int keys) {
   SeqCut c{};
   c.few = s.few > 0 || rows <= SEQ_FEW;
-  c.unit_rows = s.few > 0 ? s.few : SEQ_FEW;
-  c.tiles = rows <= c.unit_rows ? 1 : (c.few ? seq_ceil(rows, c.unit_rows) : seq_ceil(rows, SEQ_TILE));
+  c.tile_rows = c.few ? (s.few > 0 ? s.few : SEQ_FEW) : SEQ_TILE;
+  c.tiles = rows <= c.tile_rows ? 1 : seq_ceil(rows, c.tile_rows);
   int most = s.few_parts, step = SEQ_PART_FEW;
   if (!c.few) {
-    most = seq_ceil(2 * s.cus, c.tiles * s.kv_heads);
+    most = seq_ceil(2 * s.cus, (c.tiles > s.least_tiles ? c.tiles : s.least_tiles) * s.kv_heads);
     step = 64;  // a key tile
     most = most < keys / SEQ_PART_TILE ? most : keys / SEQ_PART_TILE;
     most = most < SEQ_JOIN_PARTS ? most : SEQ_JOIN_PARTS;
@@ -64,33 +70,37 @@ constexpr SeqCut seq_cut_of(const SeqShape& s, int rows, int keys) {
   most = most < 1 ? 1 : most;
   c.part_keys = seq_ceil(seq_ceil(keys, most), step) * step;
   c.parts = keys > 0 ? seq_ceil(keys, c.part_keys) : 1;
-  c.units = c.parts > 1 ? (c.few ? 1 : SEQ_TILE / SEQ_FEW) : 0;
   return c;
 }
 
 // Upper bounds, over all lengths that these totals allow, of a call's items, of
-// its units of partial results and of the rows to join.  cap: keys of a
-// sequence at most.
+// its partial results (of one row and part each) and of the rows to join.  cap:
+// keys of a sequence at most.
 struct SeqBounds {
-  int64_t items, units, join_rows;
+  int64_t items, partials, join_rows;
 };
 constexpr SeqBounds seq_bounds(const SeqShape& s, int64_t tokens, int64_t batch, int64_t cap) {
   const int64_t rows = tokens * s.group, hk = s.kv_heads, cus = s.cus;
   const int64_t few_parts = seq_least((cap + SEQ_PART_FEW - 1) / SEQ_PART_FEW, s.few_parts);
   const int64_t few_tiles = s.few ? rows / s.few + batch : batch;
-  SeqBounds b{few_tiles * hk * few_parts, 0, 0};
-  b.units = few_parts > 1 ? b.items : 0;
-  b.join_rows = few_parts > 1 ? rows * hk : 0;
+  SeqBounds b{few_tiles * hk * few_parts, few_parts > 1 ? rows * hk * few_parts : 0, 0};
   if (!s.few) {
-    const int64_t seqs = seq_least(batch, rows / (SEQ_FEW + 1));
+    const int64_t seqs = seq_least(batch, rows / (SEQ_FEW + 1));  // of more than SEQ_FEW rows
     const int64_t tiles = (rows / SEQ_TILE + seqs) * hk;
-    int64_t parts = seq_least(seq_least(cap / SEQ_PART_TILE, (2 * cus + hk - 1) / hk), SEQ_JOIN_PARTS);
+    const int64_t hl = hk * s.least_tiles;
+    int64_t parts = seq_least(seq_least(cap / SEQ_PART_TILE, (2 * cus + hl - 1) / hl), SEQ_JOIN_PARTS);
     parts = parts < 1 ? 1 : parts;
-    const int64_t items = seq_least(tiles * parts, tiles + seqs * 2 * cus);
-    b.items += items;
-    b.units += parts > 1 ? items * (SEQ_TILE / SEQ_FEW) : 0;
-    b.join_rows = b.units > 0 ? rows * hk : 0;
+    b.items += seq_least(tiles * parts, tiles + seqs * 2 * cus);
+    // Rows of sequences with few and of others, each in the most parts of its
+    // kind; or, where few sequences bring the others, for each of those at most
+    // r hk (2 cus / (t hk) + 1) of its r <= 128 t rows.
+    const int64_t few = few_parts > 1 ? few_parts : 0, tile = parts > 1 ? parts : 0;
+    const int64_t few_rows = seq_least(rows, batch * SEQ_FEW);
+    const int64_t either = tile >= few ? rows * tile : few_rows * few + (rows - few_rows) * tile;
+    const int64_t tile_most = tile ? seqs * SEQ_TILE * 2 * cus + rows * hk : 0;
+    b.partials = seq_least(either * hk, few_rows * few * hk + tile_most);
   }
+  b.join_rows = b.partials > 0 ? rows * hk : 0;
   return b;
 }
 

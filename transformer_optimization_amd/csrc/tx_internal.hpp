@@ -135,7 +135,8 @@ struct SeqAttnArgs {
   int few;   // rows of a tile where every sequence has few rows (seq_common.hpp), else 0
   int few_parts;  // most parts of the keys of such rows
   int cus;
-  float* ws;
+  float* ws;     // partial results: [rows][head_dim], normalised,
+  float* ws_ml;  // and their maxima (log2 units) and sums, [rows][2]
 };
 
 int launch_rotary_append(const RotaryArgs& a, int dt, hipStream_t st);
