@@ -291,7 +291,8 @@ int tx_flash_attn_packed(const void* q, const int64_t q_strides[2], const void* 
  * causal those up to its own, j <= kv_lens[b] - n + i.  A row that sees no key gets 0.  max_q_len bounds the
  * rows of a sequence (<= 0: T); a call with a bound that is too small is still in bounds and right, only slower.
  * workspace: at least the floats that tx_flash_attn_paged_workspace gives for the same sizes (scratch; 16-byte
- * aligned, NULL when that is 0); calls that overlap in time need one each, calls one after another may share one.
+ * aligned, NULL when that is 0); calls that overlap in time need one each, calls one after another may share one.  It may share no
+ * memory with the other arguments.
  * A row whose keys are cut into P parts takes P * (head_dim + 2) floats, P at most the lesser of max_pages *
  * page_size / 256 and 256 / kv_heads, rounded up (sequences of more than 16 rows a K/V head at head_dim 64: of / 512
  * and 512 / kv_heads, 256), and the lengths are not known on the host: up to tokens * q_heads * P rows are reserved, fewer where few sequences bring

@@ -11,7 +11,7 @@ import torch
 from transformer_optimization_amd import _C
 from _util import log
 from test_limits import _run_check
-from test_seq_ops import _attend, _cu, _i32, _paged, _randn, _same
+from test_seq_ops import _Abi, _attend, _cu, _i32, _paged, _randn, _same
 
 DTYPES = [torch.bfloat16, torch.float16]
 gpu = pytest.mark.gpu
@@ -252,6 +252,23 @@ def test_one_kv_head_over_a_very_long_cache(cuda, hd, h, new, keys):
 
 
 # -------------------------------------------------------------- workspaces
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs the host C++ compiler")
+def test_spans_among_blocks(tmp_path):
+    _run_check(tmp_path, "seq_spans_check")
+
+
+@pytest.mark.parametrize("ws", [
+    5 << 20, (5 << 20) + 63 * 1024, (5 << 20) - 16,     # q, its last row, just before it
+    1 << 33, (1 << 33) + 31 * 4096, 1 << 34,            # the caches
+    6 << 20, (6 << 20) - 16, 7 << 20, 8 << 20, (8 << 20) + 4 * 64,  # starts, lengths, the table and its last row
+    3 << 30, 16 + (3 << 30),                            # the output
+])
+def test_a_workspace_may_not_be_an_argument(ws):
+    sizes = dict(np=32, ps=16, mp=64, ld=64)
+    assert _C.flash_attn_paged_workspace(64, 2, 8, 2, 64, 16, 64) > 4
+    assert _Abi().paged(q=5 << 20, cu=6 << 20, kvl=7 << 20, table=8 << 20, ws=ws, **sizes) == _C.TX_EINVAL
+
+
 @gpu
 @pytest.mark.parametrize("hd,h,hk,new,lens", [
     (128, 16, 4, [1] * 20 + [150], [3000] * 21), (64, 8, 8, [1] * 9 + [300, 40], [5000] * 11), (128, 8, 1, [17], [40000]),

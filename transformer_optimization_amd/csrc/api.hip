@@ -630,6 +630,18 @@ int tx_flash_attn_paged(const void* q, const int64_t q_strides[2], const void* k
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_floats < need)) return TX_EINVAL;
   if (need > 0 && spans_overlap((uintptr_t)workspace, need * 4, (uintptr_t)o, ((tokens - 1) * o_strides[0] + ox) * 2))
     return TX_EINVAL;
+  // The workspace is written while the inputs are read.
+  const uintptr_t ws = (uintptr_t)workspace;
+  if (need > 0 &&
+      (span_meets_blocks(ws, need * 4, (uintptr_t)q, q_strides[0], (q_heads - 1) * q_strides[1] + head_dim, tokens) ||
+       span_meets_blocks(ws, need * 4, (uintptr_t)k_cache, k_cache_strides[0],
+                         page_extent(k_cache_strides, kv_heads, page_size, head_dim), num_pages) ||
+       span_meets_blocks(ws, need * 4, (uintptr_t)v_cache, v_cache_strides[0],
+                         page_extent(v_cache_strides, kv_heads, page_size, head_dim), num_pages) ||
+       spans_overlap(ws, need * 4, (uintptr_t)cu_seqlens, (batch + 1) * 4) ||
+       spans_overlap(ws, need * 4, (uintptr_t)kv_lens, batch * 4) ||
+       spans_overlap(ws, need * 4, (uintptr_t)block_table, ((batch - 1) * table_ld + max_pages) * 4)))
+    return TX_EINVAL;
   return launch_seq_attention(a, dt, (hipStream_t)stream);
 }
 

@@ -78,6 +78,19 @@ inline bool blocks_disjoint(uintptr_t a, int64_t a_stride, int64_t a_extent, int
   return at >= (__int128)a_extent * 2 && at + (__int128)b_extent * 2 <= row;
 }
 
+// Whether [a, a + a_bytes) meets any of `count` blocks of `extent` 16-bit
+// elements at distance `stride` from b on (between them it may lie).
+inline bool span_meets_blocks(uintptr_t a, int64_t a_bytes, uintptr_t b, int64_t stride, int64_t extent, int64_t count) {
+  if (a_bytes <= 0 || extent <= 0 || count <= 0) return false;
+  const __int128 lo = (__int128)a - (__int128)b, hi = lo + a_bytes;  // relative to the first block
+  const __int128 step = (__int128)stride * 2, len = (__int128)extent * 2;
+  if (hi <= 0 || lo >= step * (count - 1) + len) return false;
+  if (step <= 0 || lo < len) return true;
+  // The first block that ends behind lo.
+  const __int128 k = (lo - len) / step + 1;
+  return k < count && k * step < hi;
+}
+
 }  // namespace tx
 
 namespace tx {
