@@ -278,7 +278,9 @@ int tx_rotary_append(const void* q, const int64_t q_strides[2], void* q_out, con
  *   o[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h / (q_heads / kv_heads)]) v[j, ..]
  * over the keys j of t's own sequence (causal != 0: up to t itself).  fp32 scores and sums, one pass with a
  * running maximum; the weights are rounded to dt as operands of the second product only.  A key outside a
- * row's mask has no influence on it, whatever it holds (NaN and infinities included).  head_dim 64 or 128,
+ * row's mask has no influence on it, whatever it holds (NaN and infinities included); what a row sees reaches it as
+ * in IEEE arithmetic on its weights (a score of NaN or +inf makes it NaN, an infinite value its element infinite, or NaN
+ * where it meets its opposite or a weight of 0).  head_dim 64 or 128,
  * kv_heads divides q_heads.  o may not share memory with q, k or v.
  */
 int tx_flash_attn_packed(const void* q, const int64_t q_strides[2], const void* k, const int64_t k_strides[2],

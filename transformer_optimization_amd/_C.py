@@ -880,7 +880,8 @@ def flash_attn_packed(
 
 def flash_attn_paged_workspace(tokens: int, batch: int, heads: int, kv_heads: int, head_dim: int, page_size: int,
                                max_pages: int, max_q_len: int = 0) -> int:
-    """fp32 values of workspace that :func:`flash_attn_paged` needs for these sizes (0: none)."""
+    """fp32 values of workspace that :func:`flash_attn_paged` needs for these sizes (0: none): at most ``tokens * heads
+    * parts * (head_dim + 2)`` with up to ``256 / kv_heads`` parts of the keys, 512 at head dim 64 (``tx_api.h``)."""
     n = ctypes.c_int64(0)
     _check("tx_flash_attn_paged_workspace",
            load_library().tx_flash_attn_paged_workspace(tokens, batch, heads, kv_heads, head_dim, page_size, max_pages,
@@ -909,8 +910,8 @@ def flash_attn_paged(
     A page index outside ``[0, pages)`` makes the rows that need it NaN.
 
     ``max_q_len``: a bound on the rows of one sequence that the caller knows (0: T), to choose the kernel by.
-    ``workspace``: fp32, at least :func:`flash_attn_paged_workspace` values, made here when omitted; calls that
-    overlap in time need one each."""
+    ``workspace``: fp32, at least :func:`flash_attn_paged_workspace` values, made here when omitted (and kept by a
+    captured graph); calls that overlap in time need one each, others may share one."""
     t, heads, hd = _dims3("q", q)
     dtype = q.dtype
     qs = _heads3("q", q, t, heads, hd, dtype)

@@ -164,10 +164,10 @@ struct SqLoader {
 // it runs (its K tile is staged one tile ahead of V, two sets of scores).  At
 // head dim 128, where registers allow two workgroups a CU either way: one
 // prompt of 32768 tokens 3990 -> 3900 us, of 2048 48.5 -> 45 us.  At head dim 64
-// its registers (181 for 125) cost workgroups: 40.4 -> 45.9 us for 16 prompts
+// its registers (181 for 128) cost workgroups: 40.4 -> 45.9 us for 16 prompts
 // of up to 1021 tokens, so LEAD = 0 there.
 // NST, the stages of the K and V rings: 2, for two workgroups a CU at head dim
-// 128 and four at 64 (125 registers): a third stage there leaves three, 2 x 8192
+// 128 and four at 64 (128 registers): a third stage there leaves three, 2 x 8192
 // tokens 300 us for 285, 16 prompts of up to 1021 42.9 for 38.4.  (With 4 and 8
 // where a call has no more workgroups than CUs, one prompt of 1024 tokens
 // took 29.9 us for 25.9: what a lone workgroup waits for is not its loads.)
@@ -694,9 +694,11 @@ __global__ __launch_bounds__(SQ_THREADS, HD == 64 ? 4 : 2) void seq_attn_packed_
 // MFMA operand, 16 rows x 64 bytes, reach 5.9 TB/s where whole rows reach 6.8),
 // into the wave's own LDS; K is read as the A operand of S^T = K Q^T (16 keys
 // x 32 dims), V transposed as that of o^T += V^T P^T.  K's rows are replaced by
-// the next block's once its scores are formed, V's once it is used, so that a
-// block's 2 x 64 HD bytes are in flight nearly all the time in each of the 8
-// waves of a CU (16 at head dim 64).  S^T leaves lane l the keys 4 (l >> 4)
+// the next block's once its scores are formed, V's once it is used, in each of
+// the 8 waves of a CU (16 at head dim 64).  K's transfer lies beside V's and the
+// softmax; V's does not reach into the scores: the wait for q that the compiler
+// places before the first of them counts the page lookup behind the DMAs, but
+// not the DMAs, and so drains them.  S^T leaves lane l the keys 4 (l >> 4)
 // .. + 3 of both 16-key halves of row l & 15, which is a P operand as it stands
 // if V's rows are taken in that order.  The waves' results meet in LDS at the
 // end.
