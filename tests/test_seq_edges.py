@@ -176,6 +176,62 @@ def test_values_near_the_end_of_the_range_do_not_overflow(cuda, hd, new, keys):
         _strictly_same(got, want, tol, f"packed {new} hd{hd}")
 
 
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_an_infinity_with_a_weight_too_small_for_16_bits_is_seen(cuda, hd):
+    """Weights from 2^-8 to 2^-80 of the largest (below 2^-40 they round to 0 in fp16): the elements are infinite all
+    the same, in one token's rows and in a tile's."""
+    dtype, n = torch.float16, 100
+    k = torch.zeros(n, 1, hd, dtype=dtype, device=cuda)
+    k[:, 0, 0] = torch.arange(n, device=cuda) * 0.5
+    v = _randn((n, 1, hd), dtype, cuda, 270)
+    v[20:60:5, 0, 7] = math.inf
+    v[30, 0, 9] = -math.inf
+    q = torch.zeros(n, 4, hd, dtype=dtype, device=cuda)
+    q[..., 0] = 1.0
+    want, tol = _ieee(q, k, v, 1.0, True, dtype)
+    assert bool(torch.isinf(want[:, :, 7]).any()) and not bool(torch.isnan(want).any())
+    _strictly_same(_C.flash_attn_packed(q, k, v, _cu([n], cuda), 1.0, True), want, tol, "packed")
+    kc, vc = (torch.zeros(7, 1, 16, hd, dtype=dtype, device=cuda) for _ in range(2))
+    kc.view(-1, hd)[:n], vc.view(-1, hd)[:n] = k[:, 0], v[:, 0]
+    table = torch.arange(7, dtype=torch.int32, device=cuda)[None]
+    for new in (1, 3, n):
+        got = _C.flash_attn_paged(q[n - new:], kc, vc, table, _cu([new], cuda), _i32([n], cuda), 1.0)
+        _strictly_same(got, want[n - new:], tol[n - new:], f"paged {new}")
+
+
+@gpu
+def test_captured_calls_meet_values_that_are_not_finite(cuda):
+    """Graphs captured over finite values, replayed over others: every replay equals the eager call."""
+    dtype, hd, h, hk, n = torch.bfloat16, 128, 8, 2, 1500
+    q, k, v = (_randn((n, x, hd), dtype, cuda, 280 + i) for i, x in enumerate((h, hk, hk)))
+    _, _, kc, vc, table = _paged([n], hk, 16, hd, dtype, cuda, 283)
+    cu, cu1, cu90, kvl = _cu([n], cuda), _cu([1], cuda), _cu([90], cuda), _i32([n], cuda)
+
+    def step():
+        return [_C.flash_attn_packed(q, k, v, cu, hd**-0.5, True),
+                _C.flash_attn_paged(q[-1:], kc, vc, table, cu1, kvl, hd**-0.5, max_q_len=1),
+                _C.flash_attn_paged(q[-90:], kc, vc, table, cu90, kvl, hd**-0.5)]
+
+    step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step()
+    for i, (what, at) in enumerate(((0.5, 3), (math.inf, 3), (math.nan, n - 1), (-math.inf, n - 2), (1.0, 7))):
+        for c in (v, k) if i % 2 else (v,):
+            c[at, 0, 11] = what
+        vc[table[0, at // 16].long(), 0, at % 16, 5] = what
+        g.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(outs, step()):
+            assert torch.equal(got.view(torch.int16), want.view(torch.int16)), i
+
+
 def _time_us(fn):
     for _ in range(3):
         fn()
