@@ -314,6 +314,98 @@ int tx_flash_attn_paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads
                                   int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t max_q_len,
                                   int64_t* floats);
 
+/*
+ * An 8-bit cache ("mx8"): k_cache / v_cache hold e4m3 codes, and k_scales / v_scales one byte s for every 32 elements
+ * of a head, [page][kv_head][slot][head_dim / 32] at strides {page, head, slot} (bytes, the last contiguous): element d
+ * stands for code[d] * 2^(s[d / 32] - 127) (s = 255: NaN).  Cache strides are in elements (bytes) and multiples of 16.
+ * Written by tx_norm_rotary_append: s is the smallest with every finite magnitude of the block within 448 * 2^(s - 127)
+ * (at least 10 for bf16, 112 for fp16, whose codes are then all its own values), codes are rounded to nearest even,
+ * what is not finite becomes NaN; of fp16 (bf16) magnitudes above 61440 (1.875 * 2^127) count as that.
+ */
+
+/*
+ * tx_rotary_append with norms of each q and k head before the turn, positions of several axes, and 8-bit caches.
+ * norm: TX_NORM_NONE, or with the head's mean square (TX_NORM_RMS) or variance (TX_NORM_LAYER, the mean taken off)
+ * m: x / sqrt(m + eps) * weight + bias.  Weights (each nullable: 1) and biases (nullable: 0; TX_NORM_LAYER only) have
+ * head_dim values, per_head != 0: as many for each head; of param_dt, dt or TX_F32, 16-byte aligned.
+ * positions (int64, nullable as there): of axis x at positions[x * positions_ld + t]; pair i goes by axis pair_axis[i]
+ * (int32 [rotary_dim / 2]; NULL: axis 0; cut to [0, axes)).
+ * All of it in fp32, rounded once: the turned q and k to dt (q_out, k_out, a 16-bit cache) or to codes.  With scales
+ * (both or neither) the caches are 8-bit (head_dim a multiple of 32).  Otherwise as tx_rotary_append; outputs may
+ * share no memory with any input either, but for q_out and k_out that are q and k themselves.
+ */
+#define TX_NORM_NONE 0
+#define TX_NORM_RMS 1
+#define TX_NORM_LAYER 2
+int tx_norm_rotary_append(const void* q, const int64_t q_strides[2], void* q_out, const int64_t q_out_strides[2],
+                          const void* k, const int64_t k_strides[2], void* k_out, const int64_t k_out_strides[2],
+                          const void* v, const int64_t v_strides[2],
+                          void* k_cache, const int64_t k_cache_strides[3],
+                          uint8_t* k_scales, const int64_t k_scales_strides[3],
+                          void* v_cache, const int64_t v_cache_strides[3],
+                          uint8_t* v_scales, const int64_t v_scales_strides[3],
+                          const void* q_weight, const void* q_bias, const void* k_weight, const void* k_bias,
+                          int per_head, int param_dt, int norm, float eps,
+                          const int64_t* steps, const int32_t* pair_axis,
+                          const int64_t* positions, int64_t positions_ld, int64_t axes,
+                          const int32_t* cu_seqlens, const int32_t* kv_lens,
+                          const int32_t* block_table, int64_t table_ld,
+                          int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                          int64_t rotary_dim, int64_t num_pages, int64_t page_size, int64_t max_pages,
+                          float amplitude, int interleaved, int dt, void* stream);
+
+/*
+ * tx_flash_attn_paged over an 8-bit cache: the same arguments, results and workspace
+ * (tx_flash_attn_paged_workspace) for the values that codes and scales stand for, which are exact in dt (beyond
+ * fp16's range: infinite).  Scales' pointers and strides are multiples of head_dim / 32.  o and the workspace may
+ * share no memory with any input.
+ */
+int tx_flash_attn_paged_mx8(const void* q, const int64_t q_strides[2],
+                            const void* k_cache, const int64_t k_cache_strides[3],
+                            const uint8_t* k_scales, const int64_t k_scales_strides[3],
+                            const void* v_cache, const int64_t v_cache_strides[3],
+                            const uint8_t* v_scales, const int64_t v_scales_strides[3],
+                            void* o, const int64_t o_strides[2],
+                            const int32_t* cu_seqlens, const int32_t* kv_lens,
+                            const int32_t* block_table, int64_t table_ld,
+                            int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t max_q_len,
+                            float scale, int causal, float* workspace, int64_t workspace_floats, int dt, void* stream);
+
+/*
+ * Attention of the tokens of draft trees over a paged cache of 16 bits (scales NULL) or 8: row i of a sequence's n
+ * sees the keys before the new ones, j < kv_lens[b] - n, and new key kv_lens[b] - n + x if bit x % 64 of
+ * tree_mask[t * tree_ld + x / 64] is set (int64, tree_words to a row; new keys past them are not seen).  A row sees
+ * itself only if its own bit is set; a row that sees no key gets 0.  Otherwise as tx_flash_attn_paged(_mx8).
+ */
+int tx_flash_attn_tree(const void* q, const int64_t q_strides[2],
+                       const void* k_cache, const int64_t k_cache_strides[3],
+                       const uint8_t* k_scales, const int64_t k_scales_strides[3],
+                       const void* v_cache, const int64_t v_cache_strides[3],
+                       const uint8_t* v_scales, const int64_t v_scales_strides[3],
+                       void* o, const int64_t o_strides[2],
+                       const int32_t* cu_seqlens, const int32_t* kv_lens,
+                       const int32_t* block_table, int64_t table_ld,
+                       const int64_t* tree_mask, int64_t tree_ld, int64_t tree_words,
+                       int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                       int64_t num_pages, int64_t page_size, int64_t max_pages, int64_t max_q_len,
+                       float scale, float* workspace, int64_t workspace_floats, int dt, void* stream);
+
+/*
+ * The accepted path of each sequence's n = cu_seqlens[b + 1] - cu_seqlens[b] drafts moves to the front of their slots:
+ * keys and values (and scales) of key kv_lens[b] - n + path[b * path_ld + i] go to key kv_lens[b] - n + i, for i <
+ * counts[b] (cut to [0, min(n, max_path)]); lens_out[b] = kv_lens[b] - n + counts[b], the length that is left.  A path
+ * ascends, path[i] >= i (as drafts do whose parents precede them); of one that does not, which values its slots get is
+ * not said.  Entries outside [0, n), keys before 0 and keys without a page are left out.  kv_heads may be those of many
+ * layers that share a pool.  lens_out may not be kv_lens.
+ */
+int tx_cache_accept(void* k_cache, const int64_t k_cache_strides[3], uint8_t* k_scales, const int64_t k_scales_strides[3],
+                    void* v_cache, const int64_t v_cache_strides[3], uint8_t* v_scales, const int64_t v_scales_strides[3],
+                    const int32_t* cu_seqlens, const int32_t* kv_lens, const int32_t* block_table, int64_t table_ld,
+                    const int32_t* path, int64_t path_ld, int64_t max_path, const int32_t* counts, int32_t* lens_out,
+                    int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t num_pages, int64_t page_size,
+                    int64_t max_pages, int dt, void* stream);
+
 /* tx_select_kernel: for tests and timing, the kernel that the calling thread's
  * later calls of `op` take where several give the result; no counterpart in
  * the reference.  variant < 0 restores the process's choice: the dispatcher's

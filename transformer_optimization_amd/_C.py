@@ -32,6 +32,8 @@ LN_HAS_DELTA, LN_MASK_DELTA, LN_MASK_X, LN_MASK_OUT, LN_WRITE_X, LN_SPLIT_Y = 1,
 EPI_BIAS, EPI_GELU_ERF, EPI_RESIDUAL, EPI_MASK_DELTA, EPI_MASK_OUT, EPI_SPLIT_OUT = 1, 2, 4, 8, 16, 32
 SOFTMAX_EAGER, SOFTMAX_ONLINE = 0, 1
 SELECT_GEMM, SELECT_ATTN_ROWRES = 0, 1
+TX_NORM_NONE, TX_NORM_RMS, TX_NORM_LAYER = 0, 1, 2
+HEAD_NORMS = {"none": TX_NORM_NONE, "rms": TX_NORM_RMS, "layer": TX_NORM_LAYER}
 SOFTMAX_MODES = {"eager": SOFTMAX_EAGER, "online": SOFTMAX_ONLINE}
 # Longest sequence the eager-exact softmax serves (tx_flash_attn_fwd returns
 # TX_EUNSUPPORTED above it: 1024 key tiles of 64); below it, the lengths
@@ -57,6 +59,10 @@ EXPORTED_SYMBOLS = (
     "tx_flash_attn_packed",
     "tx_flash_attn_paged",
     "tx_flash_attn_paged_workspace",
+    "tx_norm_rotary_append",
+    "tx_flash_attn_paged_mx8",
+    "tx_flash_attn_tree",
+    "tx_cache_accept",
     "tx_select_kernel",
 )
 
@@ -161,6 +167,46 @@ def _declare(lib: ctypes.CDLL) -> None:
     ]
     lib.tx_flash_attn_paged_workspace.restype = _i32
     lib.tx_flash_attn_paged_workspace.argtypes = [_i64] * 8 + [_vp]
+    lib.tx_norm_rotary_append.restype = _i32
+    lib.tx_norm_rotary_append.argtypes = [
+        _vp, _vp, _vp, _vp,                 # q strides q_out strides
+        _vp, _vp, _vp, _vp, _vp, _vp,       # k strides k_out strides v strides
+        _vp, _vp, _vp, _vp,                 # k_cache strides k_scales strides
+        _vp, _vp, _vp, _vp,                 # v_cache strides v_scales strides
+        _vp, _vp, _vp, _vp, _i32, _i32, _i32, _f32,  # q_weight q_bias k_weight k_bias per_head param_dt norm eps
+        _vp, _vp, _vp, _i64, _i64,          # steps pair_axis positions positions_ld axes
+        _vp, _vp, _vp, _i64,                # cu_seqlens kv_lens block_table table_ld
+        _i64, _i64, _i64, _i64, _i64, _i64,  # tokens batch q_heads kv_heads head_dim rotary_dim
+        _i64, _i64, _i64,                   # num_pages page_size max_pages
+        _f32, _i32, _i32, _vp,              # amplitude interleaved dt stream
+    ]
+    lib.tx_flash_attn_paged_mx8.restype = _i32
+    lib.tx_flash_attn_paged_mx8.argtypes = [
+        _vp, _vp, _vp, _vp, _vp, _vp,       # q k_cache k_scales, each with its strides
+        _vp, _vp, _vp, _vp, _vp, _vp,       # v_cache v_scales o
+        _vp, _vp, _vp, _i64,                # cu_seqlens kv_lens block_table table_ld
+        _i64, _i64, _i64, _i64, _i64,       # tokens batch q_heads kv_heads head_dim
+        _i64, _i64, _i64, _i64,             # num_pages page_size max_pages max_q_len
+        _f32, _i32, _vp, _i64, _i32, _vp,   # scale causal workspace workspace_floats dt stream
+    ]
+    lib.tx_flash_attn_tree.restype = _i32
+    lib.tx_flash_attn_tree.argtypes = [
+        _vp, _vp, _vp, _vp, _vp, _vp,       # q k_cache k_scales, each with its strides
+        _vp, _vp, _vp, _vp, _vp, _vp,       # v_cache v_scales o
+        _vp, _vp, _vp, _i64,                # cu_seqlens kv_lens block_table table_ld
+        _vp, _i64, _i64,                    # tree_mask tree_ld tree_words
+        _i64, _i64, _i64, _i64, _i64,       # tokens batch q_heads kv_heads head_dim
+        _i64, _i64, _i64, _i64,             # num_pages page_size max_pages max_q_len
+        _f32, _vp, _i64, _i32, _vp,         # scale workspace workspace_floats dt stream
+    ]
+    lib.tx_cache_accept.restype = _i32
+    lib.tx_cache_accept.argtypes = [
+        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,  # k_cache k_scales v_cache v_scales, each with its strides
+        _vp, _vp, _vp, _i64,                # cu_seqlens kv_lens block_table table_ld
+        _vp, _i64, _i64, _vp, _vp,          # path path_ld max_path counts lens_out
+        _i64, _i64, _i64, _i64, _i64, _i64,  # batch kv_heads head_dim num_pages page_size max_pages
+        _i32, _vp,                          # dt stream
+    ]
 
 
 def _hip_runtime_mappings() -> set:
@@ -951,3 +997,383 @@ def flash_attn_paged(
                lambda: {"op": "flash_attn_paged", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh,
                         "head_dim": hd, "causal": bool(causal), "page_size": page_size})
     return out
+
+
+# --------------------------------------------- 8-bit caches and draft trees
+# Elements of a head that share a scale.
+MX_BLOCK = 32
+
+
+def mx8_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, *,
+              device: Optional[torch.device] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(codes, scales)`` of one side of an 8-bit cache: e4m3 codes ``[pages, kv_heads, page_size, head_dim]`` and a
+    power of two (e8m0) for every 32 elements, ``[pages, kv_heads, page_size, head_dim / 32]``, both all zero bits.
+    Of any other strides they can be views of the caller's own; scales may be uint8 too (2^(byte - 127), 255: NaN)."""
+    if head_dim <= 0 or head_dim % MX_BLOCK:
+        raise ValueError(f"an 8-bit cache needs a head_dim that is a multiple of {MX_BLOCK}")
+    codes = torch.zeros((pages, kv_heads, page_size, head_dim), dtype=torch.uint8, device=device)
+    scales = torch.zeros((pages, kv_heads, page_size, head_dim // MX_BLOCK), dtype=torch.uint8, device=device)
+    return codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu)
+
+
+def _check_mx8(k_cache, k_scales, v_cache, v_scales, block_table, batch: int, hd: int) -> tuple:
+    if k_scales is None or v_scales is None:
+        raise ValueError("an 8-bit cache needs k_scales and v_scales")
+    if hd % MX_BLOCK:
+        raise ValueError(f"an 8-bit cache needs a head_dim that is a multiple of {MX_BLOCK}")
+    if k_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"a cache with scales must be float8_e4m3fn, got {k_cache.dtype}")
+    ks, vs, sizes = _check_cache(k_cache, v_cache, block_table, batch, hd, torch.float8_e4m3fn)
+    want = (*sizes[:3], hd // MX_BLOCK)
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if t.shape != want:
+            raise ValueError(f"{name} must be {list(want)}, got {tuple(t.shape)}")
+        if t.dtype != torch.uint8 and t.dtype != torch.float8_e8m0fnu:
+            raise ValueError(f"{name} must be uint8 or float8_e8m0fnu")
+        if t.stride(3) != 1 and want[3] > 1:
+            raise ValueError(f"{name} must be contiguous in its last dim")
+    return ks, vs, sizes, k_scales.stride(), v_scales.stride()
+
+
+def norm_rotary_append(
+    q: Optional[torch.Tensor],
+    k: torch.Tensor,
+    v: Optional[torch.Tensor],
+    steps: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    *,
+    norm: str = "rms",
+    q_weight: Optional[torch.Tensor] = None,
+    k_weight: Optional[torch.Tensor] = None,
+    q_bias: Optional[torch.Tensor] = None,
+    k_bias: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    kv_lens: Optional[torch.Tensor] = None,
+    positions: Optional[torch.Tensor] = None,
+    pair_axis: Optional[torch.Tensor] = None,
+    block_table: Optional[torch.Tensor] = None,
+    k_cache: Optional[torch.Tensor] = None,
+    v_cache: Optional[torch.Tensor] = None,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
+    q_out: Optional[torch.Tensor] = None,
+    k_out: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    amplitude: float = 1.0,
+) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """:func:`rotary_append` with norms of the heads, positions of several axes and 8-bit caches
+    (``tx_norm_rotary_append``).  Returns ``(q_out, k_out)``.
+
+    Before the turn each q and k head is divided by the root of its mean square (``norm="rms"``), or of its variance
+    after its mean is taken off (``"layer"``), or left as it is (``"none"``; positions of several axes and 8-bit caches
+    without a norm).  Weights and, for ``"layer"``, biases are ``[hd]``, or ``[heads, hd]`` where each head has its own
+    (then all of them), in the tensors' dtype or fp32.
+
+    ``positions``: int64 ``[T]``, or ``[axes, T]`` with ``pair_axis`` (int32 ``[rotary_dim / 2]``), the axis that each
+    pair goes by (time, height, width).  Frequencies that start anew on each axis are ``steps`` joined of several
+    :func:`rotary_steps`.  ``k_scales``, ``v_scales``: with them the caches are 8-bit (:func:`mx8_cache`).  All else as
+    :func:`rotary_append`; the result is rounded once."""
+    t, kvh, hd = _dims3("k", k)
+    dtype = k.dtype
+    ks = _heads3("k", k, t, kvh, hd, dtype)
+    qs = qos = kos = vs = kcs = vcs = kss = vss = _NO_STRIDES
+    batch = _starts(cu_seqlens)
+    half = steps.shape[0] if steps.dim() == 1 else 0
+    if not 0 < 2 * half <= hd or steps.dtype != torch.int64 or not steps.is_contiguous():
+        raise ValueError(f"steps must be a contiguous int64 [rotary_dim / 2] tensor with rotary_dim <= {hd}")
+    kind = HEAD_NORMS.get(norm)
+    if kind is None:
+        raise ValueError(f"norm must be one of {sorted(HEAD_NORMS)}")
+    heads = kvh
+    if q is not None:
+        heads = _dims3("q", q)[1]
+        qs = _heads3("q", q, t, heads, hd, dtype)
+        if kvh <= 0 or heads % kvh:
+            raise ValueError(f"{kvh} K/V heads do not divide {heads} query heads")
+        if q_out is not None:
+            qos = _heads3("q_out", q_out, t, heads, hd, dtype)
+    elif q_out is not None or q_weight is not None or q_bias is not None:
+        raise ValueError("q_out, q_weight or q_bias without q")
+    if k_out is not None:
+        kos = _heads3("k_out", k_out, t, kvh, hd, dtype)
+    per_head = param_dt = None
+    for name, p, n in (("q_weight", q_weight, heads), ("k_weight", k_weight, kvh), ("q_bias", q_bias, heads),
+                       ("k_bias", k_bias, kvh)):
+        if p is None:
+            continue
+        if kind == TX_NORM_NONE or (kind == TX_NORM_RMS and name.endswith("bias")):
+            raise ValueError(f"{name} with norm={norm!r}")
+        if p.shape != (hd,) and p.shape != (n, hd) or not p.is_contiguous():
+            raise ValueError(f"{name} must be contiguous [{hd}] or [{n}, {hd}]")
+        if p.dtype != dtype and p.dtype != torch.float32:
+            raise ValueError(f"{name} must be {dtype} or float32")
+        if per_head is not None and (per_head != (p.dim() == 2) or param_dt != p.dtype):
+            raise ValueError("weights and biases must be alike: all of one dtype, all [hd] or all [heads, hd]")
+        per_head, param_dt = p.dim() == 2, p.dtype
+    if kv_lens is not None:
+        _int_vector("kv_lens", kv_lens, batch)
+    axes, positions_ld = 1, t
+    if positions is not None:
+        shape = positions.shape
+        if (len(shape) not in (1, 2) or shape[-1] != t or shape[0] == 0 and len(shape) == 2
+                or positions.dtype != torch.int64 or positions.stride(-1) != 1 and t > 1):
+            raise ValueError(f"positions must be int64 [{t}] or [axes, {t}] with contiguous rows")
+        if len(shape) == 2:
+            axes, positions_ld = shape[0], positions.stride(0)
+    if axes > 1 and pair_axis is None:
+        raise ValueError("positions of several axes need pair_axis")
+    if pair_axis is not None:
+        _int_vector("pair_axis", pair_axis, half)
+    pages = page_size = max_pages = table_ld = 0
+    mx = k_scales is not None or v_scales is not None
+    if k_cache is not None or v_cache is not None:
+        if k_cache is None or v_cache is None or block_table is None or kv_lens is None or v is None:
+            raise ValueError("a cache needs k_cache, v_cache, block_table, kv_lens and v")
+        vs = _heads3("v", v, t, kvh, hd, dtype)
+        if mx:
+            kcs, vcs, sizes, kss, vss = _check_mx8(k_cache, k_scales, v_cache, v_scales, block_table, batch, hd)
+        else:
+            kcs, vcs, sizes = _check_cache(k_cache, v_cache, block_table, batch, hd, dtype)
+        pages, cache_heads, page_size, max_pages, table_ld = sizes
+        if cache_heads != kvh:
+            raise ValueError("the caches must hold k's heads")
+    elif mx:
+        raise ValueError("scales without a cache")
+    else:
+        block_table = v = None
+    at = _one_device(k, q, v, steps, cu_seqlens, kv_lens, positions, pair_axis, block_table, k_cache, v_cache, k_scales,
+                     v_scales, q_weight, k_weight, q_bias, k_bias, q_out, k_out)
+    load_library()
+    if q is not None and q_out is None:
+        q_out = torch.empty((t, heads, hd), dtype=dtype, device=k.device)
+        qos = (heads * hd, hd, 1)
+    if k_cache is None and k_out is None:
+        k_out = torch.empty((t, kvh, hd), dtype=dtype, device=k.device)
+        kos = (kvh * hd, hd, 1)
+    if t == 0 or batch == 0:
+        return q_out, k_out
+    # The strides in one array, kept with the launch, and their addresses in it.
+    st = array.array("q", (*qs[:3], *qos[:3], *ks[:3], *kos[:3], *vs[:3], *kcs[:3], *vcs[:3], *kss[:3], *vss[:3]))
+    sa = st.buffer_info()[0]
+    args = (_ptr(q), sa, _ptr(q_out) if q is not None else None, sa + 24, k.data_ptr(), sa + 48, _ptr(k_out), sa + 72,
+            _ptr(v), sa + 96, _ptr(k_cache), sa + 120, _ptr(k_scales), sa + 168, _ptr(v_cache), sa + 144,
+            _ptr(v_scales), sa + 192, _ptr(q_weight), _ptr(q_bias), _ptr(k_weight), _ptr(k_bias),
+            1 if per_head else 0, _DT.get(param_dt, TX_F32), kind, float(eps), steps.data_ptr(), _ptr(pair_axis),
+            _ptr(positions), positions_ld, axes, cu_seqlens.data_ptr(), _ptr(kv_lens), _ptr(block_table), table_ld,
+            t, batch, heads, kvh, hd, 2 * half, pages, page_size, max_pages, float(amplitude), 1 if interleaved else 0,
+            _DT.get(dtype, -1))
+    _launch_on(at, "tx_norm_rotary_append", args,
+               (q, k, v, steps, cu_seqlens, kv_lens, positions, pair_axis, block_table, k_cache, v_cache, k_scales,
+                v_scales, q_weight, k_weight, q_bias, k_bias, q_out, k_out, st),
+               lambda: {"op": "norm_rotary_append", "tokens": t, "heads": heads, "kv_heads": kvh, "head_dim": hd,
+                        "norm": norm, "axes": axes, "cache": k_cache is not None, "mx8": mx})
+    return q_out, k_out
+
+
+def _paged_workspace(at: int, device, *sizes: int) -> Optional[torch.Tensor]:
+    if at != torch.cuda.current_device():
+        with torch.cuda.device(at):
+            need = flash_attn_paged_workspace(*sizes)
+    else:
+        need = flash_attn_paged_workspace(*sizes)
+    return torch.empty(need, dtype=torch.float32, device=device) if need > 0 else None
+
+
+def flash_attn_paged_mx8(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_cache: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    kv_lens: torch.Tensor,
+    scale: float,
+    causal: bool = True,
+    *,
+    max_q_len: int = 0,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """:func:`flash_attn_paged` over an 8-bit cache (``tx_flash_attn_paged_mx8``): caches ``[pages, kv_heads,
+    page_size, hd]`` of float8_e4m3fn and their scales, as :func:`norm_rotary_append` writes them.  The result is that
+    of the values that codes and scales stand for.  Workspace: :func:`flash_attn_paged_workspace`."""
+    t, heads, hd = _dims3("q", q)
+    dtype = q.dtype
+    qs = _heads3("q", q, t, heads, hd, dtype)
+    batch = _starts(cu_seqlens)
+    _int_vector("kv_lens", kv_lens, batch)
+    ks, vs, (pages, kvh, page_size, max_pages, table_ld), kss, vss = _check_mx8(k_cache, k_scales, v_cache, v_scales,
+                                                                                block_table, batch, hd)
+    if kvh <= 0 or heads % kvh:
+        raise ValueError(f"{kvh} K/V heads do not divide {heads} query heads")
+    if out is not None:
+        os_ = _heads3("out", out, t, heads, hd, dtype)
+    at = _one_device(q, k_cache, k_scales, v_cache, v_scales, block_table, cu_seqlens, kv_lens, out, workspace)
+    load_library()
+    if out is None:
+        out = torch.empty((t, heads, hd), dtype=dtype, device=q.device)
+        os_ = (heads * hd, hd, 1)
+    if t == 0 or batch == 0:
+        return out
+    if workspace is None:
+        workspace = _paged_workspace(at, q.device, t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+    elif workspace.dtype != torch.float32 or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous fp32")
+    st = array.array("q", (*qs, *ks, *kss, *vs, *vss, *os_))
+    sa = st.buffer_info()[0]
+    args = (q.data_ptr(), sa, k_cache.data_ptr(), sa + 24, k_scales.data_ptr(), sa + 56, v_cache.data_ptr(), sa + 88,
+            v_scales.data_ptr(), sa + 120, out.data_ptr(), sa + 152, cu_seqlens.data_ptr(), kv_lens.data_ptr(),
+            block_table.data_ptr(), table_ld, t, batch, heads, kvh, hd, pages, page_size, max_pages, max_q_len,
+            float(scale), 1 if causal else 0, workspace.data_ptr() if workspace is not None else None,
+            0 if workspace is None else workspace.numel(), _DT.get(dtype, -1))
+    _launch_on(at, "tx_flash_attn_paged_mx8", args,
+               (q, k_cache, k_scales, v_cache, v_scales, out, cu_seqlens, kv_lens, block_table, workspace, st),
+               lambda: {"op": "flash_attn_paged_mx8", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh,
+                        "head_dim": hd, "causal": bool(causal), "page_size": page_size})
+    return out
+
+
+def flash_attn_tree(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    kv_lens: torch.Tensor,
+    tree_mask: torch.Tensor,
+    scale: float,
+    *,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
+    max_q_len: int = 0,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of the tokens of draft trees over a paged cache that already holds them (``tx_flash_attn_tree``),
+    16-bit or, with scales, 8-bit.  Row i of a sequence's n sees all keys before the n and those of them whose bit is
+    set in its row of ``tree_mask`` (int64 ``[T, words]``: new token x is bit ``x % 64`` of word ``x // 64``), itself
+    included only by its own bit.  :func:`tree_masks` makes the rows from each token's parent.  All else as
+    :func:`flash_attn_paged`."""
+    t, heads, hd = _dims3("q", q)
+    dtype = q.dtype
+    qs = _heads3("q", q, t, heads, hd, dtype)
+    batch = _starts(cu_seqlens)
+    _int_vector("kv_lens", kv_lens, batch)
+    kss = vss = (0, 0, 0, 1)
+    if k_scales is not None or v_scales is not None:
+        ks, vs, sizes, kss, vss = _check_mx8(k_cache, k_scales, v_cache, v_scales, block_table, batch, hd)
+    else:
+        ks, vs, sizes = _check_cache(k_cache, v_cache, block_table, batch, hd, dtype)
+    pages, kvh, page_size, max_pages, table_ld = sizes
+    if kvh <= 0 or heads % kvh:
+        raise ValueError(f"{kvh} K/V heads do not divide {heads} query heads")
+    mask = tree_mask.shape
+    if len(mask) != 2 or mask[0] != t or mask[1] < 1 or tree_mask.dtype != torch.int64:
+        raise ValueError(f"tree_mask must be an int64 [{t}, words] tensor")
+    tree_ld, unit = tree_mask.stride()
+    if unit != 1 and mask[1] > 1:
+        raise ValueError("tree_mask rows must be contiguous")
+    if out is not None:
+        os_ = _heads3("out", out, t, heads, hd, dtype)
+    at = _one_device(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_seqlens, kv_lens, tree_mask, out, workspace)
+    load_library()
+    if out is None:
+        out = torch.empty((t, heads, hd), dtype=dtype, device=q.device)
+        os_ = (heads * hd, hd, 1)
+    if t == 0 or batch == 0:
+        return out
+    if workspace is None:
+        workspace = _paged_workspace(at, q.device, t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+    elif workspace.dtype != torch.float32 or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous fp32")
+    st = array.array("q", (*qs, *ks, *kss, *vs, *vss, *os_))
+    sa = st.buffer_info()[0]
+    args = (q.data_ptr(), sa, k_cache.data_ptr(), sa + 24, _ptr(k_scales), sa + 56, v_cache.data_ptr(), sa + 88,
+            _ptr(v_scales), sa + 120, out.data_ptr(), sa + 152, cu_seqlens.data_ptr(), kv_lens.data_ptr(),
+            block_table.data_ptr(), table_ld, tree_mask.data_ptr(), tree_ld, mask[1], t, batch, heads, kvh, hd, pages,
+            page_size, max_pages, max_q_len, float(scale), workspace.data_ptr() if workspace is not None else None,
+            0 if workspace is None else workspace.numel(), _DT.get(dtype, -1))
+    _launch_on(at, "tx_flash_attn_tree", args,
+               (q, k_cache, v_cache, k_scales, v_scales, out, cu_seqlens, kv_lens, block_table, tree_mask, workspace, st),
+               lambda: {"op": "flash_attn_tree", "tokens": t, "batch": batch, "heads": heads, "kv_heads": kvh,
+                        "head_dim": hd, "page_size": page_size, "mx8": k_scales is not None})
+    return out
+
+
+def tree_masks(parents, *, words: int = 0, device: Optional[torch.device] = None) -> torch.Tensor:
+    """Rows of :func:`flash_attn_tree`'s mask, int64 ``[T, words]``, of one list per sequence: the index within it of
+    each new token's parent (before the token itself; -1: the last token before the drafts).  A token sees itself and
+    what is above it.  ``words``: at least, for one captured shape (0: as many as the longest list needs)."""
+    bits, most = [], 1
+    for ps in parents:
+        first = len(bits)
+        for i, p in enumerate(ps):
+            p = int(p)
+            if not -1 <= p < i:
+                raise ValueError(f"parent {p} of new token {i}: a parent comes before its token, or is -1")
+            bits.append(1 << i | (bits[first + p] if p >= 0 else 0))
+        most = max(most, len(ps))
+    need = (most + 63) // 64
+    if words and words < need:
+        raise ValueError(f"{most} new tokens need {need} words")
+    words = words or need
+    rows = [[((b >> (64 * w)) + (1 << 63)) % (1 << 64) - (1 << 63) for w in range(words)] for b in bits]
+    return torch.tensor(rows, dtype=torch.int64, device=device).view(len(bits), words)
+
+
+def cache_accept(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    kv_lens: torch.Tensor,
+    path: torch.Tensor,
+    counts: torch.Tensor,
+    *,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
+    lens_out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """After the target model has judged a tree: the keys and values of its accepted tokens move to the front of the
+    drafts' slots (``tx_cache_accept``).  ``path`` (int32 ``[batch, max_path]``) holds the accepted ones' indices among
+    the sequence's new tokens, ascending, ``counts[b]`` (int32) of them; key ``kv_lens[b] - n + path[b, i]`` goes to
+    ``kv_lens[b] - n + i``.  Returns the lengths that are left, ``kv_lens - n + counts`` (int32 ``[batch]``, in
+    ``lens_out`` if given, which may not be ``kv_lens``).  The caches are 16-bit, or 8-bit with their scales; their
+    heads may be those of many layers that share pages."""
+    batch = _starts(cu_seqlens)
+    _int_vector("kv_lens", kv_lens, batch)
+    _int_vector("counts", counts, batch)
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache and v_cache must be [pages, kv_heads, page_size, head_dim]")
+    hd, dtype = k_cache.shape[3], k_cache.dtype
+    kss = vss = (0, 0, 0, 1)
+    if k_scales is not None or v_scales is not None:
+        ks, vs, sizes, kss, vss = _check_mx8(k_cache, k_scales, v_cache, v_scales, block_table, batch, hd)
+        dt = TX_BF16
+    else:
+        ks, vs, sizes = _check_cache(k_cache, v_cache, block_table, batch, hd, dtype)
+        dt = _DT.get(dtype, -1)
+    pages, heads, page_size, max_pages, table_ld = sizes
+    if path.dim() != 2 or path.shape[0] != batch or path.shape[1] < 1 or path.dtype != torch.int32:
+        raise ValueError("path must be an int32 [batch, max_path] tensor")
+    path_ld, unit = path.stride()
+    if unit != 1 and path.shape[1] > 1:
+        raise ValueError("path rows must be contiguous")
+    if lens_out is not None:
+        _int_vector("lens_out", lens_out, batch)
+    at = _one_device(k_cache, v_cache, k_scales, v_scales, block_table, cu_seqlens, kv_lens, path, counts, lens_out)
+    load_library()
+    if lens_out is None:
+        lens_out = torch.empty(batch, dtype=torch.int32, device=k_cache.device)
+    if batch == 0:
+        return lens_out
+    st = array.array("q", (*ks, *kss, *vs, *vss))
+    sa = st.buffer_info()[0]
+    args = (k_cache.data_ptr(), sa, _ptr(k_scales), sa + 32, v_cache.data_ptr(), sa + 64, _ptr(v_scales), sa + 96,
+            cu_seqlens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), table_ld, path.data_ptr(), path_ld,
+            path.shape[1], counts.data_ptr(), lens_out.data_ptr(), batch, heads, hd, pages, page_size, max_pages, dt)
+    _launch_on(at, "tx_cache_accept", args,
+               (k_cache, v_cache, k_scales, v_scales, cu_seqlens, kv_lens, block_table, path, counts, lens_out, st),
+               lambda: {"op": "cache_accept", "batch": batch, "heads": heads, "head_dim": hd, "mx8": k_scales is not None})
+    return lens_out

@@ -350,18 +350,49 @@ static int check_rows(const void* p, const int64_t* st, int64_t rows, int64_t he
   if (out && !view_is_nonoverlapping(st3, rows, heads, 1, hd)) return TX_EINVAL;
   return TX_OK;
 }
-// A [pages][heads][slots][head_dim] cache view.
-static int check_cache(const void* p, const int64_t* st, int64_t pages, int64_t heads, int64_t slots, int64_t hd) {
+// A [pages][heads][slots][head_dim] cache view of elements of `size` bytes.
+static int check_cache(const void* p, const int64_t* st, int64_t pages, int64_t heads, int64_t slots, int64_t hd,
+                       int size = 2) {
   if (!p || !st) return TX_EINVAL;
   for (int i = 0; i < 3; ++i) {
     if (st[i] < 0) return TX_EINVAL;
-    if (st[i] % 8 || st[i] > (int64_t)1 << 40) return TX_EUNSUPPORTED;
+    if (st[i] % (16 / size) || st[i] > (int64_t)1 << 40) return TX_EUNSUPPORTED;
   }
   if (!aligned16(p)) return TX_EUNSUPPORTED;
   // Byte strides of a page, and byte offsets within one K/V head's part of it, are 32-bit.
   if (st[2] >= 1 << 24 || st[0] >= (int64_t)1 << 31 || (slots - 1) * st[2] + hd >= (int64_t)1 << 31)
     return TX_EUNSUPPORTED;
   return view_is_nonoverlapping(st, pages, heads, slots, hd) ? TX_OK : TX_EINVAL;
+}
+// Scales of an 8-bit cache, [pages][heads][slots][n], rows aligned to `align` bytes.
+static int check_scales(const void* p, const int64_t* st, int64_t pages, int64_t heads, int64_t slots, int64_t n,
+                        int64_t align) {
+  if (!p || !st) return TX_EINVAL;
+  for (int i = 0; i < 3; ++i) {
+    if (st[i] < 0) return TX_EINVAL;
+    if (st[i] % align || st[i] > (int64_t)1 << 40) return TX_EUNSUPPORTED;
+  }
+  if ((uintptr_t)p % (uintptr_t)align) return TX_EUNSUPPORTED;
+  if (st[2] >= 1 << 24 || st[0] >= (int64_t)1 << 31 || (slots - 1) * st[2] + n >= (int64_t)1 << 31)
+    return TX_EUNSUPPORTED;
+  return view_is_nonoverlapping(st, pages, heads, slots, n) ? TX_OK : TX_EINVAL;
+}
+// Memory that a call reads or writes: `count` blocks of `extent` bytes, `stride` apart.
+struct Mem {
+  uintptr_t p;
+  __int128 stride, extent;
+  int64_t count;
+};
+static Mem mem_rows(const void* p, const int64_t* st, int64_t rows, int64_t heads, int64_t hd) {
+  return {(uintptr_t)p, (__int128)st[0] * 2, (__int128)((heads - 1) * st[1] + hd) * 2, rows};
+}
+static Mem mem_pages(const void* p, const int64_t* st, int64_t pages, int64_t heads, int64_t slots, int64_t n, int size) {
+  return {(uintptr_t)p, (__int128)st[0] * size, (__int128)((heads - 1) * st[1] + (slots - 1) * st[2] + n) * size, pages};
+}
+static Mem mem_span(const void* p, int64_t bytes) { return {(uintptr_t)p, bytes, bytes, 1}; }
+static bool disjoint(const Mem& a, const Mem& b) {
+  if (!a.p || !b.p || a.extent <= 0 || b.extent <= 0) return true;
+  return byte_blocks_disjoint(a.p, a.stride, a.extent, a.count, b.p, b.stride, b.extent, b.count);
 }
 static bool rows_disjoint(const void* a, const int64_t* as, int64_t ah, const void* b, const int64_t* bs,
                           int64_t bh, int64_t rows, int64_t hd) {
@@ -575,14 +606,22 @@ int tx_flash_attn_paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads
   return TX_OK;
 }
 
-int tx_flash_attn_paged(const void* q, const int64_t q_strides[2], const void* k_cache,
-                        const int64_t k_cache_strides[3], const void* v_cache,
-                        const int64_t v_cache_strides[3], void* o, const int64_t o_strides[2],
-                        const int32_t* cu_seqlens, const int32_t* kv_lens, const int32_t* block_table,
-                        int64_t table_ld, int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
-                        int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages,
-                        int64_t max_q_len, float scale, int causal, float* workspace, int64_t workspace_floats,
-                        int dt, void* stream) {
+// What the paged calls share.  Scales (nullptr: 16-bit caches), and a tree's mask.
+struct PagedExtra {
+  const uint8_t* k_scales;
+  const int64_t* k_scales_strides;
+  const uint8_t* v_scales;
+  const int64_t* v_scales_strides;
+  const int64_t* tree;
+  int64_t tree_ld, tree_words;
+};
+static int paged_attention(const void* q, const int64_t q_strides[2], const void* k_cache,
+                           const int64_t k_cache_strides[3], const void* v_cache, const int64_t v_cache_strides[3],
+                           void* o, const int64_t o_strides[2], const int32_t* cu_seqlens, const int32_t* kv_lens,
+                           const int32_t* block_table, int64_t table_ld, int64_t tokens, int64_t batch,
+                           int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_pages, int64_t page_size,
+                           int64_t max_pages, int64_t max_q_len, float scale, int causal, float* workspace,
+                           int64_t workspace_floats, int dt, const PagedExtra& x, bool mx, bool tree, void* stream) {
   int rc = check_seqs(tokens, batch, q_heads, kv_heads, head_dim, dt, cu_seqlens);
   if (rc != TX_OK) return rc;
   if (!kv_lens || !(scale > 0.f) || !(scale < 3.0e38f)) return TX_EINVAL;
@@ -591,15 +630,18 @@ int tx_flash_attn_paged(const void* q, const int64_t q_strides[2], const void* k
   if ((rc = check_rows(q, q_strides, tokens, q_heads, head_dim, false)) != TX_OK) return rc;
   if ((rc = check_rows(o, o_strides, tokens, q_heads, head_dim, true)) != TX_OK) return rc;
   if ((rc = check_pages(block_table, table_ld, batch, num_pages, page_size, max_pages)) != TX_OK) return rc;
-  if ((rc = check_cache(k_cache, k_cache_strides, num_pages, kv_heads, page_size, head_dim)) != TX_OK) return rc;
-  if ((rc = check_cache(v_cache, v_cache_strides, num_pages, kv_heads, page_size, head_dim)) != TX_OK) return rc;
-  const int64_t ox = (q_heads - 1) * o_strides[1] + head_dim;
-  if (!rows_disjoint(o, o_strides, q_heads, q, q_strides, q_heads, tokens, head_dim) ||
-      !blocks_disjoint((uintptr_t)o, o_strides[0], ox, tokens, (uintptr_t)k_cache, k_cache_strides[0],
-                       page_extent(k_cache_strides, kv_heads, page_size, head_dim), num_pages) ||
-      !blocks_disjoint((uintptr_t)o, o_strides[0], ox, tokens, (uintptr_t)v_cache, v_cache_strides[0],
-                       page_extent(v_cache_strides, kv_heads, page_size, head_dim), num_pages))
-    return TX_EINVAL;
+  const int size = mx ? 1 : 2;
+  const int64_t blocks = head_dim / 32;
+  if ((rc = check_cache(k_cache, k_cache_strides, num_pages, kv_heads, page_size, head_dim, size)) != TX_OK) return rc;
+  if ((rc = check_cache(v_cache, v_cache_strides, num_pages, kv_heads, page_size, head_dim, size)) != TX_OK) return rc;
+  if (mx) {
+    if ((rc = check_scales(x.k_scales, x.k_scales_strides, num_pages, kv_heads, page_size, blocks, blocks)) != TX_OK) return rc;
+    if ((rc = check_scales(x.v_scales, x.v_scales_strides, num_pages, kv_heads, page_size, blocks, blocks)) != TX_OK) return rc;
+  }
+  if (tree) {
+    if (!x.tree || x.tree_words <= 0 || x.tree_ld < 0 || (tokens > 1 && x.tree_ld < x.tree_words)) return TX_EINVAL;
+    if (((uintptr_t)x.tree & 7u) || x.tree_words > 1 << 24 || x.tree_ld > (int64_t)1 << 40) return TX_EUNSUPPORTED;
+  }
   SeqAttnArgs a{};
   a.s = {cu_seqlens, kv_lens, block_table, table_ld, (int)tokens, (int)batch, (int)num_pages,
          page_log2(page_size), (int)max_pages};
@@ -626,23 +668,314 @@ int tx_flash_attn_paged(const void* q, const int64_t q_strides[2], const void* k
   a.paged = 1;
   a.max_q_len = max_q_len <= 0 || max_q_len > tokens ? tokens : max_q_len;
   a.ws = workspace;
+  if (mx) {
+    a.k_scales = x.k_scales;
+    a.v_scales = x.v_scales;
+    a.ks_sp = x.k_scales_strides[0];
+    a.ks_sh = x.k_scales_strides[1];
+    a.ks_st = x.k_scales_strides[2];
+    a.vs_sp = x.v_scales_strides[0];
+    a.vs_sh = x.v_scales_strides[1];
+    a.vs_st = x.v_scales_strides[2];
+  }
+  if (tree) {
+    a.tree = (const uint64_t*)x.tree;
+    a.tree_ld = x.tree_ld;
+    a.tree_words = (int)x.tree_words;
+  }
   const int64_t need = seq_attention_workspace(a);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_floats < need)) return TX_EINVAL;
-  if (need > 0 && spans_overlap((uintptr_t)workspace, need * 4, (uintptr_t)o, ((tokens - 1) * o_strides[0] + ox) * 2))
-    return TX_EINVAL;
-  // The workspace is written while the inputs are read.
-  const uintptr_t ws = (uintptr_t)workspace;
-  if (need > 0 &&
-      (span_meets_blocks(ws, need * 4, (uintptr_t)q, q_strides[0], (q_heads - 1) * q_strides[1] + head_dim, tokens) ||
-       span_meets_blocks(ws, need * 4, (uintptr_t)k_cache, k_cache_strides[0],
-                         page_extent(k_cache_strides, kv_heads, page_size, head_dim), num_pages) ||
-       span_meets_blocks(ws, need * 4, (uintptr_t)v_cache, v_cache_strides[0],
-                         page_extent(v_cache_strides, kv_heads, page_size, head_dim), num_pages) ||
-       spans_overlap(ws, need * 4, (uintptr_t)cu_seqlens, (batch + 1) * 4) ||
-       spans_overlap(ws, need * 4, (uintptr_t)kv_lens, batch * 4) ||
-       spans_overlap(ws, need * 4, (uintptr_t)block_table, ((batch - 1) * table_ld + max_pages) * 4)))
-    return TX_EINVAL;
-  return launch_seq_attention(a, dt, (hipStream_t)stream);
+  // Output and workspace are written while the inputs are read.
+  const Mem out = mem_rows(o, o_strides, tokens, q_heads, head_dim);
+  const Mem in[] = {mem_rows(q, q_strides, tokens, q_heads, head_dim),
+                    mem_pages(k_cache, k_cache_strides, num_pages, kv_heads, page_size, head_dim, size),
+                    mem_pages(v_cache, v_cache_strides, num_pages, kv_heads, page_size, head_dim, size)};
+  for (const Mem& m : in)
+    if (!disjoint(out, m)) return TX_EINVAL;
+  const Mem small[] = {mem_span(cu_seqlens, (batch + 1) * 4), mem_span(kv_lens, batch * 4),
+                       mem_span(block_table, ((batch - 1) * table_ld + max_pages) * 4),
+                       mem_span(tree ? x.tree : nullptr, tree ? ((tokens - 1) * x.tree_ld + x.tree_words) * 8 : 0),
+                       mx ? mem_pages(x.k_scales, x.k_scales_strides, num_pages, kv_heads, page_size, blocks, 1) : Mem{},
+                       mx ? mem_pages(x.v_scales, x.v_scales_strides, num_pages, kv_heads, page_size, blocks, 1) : Mem{}};
+  if (mx || tree)
+    for (const Mem& m : small)
+      if (!disjoint(out, m)) return TX_EINVAL;
+  if (need > 0) {
+    const uintptr_t ws = (uintptr_t)workspace;
+    if (spans_overlap(ws, need * 4, (uintptr_t)o,
+                      ((tokens - 1) * o_strides[0] + (q_heads - 1) * o_strides[1] + head_dim) * 2))
+      return TX_EINVAL;
+    for (const Mem& m : in)
+      if (span_meets_byte_blocks(ws, need * 4, m.p, m.stride, m.extent, m.count)) return TX_EINVAL;
+    for (const Mem& m : small)
+      if (m.p && span_meets_byte_blocks(ws, need * 4, m.p, m.stride, m.extent, m.count)) return TX_EINVAL;
+  }
+  return mx || tree ? launch_cache_attention(a, dt, (hipStream_t)stream) : launch_seq_attention(a, dt, (hipStream_t)stream);
+}
+
+int tx_flash_attn_paged(const void* q, const int64_t q_strides[2], const void* k_cache,
+                        const int64_t k_cache_strides[3], const void* v_cache,
+                        const int64_t v_cache_strides[3], void* o, const int64_t o_strides[2],
+                        const int32_t* cu_seqlens, const int32_t* kv_lens, const int32_t* block_table,
+                        int64_t table_ld, int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                        int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages,
+                        int64_t max_q_len, float scale, int causal, float* workspace, int64_t workspace_floats,
+                        int dt, void* stream) {
+  return paged_attention(q, q_strides, k_cache, k_cache_strides, v_cache, v_cache_strides, o, o_strides, cu_seqlens, kv_lens,
+                         block_table, table_ld, tokens, batch, q_heads, kv_heads, head_dim, num_pages, page_size, max_pages,
+                         max_q_len, scale, causal, workspace, workspace_floats, dt, PagedExtra{}, false, false, stream);
+}
+
+int tx_flash_attn_paged_mx8(const void* q, const int64_t q_strides[2], const void* k_cache,
+                            const int64_t k_cache_strides[3], const uint8_t* k_scales,
+                            const int64_t k_scales_strides[3], const void* v_cache,
+                            const int64_t v_cache_strides[3], const uint8_t* v_scales,
+                            const int64_t v_scales_strides[3], void* o, const int64_t o_strides[2],
+                            const int32_t* cu_seqlens, const int32_t* kv_lens, const int32_t* block_table,
+                            int64_t table_ld, int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                            int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages,
+                            int64_t max_q_len, float scale, int causal, float* workspace, int64_t workspace_floats,
+                            int dt, void* stream) {
+  const PagedExtra x{k_scales, k_scales_strides, v_scales, v_scales_strides, nullptr, 0, 0};
+  return paged_attention(q, q_strides, k_cache, k_cache_strides, v_cache, v_cache_strides, o, o_strides, cu_seqlens, kv_lens,
+                         block_table, table_ld, tokens, batch, q_heads, kv_heads, head_dim, num_pages, page_size, max_pages,
+                         max_q_len, scale, causal, workspace, workspace_floats, dt, x, true, false, stream);
+}
+
+int tx_flash_attn_tree(const void* q, const int64_t q_strides[2], const void* k_cache,
+                       const int64_t k_cache_strides[3], const uint8_t* k_scales,
+                       const int64_t k_scales_strides[3], const void* v_cache, const int64_t v_cache_strides[3],
+                       const uint8_t* v_scales, const int64_t v_scales_strides[3], void* o,
+                       const int64_t o_strides[2], const int32_t* cu_seqlens, const int32_t* kv_lens,
+                       const int32_t* block_table, int64_t table_ld, const int64_t* tree_mask, int64_t tree_ld,
+                       int64_t tree_words, int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                       int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages,
+                       int64_t max_q_len, float scale, float* workspace, int64_t workspace_floats, int dt,
+                       void* stream) {
+  if ((!k_scales) != (!v_scales)) return TX_EINVAL;
+  const PagedExtra x{k_scales, k_scales_strides, v_scales, v_scales_strides, tree_mask, tree_ld, tree_words};
+  return paged_attention(q, q_strides, k_cache, k_cache_strides, v_cache, v_cache_strides, o, o_strides, cu_seqlens, kv_lens,
+                         block_table, table_ld, tokens, batch, q_heads, kv_heads, head_dim, num_pages, page_size, max_pages,
+                         max_q_len, scale, 0, workspace, workspace_floats, dt, x, k_scales != nullptr, true, stream);
+}
+
+int tx_norm_rotary_append(const void* q, const int64_t q_strides[2], void* q_out, const int64_t q_out_strides[2],
+                          const void* k, const int64_t k_strides[2], void* k_out, const int64_t k_out_strides[2],
+                          const void* v, const int64_t v_strides[2], void* k_cache,
+                          const int64_t k_cache_strides[3], uint8_t* k_scales, const int64_t k_scales_strides[3],
+                          void* v_cache, const int64_t v_cache_strides[3], uint8_t* v_scales,
+                          const int64_t v_scales_strides[3], const void* q_weight, const void* q_bias,
+                          const void* k_weight, const void* k_bias, int per_head, int param_dt, int norm, float eps,
+                          const int64_t* steps, const int32_t* pair_axis, const int64_t* positions,
+                          int64_t positions_ld, int64_t axes, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                          const int32_t* block_table, int64_t table_ld, int64_t tokens, int64_t batch,
+                          int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t num_pages,
+                          int64_t page_size, int64_t max_pages, float amplitude, int interleaved, int dt,
+                          void* stream) {
+  if (!k || !steps || (!q) != (!q_out) || (!k_cache) != (!v_cache) || (!k_scales) != (!v_scales)) return TX_EINVAL;
+  if ((!k_out && !k_cache) || (k_scales && !k_cache)) return TX_EINVAL;
+  if (!(amplitude > 0.f) || !(amplitude < 3.0e38f)) return TX_EINVAL;
+  if (norm != TX_NORM_NONE && norm != TX_NORM_RMS && norm != TX_NORM_LAYER) return TX_EINVAL;
+  if (norm != TX_NORM_NONE && (!(eps >= 0.f) || !(eps < 3.0e38f))) return TX_EINVAL;
+  if (norm != TX_NORM_LAYER && (q_bias || k_bias)) return TX_EINVAL;
+  if (norm == TX_NORM_NONE && (q_weight || k_weight)) return TX_EINVAL;
+  if (!q && (q_weight || q_bias)) return TX_EINVAL;
+  int rc = check_seqs(tokens, batch, q_heads, kv_heads, head_dim, dt, cu_seqlens);
+  if (rc != TX_OK) return rc;
+  if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > head_dim) return TX_EINVAL;
+  if (head_dim % 8 || head_dim > 256 || (k_scales && head_dim % 32)) return TX_EUNSUPPORTED;
+  const void* params[4] = {q_weight, q_bias, k_weight, k_bias};
+  bool any_param = false;
+  for (const void* p : params) {
+    any_param |= p != nullptr;
+    if (!aligned16(p)) return TX_EUNSUPPORTED;
+  }
+  if (any_param && param_dt != dt && param_dt != TX_F32) return TX_EUNSUPPORTED;
+  if (axes <= 0 || (positions && axes > 1 && positions_ld < tokens)) return TX_EINVAL;
+  if (axes > 1 << 16 || positions_ld < 0 || positions_ld > (int64_t)1 << 40) return TX_EUNSUPPORTED;
+  if (((uintptr_t)steps & 7u) || ((uintptr_t)positions & 7u) || ((uintptr_t)kv_lens & 3u) || ((uintptr_t)pair_axis & 3u))
+    return TX_EUNSUPPORTED;
+  // Rows of one workgroup's tokens are counted in 32 bits.
+  if ((q_heads + 2 * kv_heads) * head_dim > (int64_t)1 << 26) return TX_EUNSUPPORTED;
+  if (q && (rc = check_rows(q, q_strides, tokens, q_heads, head_dim, false)) != TX_OK) return rc;
+  if (q && (rc = check_rows(q_out, q_out_strides, tokens, q_heads, head_dim, true)) != TX_OK) return rc;
+  if ((rc = check_rows(k, k_strides, tokens, kv_heads, head_dim, false)) != TX_OK) return rc;
+  if (k_out && (rc = check_rows(k_out, k_out_strides, tokens, kv_heads, head_dim, true)) != TX_OK) return rc;
+  const int size = k_scales ? 1 : 2;
+  const int64_t blocks = head_dim / 32;
+  if (k_cache) {
+    if (!kv_lens) return TX_EINVAL;
+    if ((rc = check_rows(v, v_strides, tokens, kv_heads, head_dim, false)) != TX_OK) return rc;
+    if ((rc = check_pages(block_table, table_ld, batch, num_pages, page_size, max_pages)) != TX_OK) return rc;
+    if ((rc = check_cache(k_cache, k_cache_strides, num_pages, kv_heads, page_size, head_dim, size)) != TX_OK) return rc;
+    if ((rc = check_cache(v_cache, v_cache_strides, num_pages, kv_heads, page_size, head_dim, size)) != TX_OK) return rc;
+    if (k_scales) {
+      if ((rc = check_scales(k_scales, k_scales_strides, num_pages, kv_heads, page_size, blocks, 1)) != TX_OK) return rc;
+      if ((rc = check_scales(v_scales, v_scales_strides, num_pages, kv_heads, page_size, blocks, 1)) != TX_OK) return rc;
+    }
+  }
+  // Outputs: an input itself, or memory that no input and no other output uses.
+  const int64_t param_bytes = (per_head ? q_heads : 1) * head_dim * (param_dt == TX_F32 ? 4 : 2);
+  const int64_t k_param_bytes = (per_head ? kv_heads : 1) * head_dim * (param_dt == TX_F32 ? 4 : 2);
+  const Mem none{};
+  const Mem in[] = {mem_rows(k, k_strides, tokens, kv_heads, head_dim),
+                    q ? mem_rows(q, q_strides, tokens, q_heads, head_dim) : none,
+                    k_cache ? mem_rows(v, v_strides, tokens, kv_heads, head_dim) : none,
+                    mem_span(q_weight, param_bytes), mem_span(q_bias, param_bytes), mem_span(k_weight, k_param_bytes),
+                    mem_span(k_bias, k_param_bytes), mem_span(steps, rotary_dim / 2 * 8),
+                    mem_span(pair_axis, rotary_dim / 2 * 4), mem_span(positions, ((axes - 1) * positions_ld + tokens) * 8),
+                    mem_span(cu_seqlens, (batch + 1) * 4), mem_span(kv_lens, batch * 4),
+                    k_cache ? mem_span(block_table, ((batch - 1) * table_ld + max_pages) * 4) : none};
+  const Mem out[] = {k_out ? mem_rows(k_out, k_out_strides, tokens, kv_heads, head_dim) : none,
+                     q ? mem_rows(q_out, q_out_strides, tokens, q_heads, head_dim) : none,
+                     k_cache ? mem_pages(k_cache, k_cache_strides, num_pages, kv_heads, page_size, head_dim, size) : none,
+                     k_cache ? mem_pages(v_cache, v_cache_strides, num_pages, kv_heads, page_size, head_dim, size) : none,
+                     k_scales ? mem_pages(k_scales, k_scales_strides, num_pages, kv_heads, page_size, blocks, 1) : none,
+                     k_scales ? mem_pages(v_scales, v_scales_strides, num_pages, kv_heads, page_size, blocks, 1) : none};
+  for (int i = 0; i < (int)(sizeof(out) / sizeof(out[0])); ++i) {
+    for (int j = 0; j < (int)(sizeof(in) / sizeof(in[0])); ++j) {
+      if (i == 0 && j == 0 && k_out && same_rows(k_out, k_out_strides, k, k_strides)) continue;
+      if (i == 1 && j == 1 && q && same_rows(q_out, q_out_strides, q, q_strides)) continue;
+      if (!disjoint(out[i], in[j])) return TX_EINVAL;
+    }
+    for (int j = 0; j < i; ++j)
+      if (!disjoint(out[i], out[j])) return TX_EINVAL;
+  }
+  NormRotaryArgs a{};
+  a.s = {cu_seqlens, kv_lens, block_table, table_ld, (int)tokens, (int)batch, 0, 0, 0};
+  a.k = k;
+  a.k_st = k_strides[0];
+  a.k_sh = k_strides[1];
+  if (q) {
+    a.q = q;
+    a.q_st = q_strides[0];
+    a.q_sh = q_strides[1];
+    a.q_out = q_out;
+    a.qo_st = q_out_strides[0];
+    a.qo_sh = q_out_strides[1];
+  }
+  if (k_out) {
+    a.k_out = k_out;
+    a.ko_st = k_out_strides[0];
+    a.ko_sh = k_out_strides[1];
+  }
+  if (k_cache) {
+    a.s.num_pages = (int)num_pages;
+    a.s.page_log2 = page_log2(page_size);
+    a.s.max_pages = (int)max_pages;
+    a.v = v;
+    a.v_st = v_strides[0];
+    a.v_sh = v_strides[1];
+    a.k_cache = k_cache;
+    a.kc_sp = k_cache_strides[0];
+    a.kc_sh = k_cache_strides[1];
+    a.kc_st = k_cache_strides[2];
+    a.v_cache = v_cache;
+    a.vc_sp = v_cache_strides[0];
+    a.vc_sh = v_cache_strides[1];
+    a.vc_st = v_cache_strides[2];
+  }
+  if (k_scales) {
+    a.k_scales = k_scales;
+    a.ks_sp = k_scales_strides[0];
+    a.ks_sh = k_scales_strides[1];
+    a.ks_st = k_scales_strides[2];
+    a.v_scales = v_scales;
+    a.vs_sp = v_scales_strides[0];
+    a.vs_sh = v_scales_strides[1];
+    a.vs_st = v_scales_strides[2];
+  }
+  a.q_weight = q_weight;
+  a.q_bias = q_bias;
+  a.k_weight = k_weight;
+  a.k_bias = k_bias;
+  a.param_f32 = param_dt == TX_F32 ? 1 : 0;
+  a.param_sh = per_head ? (int)head_dim : 0;
+  a.norm = norm;
+  a.eps = eps;
+  a.steps = (const uint64_t*)steps;
+  a.pair_axis = pair_axis;
+  a.positions = positions;
+  a.positions_ld = positions_ld;
+  a.axes = (int)axes;
+  a.heads = (int)q_heads;
+  a.kv_heads = (int)kv_heads;
+  a.head_dim = (int)head_dim;
+  a.rotary = (int)rotary_dim;
+  a.amplitude = amplitude;
+  a.interleaved = interleaved ? 1 : 0;
+  return launch_norm_rotary_append(a, dt, (hipStream_t)stream);
+}
+
+int tx_cache_accept(void* k_cache, const int64_t k_cache_strides[3], uint8_t* k_scales,
+                    const int64_t k_scales_strides[3], void* v_cache, const int64_t v_cache_strides[3],
+                    uint8_t* v_scales, const int64_t v_scales_strides[3], const int32_t* cu_seqlens,
+                    const int32_t* kv_lens, const int32_t* block_table, int64_t table_ld, const int32_t* path,
+                    int64_t path_ld, int64_t max_path, const int32_t* counts, int32_t* lens_out, int64_t batch,
+                    int64_t kv_heads, int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages,
+                    int dt, void* stream) {
+  if (!k_cache || !v_cache || (!k_scales) != (!v_scales) || !kv_lens || !path || !counts || !lens_out) return TX_EINVAL;
+  int rc = check_seqs(1, batch, kv_heads, kv_heads, head_dim, dt, cu_seqlens);
+  if (rc != TX_OK) return rc;
+  if (max_path <= 0 || path_ld < 0 || (batch > 1 && path_ld < max_path)) return TX_EINVAL;
+  if (max_path > 1 << 24 || path_ld > (int64_t)1 << 40) return TX_EUNSUPPORTED;
+  if (((uintptr_t)kv_lens & 3u) || ((uintptr_t)path & 3u) || ((uintptr_t)counts & 3u) || ((uintptr_t)lens_out & 3u))
+    return TX_EUNSUPPORTED;
+  if (head_dim % 8 || head_dim > 256 || (k_scales && head_dim % 32)) return TX_EUNSUPPORTED;
+  if ((rc = check_pages(block_table, table_ld, batch, num_pages, page_size, max_pages)) != TX_OK) return rc;
+  const int size = k_scales ? 1 : 2;
+  const int64_t blocks = head_dim / 32;
+  if ((rc = check_cache(k_cache, k_cache_strides, num_pages, kv_heads, page_size, head_dim, size)) != TX_OK) return rc;
+  if ((rc = check_cache(v_cache, v_cache_strides, num_pages, kv_heads, page_size, head_dim, size)) != TX_OK) return rc;
+  if (k_scales) {
+    if ((rc = check_scales(k_scales, k_scales_strides, num_pages, kv_heads, page_size, blocks, 1)) != TX_OK) return rc;
+    if ((rc = check_scales(v_scales, v_scales_strides, num_pages, kv_heads, page_size, blocks, 1)) != TX_OK) return rc;
+  }
+  // (lens_out is written while other workgroups of the sequence read kv_lens)
+  const Mem none{};
+  const Mem in[] = {mem_span(cu_seqlens, (batch + 1) * 4), mem_span(kv_lens, batch * 4), mem_span(counts, batch * 4),
+                    mem_span(path, ((batch - 1) * path_ld + max_path) * 4),
+                    mem_span(block_table, ((batch - 1) * table_ld + max_pages) * 4)};
+  const Mem out[] = {mem_span(lens_out, batch * 4),
+                     mem_pages(k_cache, k_cache_strides, num_pages, kv_heads, page_size, head_dim, size),
+                     mem_pages(v_cache, v_cache_strides, num_pages, kv_heads, page_size, head_dim, size),
+                     k_scales ? mem_pages(k_scales, k_scales_strides, num_pages, kv_heads, page_size, blocks, 1) : none,
+                     k_scales ? mem_pages(v_scales, v_scales_strides, num_pages, kv_heads, page_size, blocks, 1) : none};
+  for (int i = 0; i < 5; ++i) {
+    for (const Mem& m : in)
+      if (!disjoint(out[i], m)) return TX_EINVAL;
+    for (int j = 0; j < i; ++j)
+      if (!disjoint(out[i], out[j])) return TX_EINVAL;
+  }
+  CacheAcceptArgs a{};
+  a.s = {cu_seqlens, kv_lens, block_table, table_ld, 0, (int)batch, (int)num_pages, page_log2(page_size), (int)max_pages};
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.kc_sp = k_cache_strides[0] * size;
+  a.kc_sh = k_cache_strides[1] * size;
+  a.kc_st = k_cache_strides[2] * size;
+  a.vc_sp = v_cache_strides[0] * size;
+  a.vc_sh = v_cache_strides[1] * size;
+  a.vc_st = v_cache_strides[2] * size;
+  if (k_scales) {
+    a.k_scales = k_scales;
+    a.ks_sp = k_scales_strides[0];
+    a.ks_sh = k_scales_strides[1];
+    a.ks_st = k_scales_strides[2];
+    a.v_scales = v_scales;
+    a.vs_sp = v_scales_strides[0];
+    a.vs_sh = v_scales_strides[1];
+    a.vs_st = v_scales_strides[2];
+  }
+  a.path = path;
+  a.path_ld = path_ld;
+  a.counts = counts;
+  a.lens_out = lens_out;
+  a.max_path = (int)max_path;
+  a.heads = (int)kv_heads;
+  a.chunks = (int)(head_dim * size / 16);
+  a.blocks = (int)blocks;
+  return launch_cache_accept(a, (hipStream_t)stream);
 }
 
 }  // extern "C"

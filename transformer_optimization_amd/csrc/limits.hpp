@@ -63,32 +63,40 @@ inline bool spans_overlap(uintptr_t a, int64_t a_len, uintptr_t b, int64_t b_len
 }
 
 // Whether two strided views share no byte.  Each is `count` blocks of
-// `extent` elements at distance `stride` (16-bit elements).  Either their
-// spans do not meet, or they have one stride in common and, within it, blocks
-// that lie side by side (column views of one projection, K and V of one page).
-inline bool blocks_disjoint(uintptr_t a, int64_t a_stride, int64_t a_extent, int64_t a_count,
-                            uintptr_t b, int64_t b_stride, int64_t b_extent, int64_t b_count) {
-  const __int128 a_len = ((__int128)(a_count - 1) * a_stride + a_extent) * 2;
-  const __int128 b_len = ((__int128)(b_count - 1) * b_stride + b_extent) * 2;
+// `extent` bytes at distance `stride`.  Either their spans do not meet, or they
+// have one stride in common and, within it, blocks that lie side by side
+// (column views of one projection, K and V of one page).
+inline bool byte_blocks_disjoint(uintptr_t a, __int128 a_stride, __int128 a_extent, int64_t a_count, uintptr_t b,
+                                 __int128 b_stride, __int128 b_extent, int64_t b_count) {
+  const __int128 a_len = (a_count - 1) * a_stride + a_extent;
+  const __int128 b_len = (b_count - 1) * b_stride + b_extent;
   if ((__int128)a + a_len <= (__int128)b || (__int128)b + b_len <= (__int128)a) return true;
   if (a_stride != b_stride || a_stride <= 0) return false;
-  const __int128 row = (__int128)a_stride * 2;
-  __int128 at = ((__int128)b - (__int128)a) % row;  // b's blocks start here within a's
-  if (at < 0) at += row;
-  return at >= (__int128)a_extent * 2 && at + (__int128)b_extent * 2 <= row;
+  __int128 at = ((__int128)b - (__int128)a) % a_stride;  // b's blocks start here within a's
+  if (at < 0) at += a_stride;
+  return at >= a_extent && at + b_extent <= a_stride;
+}
+// The same of 16-bit elements.
+inline bool blocks_disjoint(uintptr_t a, int64_t a_stride, int64_t a_extent, int64_t a_count,
+                            uintptr_t b, int64_t b_stride, int64_t b_extent, int64_t b_count) {
+  return byte_blocks_disjoint(a, (__int128)a_stride * 2, (__int128)a_extent * 2, a_count, b, (__int128)b_stride * 2,
+                              (__int128)b_extent * 2, b_count);
 }
 
-// Whether [a, a + a_bytes) meets any of `count` blocks of `extent` 16-bit
-// elements at distance `stride` from b on (between them it may lie).
-inline bool span_meets_blocks(uintptr_t a, int64_t a_bytes, uintptr_t b, int64_t stride, int64_t extent, int64_t count) {
-  if (a_bytes <= 0 || extent <= 0 || count <= 0) return false;
+// Whether [a, a + a_bytes) meets any of `count` blocks of `len` bytes at
+// distance `step` from b on (between them it may lie).
+inline bool span_meets_byte_blocks(uintptr_t a, int64_t a_bytes, uintptr_t b, __int128 step, __int128 len, int64_t count) {
+  if (a_bytes <= 0 || len <= 0 || count <= 0) return false;
   const __int128 lo = (__int128)a - (__int128)b, hi = lo + a_bytes;  // relative to the first block
-  const __int128 step = (__int128)stride * 2, len = (__int128)extent * 2;
   if (hi <= 0 || lo >= step * (count - 1) + len) return false;
   if (step <= 0 || lo < len) return true;
   // The first block that ends behind lo.
   const __int128 k = (lo - len) / step + 1;
   return k < count && k * step < hi;
+}
+// The same of 16-bit elements.
+inline bool span_meets_blocks(uintptr_t a, int64_t a_bytes, uintptr_t b, int64_t stride, int64_t extent, int64_t count) {
+  return span_meets_byte_blocks(a, a_bytes, b, (__int128)stride * 2, (__int128)extent * 2, count);
 }
 
 }  // namespace tx

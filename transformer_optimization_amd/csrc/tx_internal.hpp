@@ -118,6 +118,58 @@ struct RotaryArgs {
   SeqDiv by_units, by_v_units, by_token;
 };
 
+// rotary_append with norms, positions of several axes and 8-bit caches.  Strides
+// of caches and scales are in their own elements (a code or a scale: a byte).
+struct NormRotaryArgs {
+  SeqArgs s;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_out;
+  void* k_cache;
+  void* v_cache;
+  uint8_t* k_scales;  // nullptr: 16-bit caches
+  uint8_t* v_scales;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh, ko_st, ko_sh;
+  int64_t kc_sp, kc_sh, kc_st, vc_sp, vc_sh, vc_st;
+  int64_t ks_sp, ks_sh, ks_st, vs_sp, vs_sh, vs_st;
+  const void* q_weight;  // gains and shifts; each may be nullptr
+  const void* q_bias;
+  const void* k_weight;
+  const void* k_bias;
+  int param_f32;  // they are fp32 (else of the tensors' type)
+  int param_sh;   // elements from one head's to the next's: head_dim, or 0
+  int norm;       // TX_NORM_*
+  float eps;
+  const uint64_t* steps;
+  const int32_t* pair_axis;
+  const int64_t* positions;
+  int64_t positions_ld;
+  int axes;
+  int heads, kv_heads, head_dim, rotary;
+  float amplitude;
+  int interleaved;
+  SeqDiv by_rows;  // rows (heads of q, k and v) of a token
+};
+
+struct CacheAcceptArgs {
+  SeqArgs s;
+  void* k_cache;
+  void* v_cache;
+  uint8_t* k_scales;  // nullptr: 16-bit caches
+  uint8_t* v_scales;
+  // bytes
+  int64_t kc_sp, kc_sh, kc_st, vc_sp, vc_sh, vc_st;
+  int64_t ks_sp, ks_sh, ks_st, vs_sp, vs_sh, vs_st;
+  const int32_t* path;
+  int64_t path_ld;
+  const int32_t* counts;
+  int32_t* lens_out;
+  int max_path, heads;
+  int chunks, blocks;  // 16-byte chunks and scales of a head's row
+};
+
 struct SeqAttnArgs {
   SeqArgs s;
   const void* q;
@@ -137,10 +189,22 @@ struct SeqAttnArgs {
   int cus;
   float* ws;     // partial results: [rows][head_dim], normalised,
   float* ws_ml;  // and their maxima (log2 units) and sums, [rows][2]
+  // 8-bit caches (strides of k and v in bytes): scales, one byte for 32 elements.
+  const uint8_t* k_scales;  // nullptr: 16-bit caches
+  const uint8_t* v_scales;
+  int64_t ks_sp, ks_sh, ks_st, vs_sp, vs_sh, vs_st;
+  // Draft trees: which of its sequence's new tokens a token sees.
+  const uint64_t* tree;  // nullptr: none
+  int64_t tree_ld;
+  int tree_words;
 };
 
 int launch_rotary_append(const RotaryArgs& a, int dt, hipStream_t st);
 int launch_seq_attention(const SeqAttnArgs& a, int dt, hipStream_t st);
+int launch_norm_rotary_append(const NormRotaryArgs& a, int dt, hipStream_t st);
+int launch_cache_accept(const CacheAcceptArgs& a, hipStream_t st);
+// Paged attention over an 8-bit cache, or of a draft tree, or both.
+int launch_cache_attention(const SeqAttnArgs& a, int dt, hipStream_t st);
 // Floats of workspace a paged call of these sizes needs.
 int64_t seq_attention_workspace(const SeqAttnArgs& a);
 
