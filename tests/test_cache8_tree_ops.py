@@ -779,11 +779,17 @@ def test_what_a_tree_mask_hides_has_no_influence(cuda, mx, hd, n, m):
     got = _C.flash_attn_tree(q, kc, vc, *args, **sc)
     g = h // hk
     hit_k, hit_v = seen[:, key], seen[:, val]
-    assert torch.equal(got[:, :g][~hit_k], clean[:, :g][~hit_k]) and bool(torch.isnan(got[:, :g][hit_k]).all())
+    assert bool(torch.isfinite(clean).all()) and bool(torch.isnan(got[:, :g][hit_k]).all())
     d = [i for i in range(hd) if i != 7]
-    assert torch.equal(got[:, g:][~hit_v], clean[:, g:][~hit_v])
-    # rows with a value that is not finite are formed again: their other elements within tolerance
+    # Not every bit: rows side by side renew the base that their weights are measured from together, and another base
+    # rounds other weights up and down, each by half a step at most as before.
+    # Rows that meet 0 times a value that is not finite are formed again, with weights that are rounded after the
+    # division by their sum w_j / l, where the first pass rounds w_j and divides the sum of products.  Either way a
+    # weight is off by half a step, eps / 2 of p_j, and the result is rounded once, so the tolerance is the same
+    # (of its eps A for the weights the second half, for the sum, is not even used), but not every bit is.
     want, tol = _attend(q, ks[0], vs[0], hd**-0.5, seen, dtype)
+    _same(got[:, :g][~hit_k], want[:, :g][~hit_k], tol[:, :g][~hit_k], "rows that do not see the key")
+    _same(got[:, g:][~hit_v], want[:, g:][~hit_v], tol[:, g:][~hit_v], "rows that do not see it")
     _same(got[:, g:][..., d], want[:, g:][..., d], tol[:, g:][..., d], "other elements")
     assert bool((~torch.isfinite(got[:, g:, 7][hit_v])).all())
 
@@ -803,7 +809,10 @@ def test_hidden_nan_of_an_8_bit_cache_has_no_influence(cuda, hd, n):
     sc["k_scales"][pg, 0, slot, 0] = 255
     vc.view(torch.uint8)[pg, 1, slot, 9] = 0x7F
     got = _mx8(q, kc, vc, sc, *args)
-    assert torch.equal(got[:-1], clean[:-1])
+    assert bool(torch.isfinite(clean).all())
+    # (within tolerance, not every bit, as above)
+    want, tol = _attend(q, ks[0], vs[0], hd**-0.5, _causal(n, m, cuda), dtype)
+    _same(got[:-1], want[:-1], tol[:-1], "rows before it")
     assert bool(torch.isnan(got[-1, :2]).all()) and bool(torch.isnan(got[-1, 2:, 9]).all())
     assert bool(torch.isfinite(got[-1, 2:, :9]).all())
 
@@ -847,12 +856,13 @@ def test_a_tree_s_rows_do_not_need_the_pages_they_do_not_see(cuda, mx):
     parents = [-1, 0, 1, 2] + [0] * 12 + [4 + i % 4 for i in range(24)]
     q = _randn((n, h, hd), dtype, cuda, 146)
     args = (_cu([n], cuda), _i32([m], cuda), _C.tree_masks([parents], device=cuda), hd**-0.5)
-    good = _C.flash_attn_tree(q, kc, vc, table, *args, **sc)
     table[0, (m - n + 8) // page] = -1  # drafts 8 .. 15
     got = _C.flash_attn_tree(q, kc, vc, table, *args, **sc)
-    lost = _tree_seen(parents, m, cuda)[:, m - n + 8:m - n + 16].any(1)
+    seen = _tree_seen(parents, m, cuda)
+    lost = seen[:, m - n + 8:m - n + 16].any(1)
     assert bool(torch.isnan(got[lost]).all())
-    assert torch.equal(got[~lost], good[~lost])
+    want, tol = _attend(q, ks[0], vs[0], hd**-0.5, seen, dtype)
+    _same(got[~lost], want[~lost], tol[~lost], "the other rows")
 
 
 @gpu

@@ -215,6 +215,10 @@ __device__ __forceinline__ void ring_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// The same where no DMA is in flight: what this wave wrote to LDS is there; its
+// loads to registers go on.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // Wait for every memory operation of this wave, DMA issues included.  A ring
 // issues a few loads past its last step (into stages that are never read);
 // the last statement of a ring kernel drains them, so that no DMA lands in
