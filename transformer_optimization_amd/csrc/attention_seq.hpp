@@ -391,25 +391,25 @@ struct SqTile {
     // Codes: K of tile kk and V of tile kv (kk - LEAD) to registers, and from there to LDS.
     auto load8 = [&](int kk, int kv) {
       if constexpr (MX) {
-        if (LEAD && kv < kt1) ld.load(kv, ld.v);  // (its pages are those of the last K tile)
-        if (kk < kt1) {
-          ld.advance(kk);
-          ld.load(kk, ld.k);
-        }
-        if (!LEAD && kv < kt1) ld.load(kv, ld.v);
+        // (In every step, so that the compiler can count the loads in flight: past
+        // the last tile its last key again.)
+        if (LEAD && kv >= 0) ld.load(kv, ld.v);  // (its pages are those of the last K tile)
+        ld.advance(kk);
+        ld.load(kk, ld.k);
+        if (!LEAD) ld.load(kv, ld.v);
       }
     };
     auto put8 = [&](int kk, int kv) {
       if constexpr (MX) {
-        if (kk < kt1) ld.template put<true>(lds + (kk % NST) * L::ELEMS, ld.k);
-        if (kv < kt1) ld.template put<false>(lds + (NST + kv % NST) * L::ELEMS, ld.v);
+        ld.template put<true>(lds + (kk % NST) * L::ELEMS, ld.k);
+        if (!LEAD || kv >= 0) ld.template put<false>(lds + (NST + kv % NST) * L::ELEMS, ld.v);
       }
     };
     if constexpr (MX) {
       ld.lookup(kt0);
       if constexpr (LEAD) {
-        load8(kt0, kt1);
-        put8(kt0, kt1);
+        load8(kt0, -1);
+        put8(kt0, -1);
       }
       load8(kt0 + LEAD, kt0);
       put8(kt0 + LEAD, kt0);
@@ -722,7 +722,7 @@ __device__ __forceinline__ void sq_odd_rows(int b, int q0, int hk, int base, int
   for (int k0 = j0; k0 < lim; k0 += 32) {
     if ((k0 - j0) % 64 == 0) {  // look through 64 keys
       uint32_t any = 0;
-#pragma unroll
+#pragma unroll(MX ? 1 : HD / 8)  // (of codes: the kernels' registers again)
       for (int i = 0; i < HD / 8; ++i) {
         const Elem *kr, *vr;
         const int x = 64 * i + lane;
@@ -794,14 +794,20 @@ __device__ __forceinline__ void sq_odd_rows(int b, int q0, int hk, int base, int
 #pragma unroll 1
   for (int k0 = j0; k0 < lim; k0 += 32) {
     uint32_t v[HD / 16][8];  // asked for before the keys, whose loads they overlap
+    if constexpr (!MX) {
 #pragma unroll
-    for (int d = 0; d < HD / 16; ++d) values(k0, d, v[d]);
+      for (int d = 0; d < HD / 16; ++d) values(k0, d, v[d]);
+    }
     f32x4 w[2];
     weights(k0, w);
     const u32x4 pw = {pack2<T>(w[0][0] * f, w[0][1] * f), pack2<T>(w[0][2] * f, w[0][3] * f),
                       pack2<T>(w[1][0] * f, w[1][1] * f), pack2<T>(w[1][2] * f, w[1][3] * f)};
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) {
+      if constexpr (MX) {
+        values(k0, d, v[d]);
+        asm volatile("" ::: "memory");  // one after another: two loads a value
+      }
       u32x4 vv;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -952,50 +958,164 @@ __global__ __launch_bounds__(SQ_THREADS, HD == 64 ? 4 : 2) void seq_attn_packed_
 // .. + 3 of both 16-key halves of row l & 15, which is a P operand as it stands
 // if V's rows are taken in that order.  The waves' results meet in LDS at the
 // end.
-template <typename T, int HD>
+//
+// 8-bit rows come through registers instead, AHEAD blocks before their use, and
+// are converted into the same layout of one LDS block, K's first, V's in its
+// place once the scores are formed.
+template <typename T, int HD, bool MX>
 struct SqFew {
   typedef typename Mfma16<T>::vec vec;
   static constexpr int CH = HD / 8, RPI = 64 / CH, LDB = 32 / RPI;  // rows per instruction, instructions per block
   static constexpr int ELEMS = 32 * HD;                             // a block of K or V; o of 16 rows in fp32
-  static constexpr int WAVE_ELEMS = 2 * ELEMS;
+  static constexpr int WAVE_ELEMS = MX ? ELEMS : 2 * ELEMS;
   static constexpr float BIAS = SqTile<T, HD, SQ_PAGED>::BIAS;
   // Instruction x moves the keys LDB (lane / CH) + x, so that a lane's keys lie
   // in one page (LDB divides 8); they land at LDS row x RPI + lane / CH.  The
   // 16-byte chunks of a key are xor-ed for the reads: 16 keys at one chunk (K),
   // 8 keys x 32 bytes (V) fall on different banks.
-  // 8-bit rows: 16-code chunks; a lane's keys of a block are LDB8 (lane / CH8) + x.
+  // 8-bit rows: CH8 chunks of 16 codes; a lane's keys of a block are LDB8 (lane /
+  // CH8) + x.  Its two 16-byte halves of a chunk go to even and odd places, so
+  // the swizzles' lowest bit is one that differs between neighbouring rows of a
+  // write (16 lanes then fill all banks).
   static constexpr int CH8 = HD / 16, LDB8 = 32 * CH8 / 64;
+  #ifndef SQ8_AHEAD
+#define SQ8_AHEAD 2
+#define SQ8_RES 2
+#endif
+  static constexpr int AHEAD = HD == 128 ? SQ8_AHEAD : 1;
   static __device__ __forceinline__ int lds_row(int key) { return key % LDB * RPI + key / LDB; }
   static __device__ __forceinline__ int kswz(int key) {
+    if (MX) return HD == 128 ? ((key >> 2) & 3) | ((key & 3) << 2) : ((key >> 1) & 1) | ((key & 1) << 1) | ((key >> 1) & 4);
     return HD == 128 ? key & 15 : (key & 3) | ((key >> 1) & 4);
   }
-  static __device__ __forceinline__ int vswz(int key) { return HD == 128 ? (key & 7) << 1 : (key & 3) << 1; }
+  static __device__ __forceinline__ int vswz(int key) {
+    if (MX) return HD == 128 ? (key & 7) << 1 | ((key >> 2) & 1) : (key & 3) << 1 | ((key >> 1) & 1);
+    return HD == 128 ? (key & 7) << 1 : (key & 3) << 1;
+  }
 };
+
+// The maximum over lanes l, l ^ 16, l ^ 32 and l ^ 48, on the vector ALU alone.
+__device__ __forceinline__ float sq_max_groups(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+  const uint32_t v = __builtin_bit_cast(uint32_t, x);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
 
 // The x-th lane's value of each four lanes.
 template <int X> __device__ __forceinline__ uint32_t sq_quad(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, X * 0x55, 0xf, 0xf, true);
 }
 
-template <typename T, int HD, int K>
+// The keys of an item of few rows (wave-uniform).
+struct SqKeys {
+  int b, hk, j0, lim;
+};
+// Keys that the rows of an item see at most.
+template <int K>
+__device__ __forceinline__ int sq_few_lim(const SeqAttnArgs& a, const SeqWork& w, int r0, int j1) {
+  const int last = min(w.qn * a.group - r0, w.cut.tile_rows) + r0 - 1;
+  const int sees = !(K & SQ_TREE) && a.causal ? w.kvn - w.qn + seq_div(last, a.by_group) + 1 : w.kvn;
+  return seq_uni(min(min(max(sees, 0), a.s.max_pages << a.s.page_log2), j1));
+}
+// Codes of a wave's blocks on their way through its registers: of each slot
+// (block n of an item goes to slot n % N), a lane's codes of LDB8 keys at one
+// chunk, and for each four lanes the scales of their keys, one key a lane.
+// A lane's keys lie in one page, so those past the last are read too.  What a
+// slot is loaded with once it is used: the item's next block of that slot, or,
+// past its last, the next item's first, so that an item's first keys arrive while
+// the waves of the one before it meet.  Every block loads the same number of
+// times, so that the compiler can count the loads in flight and waits for those
+// it needs alone.
+template <typename T, int HD>
+struct SqAhead8 {
+  typedef SqFew<T, HD, true> F;
+  static constexpr int N = F::AHEAD, STEP = 128 * N;
+  struct Side {
+    u32x4 x[F::LDB8];
+    uint32_t s;
+  };
+  Side k[N], v[N];
+  uint32_t at[N];    // pages that the slots are loaded from
+  uint32_t page[N];  // and the ones after them
+  int chunk, key0;   // this lane's chunk; its first key within a block
+
+  __device__ __forceinline__ int first(const SqKeys& c, int wave) const { return c.j0 + 32 * wave; }
+  // (keys past the last: the last ones; without any, the first slot of the table)
+  __device__ __forceinline__ int key(const SqKeys& c, int kb) const { return min(kb + key0, (max(c.lim, 1) - 1) & ~(F::LDB8 - 1)); }
+  __device__ __forceinline__ uint32_t lookup(const SeqAttnArgs& a, const SqKeys& c, int kb) const {
+    return (uint32_t)a.s.table[(int64_t)c.b * a.s.table_ld + (key(c, kb) >> a.s.page_log2)];
+  }
+  __device__ __forceinline__ void fetch(const SeqAttnArgs& a, const SqKeys& c, int kb, uint32_t page, Side& y, const void* head,
+                                        const uint8_t* scales, int64_t sp, int64_t st, int64_t ssp, int64_t sst, int lane) const {
+    page = page < (uint32_t)a.s.num_pages ? page : 0;  // page 0 in the place of one that is not there
+    const uint32_t slot = (uint32_t)(key(c, kb) & ((1 << a.s.page_log2) - 1));
+    const uint8_t* row = (const uint8_t*)head + ((uint64_t)page * (uint32_t)sp + slot * (uint32_t)st) + 16 * chunk;
+#pragma unroll
+    for (int i = 0; i < F::LDB8; ++i) y.x[i] = __builtin_nontemporal_load((const u32x4*)(row + (uint32_t)i * (uint32_t)st));
+    const uint8_t* from = scales + ((uint64_t)page * (uint32_t)ssp + (slot + (lane & (F::LDB8 - 1))) * (uint32_t)sst);
+    if constexpr (HD == 128) y.s = *(const uint32_t*)from;
+    else y.s = *(const uint16_t*)from;
+  }
+  __device__ __forceinline__ void fetch_k(const SeqAttnArgs& a, const SqKeys& c, int kb, uint32_t page, Side& y, int lane) const {
+    fetch(a, c, kb, page, y, (const uint8_t*)a.k + c.hk * a.k_sh, a.k_scales + c.hk * a.ks_sh, a.k_sp, a.k_st, a.ks_sp, a.ks_st, lane);
+  }
+  __device__ __forceinline__ void fetch_v(const SeqAttnArgs& a, const SqKeys& c, int kb, uint32_t page, Side& y, int lane) const {
+    fetch(a, c, kb, page, y, (const uint8_t*)a.v + c.hk * a.v_sh, a.v_scales + c.hk * a.vs_sh, a.v_sp, a.v_st, a.vs_sp, a.vs_st, lane);
+  }
+  // The first blocks of an item.
+  __device__ __forceinline__ void start(const SeqAttnArgs& a, const SqKeys& c, int lane, int wave) {
+    chunk = lane % F::CH8;
+    key0 = lane / F::CH8 * F::LDB8;
+    static_for<N>([&](auto ic) { load<decltype(ic)::value>(a, c, lane, wave); });
+  }
+  template <int I> __device__ __forceinline__ void load(const SeqAttnArgs& a, const SqKeys& c, int lane, int wave) {
+    const int kb = first(c, wave) + 128 * I;
+    at[I] = lookup(a, c, kb);
+    fetch_k(a, c, kb, at[I], k[I], lane);
+    fetch_v(a, c, kb, at[I], v[I], lane);
+  }
+  // 16-bit rows of a block, to LDS.  (A wave's LDS operations complete in the order that they are written in.)
+  template <typename Swz> __device__ __forceinline__ void put(const Side& y, T* to, Swz swz) const {
+    asm volatile("" ::: "memory");
+    static_for<F::LDB8>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      const int kk = key0 + i, z = swz(kk);
+      const float sc = mx_scale(__builtin_amdgcn_ubfe(sq_quad<i>(y.s), 8 * (chunk >> 1), 8));
+      T* row = to + F::lds_row(kk) * HD;
+      st128(row + (((2 * chunk) ^ z) << 3), mx_values<T>(y.x[i][0], y.x[i][1], sc));
+      st128(row + (((2 * chunk + 1) ^ z) << 3), mx_values<T>(y.x[i][2], y.x[i][3], sc));
+    });
+    asm volatile("" ::: "memory");
+  }
+};
+struct SqNoAhead {};
+
+// next: the keys of the workgroup's next item, whose first blocks `ahead` holds
+// on return (8-bit; those of this item it holds already).
+template <typename T, int HD, int K, typename Ahead>
 __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork& w, int hk, int r0, int j0, int j1,
                                             float* part, float* ml, T* lds, float* stat, int* bad, int lane,
-                                            int wave) {
+                                            int wave, Ahead& ahead, const SqKeys& next) {
   constexpr bool MX = (K & SQ_MX8) != 0, TREE = (K & SQ_TREE) != 0;
-  typedef SqFew<T, HD> F;
+  typedef SqFew<T, HD, MX> F;
   typedef typename F::vec vec;
   const float NEG_INF = -__builtin_inff();
   const float c = a.scale * SQ_LOG2E;
   const int G = a.group, n = min(w.qn * G - r0, w.cut.tile_rows);
   const int cap = a.s.max_pages << a.s.page_log2, ps1 = (1 << a.s.page_log2) - 1;
   auto keys_of = [&](int r) { return max(!TREE && a.causal ? w.kvn - w.qn + seq_div(r, a.by_group) + 1 : w.kvn, 0); };
-  const int lim = seq_uni(min(min(keys_of(r0 + n - 1), cap), j1));
+  const int lim = sq_few_lim<K>(a, w, r0, j1);
   const int col = lane & 15, g = lane >> 4;
   const int r = r0 + min(col, n - 1);
   const int i0 = seq_div(r, a.by_group);
   const int64_t tok = w.q0 + i0;
   const int h = hk * G + r - i0 * G;
   const int mylim = min(keys_of(r), lim);
+  // Keys that every row sees.
+  const int lim_min = seq_uni(min(TREE ? max(w.kvn - w.qn, 0) : keys_of(r0), lim));
   SqTreeRow tr;
   if constexpr (TREE) tr.init(a, tok, w.kvn - w.qn);
   SeqHead<T, K> hp;
@@ -1025,7 +1145,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   auto key0 = [&](int kb) { return min(kb + lane / F::CH * F::LDB, (lim - 1) & ~(F::LDB - 1)); };
   auto lookup = [&](int kb) { return (uint32_t)table[key0(kb) >> a.s.page_log2]; };
   T* ks = lds + wave * F::WAVE_ELEMS;
-  T* vs = ks + F::ELEMS;
+  T* vs = MX ? ks : ks + F::ELEMS;
   auto load = [&](int kb, uint32_t page, T* to, const T* head, int64_t sp, int64_t st, auto swz) {
     const int key = key0(kb), left = lim - 1 - key;
     if (page >= (uint32_t)a.s.num_pages) {  // page 0 in the place of one that is not there
@@ -1045,66 +1165,15 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   auto load_v = [&](int kb, uint32_t page) {
     if constexpr (!MX) load(kb, page, vs, hp.v, a.v_sp, a.v_st, F::vswz);
   };
-  // 8-bit rows come through registers: codes of a lane's keys at one chunk, and
-  // for each four lanes the scales of their keys, one key a lane.
-  struct Block {
-    u32x4 k[F::LDB8], v[F::LDB8];
-    uint32_t ks, vs;
-  };
-  const int c8 = lane % F::CH8, g8 = lane / F::CH8 * F::LDB8;
-  auto key8 = [&](int kb) { return min(kb + g8, (lim - 1) & ~(F::LDB8 - 1)); };
-  auto lookup8 = [&](int kb) { return (uint32_t)table[key8(kb) >> a.s.page_log2]; };
-  auto fetch = [&](int kb, uint32_t page, Block& x) {
-    if constexpr (MX) {
-      const int key = key8(kb), left = lim - 1 - key;
-      if (page >= (uint32_t)a.s.num_pages) {
-        bad_from = min(bad_from, key & ~ps1);
-        page = 0;
-      }
-      const uint32_t slot = (uint32_t)(key & ps1);
-      auto side = [&](const uint8_t* head, const uint8_t* scales, int64_t sp, int64_t st, int64_t ssp, int64_t sst, u32x4* y,
-                      uint32_t& s) {
-        const uint8_t* row = head + ((uint64_t)page * (uint32_t)sp + slot * (uint32_t)st) + 16 * c8;
-#pragma unroll
-        for (int i = 0; i < F::LDB8; ++i)
-          y[i] = __builtin_nontemporal_load((const u32x4*)(row + (uint32_t)min(i, left) * (uint32_t)st));
-        const uint32_t i = (uint32_t)min(lane & (F::LDB8 - 1), left);
-        const uint8_t* at = scales + ((uint64_t)page * (uint32_t)ssp + (slot + i) * (uint32_t)sst);
-        if constexpr (HD == 128) s = *(const uint32_t*)at;
-        else s = *(const uint16_t*)at;
-      };
-      side(hp.k, a.k_scales + hk * a.ks_sh, a.k_sp, a.k_st, a.ks_sp, a.ks_st, x.k, x.ks);
-      side(hp.v, a.v_scales + hk * a.vs_sh, a.v_sp, a.v_st, a.vs_sp, a.vs_st, x.v, x.vs);
-    }
-  };
-  auto put = [&](const Block& x) {
-    if constexpr (MX) {
-      asm volatile("" ::: "memory");  // the block before this one is read
-      static_for<F::LDB8>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        const int key = g8 + i;
-        const float sk = mx_scale((sq_quad<i>(x.ks) >> (8 * (c8 >> 1))) & 0xFFu);
-        const float sv = mx_scale((sq_quad<i>(x.vs) >> (8 * (c8 >> 1))) & 0xFFu);
-        T* kr = ks + F::lds_row(key) * HD;
-        T* vr = vs + F::lds_row(key) * HD;
-        st128(kr + (((2 * c8) ^ F::kswz(key)) << 3), mx_values<T>(x.k[i][0], x.k[i][1], sk));
-        st128(kr + (((2 * c8 + 1) ^ F::kswz(key)) << 3), mx_values<T>(x.k[i][2], x.k[i][3], sk));
-        st128(vr + (((2 * c8) ^ F::vswz(key)) << 3), mx_values<T>(x.v[i][0], x.v[i][1], sv));
-        st128(vr + (((2 * c8 + 1) ^ F::vswz(key)) << 3), mx_values<T>(x.v[i][2], x.v[i][3], sv));
-      });
-      // (a wave's LDS operations complete in order)
-      asm volatile("" ::: "memory");
-    }
-  };
   const uint32_t vbase = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) T*)vs;
   // Transposing reads: lane j of a 16-lane group g addresses key 4 g + j / 4
   // (and + 16) at dims 16 d + 4 (j % 4) and receives dim 16 d + j of 4 keys.
   const int vkey = 4 * g + (col >> 2);
   const uint32_t vrow = vbase + (uint32_t)(F::lds_row(vkey) * HD * 2 + (col & 1) * 8);
-  const int vx = (col & 3) >> 1, vsw = F::vswz(vkey);
+  const int vx = ((col & 3) >> 1) ^ (F::vswz(vkey) & 1), vsw = F::vswz(vkey) & ~1;
   const T* krow = ks + F::lds_row(col) * HD;
   const int ksw = F::kswz(col);
-  auto compute = [&](int kb, uint32_t page, bool more) {
+  auto compute = [&](int kb, uint32_t page, bool more, auto between) {
     // This block's K rows are there: only its V rows may still be on the way
     // (a page lookup among them makes the wait stricter).
     if constexpr (!MX) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(F::LDB) : "memory");
@@ -1116,10 +1185,13 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
       for (int i = 0; i < HD / 32; ++i)
         acc = Mfma16<T>::mma(__builtin_bit_cast(vec, ld128(krow + 16 / F::LDB * x * HD + (((4 * i + g) ^ ksw) << 3))), qf[i], acc);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[4 * x + e] = (kb + 16 * x + 4 * g + e < mylim) ? acc[e] : NEG_INF;
+      for (int e = 0; e < 4; ++e) s[4 * x + e] = acc[e];
     }
-    if constexpr (TREE) {
-      if (kb + 32 > tr.base) {
+    if (kb + 32 > lim_min) {
+      const int d = mylim - kb - 4 * g;  // slot of key kb + 4 g + x is seen if x < d
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = (16 * (e >> 2) + (e & 3) < d) ? s[e] : NEG_INF;
+      if constexpr (TREE) {
         const uint32_t seen = (uint32_t)(tr.window(kb) >> (4 * g));
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] = (seen >> (16 * (e >> 2) + (e & 3))) & 1u ? s[e] : NEG_INF;
@@ -1132,8 +1204,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
     float mx = NEG_INF;
 #pragma unroll
     for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    mx = sq_max_groups(mx);
     mx *= c;
     if (__any(mx > m_run + 8.f)) {
       const float m_new = fmaxf(m_run, mx);
@@ -1151,6 +1222,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
                                                  pack2_raw<T>(p[4], p[5]), pack2_raw<T>(p[6], p[7])});
     lsum = Mfma16<T>::mma(ones, pf, lsum);
     // This block's V rows: only the next one's K may still be on the way.
+    between();
     if constexpr (!MX) {
       if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(F::LDB) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1175,25 +1247,51 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
 
   const int first = j0 + 32 * wave;
   if constexpr (MX) {
-    // Two blocks ahead in registers.
-    if (first < lim) {
-      uint32_t p2 = lookup8(first + 256), p3 = lookup8(first + 384);
-      Block x, y;
-      fetch(first, lookup8(first), x);
-      if (first + 128 < lim) fetch(first + 128, lookup8(first + 128), y);
-      for (int kb = first; kb < lim; kb += 256) {
-        put(x);
-        if (kb + 256 < lim) fetch(kb + 256, p2, x);
-        p2 = lookup8(kb + 512);
-        compute(kb, 0, false);
-        if (kb + 128 < lim) {
-          put(y);
-          if (kb + 384 < lim) fetch(kb + 384, p3, y);
-          p3 = lookup8(kb + 640);
-          compute(kb + 128, 0, false);
+    constexpr int N = F::AHEAD, STEP = Ahead::STEP;
+    const SqKeys cur{w.b, hk, j0, lim};
+    const int next_first = ahead.first(next, wave);
+    static_for<N>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      const bool more = first + 128 * i + STEP < lim;
+      ahead.page[i] = ahead.lookup(a, more ? cur : next, more ? first + 128 * i + STEP : next_first + 128 * i);
+    });
+    auto block = [&](auto ic, int kb) {
+      constexpr int i = decltype(ic)::value;
+      if (ahead.at[i] >= (uint32_t)a.s.num_pages) bad_from = min(bad_from, ahead.key(cur, kb) & ~ps1);
+      const uint32_t page = ahead.page[i];
+      const bool more = kb + STEP < lim, more2 = kb + 2 * STEP < lim;
+      const SqKeys to = more ? cur : next;
+      const int then = more ? kb + STEP : next_first + 128 * i;
+      ahead.page[i] = ahead.lookup(a, more2 ? cur : next, more2 ? kb + 2 * STEP : next_first + 128 * i);
+      ahead.put(ahead.k[i], ks, F::kswz);
+      ahead.fetch_k(a, to, then, page, ahead.k[i], lane);
+      compute(kb, 0, false, [&]() {
+        auto& y = ahead.v[i];
+        if (kb + 32 > lim) {  // (weights of 0 times what the slots past the last key hold)
+#pragma unroll
+          for (int e = 0; e < F::LDB8; ++e)
+            if (kb + ahead.key0 + e >= lim) y.x[e] = u32x4{0, 0, 0, 0};
         }
+        ahead.put(y, ks, F::vswz);
+        ahead.fetch_v(a, to, then, page, y, lane);
+        ahead.at[i] = page;
+      });
+    };
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the slots' order differs from item to item
+    int kb = first;
+    if constexpr (N == 2) {
+      for (; kb + 128 < lim; kb += 256) {
+        block(std::integral_constant<int, 0>{}, kb);
+        block(std::integral_constant<int, N - 1>{}, kb + 128);
       }
+      if (kb < lim) block(std::integral_constant<int, 0>{}, kb);
+    } else {
+      for (; kb < lim; kb += 128) block(std::integral_constant<int, 0>{}, kb);
     }
+    static_for<N>([&](auto ic) {  // slots that this item has no block for
+      constexpr int i = decltype(ic)::value;
+      if (first + 128 * i >= lim) ahead.template load<i>(a, next, lane, wave);
+    });
   } else if (first < lim) {
     uint32_t page = lookup(first), next = lookup(first + 128);
     load_k(first, page);
@@ -1201,10 +1299,15 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
     for (int kb = first; kb < lim; kb += 128) {
       page = next;
       next = lookup(kb + 256);
-      compute(kb, page, kb + 128 < lim);
+      compute(kb, page, kb + 128 < lim, []() {});
     }
   }
 
+  // (8-bit: loads go on across the barriers)
+  auto meet = []() {
+    if constexpr (MX) lds_barrier();
+    else __syncthreads();
+  };
   // Join the waves: o in fp32 over each wave's K block, m and l beside it.
   if (threadIdx.x == 0) *bad = cap;
   float* ow = (float*)ks;
@@ -1212,7 +1315,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   float* sm = stat + wave * 16;
   float* sl = stat + 64 + wave * 16;
   int* sagain = (int*)(stat + 128);
-  __syncthreads();
+  meet();
   if (bad_from < cap) atomicMin(bad, bad_from);
 #pragma unroll
   // (4-value chunks xor the row: 16 rows at one chunk would share 4 banks)
@@ -1222,7 +1325,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
     sl[col] = lsum[0];
   }
   if (threadIdx.x < 16) sagain[threadIdx.x] = 0;
-  __syncthreads();
+  meet();
   const int lost_from = *bad;
   constexpr int DT = HD / 16;  // dims a thread joins: 16 threads a row
   const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 4;
@@ -1267,7 +1370,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   // (as in a tile)
   const bool redo = active && !lost && (TREE ? some : sees > j0) && L == L && (L != 0.f || part) && !(odd == 0.f);
   if (redo) sagain[row] = 1;
-  __syncthreads();
+  meet();
   const int hh = hk * G + rr - ir * G;
   if (active) {
     if (part) {
@@ -1302,48 +1405,93 @@ __host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
   return SeqShape{a.group, a.kv_heads, a.cus, a.head_dim == 128 ? 2 : 1, a.few_parts, a.few};
 }
 
+// Workgroups of a call that are resident on a CU.
+template <int HD, bool FEW_ONLY, int K>
+constexpr int sq_resident() {
+  if (FEW_ONLY && (K & SQ_MX8)) return HD == 64 ? 4 : SQ8_RES;
+  return HD == 64 ? (FEW_ONLY ? 4 : 3) : 2;
+}
+
 // Persistent workgroups over the items of a call (SeqWalk); a grid of at most
 // the items, so every workgroup's loop ends.
 template <typename T, int HD, bool FEW_ONLY, int K>
-__global__ __launch_bounds__(SQ_THREADS, HD == 64 ? (FEW_ONLY ? 4 : 3) : 2) void seq_attn_paged_kernel(SeqAttnArgs a) {
-  constexpr int TILE_ELEMS = SqTile<T, HD, K>::LDS_ELEMS, FEW_ELEMS = 4 * SqFew<T, HD>::WAVE_ELEMS;
+__global__ __launch_bounds__(SQ_THREADS, (sq_resident<HD, FEW_ONLY, K>())) void seq_attn_paged_kernel(SeqAttnArgs a) {
+  constexpr int TILE_ELEMS = SqTile<T, HD, K>::LDS_ELEMS, FEW_ELEMS = 4 * SqFew<T, HD, (K & SQ_MX8) != 0>::WAVE_ELEMS;
   constexpr int ELEMS = FEW_ONLY || FEW_ELEMS > TILE_ELEMS ? FEW_ELEMS : TILE_ELEMS;
   __shared__ __attribute__((aligned(16))) T lds[ELEMS];
   __shared__ float stat[144];
   __shared__ int bad[4];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  constexpr bool MX = (K & SQ_MX8) != 0;
   const SeqShape sh = sq_shape(a);
   __shared__ int seqs[SeqWalk::LDS_INTS];
   SeqWalk walk;
   walk.init(a.s, sh, false, seqs);
-  SeqWork w;
-  for (int i = blockIdx.x; walk.find(a.s, sh, false, i, w); i += gridDim.x) {
+  // Item i: its place in the call.
+  struct Item {
+    SeqWork w;
+    int hk, r0, j0, j1, np, pair;
+  };
+  auto find = [&](int i, Item& x) {
+    if (!walk.find(a.s, sh, false, i, x.w)) return false;
+    // Item u of a sequence: its (part, K/V head) pairs first, then its tiles:
+    // the tiles that share keys meet on one XCD when the pairs are a multiple
+    // of 8.
+    const int u = i - x.w.item;
+    x.np = x.w.cut.parts * a.kv_heads;
+    const int tile = x.w.cut.tiles > 1 ? seq_uni(u / x.np) : 0;
+    x.pair = u - tile * x.np;
+    const int p = seq_uni(seq_div(x.pair, a.by_kv_heads));
+    x.hk = x.pair - p * a.kv_heads;
+    x.j0 = p * x.w.cut.part_keys;
+    x.j1 = p + 1 < x.w.cut.parts ? x.j0 + x.w.cut.part_keys : 0x7fffffff;
+    x.r0 = tile * x.w.cut.tile_rows;
+    return true;
+  };
+  // 8-bit rows of few-row items: the first blocks of the next item are loaded within this one.
+  typename std::conditional<MX, SqAhead8<T, HD>, SqNoAhead>::type ahead;
+  Item x, y;
+  bool have = find(blockIdx.x, x);
+  if constexpr (MX && FEW_ONLY) {
+    if (have) ahead.start(a, SqKeys{x.w.b, x.hk, x.j0, sq_few_lim<K>(a, x.w, x.r0, x.j1)}, threadIdx.x & 63, wave);
+  }
+  for (int i = blockIdx.x; have;) {
+    i += gridDim.x;
+    SqKeys next{x.w.b, x.hk, 0, 1};  // none: the sequence's first key
+    bool have_next = false;
+    if constexpr (MX && FEW_ONLY) {
+      have_next = find(i, y);
+      if (have_next) next = SqKeys{y.w.b, y.hk, y.j0, sq_few_lim<K>(a, y.w, y.r0, y.j1)};
+    }
+    const SeqWork& w = x.w;
     // An item's lane constants are formed within it: held across the items
     // they cost the registers that its loads need (56 spills).
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
-    // Item u of a sequence: its (part, K/V head) pairs first, then its tiles:
-    // the tiles that share keys meet on one XCD when the pairs are a multiple
-    // of 8.
-    const int u = i - w.item, np = w.cut.parts * a.kv_heads;
-    const int tile = w.cut.tiles > 1 ? seq_uni(u / np) : 0, pair = u - tile * np;
-    const int p = seq_uni(seq_div(pair, a.by_kv_heads)), hk = pair - p * a.kv_heads;
-    const int j0 = p * w.cut.part_keys, j1 = p + 1 < w.cut.parts ? j0 + w.cut.part_keys : 0x7fffffff;
     // Partial results of a sequence: by tile, part, K/V head, row of the tile.
-    const int r0 = tile * w.cut.tile_rows;
     float *part = nullptr, *ml = nullptr;
     if (w.cut.parts > 1) {
-      const int64_t at = w.partial + r0 * np + pair * min(w.qn * a.group - r0, w.cut.tile_rows);
+      const int64_t at = w.partial + x.r0 * x.np + x.pair * min(w.qn * a.group - x.r0, w.cut.tile_rows);
       part = a.ws + at * HD;
       ml = a.ws_ml + at * 2;
     }
     if constexpr (FEW_ONLY) {
-      sq_few_item<T, HD, K>(a, w, hk, r0, j0, j1, part, ml, lds, stat, bad, lane, wave);
+      sq_few_item<T, HD, K>(a, w, x.hk, x.r0, x.j0, x.j1, part, ml, lds, stat, bad, lane, wave, ahead, next);
+    } else if (w.cut.few) {
+      if constexpr (MX) ahead.start(a, SqKeys{w.b, x.hk, x.j0, sq_few_lim<K>(a, w, x.r0, x.j1)}, lane, wave);
+      sq_few_item<T, HD, K>(a, w, x.hk, x.r0, x.j0, x.j1, part, ml, lds, stat, bad, lane, wave, ahead, next);
     } else {
-      if (w.cut.few) sq_few_item<T, HD, K>(a, w, hk, r0, j0, j1, part, ml, lds, stat, bad, lane, wave);
-      else sq_tile_item<T, HD, K>(a, w.b, w.q0, w.qn, w.kvn, hk, r0, j0, j1, part, ml, lds, bad, lane, wave);
+      sq_tile_item<T, HD, K>(a, w.b, w.q0, w.qn, w.kvn, x.hk, x.r0, x.j0, x.j1, part, ml, lds, bad, lane, wave);
     }
-    __syncthreads();  // LDS belongs to the next item
+    // LDS belongs to the next item.
+    if constexpr (MX && FEW_ONLY) {
+      lds_barrier();
+      x = y;
+      have = have_next;
+    } else {
+      __syncthreads();
+      have = find(i, x);
+    }
   }
 }
 
@@ -1506,10 +1654,8 @@ int sq_launch_paged(SeqAttnArgs a, hipStream_t st) {
   const SeqBounds b = sq_bounds(a);
   a.ws_ml = a.ws + b.partials * HD;
   auto grid = [](int64_t items, int64_t most) { return dim3((unsigned)(items < most ? items : most)); };
-  // As many workgroups as are resident: few rows 4 a CU at head dim 64 and 2 at
-  // 128, tiles 3 and 2.
-  if (a.few) seq_attn_paged_kernel<T, HD, true, K><<<grid(b.items, (HD == 64 ? 4 : 2) * a.cus), block, 0, st>>>(a);
-  else seq_attn_paged_kernel<T, HD, false, K><<<grid(b.items, (HD == 64 ? 3 : 2) * a.cus), block, 0, st>>>(a);
+  if (a.few) seq_attn_paged_kernel<T, HD, true, K><<<grid(b.items, sq_resident<HD, true, K>() * a.cus), block, 0, st>>>(a);
+  else seq_attn_paged_kernel<T, HD, false, K><<<grid(b.items, sq_resident<HD, false, K>() * a.cus), block, 0, st>>>(a);
   if (hipGetLastError() != hipSuccess) return TX_EHIP;
   if (b.partials > 0) {
     seq_attn_join_kernel<T, HD, (K & SQ_TREE) != 0><<<grid(b.join_rows, 4 * a.cus), block, 0, st>>>(a);
