@@ -974,22 +974,25 @@ struct SqFew {
   // 16-byte chunks of a key are xor-ed for the reads: 16 keys at one chunk (K),
   // 8 keys x 32 bytes (V) fall on different banks.
   // 8-bit rows: CH8 chunks of 16 codes; a lane's keys of a block are LDB8 (lane /
-  // CH8) + x.  Its two 16-byte halves of a chunk go to even and odd places, so
-  // the swizzles' lowest bit is one that differs between neighbouring rows of a
-  // write (16 lanes then fill all banks).
+  // CH8) + x.  It writes a chunk as two of 16 bytes, and eight lanes' writes are
+  // free of bank conflicts where they fill 128 bytes of addresses modulo 128 (16
+  // cycles an instruction otherwise, for 8): at head dim 128, where they lie in one
+  // row, pos() swaps the two in the row's second half; at 64, in two rows, the
+  // lowest bit of the swizzles differs between those.
   static constexpr int CH8 = HD / 16, LDB8 = 32 * CH8 / 64;
-  #ifndef SQ8_AHEAD
+#ifndef SQ8_AHEAD
 #define SQ8_AHEAD 2
 #define SQ8_RES 2
 #endif
   static constexpr int AHEAD = HD == 128 ? SQ8_AHEAD : 1;
+  static __device__ __forceinline__ int pos(int chunk) { return MX && HD == 128 ? chunk ^ (chunk >> 3) : chunk; }
   static __device__ __forceinline__ int lds_row(int key) { return key % LDB * RPI + key / LDB; }
   static __device__ __forceinline__ int kswz(int key) {
-    if (MX) return HD == 128 ? ((key >> 2) & 3) | ((key & 3) << 2) : ((key >> 1) & 1) | ((key & 1) << 1) | ((key >> 1) & 4);
+    if (MX && HD == 64) return ((key >> 1) & 1) | ((key & 1) << 1) | ((key >> 1) & 4);
     return HD == 128 ? key & 15 : (key & 3) | ((key >> 1) & 4);
   }
   static __device__ __forceinline__ int vswz(int key) {
-    if (MX) return HD == 128 ? (key & 7) << 1 | ((key >> 2) & 1) : (key & 3) << 1 | ((key >> 1) & 1);
+    if (MX && HD == 64) return (key & 3) << 1 | ((key >> 1) & 1);
     return HD == 128 ? (key & 7) << 1 : (key & 3) << 1;
   }
 };
@@ -1085,8 +1088,8 @@ struct SqAhead8 {
       const int kk = key0 + i, z = swz(kk);
       const float sc = mx_scale(__builtin_amdgcn_ubfe(sq_quad<i>(y.s), 8 * (chunk >> 1), 8));
       T* row = to + F::lds_row(kk) * HD;
-      st128(row + (((2 * chunk) ^ z) << 3), mx_values<T>(y.x[i][0], y.x[i][1], sc));
-      st128(row + (((2 * chunk + 1) ^ z) << 3), mx_values<T>(y.x[i][2], y.x[i][3], sc));
+      st128(row + ((F::pos(2 * chunk) ^ z) << 3), mx_values<T>(y.x[i][0], y.x[i][1], sc));
+      st128(row + ((F::pos(2 * chunk + 1) ^ z) << 3), mx_values<T>(y.x[i][2], y.x[i][3], sc));
     });
     asm volatile("" ::: "memory");
   }
@@ -1183,7 +1186,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i)
-        acc = Mfma16<T>::mma(__builtin_bit_cast(vec, ld128(krow + 16 / F::LDB * x * HD + (((4 * i + g) ^ ksw) << 3))), qf[i], acc);
+        acc = Mfma16<T>::mma(__builtin_bit_cast(vec, ld128(krow + 16 / F::LDB * x * HD + (((F::pos(4 * i) ^ g) ^ ksw) << 3))), qf[i], acc);
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[4 * x + e] = acc[e];
     }
@@ -1232,7 +1235,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
       u32x4 vop[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t at = vrow + (uint32_t)((((2 * (4 * d4 + i)) ^ vsw) + vx) << 4);
+        const uint32_t at = vrow + (uint32_t)((((2 * (4 * d4 + i)) ^ vsw) + (vx ^ (F::pos(8 * d4) & 1))) << 4);
         u32x2 lo, hi;
         asm volatile("ds_read_b64_tr_b16 %0, %1" : "=v"(lo) : "v"(at));
         asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(hi) : "v"(at), "n"(16 / F::LDB * HD * 2));
