@@ -959,8 +959,7 @@ __global__ __launch_bounds__(SQ_THREADS, HD == 64 ? 4 : 2) void seq_attn_packed_
 // if V's rows are taken in that order.  The waves' results meet in LDS at the
 // end.
 //
-// 8-bit rows come through registers instead, AHEAD blocks before their use, and
-// are converted into the same layout of one LDS block, K's first, V's in its
+// 8-bit rows come through registers instead, a block before their use, and are converted into the same layout of one LDS block, K's first, V's in its
 // place once the scores are formed.
 template <typename T, int HD, bool MX>
 struct SqFew {
@@ -980,11 +979,6 @@ struct SqFew {
   // row, pos() swaps the two in the row's second half; at 64, in two rows, the
   // lowest bit of the swizzles differs between those.
   static constexpr int CH8 = HD / 16, LDB8 = 32 * CH8 / 64;
-#ifndef SQ8_AHEAD
-#define SQ8_AHEAD 2
-#define SQ8_RES 2
-#endif
-  static constexpr int AHEAD = HD == 128 ? SQ8_AHEAD : 1;
   static __device__ __forceinline__ int pos(int chunk) { return MX && HD == 128 ? chunk ^ (chunk >> 3) : chunk; }
   static __device__ __forceinline__ int lds_row(int key) { return key % LDB * RPI + key / LDB; }
   static __device__ __forceinline__ int kswz(int key) {
@@ -1012,9 +1006,10 @@ template <int X> __device__ __forceinline__ uint32_t sq_quad(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, X * 0x55, 0xf, 0xf, true);
 }
 
-// The keys of an item of few rows (wave-uniform).
+// The keys and the rows of an item of few rows (wave-uniform).
 struct SqKeys {
   int b, hk, j0, lim;
+  int q0, r0, n;
 };
 // Keys that the rows of an item see at most.
 template <int K>
@@ -1023,28 +1018,39 @@ __device__ __forceinline__ int sq_few_lim(const SeqAttnArgs& a, const SeqWork& w
   const int sees = !(K & SQ_TREE) && a.causal ? w.kvn - w.qn + seq_div(last, a.by_group) + 1 : w.kvn;
   return seq_uni(min(min(max(sees, 0), a.s.max_pages << a.s.page_log2), j1));
 }
-// Codes of a wave's blocks on their way through its registers: of each slot
-// (block n of an item goes to slot n % N), a lane's codes of LDB8 keys at one
-// chunk, and for each four lanes the scales of their keys, one key a lane.
-// A lane's keys lie in one page, so those past the last are read too.  What a
-// slot is loaded with once it is used: the item's next block of that slot, or,
-// past its last, the next item's first, so that an item's first keys arrive while
-// the waves of the one before it meet.  Every block loads the same number of
-// times, so that the compiler can count the loads in flight and waits for those
-// it needs alone.
+template <int K>
+__device__ __forceinline__ SqKeys sq_keys(const SeqAttnArgs& a, const SeqWork& w, int hk, int r0, int j0, int j1) {
+  return SqKeys{w.b, hk, j0, sq_few_lim<K>(a, w, r0, j1), w.q0, r0, min(w.qn * a.group - r0, w.cut.tile_rows)};
+}
+// Codes of a wave's next block on their way through its registers: a lane's codes
+// of LDB8 keys at one chunk, and for each four lanes the scales of their keys,
+// one key a lane.  A lane's keys lie in one page, so those past the last are read
+// too.  Behind an item's last block comes the next item's first, so that its keys
+// arrive while the waves of the one before it meet; so do its rows of q, once this
+// one's are used.  Every block loads the same number of times, and nothing waits
+// for more than the loads that it needs: the compiler counts those in flight.
+// (Loads behind an item's stores would wait for these to arrive: 64 streams of up
+// to 30000 keys took 246 us with q and the second block's page loaded there.  Two
+// blocks ahead they are no faster.)
 template <typename T, int HD>
 struct SqAhead8 {
   typedef SqFew<T, HD, true> F;
-  static constexpr int N = F::AHEAD, STEP = 128 * N;
   struct Side {
     u32x4 x[F::LDB8];
     uint32_t s;
   };
-  Side k[N], v[N];
-  uint32_t at[N];    // pages that the slots are loaded from
-  uint32_t page[N];  // and the ones after them
+  Side k, v;
+  uint32_t at;       // page that they are loaded from
+  uint32_t page;     // and the one after it
   int chunk, key0;   // this lane's chunk; its first key within a block
+  typename F::vec q[HD / 32];  // of the item's rows
 
+  __device__ __forceinline__ void load_q(const SeqAttnArgs& a, const SqKeys& c, int lane) {
+    const int r = c.r0 + min(lane & 15, c.n - 1), i = seq_div(r, a.by_group);
+    const T* row = (const T*)a.q + (int64_t)(c.q0 + i) * a.q_st + (c.hk * a.group + r - i * a.group) * a.q_sh + 8 * (lane >> 4);
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) q[e] = __builtin_bit_cast(typename F::vec, ld128(row + 32 * e));
+  }
   __device__ __forceinline__ int first(const SqKeys& c, int wave) const { return c.j0 + 32 * wave; }
   // (keys past the last: the last ones; without any, the first slot of the table)
   __device__ __forceinline__ int key(const SqKeys& c, int kb) const { return min(kb + key0, (max(c.lim, 1) - 1) & ~(F::LDB8 - 1)); }
@@ -1068,17 +1074,19 @@ struct SqAhead8 {
   __device__ __forceinline__ void fetch_v(const SeqAttnArgs& a, const SqKeys& c, int kb, uint32_t page, Side& y, int lane) const {
     fetch(a, c, kb, page, y, (const uint8_t*)a.v + c.hk * a.v_sh, a.v_scales + c.hk * a.vs_sh, a.v_sp, a.v_st, a.vs_sp, a.vs_st, lane);
   }
-  // The first blocks of an item.
+  // The first block of an item.
   __device__ __forceinline__ void start(const SeqAttnArgs& a, const SqKeys& c, int lane, int wave) {
     chunk = lane % F::CH8;
     key0 = lane / F::CH8 * F::LDB8;
-    static_for<N>([&](auto ic) { load<decltype(ic)::value>(a, c, lane, wave); });
+    load_q(a, c, lane);
+    load(a, c, lane, wave);
   }
-  template <int I> __device__ __forceinline__ void load(const SeqAttnArgs& a, const SqKeys& c, int lane, int wave) {
-    const int kb = first(c, wave) + 128 * I;
-    at[I] = lookup(a, c, kb);
-    fetch_k(a, c, kb, at[I], k[I], lane);
-    fetch_v(a, c, kb, at[I], v[I], lane);
+  __device__ __forceinline__ void load(const SeqAttnArgs& a, const SqKeys& c, int lane, int wave) {
+    const int kb = first(c, wave);
+    at = lookup(a, c, kb);
+    page = lookup(a, c, kb + 128);
+    fetch_k(a, c, kb, at, k, lane);
+    fetch_v(a, c, kb, at, v, lane);
   }
   // 16-bit rows of a block, to LDS.  (A wave's LDS operations complete in the order that they are written in.)
   template <typename Swz> __device__ __forceinline__ void put(const Side& y, T* to, Swz swz) const {
@@ -1096,7 +1104,7 @@ struct SqAhead8 {
 };
 struct SqNoAhead {};
 
-// next: the keys of the workgroup's next item, whose first blocks `ahead` holds
+// next: the keys of the workgroup's next item, whose first block `ahead` holds
 // on return (8-bit; those of this item it holds already).
 template <typename T, int HD, int K, typename Ahead>
 __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork& w, int hk, int r0, int j0, int j1,
@@ -1125,12 +1133,14 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   hp.init(a, w.b, w.q0, hk);
   const int32_t* table = a.s.table + (int64_t)w.b * a.s.table_ld;
 
-  vec qf[HD / 32];
-  {
+  vec qf_own[MX ? 1 : HD / 32];
+  if constexpr (!MX) {
     const T* qrow = (const T*)a.q + tok * a.q_st + h * a.q_sh + 8 * g;
 #pragma unroll
-    for (int ks = 0; ks < HD / 32; ++ks) qf[ks] = __builtin_bit_cast(vec, ld128(qrow + 32 * ks));
+    for (int ks = 0; ks < HD / 32; ++ks) qf_own[ks] = __builtin_bit_cast(vec, ld128(qrow + 32 * ks));
   }
+  const vec* qf = qf_own;
+  if constexpr (MX) qf = ahead.q;
   vec ones;
   {
     const uint32_t one2 = std::is_same<T, bf16>::value ? 0x3F803F80u : 0x3C003C00u;
@@ -1250,51 +1260,33 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
 
   const int first = j0 + 32 * wave;
   if constexpr (MX) {
-    constexpr int N = F::AHEAD, STEP = Ahead::STEP;
-    const SqKeys cur{w.b, hk, j0, lim};
+    const SqKeys cur{w.b, hk, j0, lim, w.q0, r0, n};
     const int next_first = ahead.first(next, wave);
-    static_for<N>([&](auto ic) {
-      constexpr int i = decltype(ic)::value;
-      const bool more = first + 128 * i + STEP < lim;
-      ahead.page[i] = ahead.lookup(a, more ? cur : next, more ? first + 128 * i + STEP : next_first + 128 * i);
-    });
-    auto block = [&](auto ic, int kb) {
-      constexpr int i = decltype(ic)::value;
-      if (ahead.at[i] >= (uint32_t)a.s.num_pages) bad_from = min(bad_from, ahead.key(cur, kb) & ~ps1);
-      const uint32_t page = ahead.page[i];
-      const bool more = kb + STEP < lim, more2 = kb + 2 * STEP < lim;
+    if (first + 128 >= lim) ahead.page = ahead.lookup(a, next, next_first);
+    for (int kb = first; kb < lim; kb += 128) {
+      if (ahead.at >= (uint32_t)a.s.num_pages) bad_from = min(bad_from, ahead.key(cur, kb) & ~ps1);
+      const uint32_t page = ahead.page;
+      const bool more = kb + 128 < lim, more2 = kb + 256 < lim;
       const SqKeys to = more ? cur : next;
-      const int then = more ? kb + STEP : next_first + 128 * i;
-      ahead.page[i] = ahead.lookup(a, more2 ? cur : next, more2 ? kb + 2 * STEP : next_first + 128 * i);
-      ahead.put(ahead.k[i], ks, F::kswz);
-      ahead.fetch_k(a, to, then, page, ahead.k[i], lane);
+      const int then = more ? kb + 128 : next_first;
+      ahead.page = ahead.lookup(a, more2 ? cur : next, more2 ? kb + 256 : (more ? next_first : next_first + 128));
+      ahead.put(ahead.k, ks, F::kswz);
+      ahead.fetch_k(a, to, then, page, ahead.k, lane);
       compute(kb, 0, false, [&]() {
-        auto& y = ahead.v[i];
+        auto& y = ahead.v;
         if (kb + 32 > lim) {  // (weights of 0 times what the slots past the last key hold)
 #pragma unroll
           for (int e = 0; e < F::LDB8; ++e)
             if (kb + ahead.key0 + e >= lim) y.x[e] = u32x4{0, 0, 0, 0};
+          if (kb + ahead.key0 + (lane & (F::LDB8 - 1)) >= lim) y.s = 0;
         }
         ahead.put(y, ks, F::vswz);
         ahead.fetch_v(a, to, then, page, y, lane);
-        ahead.at[i] = page;
+        ahead.at = page;
       });
-    };
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the slots' order differs from item to item
-    int kb = first;
-    if constexpr (N == 2) {
-      for (; kb + 128 < lim; kb += 256) {
-        block(std::integral_constant<int, 0>{}, kb);
-        block(std::integral_constant<int, N - 1>{}, kb + 128);
-      }
-      if (kb < lim) block(std::integral_constant<int, 0>{}, kb);
-    } else {
-      for (; kb < lim; kb += 128) block(std::integral_constant<int, 0>{}, kb);
     }
-    static_for<N>([&](auto ic) {  // slots that this item has no block for
-      constexpr int i = decltype(ic)::value;
-      if (first + 128 * i >= lim) ahead.template load<i>(a, next, lane, wave);
-    });
+    if (first >= lim) ahead.load(a, next, lane, wave);  // (no block of this item)
+    ahead.load_q(a, next, lane);
   } else if (first < lim) {
     uint32_t page = lookup(first), next = lookup(first + 128);
     load_k(first, page);
@@ -1306,20 +1298,26 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
     }
   }
 
-  // (8-bit: loads go on across the barriers)
-  auto meet = []() {
-    if constexpr (MX) lds_barrier();
-    else __syncthreads();
-  };
   // Join the waves: o in fp32 over each wave's K block, m and l beside it.
-  if (threadIdx.x == 0) *bad = cap;
+  // (8-bit: once for an item, by a barrier that loads in flight go on across, and
+  // a wave sees to its own rows that are not finite: the next item's keys are on
+  // their way, but no more than a block of them.)
   float* ow = (float*)ks;
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   float* sm = stat + wave * 16;
   float* sl = stat + 64 + wave * 16;
   int* sagain = (int*)(stat + 128);
-  meet();
-  if (bad_from < cap) atomicMin(bad, bad_from);
+  if constexpr (MX) {
+    if (__any(bad_from < cap)) {
+#pragma unroll
+      for (int x = 32; x > 0; x >>= 1) bad_from = min(bad_from, __shfl_xor(bad_from, x, 64));
+    }
+    if (lane == 0) bad[wave] = bad_from;
+  } else {
+    if (threadIdx.x == 0) *bad = cap;
+    __syncthreads();
+    if (bad_from < cap) atomicMin(bad, bad_from);
+  }
 #pragma unroll
   // (4-value chunks xor the row: 16 rows at one chunk would share 4 banks)
   for (int d = 0; d < HD / 16; ++d) *reinterpret_cast<f32x4*>(ow + col * HD + 4 * ((4 * d + g) ^ col)) = o[d];
@@ -1327,9 +1325,10 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
     sm[col] = m_run;
     sl[col] = lsum[0];
   }
-  if (threadIdx.x < 16) sagain[threadIdx.x] = 0;
-  meet();
-  const int lost_from = *bad;
+  if (!MX && threadIdx.x < 16) sagain[threadIdx.x] = 0;
+  if constexpr (MX) lds_barrier();
+  else __syncthreads();
+  const int lost_from = MX ? min(min(bad[0], bad[1]), min(bad[2], bad[3])) : *bad;
   constexpr int DT = HD / 16;  // dims a thread joins: 16 threads a row
   const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 4;
   const float* s0 = stat + row;
@@ -1372,8 +1371,10 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   }
   // (as in a tile)
   const bool redo = active && !lost && (TREE ? some : sees > j0) && L == L && (L != 0.f || part) && !(odd == 0.f);
-  if (redo) sagain[row] = 1;
-  meet();
+  if constexpr (!MX) {
+    if (redo) sagain[row] = 1;
+    __syncthreads();
+  }
   const int hh = hk * G + rr - ir * G;
   if (active) {
     if (part) {
@@ -1390,6 +1391,19 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
       for (int y = 0; y < DT / 4; ++y) store4<T>(orow + 64 * y, res + 4 * y);
     }
   }
+  if constexpr (MX) {
+    const uint64_t again = __ballot(redo);
+    if (__builtin_expect(again == 0, 1)) return;
+    // Lane: row lane & 15; this wave's are 4 wave .. + 3, stored above.
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    const int from = 16 * (col & 3), ro = min(col, n - 1);
+    const bool need = (col >> 2) == wave && ((again >> from) & 0xFFFFu) != 0;
+    const float m_row = __shfl(M, from, 64), l_row = __shfl(L, from, 64);
+    sq_odd_rows<T, HD, K>(w.b, w.q0, hk, w.kvn - w.qn, r0 + ro, need, min(keys_of(r0 + ro), lim), j0, m_row, l_row, F::BIAS,
+                          part ? part + ro * HD : nullptr, lane);
+    return;
+  }
   if (__builtin_expect(!__any(sagain[col]), 1)) return;  // (the same in every wave)
   // Wave 0 sees to the rows that are not finite, once all are stored.
   if ((threadIdx.x & 15) == 0) {
@@ -1400,7 +1414,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
   if (wave != 0) return;
   const int ro = min(col, n - 1);
   sq_odd_rows<T, HD, K>(w.b, w.q0, hk, w.kvn - w.qn, r0 + ro, col < n && sagain[col] != 0, min(keys_of(r0 + ro), lim), j0, stat[col],
-                           stat[64 + col], F::BIAS, part ? part + ro * HD : nullptr, lane);
+                        stat[64 + col], F::BIAS, part ? part + ro * HD : nullptr, lane);
 }
 
 // ---------------------------------------------------------------- paged calls
@@ -1411,7 +1425,7 @@ __host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
 // Workgroups of a call that are resident on a CU.
 template <int HD, bool FEW_ONLY, int K>
 constexpr int sq_resident() {
-  if (FEW_ONLY && (K & SQ_MX8)) return HD == 64 ? 4 : SQ8_RES;
+  if (FEW_ONLY && (K & SQ_MX8)) return HD == 64 ? 4 : 2;
   return HD == 64 ? (FEW_ONLY ? 4 : 3) : 2;
 }
 
@@ -1451,20 +1465,20 @@ __global__ __launch_bounds__(SQ_THREADS, (sq_resident<HD, FEW_ONLY, K>())) void 
     x.r0 = tile * x.w.cut.tile_rows;
     return true;
   };
-  // 8-bit rows of few-row items: the first blocks of the next item are loaded within this one.
+  // 8-bit rows of few-row items: the first block of the next item is loaded within this one.
   typename std::conditional<MX, SqAhead8<T, HD>, SqNoAhead>::type ahead;
   Item x, y;
   bool have = find(blockIdx.x, x);
   if constexpr (MX && FEW_ONLY) {
-    if (have) ahead.start(a, SqKeys{x.w.b, x.hk, x.j0, sq_few_lim<K>(a, x.w, x.r0, x.j1)}, threadIdx.x & 63, wave);
+    if (have) ahead.start(a, sq_keys<K>(a, x.w, x.hk, x.r0, x.j0, x.j1), threadIdx.x & 63, wave);
   }
   for (int i = blockIdx.x; have;) {
     i += gridDim.x;
-    SqKeys next{x.w.b, x.hk, 0, 1};  // none: the sequence's first key
+    SqKeys next{x.w.b, x.hk, 0, 1, x.w.q0, x.r0, 1};  // none: the sequence's first key
     bool have_next = false;
     if constexpr (MX && FEW_ONLY) {
       have_next = find(i, y);
-      if (have_next) next = SqKeys{y.w.b, y.hk, y.j0, sq_few_lim<K>(a, y.w, y.r0, y.j1)};
+      if (have_next) next = sq_keys<K>(a, y.w, y.hk, y.r0, y.j0, y.j1);
     }
     const SeqWork& w = x.w;
     // An item's lane constants are formed within it: held across the items
@@ -1481,7 +1495,7 @@ __global__ __launch_bounds__(SQ_THREADS, (sq_resident<HD, FEW_ONLY, K>())) void 
     if constexpr (FEW_ONLY) {
       sq_few_item<T, HD, K>(a, w, x.hk, x.r0, x.j0, x.j1, part, ml, lds, stat, bad, lane, wave, ahead, next);
     } else if (w.cut.few) {
-      if constexpr (MX) ahead.start(a, SqKeys{w.b, x.hk, x.j0, sq_few_lim<K>(a, w, x.r0, x.j1)}, lane, wave);
+      if constexpr (MX) ahead.start(a, sq_keys<K>(a, w, x.hk, x.r0, x.j0, x.j1), lane, wave);
       sq_few_item<T, HD, K>(a, w, x.hk, x.r0, x.j0, x.j1, part, ml, lds, stat, bad, lane, wave, ahead, next);
     } else {
       sq_tile_item<T, HD, K>(a, w.b, w.q0, w.qn, w.kvn, x.hk, x.r0, x.j0, x.j1, part, ml, lds, bad, lane, wave);
