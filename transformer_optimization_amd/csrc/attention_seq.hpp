@@ -252,7 +252,8 @@ struct SqLoader8 {
   int row, ch;          // this thread's first row of a tile, its chunk
   int last;             // last key that may be read
   int bad_from;         // first key found without a page (over the lane's lookups)
-  uint32_t at[N], next[N];  // pages of the tile that issue_k loaded last, of the one behind it
+  uint32_t at[N], next[N];  // pages of the K tile that was loaded last, of the one behind it
+  uint32_t before[N];       // and of the one before it
 
   template <typename H>
   __device__ __forceinline__ void init(const SeqAttnArgs& a, const H& hp, int wave, int lane) {
@@ -285,6 +286,7 @@ struct SqLoader8 {
   __device__ __forceinline__ void advance(int kt) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
+      before[i] = at[i];
       at[i] = next[i];
       if (at[i] >= (uint32_t)num_pages) {  // page 0 in its place
         bad_from = min(bad_from, (key(kt, i) >> psl) << psl);
@@ -293,23 +295,23 @@ struct SqLoader8 {
     }
     lookup(kt + 1);
   }
-  __device__ __forceinline__ void load(int kt, Side& x) {
+  __device__ __forceinline__ void load(int kt, Side& x, const uint32_t* page) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint32_t slot = (uint32_t)key(kt, i) & ((1u << psl) - 1);
-      x.x[i] = ld128(x.head + ((uint64_t)at[i] * x.sp + slot * x.st));
-      x.s[i] = x.scales[(uint64_t)at[i] * x.ssp + slot * x.sst];
+      x.x[i] = ld128(x.head + ((uint64_t)page[i] * x.sp + slot * x.st));
+      x.s[i] = x.scales[(uint64_t)page[i] * x.ssp + slot * x.sst];
     }
   }
   template <bool IS_K> __device__ __forceinline__ void put(T* tile, const Side& x) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int r = row + i * RPR;
-      const int swz = IS_K ? ax_kswz<HD>(r) : ax_vswz<HD>(r);
+      const int swz = IS_K ? ax_kswz<HD>(r) : ax_vswz_w<HD, true>(r);
       T* to = tile + r * HD;
       const float s = mx_scale(x.s[i]);
-      st128(to + (((2 * ch) ^ swz) << 3), mx_values<T>(x.x[i][0], x.x[i][1], s));
-      st128(to + (((2 * ch + 1) ^ swz) << 3), mx_values<T>(x.x[i][2], x.x[i][3], s));
+      st128(to + ((ax_pos<HD, true>(2 * ch) ^ swz) << 3), mx_values<T>(x.x[i][0], x.x[i][1], s));
+      st128(to + ((ax_pos<HD, true>(2 * ch + 1) ^ swz) << 3), mx_values<T>(x.x[i][2], x.x[i][3], s));
     }
   }
 };
@@ -334,7 +336,7 @@ struct SqTile {
   typedef typename Mfma<T>::vec vec;
   typedef typename Mfma16<T>::vec vec16;
   typedef typename std::conditional<MX, SqLoader8<T, HD>, SqLoader<T, HD, K & SQ_PAGED>>::type L;
-  static constexpr int LEAD = HD == 128 ? 1 : 0;
+  static constexpr int LEAD = HD == 128 && !MX ? 1 : 0;
   static constexpr int NST = 2;
   static constexpr int LDS_ELEMS = NST * 2 * L::ELEMS;
   static constexpr int LPW = 2 * L::LD;
@@ -359,9 +361,9 @@ struct SqTile {
     for (int ks = 0; ks < HD / 16; ++ks) qf[ks] = __builtin_bit_cast(vec, ld128(qrow + 8 * half + 16 * ks));
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) settle(qf[ks]);
-    AxKOff<HD> ko;
+    AxKOff<HD, MX> ko;
     ko.init_perm(lane);
-    AxVNatOff<HD> vn;
+    AxVNatOff<HD, MX> vn;
     vn.init(lane);
     // Row sum on the matrix cores: a 0/1 selector against P, 16 keys a step
     // (register 0 of a lane receives its own query's sum).
@@ -388,32 +390,37 @@ struct SqTile {
     auto issue_v = [&](int kt) {
       if constexpr (!MX) ld.issue_v(min(kt, kt1 - 1), v_at(kt));
     };
-    // Codes: K of tile kk and V of tile kv (kk - LEAD) to registers, and from there to LDS.
-    auto load8 = [&](int kk, int kv) {
+    // Codes: the K or V tile in registers to LDS, and the next one to registers (in
+    // every step, so that the compiler can count the loads in flight: past the
+    // last tile its last key again).
+    auto load_k8 = [&](int kt) {
       if constexpr (MX) {
-        // (In every step, so that the compiler can count the loads in flight: past
-        // the last tile its last key again.)
-        if (LEAD && kv >= 0) ld.load(kv, ld.v);  // (its pages are those of the last K tile)
-        ld.advance(kk);
-        ld.load(kk, ld.k);
-        if (!LEAD) ld.load(kv, ld.v);
+        ld.advance(kt);
+        ld.load(kt, ld.k, ld.at);
       }
     };
-    auto put8 = [&](int kk, int kv) {
+    auto load_v8 = [&](int kt) {  // (K is LEAD tiles ahead)
+      if constexpr (MX) ld.load(kt, ld.v, LEAD ? ld.before : ld.at);
+    };
+    auto next_k8 = [&](int kt) {
       if constexpr (MX) {
-        ld.template put<true>(lds + (kk % NST) * L::ELEMS, ld.k);
-        if (!LEAD || kv >= 0) ld.template put<false>(lds + (NST + kv % NST) * L::ELEMS, ld.v);
+        ld.template put<true>(lds + (kt % NST) * L::ELEMS, ld.k);
+        load_k8(kt + 1);
+      }
+    };
+    auto next_v8 = [&](int kt) {
+      if constexpr (MX) {
+        ld.template put<false>(lds + (NST + kt % NST) * L::ELEMS, ld.v);
+        load_v8(kt + 1);
       }
     };
     if constexpr (MX) {
       ld.lookup(kt0);
-      if constexpr (LEAD) {
-        load8(kt0, -1);
-        put8(kt0, -1);
-      }
-      load8(kt0 + LEAD, kt0);
-      put8(kt0 + LEAD, kt0);
-      load8(kt0 + LEAD + 1, kt0 + 1);
+      load_k8(kt0);
+      if constexpr (LEAD) next_k8(kt0);
+      load_v8(kt0);
+      next_k8(kt0 + LEAD);
+      next_v8(kt0);
     } else {
       if constexpr (LEAD) issue_k(kt0);
 #pragma unroll
@@ -443,8 +450,10 @@ struct SqTile {
       const int j0 = kt * AX_BN;
       if constexpr (MX) {
         lds_barrier();
-        put8(kt + LEAD + 1, kt + 1);
-        load8(kt + LEAD + 2, kt + 2);
+        if (j0 >= wlim_max) {
+          next_k8(kt + LEAD + 1);
+          next_v8(kt + 1);
+        }
       } else {
         ring_barrier<LPW * (NST - 2)>();  // K of tile kt + LEAD, V of tile kt
         issue_k(kt + LEAD + NST - 1);
@@ -534,8 +543,11 @@ struct SqTile {
       if constexpr (LEAD) {
 #pragma unroll
         for (int ks = HD / 64; ks < HD / 16; ++ks) qk(Kn, ks, sn);
+        next_k8(kt + LEAD + 1);
         weights(0);
         weights(1);
+      } else {
+        next_k8(kt + LEAD + 1);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -556,6 +568,7 @@ struct SqTile {
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt)
           o[dt] = Mfma<T>::mma32(__builtin_bit_cast(vec, vop[dt]), __builtin_bit_cast(vec, pk[u]), o[dt]);
+        if (u == 1) next_v8(kt + 1);
       }
     };
     f32x16 sa[2];
@@ -1425,7 +1438,7 @@ __host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
 // Workgroups of a call that are resident on a CU.
 template <int HD, bool FEW_ONLY, int K>
 constexpr int sq_resident() {
-  if (FEW_ONLY && (K & SQ_MX8)) return HD == 64 ? 4 : 2;
+  if (FEW_ONLY && (K & SQ_MX8)) return HD == 64 ? 3 : 2;
   return HD == 64 ? (FEW_ONLY ? 4 : 3) : 2;
 }
 

@@ -29,10 +29,21 @@ __device__ __forceinline__ int ax_vswz(int key) {
   if constexpr (HD == 128) return (key & 3) << 2;
   else return ((key >> 1) & 1) << 2;
 }
+// Tiles that are written by threads of 32 bytes a row (8-bit rows converted on
+// their way) instead of DMA: eight lanes' 16-byte writes are free of bank
+// conflicts where they differ modulo 128 bytes.  At head dim 128 the eight lie in
+// one row, whose second half swaps each two chunks; at 64 in two rows, whose
+// swizzles differ in the lowest bit.
+template <int HD, bool W32> __device__ __forceinline__ int ax_pos(int chunk) {
+  return W32 && HD == 128 ? chunk ^ (chunk >> 3) : chunk;
+}
+template <int HD, bool W32> __device__ __forceinline__ int ax_vswz_w(int key) {
+  return ax_vswz<HD>(key) | (W32 && HD == 64 ? key & 1 : 0);
+}
 // Per-lane element offsets of the K fragments inside a K tile, one per
 // 16-wide k step: key (lane & 31) (the t = 1 half adds 32 * HD), its
 // swizzled chunk 2 ks + (lane >> 5).  Tile-independent, computed once.
-template <int HD>
+template <int HD, bool W32 = false>
 struct AxKOff {
   int off[HD / 16];
   __device__ __forceinline__ void init(int lane) {
@@ -50,7 +61,8 @@ struct AxKOff {
     const int col = lane & 31, half = lane >> 5;
     const int row = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) off[ks] = row * HD + (((2 * ks + half) ^ ax_kswz<HD>(row)) << 3);
+    for (int ks = 0; ks < HD / 16; ++ks)
+      off[ks] = row * HD + ((ax_pos<HD, W32>(2 * ks + half) ^ ax_kswz<HD>(row)) << 3);
   }
 };
 // Natural-layout V: per-lane element offsets of the transposed operand reads.
@@ -64,7 +76,7 @@ struct AxKOff {
 // 32 dt + 16 (g & 1) + j of keys 4r .. 4r + 3.  off[dt] is the element
 // offset for u = 0, r = 0; step u adds 16 u HD, read r adds 4 r HD (the
 // swizzle depends on key % 4 only, which u and r leave unchanged).
-template <int HD>
+template <int HD, bool W32 = false>
 struct AxVNatOff {
   int off[HD / 32];
   __device__ __forceinline__ void init(int lane) {
@@ -73,7 +85,7 @@ struct AxVNatOff {
 #pragma unroll
     for (int dt = 0; dt < HD / 32; ++dt) {
       const int d = 32 * dt + 16 * (g & 1) + 4 * (j & 3);
-      off[dt] = key * HD + (((d >> 3) ^ ax_vswz<HD>(key)) << 3) + (d & 7);
+      off[dt] = key * HD + ((ax_pos<HD, W32>(d >> 3) ^ ax_vswz_w<HD, W32>(key)) << 3) + (d & 7);
     }
   }
 };
