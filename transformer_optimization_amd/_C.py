@@ -14,6 +14,7 @@ from __future__ import annotations
 import array
 import contextlib
 import ctypes
+import functools
 import math
 import os
 import threading
@@ -780,7 +781,7 @@ def _one_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> int:
 
 def _launch_on(at: int, fn: str, args: tuple, keep: tuple, info) -> None:
     """``_launch`` on the current stream of device ``at``; ``info`` is called when a recording is active."""
-    if at != torch.cuda.current_device():
+    if at != torch._C._cuda_getDevice():  # (initialised: the tensors are on a device)
         with torch.cuda.device(at):
             _launch_on(at, fn, args, keep, info)
         return
@@ -792,6 +793,7 @@ def _launch_on(at: int, fn: str, args: tuple, keep: tuple, info) -> None:
 
 
 _NO_STRIDES = (0, 0, 0)
+_NO_STRIDES4 = (0, 0, 0, 1)
 
 
 def rotary_append(
@@ -1002,6 +1004,7 @@ def flash_attn_paged(
 # --------------------------------------------- 8-bit caches and draft trees
 # Elements of a head that share a scale.
 MX_BLOCK = 32
+_MX_SCALES = (torch.float8_e8m0fnu, torch.uint8)
 
 
 def mx8_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, *,
@@ -1024,15 +1027,35 @@ def _check_mx8(k_cache, k_scales, v_cache, v_scales, block_table, batch: int, hd
     if k_cache.dtype != torch.float8_e4m3fn:
         raise ValueError(f"a cache with scales must be float8_e4m3fn, got {k_cache.dtype}")
     ks, vs, sizes = _check_cache(k_cache, v_cache, block_table, batch, hd, torch.float8_e4m3fn)
-    want = (*sizes[:3], hd // MX_BLOCK)
-    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-        if t.shape != want:
-            raise ValueError(f"{name} must be {list(want)}, got {tuple(t.shape)}")
-        if t.dtype != torch.uint8 and t.dtype != torch.float8_e8m0fnu:
-            raise ValueError(f"{name} must be uint8 or float8_e8m0fnu")
-        if t.stride(3) != 1 and want[3] > 1:
-            raise ValueError(f"{name} must be contiguous in its last dim")
-    return ks, vs, sizes, k_scales.stride(), v_scales.stride()
+    want = (sizes[0], sizes[1], sizes[2], hd // MX_BLOCK)
+    kss, vss = k_scales.stride(), v_scales.stride()
+    if (k_scales.shape != want or v_scales.shape != want or k_scales.dtype not in _MX_SCALES
+            or v_scales.dtype not in _MX_SCALES or (kss[3] != 1 or vss[3] != 1) and want[3] > 1):
+        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+            if t.shape != want:
+                raise ValueError(f"{name} must be {list(want)}, got {tuple(t.shape)}")
+            if t.dtype not in _MX_SCALES:
+                raise ValueError(f"{name} must be uint8 or float8_e8m0fnu")
+            if t.stride(3) != 1 and want[3] > 1:
+                raise ValueError(f"{name} must be contiguous in its last dim")
+    return ks, vs, sizes, kss, vss
+
+
+def _bad_norm_params(norm, kind, hd, dtype, params) -> None:
+    """Why the weights and biases of a norm are refused."""
+    seen = None
+    for name, p, n in params:
+        if p is None:
+            continue
+        if kind == TX_NORM_NONE or (kind == TX_NORM_RMS and name.endswith("bias")):
+            raise ValueError(f"{name} with norm={norm!r}")
+        if p.shape != (hd,) and p.shape != (n, hd) or not p.is_contiguous():
+            raise ValueError(f"{name} must be contiguous [{hd}] or [{n}, {hd}]")
+        if p.dtype != dtype and p.dtype != torch.float32:
+            raise ValueError(f"{name} must be {dtype} or float32")
+        if seen is not None and seen != (p.dim(), p.dtype):
+            raise ValueError("weights and biases must be alike: all of one dtype, all [hd] or all [heads, hd]")
+        seen = (p.dim(), p.dtype)
 
 
 def norm_rotary_append(
@@ -1075,8 +1098,11 @@ def norm_rotary_append(
     :func:`rotary_append`; the result is rounded once."""
     t, kvh, hd = _dims3("k", k)
     dtype = k.dtype
-    ks = _heads3("k", k, t, kvh, hd, dtype)
-    qs = qos = kos = vs = kcs = vcs = kss = vss = _NO_STRIDES
+    ks = k.stride()
+    if ks[2] != 1 and hd > 1:
+        raise ValueError("k must be contiguous in head_dim")
+    qs = qos = kos = vs = _NO_STRIDES
+    kcs = vcs = kss = vss = _NO_STRIDES4
     batch = _starts(cu_seqlens)
     half = steps.shape[0] if steps.dim() == 1 else 0
     if not 0 < 2 * half <= hd or steps.dtype != torch.int64 or not steps.is_contiguous():
@@ -1085,33 +1111,41 @@ def norm_rotary_append(
     if kind is None:
         raise ValueError(f"norm must be one of {sorted(HEAD_NORMS)}")
     heads = kvh
+    tensors = [k, steps, cu_seqlens]
     if q is not None:
         heads = _dims3("q", q)[1]
         qs = _heads3("q", q, t, heads, hd, dtype)
         if kvh <= 0 or heads % kvh:
             raise ValueError(f"{kvh} K/V heads do not divide {heads} query heads")
+        tensors.append(q)
         if q_out is not None:
             qos = _heads3("q_out", q_out, t, heads, hd, dtype)
+            tensors.append(q_out)
     elif q_out is not None or q_weight is not None or q_bias is not None:
         raise ValueError("q_out, q_weight or q_bias without q")
     if k_out is not None:
         kos = _heads3("k_out", k_out, t, kvh, hd, dtype)
-    per_head = param_dt = None
-    for name, p, n in (("q_weight", q_weight, heads), ("k_weight", k_weight, kvh), ("q_bias", q_bias, heads),
-                       ("k_bias", k_bias, kvh)):
-        if p is None:
-            continue
-        if kind == TX_NORM_NONE or (kind == TX_NORM_RMS and name.endswith("bias")):
-            raise ValueError(f"{name} with norm={norm!r}")
-        if p.shape != (hd,) and p.shape != (n, hd) or not p.is_contiguous():
-            raise ValueError(f"{name} must be contiguous [{hd}] or [{n}, {hd}]")
-        if p.dtype != dtype and p.dtype != torch.float32:
-            raise ValueError(f"{name} must be {dtype} or float32")
-        if per_head is not None and (per_head != (p.dim() == 2) or param_dt != p.dtype):
-            raise ValueError("weights and biases must be alike: all of one dtype, all [hd] or all [heads, hd]")
-        per_head, param_dt = p.dim() == 2, p.dtype
+        tensors.append(k_out)
+    per_head, param_dt = 0, TX_F32
+    qw = qb = kw = kb = None
+    if q_weight is not None or k_weight is not None or q_bias is not None or k_bias is not None:
+        # One tensor decides, the others are like it.
+        one = q_weight if q_weight is not None else k_weight if k_weight is not None else q_bias if q_bias is not None else k_bias
+        per_head, kind_of = one.dim() - 1, one.dtype
+        ok = kind != TX_NORM_NONE and (kind_of == dtype or kind_of == torch.float32)
+        q_shape, k_shape = ((heads, hd), (kvh, hd)) if per_head else ((hd,), (hd,))
+        for p, shape in ((q_weight, q_shape), (k_weight, k_shape), (q_bias, q_shape), (k_bias, k_shape)):
+            if p is not None:
+                ok = ok and p.shape == shape and p.dtype == kind_of and p.is_contiguous()
+                tensors.append(p)
+        if not ok or kind == TX_NORM_RMS and (q_bias is not None or k_bias is not None):
+            _bad_norm_params(norm, kind, hd, dtype, (("q_weight", q_weight, heads), ("k_weight", k_weight, kvh),
+                                                     ("q_bias", q_bias, heads), ("k_bias", k_bias, kvh)))
+        param_dt = _DT[kind_of]
+        qw, qb, kw, kb = _ptr(q_weight), _ptr(q_bias), _ptr(k_weight), _ptr(k_bias)
     if kv_lens is not None:
         _int_vector("kv_lens", kv_lens, batch)
+        tensors.append(kv_lens)
     axes, positions_ld = 1, t
     if positions is not None:
         shape = positions.shape
@@ -1120,10 +1154,12 @@ def norm_rotary_append(
             raise ValueError(f"positions must be int64 [{t}] or [axes, {t}] with contiguous rows")
         if len(shape) == 2:
             axes, positions_ld = shape[0], positions.stride(0)
-    if axes > 1 and pair_axis is None:
-        raise ValueError("positions of several axes need pair_axis")
+        tensors.append(positions)
     if pair_axis is not None:
         _int_vector("pair_axis", pair_axis, half)
+        tensors.append(pair_axis)
+    elif axes > 1:
+        raise ValueError("positions of several axes need pair_axis")
     pages = page_size = max_pages = table_ld = 0
     mx = k_scales is not None or v_scales is not None
     if k_cache is not None or v_cache is not None:
@@ -1132,51 +1168,47 @@ def norm_rotary_append(
         vs = _heads3("v", v, t, kvh, hd, dtype)
         if mx:
             kcs, vcs, sizes, kss, vss = _check_mx8(k_cache, k_scales, v_cache, v_scales, block_table, batch, hd)
+            tensors += (k_scales, v_scales)
         else:
             kcs, vcs, sizes = _check_cache(k_cache, v_cache, block_table, batch, hd, dtype)
         pages, cache_heads, page_size, max_pages, table_ld = sizes
         if cache_heads != kvh:
             raise ValueError("the caches must hold k's heads")
+        tensors += (v, k_cache, v_cache, block_table)
     elif mx:
         raise ValueError("scales without a cache")
     else:
         block_table = v = None
-    at = _one_device(k, q, v, steps, cu_seqlens, kv_lens, positions, pair_axis, block_table, k_cache, v_cache, k_scales,
-                     v_scales, q_weight, k_weight, q_bias, k_bias, q_out, k_out)
-    load_library()
+    at = _one_device(*tensors)
+    if _lib is None:
+        load_library()
     if q is not None and q_out is None:
-        q_out = torch.empty((t, heads, hd), dtype=dtype, device=k.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         qos = (heads * hd, hd, 1)
     if k_cache is None and k_out is None:
-        k_out = torch.empty((t, kvh, hd), dtype=dtype, device=k.device)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         kos = (kvh * hd, hd, 1)
     if t == 0 or batch == 0:
         return q_out, k_out
     # The strides in one array, kept with the launch, and their addresses in it.
-    st = array.array("q", (*qs[:3], *qos[:3], *ks[:3], *kos[:3], *vs[:3], *kcs[:3], *vcs[:3], *kss[:3], *vss[:3]))
+    st = array.array("q", (*qs, *qos, *ks, *kos, *vs, *kcs, *vcs, *kss, *vss))
     sa = st.buffer_info()[0]
     args = (_ptr(q), sa, _ptr(q_out) if q is not None else None, sa + 24, k.data_ptr(), sa + 48, _ptr(k_out), sa + 72,
-            _ptr(v), sa + 96, _ptr(k_cache), sa + 120, _ptr(k_scales), sa + 168, _ptr(v_cache), sa + 144,
-            _ptr(v_scales), sa + 192, _ptr(q_weight), _ptr(q_bias), _ptr(k_weight), _ptr(k_bias),
-            1 if per_head else 0, _DT.get(param_dt, TX_F32), kind, float(eps), steps.data_ptr(), _ptr(pair_axis),
+            _ptr(v), sa + 96, _ptr(k_cache), sa + 120, _ptr(k_scales), sa + 184, _ptr(v_cache), sa + 152,
+            _ptr(v_scales), sa + 216, qw, qb, kw, kb, per_head, param_dt, kind, eps, steps.data_ptr(), _ptr(pair_axis),
             _ptr(positions), positions_ld, axes, cu_seqlens.data_ptr(), _ptr(kv_lens), _ptr(block_table), table_ld,
-            t, batch, heads, kvh, hd, 2 * half, pages, page_size, max_pages, float(amplitude), 1 if interleaved else 0,
+            t, batch, heads, kvh, hd, 2 * half, pages, page_size, max_pages, amplitude, 1 if interleaved else 0,
             _DT.get(dtype, -1))
-    _launch_on(at, "tx_norm_rotary_append", args,
-               (q, k, v, steps, cu_seqlens, kv_lens, positions, pair_axis, block_table, k_cache, v_cache, k_scales,
-                v_scales, q_weight, k_weight, q_bias, k_bias, q_out, k_out, st),
+    _launch_on(at, "tx_norm_rotary_append", args, (tensors, q_out, k_out, st),
                lambda: {"op": "norm_rotary_append", "tokens": t, "heads": heads, "kv_heads": kvh, "head_dim": hd,
                         "norm": norm, "axes": axes, "cache": k_cache is not None, "mx8": mx})
     return q_out, k_out
 
 
-def _paged_workspace(at: int, device, *sizes: int) -> Optional[torch.Tensor]:
-    if at != torch.cuda.current_device():
-        with torch.cuda.device(at):
-            need = flash_attn_paged_workspace(*sizes)
-    else:
-        need = flash_attn_paged_workspace(*sizes)
-    return torch.empty(need, dtype=torch.float32, device=device) if need > 0 else None
+@functools.lru_cache(maxsize=256)
+def _workspace_floats(at: int, *sizes: int) -> int:
+    with torch.cuda.device(at):  # (the device's CUs decide)
+        return flash_attn_paged_workspace(*sizes)
 
 
 def flash_attn_paged_mx8(
@@ -1210,14 +1242,17 @@ def flash_attn_paged_mx8(
     if out is not None:
         os_ = _heads3("out", out, t, heads, hd, dtype)
     at = _one_device(q, k_cache, k_scales, v_cache, v_scales, block_table, cu_seqlens, kv_lens, out, workspace)
-    load_library()
+    if _lib is None:
+        load_library()
     if out is None:
-        out = torch.empty((t, heads, hd), dtype=dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os_ = (heads * hd, hd, 1)
     if t == 0 or batch == 0:
         return out
     if workspace is None:
-        workspace = _paged_workspace(at, q.device, t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+        need = _workspace_floats(at, t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+        if need > 0:
+            workspace = q.new_empty(need, dtype=torch.float32)
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous fp32")
     st = array.array("q", (*qs, *ks, *kss, *vs, *vss, *os_))
@@ -1225,7 +1260,7 @@ def flash_attn_paged_mx8(
     args = (q.data_ptr(), sa, k_cache.data_ptr(), sa + 24, k_scales.data_ptr(), sa + 56, v_cache.data_ptr(), sa + 88,
             v_scales.data_ptr(), sa + 120, out.data_ptr(), sa + 152, cu_seqlens.data_ptr(), kv_lens.data_ptr(),
             block_table.data_ptr(), table_ld, t, batch, heads, kvh, hd, pages, page_size, max_pages, max_q_len,
-            float(scale), 1 if causal else 0, workspace.data_ptr() if workspace is not None else None,
+            scale, 1 if causal else 0, workspace.data_ptr() if workspace is not None else None,
             0 if workspace is None else workspace.numel(), _DT.get(dtype, -1))
     _launch_on(at, "tx_flash_attn_paged_mx8", args,
                (q, k_cache, k_scales, v_cache, v_scales, out, cu_seqlens, kv_lens, block_table, workspace, st),
@@ -1260,7 +1295,7 @@ def flash_attn_tree(
     qs = _heads3("q", q, t, heads, hd, dtype)
     batch = _starts(cu_seqlens)
     _int_vector("kv_lens", kv_lens, batch)
-    kss = vss = (0, 0, 0, 1)
+    kss = vss = _NO_STRIDES4
     if k_scales is not None or v_scales is not None:
         ks, vs, sizes, kss, vss = _check_mx8(k_cache, k_scales, v_cache, v_scales, block_table, batch, hd)
     else:
@@ -1277,14 +1312,17 @@ def flash_attn_tree(
     if out is not None:
         os_ = _heads3("out", out, t, heads, hd, dtype)
     at = _one_device(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_seqlens, kv_lens, tree_mask, out, workspace)
-    load_library()
+    if _lib is None:
+        load_library()
     if out is None:
-        out = torch.empty((t, heads, hd), dtype=dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os_ = (heads * hd, hd, 1)
     if t == 0 or batch == 0:
         return out
     if workspace is None:
-        workspace = _paged_workspace(at, q.device, t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+        need = _workspace_floats(at, t, batch, heads, kvh, hd, page_size, max_pages, max_q_len)
+        if need > 0:
+            workspace = q.new_empty(need, dtype=torch.float32)
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous fp32")
     st = array.array("q", (*qs, *ks, *kss, *vs, *vss, *os_))
@@ -1292,7 +1330,7 @@ def flash_attn_tree(
     args = (q.data_ptr(), sa, k_cache.data_ptr(), sa + 24, _ptr(k_scales), sa + 56, v_cache.data_ptr(), sa + 88,
             _ptr(v_scales), sa + 120, out.data_ptr(), sa + 152, cu_seqlens.data_ptr(), kv_lens.data_ptr(),
             block_table.data_ptr(), table_ld, tree_mask.data_ptr(), tree_ld, mask[1], t, batch, heads, kvh, hd, pages,
-            page_size, max_pages, max_q_len, float(scale), workspace.data_ptr() if workspace is not None else None,
+            page_size, max_pages, max_q_len, scale, workspace.data_ptr() if workspace is not None else None,
             0 if workspace is None else workspace.numel(), _DT.get(dtype, -1))
     _launch_on(at, "tx_flash_attn_tree", args,
                (q, k_cache, v_cache, k_scales, v_scales, out, cu_seqlens, kv_lens, block_table, tree_mask, workspace, st),
@@ -1347,7 +1385,7 @@ def cache_accept(
     if k_cache.dim() != 4:
         raise ValueError("k_cache and v_cache must be [pages, kv_heads, page_size, head_dim]")
     hd, dtype = k_cache.shape[3], k_cache.dtype
-    kss = vss = (0, 0, 0, 1)
+    kss = vss = _NO_STRIDES4
     if k_scales is not None or v_scales is not None:
         ks, vs, sizes, kss, vss = _check_mx8(k_cache, k_scales, v_cache, v_scales, block_table, batch, hd)
         dt = TX_BF16
@@ -1363,9 +1401,10 @@ def cache_accept(
     if lens_out is not None:
         _int_vector("lens_out", lens_out, batch)
     at = _one_device(k_cache, v_cache, k_scales, v_scales, block_table, cu_seqlens, kv_lens, path, counts, lens_out)
-    load_library()
+    if _lib is None:
+        load_library()
     if lens_out is None:
-        lens_out = torch.empty(batch, dtype=torch.int32, device=k_cache.device)
+        lens_out = torch.empty_like(kv_lens)
     if batch == 0:
         return lens_out
     st = array.array("q", (*ks, *kss, *vs, *vss))
