@@ -42,16 +42,15 @@ template <typename T> __device__ __forceinline__ float mx_magnitude(float x) {
   const float a = __builtin_fabsf(x);
   return a < __builtin_inff() ? fminf(a, Mx<T>::TOP) : 0.f;
 }
-// Codes of four values (times 2^-e): rounded to nearest even; what is not finite becomes NaN.
-template <typename T> __device__ __forceinline__ uint32_t mx_codes(const float* x, float inv) {
-  float y[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = __builtin_fabsf(x[i]);
-    y[i] = (a < __builtin_inff() ? __builtin_copysignf(fminf(a, Mx<T>::TOP), x[i]) : x[i]) * inv;
-  }
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-  r = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], r, true);
+// x as it is held: magnitudes above TOP count as that; NaN for what is not finite.
+template <typename T> __device__ __forceinline__ float mx_within(float x) {
+  const float a = __builtin_fabsf(x);
+  return a < __builtin_inff() ? __builtin_copysignf(fminf(a, Mx<T>::TOP), x) : __builtin_nanf("");
+}
+// Codes of four values times inv = 2^-e: rounded to nearest even.
+__device__ __forceinline__ uint32_t mx_codes(const float* x, float inv) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, r, true);
   return (uint32_t)r;
 }
 

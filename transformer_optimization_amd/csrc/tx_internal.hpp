@@ -150,7 +150,7 @@ struct NormRotaryArgs {
   int heads, kv_heads, head_dim, rotary;
   float amplitude;
   int interleaved;
-  SeqDiv by_rows;  // rows (heads of q, k and v) of a token
+  SeqDiv by_heads, by_kv_heads, by_half;
 };
 
 struct CacheAcceptArgs {
