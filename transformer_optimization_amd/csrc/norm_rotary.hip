@@ -63,48 +63,51 @@ __device__ __forceinline__ void nr_params(const void* p, int f32, int64_t i, flo
 }
 
 // LPR lanes a row (the power of two that holds head_dim / 8); TOK: tokens a
-// workgroup takes.  A head's row goes round as (token, head) of q, then of k, then
-// of v, so that a wave's rows are of one kind but where kinds meet, and what only
-// others need is skipped.
+// workgroup takes.  A wave takes 64 / LPR rows of one kind at a time, (token,
+// head) of q, of k or of v, so that pointers, strides and what is to be done are
+// the whole wave's, and one token's kinds go side by side.
 template <typename T, int LPR, int TURN, int TOK>
 __global__ __launch_bounds__(NR_THREADS) void norm_rotary_kernel(NormRotaryArgs a) {
-  __shared__ __attribute__((aligned(16))) float2 cs[TOK][128];
-  __shared__ float meet[TURN == NR_CROSS ? NR_THREADS * 8 : 1];
-  const int tid = threadIdx.x;
+  __shared__ __attribute__((aligned(16))) float cosines[TOK][128], sines[TOK][128];
+  __shared__ __attribute__((aligned(16))) float meet[TURN == NR_CROSS ? NR_THREADS * 8 : 4];
+  constexpr int RW = 64 / LPR;
+  const int tid = threadIdx.x, lane = tid & 63, wave = seq_uni(tid >> 6);
   const SeqTile t = seq_find(a.s, 1, TOK, blockIdx.x);
   const int r0 = t.tile * TOK;
   if (r0 >= t.qn) return;
   const int n = t.qn - r0 < TOK ? t.qn - r0 : TOK;
   const int half = a.rotary >> 1, HK = a.kv_heads, hd = a.head_dim, H = a.heads;
   const int key0 = t.kvn - t.qn + r0;  // key index of the first row
-  const int c = tid % LPR, d = 8 * c;  // this lane's chunk of its row
+  const int c = lane % LPR, d = 8 * c;  // this lane's chunk of its row
   const bool in = d < hd;
-  const int nq = a.q ? n * H : 0, nk = n * HK, rows = nq + nk + (a.k_cache ? nk : 0);
+  const int nq = a.q ? n * H : 0, nk = n * HK;
+  // Units of RW rows: q's, k's, v's.
+  const int uq = (nq + RW - 1) / RW, uk = uq + (nk + RW - 1) / RW, units = uk + (a.k_cache ? uk - uq : 0);
 
-  // A row: its place, and what is loaded of it before the one in front is done.
   struct Row {
-    int kind, tt, h;  // 0: q, 1: k, 2: v, 3: none
+    int tt, h;  // token of the workgroup's, head
+    bool some;
     u32x4 raw;
     int page;
   };
-  auto fetch = [&](int i0, Row& w) {
-    int i = i0 + tid / LPR;
-    w.kind = i < nq ? 0 : (i < nq + nk ? 1 : (i < rows ? 2 : 3));
-    i -= w.kind == 0 ? 0 : (w.kind == 1 ? nq : nq + nk);
-    if (w.kind == 3) i = 0;
-    w.tt = seq_div(i, w.kind == 0 ? a.by_heads : a.by_kv_heads);
-    w.h = i - w.tt * (w.kind == 0 ? H : HK);
-    const int64_t row = t.q0 + r0 + w.tt;
-    const T* src = w.kind == 0   ? (const T*)a.q + row * a.q_st + w.h * a.q_sh
-                   : w.kind == 1 ? (const T*)a.k + row * a.k_st + w.h * a.k_sh
-                                 : (const T*)a.v + row * a.v_st + w.h * a.v_sh;
+  // The rows of unit u, asked for one unit ahead.
+  auto fetch = [&](int u, Row& w) {
+    const bool q = u < uq, k = !q && u < uk;
+    int i = (u - (q ? 0 : (k ? uq : uk))) * RW + lane / LPR;
+    w.some = i < (q ? nq : nk);
+    i = w.some ? i : 0;
+    w.tt = seq_div(i, q ? a.by_heads : a.by_kv_heads);
+    w.h = i - w.tt * (q ? H : HK);
+    const T* p = (const T*)(q ? a.q : (k ? a.k : a.v));
+    const int64_t st = q ? a.q_st : (k ? a.k_st : a.v_st), sh = q ? a.q_sh : (k ? a.k_sh : a.v_sh);
+    p += (int64_t)(t.q0 + r0) * st;
     w.raw = u32x4{0, 0, 0, 0};
-    if (in && w.kind != 3) w.raw = ld128(src + d);
+    if (in && w.some) w.raw = ld128(p + (w.tt * st + w.h * sh + d));
     w.page = -1;
-    if (a.k_cache && (w.kind == 1 || w.kind == 2)) w.page = seq_page(a.s, t.b, key0 + w.tt);
+    if (!q && a.k_cache && w.some) w.page = seq_page(a.s, t.b, key0 + w.tt);
   };
   Row w, next;
-  fetch(0, w);  // in flight beside the angles
+  if (wave < units) fetch(wave, w);  // in flight beside the angles
 
   for (int i = tid; i < n * half; i += NR_THREADS) {
     const int tt = seq_div(i, a.by_half), p = i - tt * half;
@@ -113,90 +116,86 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotary_kernel(NormRotaryArgs 
     const uint64_t phase = (uint64_t)pos * a.steps[p];
     float sn, cn;
     sincospif((float)(int64_t)phase * 0x1p-63f, &sn, &cn);
-    cs[tt][p] = make_float2(cn * a.amplitude, sn * a.amplitude);
+    cosines[tt][p] = cn * a.amplitude;
+    sines[tt][p] = sn * a.amplitude;
   }
   __syncthreads();
 
   const float inv_hd = 1.0f / (float)hd;
-  // Every lane of a wave runs the same iterations: the lanes of a row meet.
-  for (int i0 = 0; i0 < rows; i0 += NR_THREADS / LPR) {
-    if (i0 + NR_THREADS / LPR < rows) fetch(i0 + NR_THREADS / LPR, next);
-    const bool is_q = w.kind == 0, turned = w.kind < 2;
-    const int64_t row = t.q0 + r0 + w.tt;
+  for (int u = wave; u < units; u += NR_THREADS / 64) {
+    if (u + NR_THREADS / 64 < units) fetch(u + NR_THREADS / 64, next);
+    const bool is_q = u < uq, is_v = u >= uk;
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = unpack8<T>(w.raw, e);
     u32x4 out = w.raw;
-    if (__any(turned)) {
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = x[e];
+    if (!is_v) {
       if (a.norm != TX_NORM_NONE) {
         if (a.norm == TX_NORM_LAYER) {
           float s = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s += y[e];
+          for (int e = 0; e < 8; ++e) s += x[e];
           const float mu = nr_sum<LPR>(s) * inv_hd;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = in ? y[e] - mu : 0.f;
+          for (int e = 0; e < 8; ++e) x[e] = in ? x[e] - mu : 0.f;
         }
         float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += y[e] * y[e];
-        const float r = 1.0f / sqrtf(nr_sum<LPR>(s) * inv_hd + a.eps);
+        for (int e = 0; e < 8; ++e) s += x[e] * x[e];
+        const float r = rsqrtf(nr_sum<LPR>(s) * inv_hd + a.eps);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= r;
+        for (int e = 0; e < 8; ++e) x[e] *= r;
         const void* weight = is_q ? a.q_weight : a.k_weight;
         const void* bias = is_q ? a.q_bias : a.k_bias;
+        const int at = (in ? d : 0) + w.h * a.param_sh;
         float p[8];
-        if (weight && in && turned) {
-          nr_params<T>(weight, a.param_f32, (int64_t)w.h * a.param_sh + d, p);
+        if (weight) {
+          nr_params<T>(weight, a.param_f32, at, p);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] *= p[e];
+          for (int e = 0; e < 8; ++e) x[e] *= p[e];
         }
-        if (bias && in && turned) {
-          nr_params<T>(bias, a.param_f32, (int64_t)w.h * a.param_sh + d, p);
+        if (bias) {
+          nr_params<T>(bias, a.param_f32, at, p);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] += p[e];
+          for (int e = 0; e < 8; ++e) x[e] += p[e];
         }
       }
       // The turn.
-      const float2* angles = cs[w.tt];
+      const float *cw = cosines[w.tt], *sw = sines[w.tt];
       if constexpr (TURN == NR_INTER) {
+        const int p0 = d >> 1;
+        if (d < a.rotary) {
+          const f32x4 cn = *reinterpret_cast<const f32x4*>(cw + p0), sn = *reinterpret_cast<const f32x4*>(sw + p0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (d + 2 * j < a.rotary) {
-            const float2 w2 = angles[(d >> 1) + j];
-            const float p = y[2 * j], q = y[2 * j + 1];
-            y[2 * j] = p * w2.x - q * w2.y;
-            y[2 * j + 1] = q * w2.x + p * w2.y;
+          for (int j = 0; j < 4; ++j) {
+            const float p = x[2 * j], q = x[2 * j + 1];
+            if (d + 2 * j < a.rotary) {
+              x[2 * j] = p * cn[j] - q * sn[j];
+              x[2 * j + 1] = q * cn[j] + p * sn[j];
+            }
           }
         }
-      } else if constexpr (TURN == NR_ROW) {
-        const bool first = c < LPR / 2;
-        const float2* mine = angles + (first ? d : d - half);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float z = nr_across<LPR>(y[e]);
-          const float2 w2 = mine[e];
-          y[e] = y[e] * w2.x + z * (first ? -w2.y : w2.y);
-        }
-      } else if constexpr (TURN == NR_LANES) {
+      } else if constexpr (TURN == NR_ROW || TURN == NR_LANES) {
         const int hc = half >> 3;  // chunks of a half
-        const bool first = c < hc, turns = c < 2 * hc;
-        const int from = turns ? (tid & 63) + (first ? hc : -hc) : (tid & 63);
+        const bool first = c < hc, turns = TURN == NR_ROW || c < 2 * hc;
+        const int p0 = turns ? d - (first ? 0 : half) : 0;
+        const uint32_t sign = first ? 0x80000000u : 0u;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float z = __shfl(y[e], from, 64);
-          if (turns) {
-            const float2 w2 = angles[d - (first ? 0 : half) + e];
-            y[e] = first ? y[e] * w2.x - z * w2.y : y[e] * w2.x + z * w2.y;
+        for (int g = 0; g < 2; ++g) {
+          const f32x4 cn = *reinterpret_cast<const f32x4*>(cw + p0 + 4 * g), sn = *reinterpret_cast<const f32x4*>(sw + p0 + 4 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float& y = x[4 * g + e];
+            const float z = TURN == NR_ROW ? nr_across<LPR>(y) : __shfl(y, turns ? lane + (first ? hc : -hc) : lane, 64);
+            // first half: y cos - z sin; second: y cos + z sin
+            const float v = y * cn[e] + __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, z) ^ sign) * sn[e];
+            y = turns ? v : y;
           }
         }
       } else {
         float* mine = meet + (tid - c) * 8;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mine[d + e] = y[e];
+        for (int e = 0; e < 8; ++e) mine[d + e] = x[e];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -205,31 +204,30 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotary_kernel(NormRotaryArgs 
           if (at < a.rotary) {
             const bool first = at < half;
             const float z = mine[first ? at + half : at - half];
-            const float2 w2 = angles[first ? at : at - half];
-            y[e] = first ? y[e] * w2.x - z * w2.y : y[e] * w2.x + z * w2.y;
+            const int p = first ? at : at - half;
+            x[e] = first ? x[e] * cw[p] - z * sw[p] : x[e] * cw[p] + z * sw[p];
           }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
       }
-      if (turned) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = y[e];
+      if (is_q || a.k_out || !a.k_scales) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) out[j] = pack2<T>(x[2 * j], x[2 * j + 1]);
-        if (in) {
-          if (is_q) st128((T*)a.q_out + row * a.qo_st + w.h * a.qo_sh + d, out);
-          else if (a.k_out) st128((T*)a.k_out + row * a.ko_st + w.h * a.ko_sh + d, out);
-        }
+      }
+      T* to = (T*)(is_q ? a.q_out : a.k_out);
+      if (to && in && w.some) {
+        const int64_t st = is_q ? a.qo_st : a.ko_st, sh = is_q ? a.qo_sh : a.ko_sh;
+        to += (int64_t)(t.q0 + r0) * st;
+        st128(to + (w.tt * st + w.h * sh + d), out);
       }
     }
-    if (a.k_cache && __any(w.page >= 0)) {
-      const bool is_v = w.kind == 2;
+    if (!is_q && a.k_cache) {
       const int slot = (key0 + w.tt) & ((1 << a.s.page_log2) - 1);
+      const int64_t sp = is_v ? a.vc_sp : a.kc_sp, sh = is_v ? a.vc_sh : a.kc_sh, st = is_v ? a.vc_st : a.kc_st;
+      void* cache = is_v ? a.v_cache : a.k_cache;
       if (!a.k_scales) {
-        if (w.page >= 0 && in)
-          st128(is_v ? (T*)a.v_cache + w.page * a.vc_sp + w.h * a.vc_sh + slot * a.vc_st + d
-                     : (T*)a.k_cache + w.page * a.kc_sp + w.h * a.kc_sh + slot * a.kc_st + d, out);
+        if (w.page >= 0 && in) st128((T*)cache + (w.page * sp + w.h * sh + slot * st + d), out);
       } else {
         // The block's largest magnitude, by its bits (of 32 elements: four lanes).
         uint32_t top = 0;
@@ -254,13 +252,11 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotary_kernel(NormRotaryArgs 
         const int ex = mx_exponent<T>(m);
         const float inv = mx_power(-ex);
         if (w.page >= 0 && in) {
-          uint8_t* to = is_v ? (uint8_t*)a.v_cache + w.page * a.vc_sp + w.h * a.vc_sh + slot * a.vc_st
-                             : (uint8_t*)a.k_cache + w.page * a.kc_sp + w.h * a.kc_sh + slot * a.kc_st;
-          st64(to + d, u32x2{mx_codes(x, inv), mx_codes(x + 4, inv)});
+          st64((uint8_t*)cache + (w.page * sp + w.h * sh + slot * st + d), u32x2{mx_codes(x, inv), mx_codes(x + 4, inv)});
           if ((c & 3) == 0) {
-            uint8_t* s = is_v ? a.v_scales + w.page * a.vs_sp + w.h * a.vs_sh + slot * a.vs_st
-                              : a.k_scales + w.page * a.ks_sp + w.h * a.ks_sh + slot * a.ks_st;
-            s[c >> 2] = (uint8_t)(ex + 127);
+            uint8_t* s = is_v ? a.v_scales : a.k_scales;
+            const int64_t ssp = is_v ? a.vs_sp : a.ks_sp, ssh = is_v ? a.vs_sh : a.ks_sh, sst = is_v ? a.vs_st : a.ks_st;
+            s[w.page * ssp + w.h * ssh + slot * sst + (c >> 2)] = (uint8_t)(ex + 127);
           }
         }
       }
