@@ -252,8 +252,7 @@ struct SqLoader8 {
   int row, ch;          // this thread's first row of a tile, its chunk
   int last;             // last key that may be read
   int bad_from;         // first key found without a page (over the lane's lookups)
-  uint32_t at[N], next[N];  // pages of the K tile that was loaded last, of the one behind it
-  uint32_t before[N];       // and of the one before it
+  uint32_t at[N], next[N];  // pages of the tile that was loaded last, of the one behind it
 
   template <typename H>
   __device__ __forceinline__ void init(const SeqAttnArgs& a, const H& hp, int wave, int lane) {
@@ -286,7 +285,6 @@ struct SqLoader8 {
   __device__ __forceinline__ void advance(int kt) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      before[i] = at[i];
       at[i] = next[i];
       if (at[i] >= (uint32_t)num_pages) {  // page 0 in its place
         bad_from = min(bad_from, (key(kt, i) >> psl) << psl);
@@ -295,12 +293,12 @@ struct SqLoader8 {
     }
     lookup(kt + 1);
   }
-  __device__ __forceinline__ void load(int kt, Side& x, const uint32_t* page) {
+  __device__ __forceinline__ void load(int kt, Side& x) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint32_t slot = (uint32_t)key(kt, i) & ((1u << psl) - 1);
-      x.x[i] = ld128(x.head + ((uint64_t)page[i] * x.sp + slot * x.st));
-      x.s[i] = x.scales[(uint64_t)page[i] * x.ssp + slot * x.sst];
+      x.x[i] = ld128(x.head + ((uint64_t)at[i] * x.sp + slot * x.st));
+      x.s[i] = x.scales[(uint64_t)at[i] * x.ssp + slot * x.sst];
     }
   }
   template <bool IS_K> __device__ __forceinline__ void put(T* tile, const Side& x) {
@@ -390,36 +388,30 @@ struct SqTile {
     auto issue_v = [&](int kt) {
       if constexpr (!MX) ld.issue_v(min(kt, kt1 - 1), v_at(kt));
     };
-    // Codes: the K or V tile in registers to LDS, and the next one to registers (in
-    // every step, so that the compiler can count the loads in flight: past the
-    // last tile its last key again).
-    auto load_k8 = [&](int kt) {
-      if constexpr (MX) {
-        ld.advance(kt);
-        ld.load(kt, ld.k, ld.at);
-      }
-    };
-    auto load_v8 = [&](int kt) {  // (K is LEAD tiles ahead)
-      if constexpr (MX) ld.load(kt, ld.v, LEAD ? ld.before : ld.at);
-    };
+    // Codes (no LEAD): tile kt from registers to LDS, K's and V's each where the
+    // matrix instructions have work, and the one behind it to registers (in every
+    // step, so that the compiler can count the loads in flight: past the last tile
+    // its last key again).  With two tiles in registers they spill: a chunk of 512
+    // over 32768 keys 167 -> 202 us.
     auto next_k8 = [&](int kt) {
       if constexpr (MX) {
         ld.template put<true>(lds + (kt % NST) * L::ELEMS, ld.k);
-        load_k8(kt + 1);
+        ld.advance(kt + 1);
+        ld.load(kt + 1, ld.k);
       }
     };
     auto next_v8 = [&](int kt) {
       if constexpr (MX) {
         ld.template put<false>(lds + (NST + kt % NST) * L::ELEMS, ld.v);
-        load_v8(kt + 1);
+        ld.load(kt + 1, ld.v);
       }
     };
     if constexpr (MX) {
       ld.lookup(kt0);
-      load_k8(kt0);
-      if constexpr (LEAD) next_k8(kt0);
-      load_v8(kt0);
-      next_k8(kt0 + LEAD);
+      ld.advance(kt0);
+      ld.load(kt0, ld.k);
+      ld.load(kt0, ld.v);
+      next_k8(kt0);
       next_v8(kt0);
     } else {
       if constexpr (LEAD) issue_k(kt0);
@@ -451,7 +443,7 @@ struct SqTile {
       if constexpr (MX) {
         lds_barrier();
         if (j0 >= wlim_max) {
-          next_k8(kt + LEAD + 1);
+          next_k8(kt + 1);
           next_v8(kt + 1);
         }
       } else {
@@ -543,12 +535,10 @@ struct SqTile {
       if constexpr (LEAD) {
 #pragma unroll
         for (int ks = HD / 64; ks < HD / 16; ++ks) qk(Kn, ks, sn);
-        next_k8(kt + LEAD + 1);
         weights(0);
         weights(1);
-      } else {
-        next_k8(kt + LEAD + 1);
       }
+      next_k8(kt + 1);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         u32x4 vop[HD / 32];
