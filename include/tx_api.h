@@ -355,11 +355,15 @@ int tx_norm_rotary_append(const void* q, const int64_t q_strides[2], void* q_out
                           float amplitude, int interleaved, int dt, void* stream);
 
 /*
- * tx_flash_attn_paged over an 8-bit cache: the same arguments, results and workspace
- * (tx_flash_attn_paged_workspace) for the values that codes and scales stand for, which are exact in dt (beyond
- * fp16's range: infinite).  Scales' pointers and strides are multiples of head_dim / 32.  o and the workspace may
- * share no memory with any input.
+ * tx_flash_attn_paged over an 8-bit cache: the same arguments and results for the values that codes and scales stand
+ * for, which are exact in dt (beyond fp16's range: infinite).  Scales' pointers and strides are multiples of head_dim
+ * / 32.  o and the workspace (tx_flash_attn_cache_workspace gives its floats, for trees too) may share no memory with
+ * any input.  Where a sequence brings more than 16 rows a K/V head, how its keys are cut into parts, and with it the
+ * rounding of its result, goes by the call's tokens, batch and max_q_len; the same call gives the same bits.
  */
+int tx_flash_attn_cache_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                  int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t max_q_len,
+                                  int64_t* floats);
 int tx_flash_attn_paged_mx8(const void* q, const int64_t q_strides[2],
                             const void* k_cache, const int64_t k_cache_strides[3],
                             const uint8_t* k_scales, const int64_t k_scales_strides[3],

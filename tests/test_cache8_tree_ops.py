@@ -14,6 +14,7 @@ Tolerances, per element, from the roundings alone (eps = finfo(dtype).eps, half 
 """
 
 import math
+import shutil
 
 import pytest
 import torch
@@ -330,6 +331,20 @@ def test_wrappers_check_their_arguments_before_the_device():
             append(**bad)
     with pytest.raises(ValueError, match="multiple of 32"):
         _C.mx8_cache(1, 1, 16, 48)
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs the host C++ compiler")
+def test_cut_of_a_call_by_its_totals(tmp_path):
+    from test_seq_edges import _run_check
+    _run_check(tmp_path, "cache_cut_check")
+
+
+def test_cache_workspace_refusals():
+    for bad in ((0, 1, 8, 2, 64, 16, 8), (1, 0, 8, 2, 64, 16, 8), (1, 1, 8, 3, 64, 16, 8), (1, 1, 8, 2, 96, 16, 8),
+                (1, 1, 8, 2, 64, 12, 8), (1, 1, 8, 2, 64, 16, 0)):
+        with pytest.raises(_C.TxError):
+            _C.flash_attn_cache_workspace(*bad)
+    assert _C.flash_attn_cache_workspace(4, 4, 8, 2, 64, 16, 8) >= 0
 
 
 def test_tree_masks():
@@ -878,11 +893,18 @@ def test_a_sequence_does_not_depend_on_the_batch(cuda, mx, new):
     calls = [lambda q, table, cu, kvl, mask, most: _C.flash_attn_tree(q, kc, vc, table, cu, kvl, mask, 0.1, max_q_len=most, **sc)]
     if mx:
         calls.append(lambda q, table, cu, kvl, mask, most: _mx8(q, kc, vc, sc, table, cu, kvl, 0.1, max_q_len=most))
-    for f in calls:
+    for i, f in enumerate(calls):
         both = f(q, table, cu, kvl, mask, max(news))
         alone = f(q[:new], table[:1], _cu([new], cuda), _i32([3000], cuda), mask[:new], new)
-        assert torch.equal(both[:new], alone)
         assert torch.equal(both, f(q, table, cu, kvl, mask, max(news)))
+        if new * h // hk <= 16:
+            assert torch.equal(both[:new], alone)
+            continue
+        # more rows: the keys are cut by the call's totals
+        seen = _tree_seen(_tree(new, 152), 3000, cuda) if i == 0 else _causal(new, 3000, cuda)
+        want, tol = _attend(q[:new], ks[0], vs[0], 0.1, seen, dtype)
+        _same(both[:new], want, tol, "in the batch")
+        _same(alone, want, tol, "alone")
 
 
 @gpu
@@ -894,7 +916,7 @@ def test_a_bound_that_is_too_small_and_the_workspace(cuda, hint, mx):
     ks, vs, kc, vc, sc, table = _cache(lens, hk, 16, hd, dtype, cuda, 160, mx)
     q = _randn((sum(new), h, hd), dtype, cuda, 161)
     trees = [_tree(n, 162) for n in new]
-    need = _C.flash_attn_paged_workspace(sum(new), len(new), h, hk, hd, 16, table.shape[1], hint)
+    need = _C.flash_attn_cache_workspace(sum(new), len(new), h, hk, hd, 16, table.shape[1], hint)
     ws = torch.full((need + 64,), 2.0, device=cuda)
     got = _C.flash_attn_tree(q, kc, vc, table, _cu(new, cuda), _i32(lens, cuda), _C.tree_masks(trees, device=cuda), 0.125,
                              max_q_len=hint, workspace=ws[:need], **sc)
@@ -940,7 +962,7 @@ def test_starts_that_do_not_ascend_stay_in_bounds(cuda, starts):
     x = _randn((30, h + 2 * hk, hd), dtype, cuda, 181)
     mask = torch.full((30, 1), -1, dtype=torch.int64, device=cuda)
     for most in (0, 1):
-        ws = torch.full((_C.flash_attn_paged_workspace(30, batch, h, hk, hd, 16, table.shape[1], most) + 64,), 2.0, device=cuda)
+        ws = torch.full((_C.flash_attn_cache_workspace(30, batch, h, hk, hd, 16, table.shape[1], most) + 64,), 2.0, device=cuda)
         _mx8(x[:, :h], kc, vc, sc, table, cu, kvl, 0.1, max_q_len=most, out=out, workspace=ws[:-64])
         _C.flash_attn_tree(x[:, :h], kc, vc, table, cu, kvl, mask, 0.1, max_q_len=most, out=out, workspace=ws[:-64], **sc)
         assert bool((ws[-64:] == 2).all())
@@ -1146,8 +1168,9 @@ def test_one_captured_step_serves_other_lengths(cuda, mx):
     kvl, path, counts = _i32(lens, cuda), torch.zeros(batch, 4, dtype=torch.int32, device=cuda), _i32([1] * batch, cuda)
     x = _randn((batch * n, h + 2 * hk, hd), dtype, cuda, 221)
     mask = torch.zeros(batch * n, 1, dtype=torch.int64, device=cuda)
-    need = _C.flash_attn_paged_workspace(batch * n, batch, h, hk, hd, page, table.shape[1], n)
-    ws = torch.empty(max(need, _C.flash_attn_paged_workspace(batch, batch, h, hk, hd, page, table.shape[1], 1)), device=cuda)
+    need = [f(t, batch, h, hk, hd, page, table.shape[1], m) for t, m in ((batch * n, n), (batch, 1))
+            for f in (_C.flash_attn_cache_workspace, _C.flash_attn_paged_workspace)]
+    ws = torch.empty(max(need), device=cuda)
 
     def step():
         q, _ = _C.norm_rotary_append(x[:, :h], x[:, h:h + hk], x[:, h + hk:], steps, cu, kv_lens=kvl, block_table=table,

@@ -61,6 +61,7 @@ EXPORTED_SYMBOLS = (
     "tx_flash_attn_paged",
     "tx_flash_attn_paged_workspace",
     "tx_norm_rotary_append",
+    "tx_flash_attn_cache_workspace",
     "tx_flash_attn_paged_mx8",
     "tx_flash_attn_tree",
     "tx_cache_accept",
@@ -181,6 +182,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         _i64, _i64, _i64,                   # num_pages page_size max_pages
         _f32, _i32, _i32, _vp,              # amplitude interleaved dt stream
     ]
+    lib.tx_flash_attn_cache_workspace.restype = _i32
+    lib.tx_flash_attn_cache_workspace.argtypes = [_i64] * 8 + [_vp]
     lib.tx_flash_attn_paged_mx8.restype = _i32
     lib.tx_flash_attn_paged_mx8.argtypes = [
         _vp, _vp, _vp, _vp, _vp, _vp,       # q k_cache k_scales, each with its strides
@@ -1205,10 +1208,21 @@ def norm_rotary_append(
     return q_out, k_out
 
 
+def flash_attn_cache_workspace(tokens: int, batch: int, heads: int, kv_heads: int, head_dim: int, page_size: int,
+                               max_pages: int, max_q_len: int = 0) -> int:
+    """fp32 values of workspace that :func:`flash_attn_paged_mx8` and :func:`flash_attn_tree` need for these sizes (0:
+    none), on the current device."""
+    n = ctypes.c_int64(0)
+    _check("tx_flash_attn_cache_workspace",
+           load_library().tx_flash_attn_cache_workspace(tokens, batch, heads, kv_heads, head_dim, page_size, max_pages,
+                                                        max_q_len, ctypes.addressof(n)))
+    return n.value
+
+
 @functools.lru_cache(maxsize=256)
 def _workspace_floats(at: int, *sizes: int) -> int:
     with torch.cuda.device(at):  # (the device's CUs decide)
-        return flash_attn_paged_workspace(*sizes)
+        return flash_attn_cache_workspace(*sizes)
 
 
 def flash_attn_paged_mx8(
@@ -1229,7 +1243,7 @@ def flash_attn_paged_mx8(
 ) -> torch.Tensor:
     """:func:`flash_attn_paged` over an 8-bit cache (``tx_flash_attn_paged_mx8``): caches ``[pages, kv_heads,
     page_size, hd]`` of float8_e4m3fn and their scales, as :func:`norm_rotary_append` writes them.  The result is that
-    of the values that codes and scales stand for.  Workspace: :func:`flash_attn_paged_workspace`."""
+    of the values that codes and scales stand for.  Workspace: :func:`flash_attn_cache_workspace`."""
     t, heads, hd = _dims3("q", q)
     dtype = q.dtype
     qs = _heads3("q", q, t, heads, hd, dtype)
@@ -1289,7 +1303,7 @@ def flash_attn_tree(
     16-bit or, with scales, 8-bit.  Row i of a sequence's n sees all keys before the n and those of them whose bit is
     set in its row of ``tree_mask`` (int64 ``[T, words]``: new token x is bit ``x % 64`` of word ``x // 64``), itself
     included only by its own bit.  :func:`tree_masks` makes the rows from each token's parent.  All else as
-    :func:`flash_attn_paged`."""
+    :func:`flash_attn_paged`; workspace: :func:`flash_attn_cache_workspace`."""
     t, heads, hd = _dims3("q", q)
     dtype = q.dtype
     qs = _heads3("q", q, t, heads, hd, dtype)

@@ -582,9 +582,8 @@ int tx_flash_attn_packed(const void* q, const int64_t q_strides[2], const void* 
   return launch_seq_attention(a, dt, (hipStream_t)stream);
 }
 
-int tx_flash_attn_paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
-                                  int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t max_q_len,
-                                  int64_t* floats) {
+static int paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                           int64_t page_size, int64_t max_pages, int64_t max_q_len, bool cache, int64_t* floats) {
   const int32_t some = 0;
   int rc = check_seqs(tokens, batch, q_heads, kv_heads, head_dim, TX_BF16, &some);
   if (rc != TX_OK) return rc;
@@ -602,8 +601,20 @@ int tx_flash_attn_paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads
   a.head_dim = (int)head_dim;
   a.paged = 1;
   a.max_q_len = max_q_len <= 0 || max_q_len > tokens ? tokens : max_q_len;
-  *floats = seq_attention_workspace(a);
+  *floats = cache ? cache_attention_workspace(a) : seq_attention_workspace(a);
   return TX_OK;
+}
+
+int tx_flash_attn_paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                  int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t max_q_len,
+                                  int64_t* floats) {
+  return paged_workspace(tokens, batch, q_heads, kv_heads, head_dim, page_size, max_pages, max_q_len, false, floats);
+}
+
+int tx_flash_attn_cache_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                  int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t max_q_len,
+                                  int64_t* floats) {
+  return paged_workspace(tokens, batch, q_heads, kv_heads, head_dim, page_size, max_pages, max_q_len, true, floats);
 }
 
 // What the paged calls share.  Scales (nullptr: 16-bit caches), and a tree's mask.
@@ -683,7 +694,7 @@ static int paged_attention(const void* q, const int64_t q_strides[2], const void
     a.tree_ld = x.tree_ld;
     a.tree_words = (int)x.tree_words;
   }
-  const int64_t need = seq_attention_workspace(a);
+  const int64_t need = mx || tree ? cache_attention_workspace(a) : seq_attention_workspace(a);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_floats < need)) return TX_EINVAL;
   // Output and workspace are written while the inputs are read.
   const Mem out = mem_rows(o, o_strides, tokens, q_heads, head_dim);

@@ -6,6 +6,12 @@
 
 namespace tx {
 
+int64_t cache_attention_workspace(const SeqAttnArgs& a0) {
+  SeqAttnArgs a = a0;
+  sq_finish<SQ_PAGED | SQ_MX8>(a);
+  return sq_bounds(a).partials * (a.head_dim + 2);
+}
+
 template <typename T, int HD>
 static int launch_hd(const SeqAttnArgs& a, hipStream_t st) {
   if (!a.tree) return sq_launch_paged<T, HD, SQ_PAGED | SQ_MX8>(a, st);

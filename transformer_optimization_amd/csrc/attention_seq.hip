@@ -5,7 +5,7 @@ namespace tx {
 
 int64_t seq_attention_workspace(const SeqAttnArgs& a0) {
   SeqAttnArgs a = a0;
-  sq_finish(a);
+  sq_finish<SQ_PAGED>(a);
   return sq_bounds(a).partials * (a.head_dim + 2);
 }
 

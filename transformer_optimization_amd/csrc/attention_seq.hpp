@@ -1422,7 +1422,7 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
 
 // ---------------------------------------------------------------- paged calls
 __host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
-  return SeqShape{a.group, a.kv_heads, a.cus, a.head_dim == 128 ? 2 : 1, a.few_parts, a.few};
+  return SeqShape{a.group, a.kv_heads, a.cus, a.head_dim == 128 ? 2 : 1, a.few_parts, a.few, a.call_items};
 }
 
 // Workgroups of a call that are resident on a CU.
@@ -1657,12 +1657,14 @@ __global__ __launch_bounds__(256, 4) void seq_attn_join_kernel(SeqAttnArgs a) {
 inline SeqBounds sq_bounds(const SeqAttnArgs& a) {
   return seq_bounds(sq_shape(a), a.s.tokens, a.s.batch, (int64_t)a.s.max_pages << a.s.page_log2);
 }
-inline void sq_finish(SeqAttnArgs& a) {
+template <int K>
+void sq_finish(SeqAttnArgs& a) {
   const int cus = device_cu_count();
   const SeqShape s = seq_shape(a.s.tokens, a.s.batch, a.group, a.kv_heads, a.head_dim, a.max_q_len, cus > 0 ? cus : 256);
   a.cus = s.cus;
   a.few_parts = s.few_parts;
   a.few = s.few;
+  a.call_items = (K & (SQ_MX8 | SQ_TREE)) ? (int)seq_call_items(a.s.tokens, a.s.batch, a.group, a.kv_heads, a.max_q_len) : 0;
   a.by_group = seq_div_by(a.group);
   a.by_kv_heads = seq_div_by(a.kv_heads);
 }
@@ -1670,7 +1672,7 @@ inline void sq_finish(SeqAttnArgs& a) {
 template <typename T, int HD, int K>
 int sq_launch_paged(SeqAttnArgs a, hipStream_t st) {
   const dim3 block(SQ_THREADS);
-  sq_finish(a);
+  sq_finish<K>(a);
   const SeqBounds b = sq_bounds(a);
   a.ws_ml = a.ws + b.partials * HD;
   auto grid = [](int64_t items, int64_t most) { return dim3((unsigned)(items < most ? items : most)); };

@@ -34,6 +34,9 @@ struct SeqShape {
   int least_tiles;
   int few_parts;  // most parts of few-row items
   int few;  // rows of a tile when the call has few-row items only (<= SEQ_FEW), else 0
+  // Tiles' items of a call whose totals cut their keys (seq_call_items); 0: the
+  // sequence's own tiles do.
+  int call_items;
 };
 struct SeqCut {
   int tiles, tile_rows;
@@ -55,6 +58,34 @@ constexpr SeqShape seq_shape(int64_t tokens, int64_t batch, int group, int kv_he
   return s;
 }
 
+// Calls over an 8-bit cache or of a draft tree cut the keys of tiles by the
+// call's totals (its tokens, batch and longest sequence), since a partial row
+// costs as many bytes as 4 (8 bits) of its tile's keys:
+//  * a CU without an item gets one, of 128 keys or more (a lone workgroup takes
+//    1.5 us for 64 keys, the join and a first tile 10);
+//  * two items to a CU from 512 keys each on;
+//  * parts of 4096 keys, up to 4, for sequences of different lengths.
+// One tree of 64 tokens over 1000 keys 38 -> 20 us, of 512 17 for 25; 24 trees
+// over 1000 keys stay whole (44 us; 58 in two parts, 68 in eight); 24 over up to
+// 16384 keys 290 -> 256 (in 32 parts their partial rows were more bytes than the
+// keys).  A sequence that brings more than SEQ_FEW rows then gets other roundings
+// in a call of other totals (not elsewhere in a call, nor in another of the same).
+constexpr int SEQ_PART_CALL = 128, SEQ_CALL_PARTS = 16;
+constexpr int64_t seq_call_items(int64_t tokens, int64_t batch, int group, int kv_heads, int64_t max_q_len) {
+  const int64_t all = (tokens * group + SEQ_TILE - 1) / SEQ_TILE, one = (max_q_len * group + SEQ_TILE - 1) / SEQ_TILE;
+  const int64_t tiles = batch * one > all ? batch * one : all;  // (max_q_len may be too small)
+  return seq_least(seq_least(tiles, 2 * all) * kv_heads, 1 << 30);
+}
+constexpr int64_t seq_call_parts(int cus, int items, int64_t keys) {
+  int64_t fine = seq_least(keys / SEQ_PART_CALL, SEQ_CALL_PARTS);
+  fine = fine > keys / SEQ_PART_TILE ? fine : keys / SEQ_PART_TILE;
+  const int64_t one = seq_least(cus / items, fine), two = seq_least(2 * cus / items, keys / SEQ_PART_TILE);
+  const int64_t four = items <= 2 * cus ? seq_least(keys / 4096, 4) : 1;
+  int64_t parts = one > two ? one : two;
+  parts = parts > four ? parts : four;
+  return seq_least(parts > 1 ? parts : 1, SEQ_JOIN_PARTS);
+}
+
 constexpr SeqCut seq_cut_of(const SeqShape& s, int rows, int keys) {
   SeqCut c{};
   c.few = s.few > 0 || rows <= SEQ_FEW;
@@ -65,6 +96,7 @@ constexpr SeqCut seq_cut_of(const SeqShape& s, int rows, int keys) {
     most = seq_ceil(2 * s.cus, (c.tiles > s.least_tiles ? c.tiles : s.least_tiles) * s.kv_heads);
     step = 64;  // a key tile
     most = most < keys / SEQ_PART_TILE ? most : keys / SEQ_PART_TILE;
+    if (s.call_items > 0) most = (int)seq_call_parts(s.cus, s.call_items, keys);
     most = most < SEQ_JOIN_PARTS ? most : SEQ_JOIN_PARTS;
   }
   most = most < 1 ? 1 : most;
@@ -89,8 +121,9 @@ constexpr SeqBounds seq_bounds(const SeqShape& s, int64_t tokens, int64_t batch,
     const int64_t tiles = (rows / SEQ_TILE + seqs) * hk;
     const int64_t hl = hk * s.least_tiles;
     int64_t parts = seq_least(seq_least(cap / SEQ_PART_TILE, (2 * cus + hl - 1) / hl), SEQ_JOIN_PARTS);
+    if (s.call_items > 0) parts = seq_call_parts(s.cus, s.call_items, cap);
     parts = parts < 1 ? 1 : parts;
-    b.items += seq_least(tiles * parts, tiles + seqs * 2 * cus);
+    b.items += s.call_items > 0 ? tiles * parts : seq_least(tiles * parts, tiles + seqs * 2 * cus);
     // Rows of sequences with few and of others, each in the most parts of its
     // kind; or, where few sequences bring the others, for each of those at most
     // r hk (2 cus / (t hk) + 1) of its r <= 128 t rows.
@@ -98,7 +131,7 @@ constexpr SeqBounds seq_bounds(const SeqShape& s, int64_t tokens, int64_t batch,
     const int64_t few_rows = seq_least(rows, batch * SEQ_FEW);
     const int64_t either = tile >= few ? rows * tile : few_rows * few + (rows - few_rows) * tile;
     const int64_t tile_most = tile ? seqs * SEQ_TILE * 2 * cus + rows * hk : 0;
-    b.partials = seq_least(either * hk, few_rows * few * hk + tile_most);
+    b.partials = s.call_items > 0 ? either * hk : seq_least(either * hk, few_rows * few * hk + tile_most);
   }
   b.join_rows = b.partials > 0 ? rows * hk : 0;
   return b;

@@ -186,6 +186,7 @@ struct SeqAttnArgs {
   int64_t max_q_len;
   int few;   // rows of a tile where every sequence has few rows (seq_common.hpp), else 0
   int few_parts;  // most parts of the keys of such rows
+  int call_items;  // of tiles, where the call's totals cut their keys, else 0
   int cus;
   float* ws;     // partial results: [rows][head_dim], normalised,
   float* ws_ml;  // and their maxima (log2 units) and sums, [rows][2]
@@ -205,8 +206,9 @@ int launch_norm_rotary_append(const NormRotaryArgs& a, int dt, hipStream_t st);
 int launch_cache_accept(const CacheAcceptArgs& a, hipStream_t st);
 // Paged attention over an 8-bit cache, or of a draft tree, or both.
 int launch_cache_attention(const SeqAttnArgs& a, int dt, hipStream_t st);
-// Floats of workspace a paged call of these sizes needs.
+// Floats of workspace a paged call of these sizes needs; over an 8-bit cache or of a draft tree.
 int64_t seq_attention_workspace(const SeqAttnArgs& a);
+int64_t cache_attention_workspace(const SeqAttnArgs& a);
 
 int launch_layernorm(const LayerNormArgs& a, hipStream_t st);
 int launch_gemm(const GemmArgs& g, int ab_dt, int c_dt, int bias_dt, int res_dt, bool qkv,
