@@ -1198,9 +1198,9 @@ def norm_rotary_append(
     sa = st.buffer_info()[0]
     args = (_ptr(q), sa, _ptr(q_out) if q is not None else None, sa + 24, k.data_ptr(), sa + 48, _ptr(k_out), sa + 72,
             _ptr(v), sa + 96, _ptr(k_cache), sa + 120, _ptr(k_scales), sa + 184, _ptr(v_cache), sa + 152,
-            _ptr(v_scales), sa + 216, qw, qb, kw, kb, per_head, param_dt, kind, eps, steps.data_ptr(), _ptr(pair_axis),
-            _ptr(positions), positions_ld, axes, cu_seqlens.data_ptr(), _ptr(kv_lens), _ptr(block_table), table_ld,
-            t, batch, heads, kvh, hd, 2 * half, pages, page_size, max_pages, amplitude, 1 if interleaved else 0,
+            _ptr(v_scales), sa + 216, qw, qb, kw, kb, per_head, param_dt, kind, float(eps), steps.data_ptr(),
+            _ptr(pair_axis), _ptr(positions), positions_ld, axes, cu_seqlens.data_ptr(), _ptr(kv_lens), _ptr(block_table), table_ld,
+            t, batch, heads, kvh, hd, 2 * half, pages, page_size, max_pages, float(amplitude), 1 if interleaved else 0,
             _DT.get(dtype, -1))
     _launch_on(at, "tx_norm_rotary_append", args, (tensors, q_out, k_out, st),
                lambda: {"op": "norm_rotary_append", "tokens": t, "heads": heads, "kv_heads": kvh, "head_dim": hd,
@@ -1274,7 +1274,7 @@ def flash_attn_paged_mx8(
     args = (q.data_ptr(), sa, k_cache.data_ptr(), sa + 24, k_scales.data_ptr(), sa + 56, v_cache.data_ptr(), sa + 88,
             v_scales.data_ptr(), sa + 120, out.data_ptr(), sa + 152, cu_seqlens.data_ptr(), kv_lens.data_ptr(),
             block_table.data_ptr(), table_ld, t, batch, heads, kvh, hd, pages, page_size, max_pages, max_q_len,
-            scale, 1 if causal else 0, workspace.data_ptr() if workspace is not None else None,
+            float(scale), 1 if causal else 0, workspace.data_ptr() if workspace is not None else None,
             0 if workspace is None else workspace.numel(), _DT.get(dtype, -1))
     _launch_on(at, "tx_flash_attn_paged_mx8", args,
                (q, k_cache, k_scales, v_cache, v_scales, out, cu_seqlens, kv_lens, block_table, workspace, st),
@@ -1344,7 +1344,7 @@ def flash_attn_tree(
     args = (q.data_ptr(), sa, k_cache.data_ptr(), sa + 24, _ptr(k_scales), sa + 56, v_cache.data_ptr(), sa + 88,
             _ptr(v_scales), sa + 120, out.data_ptr(), sa + 152, cu_seqlens.data_ptr(), kv_lens.data_ptr(),
             block_table.data_ptr(), table_ld, tree_mask.data_ptr(), tree_ld, mask[1], t, batch, heads, kvh, hd, pages,
-            page_size, max_pages, max_q_len, scale, workspace.data_ptr() if workspace is not None else None,
+            page_size, max_pages, max_q_len, float(scale), workspace.data_ptr() if workspace is not None else None,
             0 if workspace is None else workspace.numel(), _DT.get(dtype, -1))
     _launch_on(at, "tx_flash_attn_tree", args,
                (q, k_cache, v_cache, k_scales, v_scales, out, cu_seqlens, kv_lens, block_table, tree_mask, workspace, st),

@@ -1032,9 +1032,9 @@ __device__ __forceinline__ SqKeys sq_keys(const SeqAttnArgs& a, const SeqWork& w
 // arrive while the waves of the one before it meet; so do its rows of q, once this
 // one's are used.  Every block loads the same number of times, and nothing waits
 // for more than the loads that it needs: the compiler counts those in flight.
-// (Loads behind an item's stores would wait for these to arrive: 64 streams of up
-// to 30000 keys took 246 us with q and the second block's page loaded there.  Two
-// blocks ahead they are no faster.)
+// 64 streams of 3000 to 30000 keys: 245 us, 5.1 TB/s, where reading the same
+// pages alone takes 193; 30 of it are the partial rows' stores.  (Two blocks ahead,
+// or three workgroups a CU, which spill: 245 and 285.)
 template <typename T, int HD>
 struct SqAhead8 {
   typedef SqFew<T, HD, true> F;
@@ -1447,70 +1447,83 @@ __global__ __launch_bounds__(SQ_THREADS, (sq_resident<HD, FEW_ONLY, K>())) void 
   __shared__ int seqs[SeqWalk::LDS_INTS];
   SeqWalk walk;
   walk.init(a.s, sh, false, seqs);
-  // Item i: its place in the call.
-  struct Item {
-    SeqWork w;
-    int hk, r0, j0, j1, np, pair;
+  // Item u of a sequence: its (part, K/V head) pairs first, then its tiles: the
+  // tiles that share keys meet on one XCD when the pairs are a multiple of 8.
+  struct Place {
+    int np, pair, hk, r0, j0, j1;
   };
-  auto find = [&](int i, Item& x) {
-    if (!walk.find(a.s, sh, false, i, x.w)) return false;
-    // Item u of a sequence: its (part, K/V head) pairs first, then its tiles:
-    // the tiles that share keys meet on one XCD when the pairs are a multiple
-    // of 8.
-    const int u = i - x.w.item;
-    x.np = x.w.cut.parts * a.kv_heads;
-    const int tile = x.w.cut.tiles > 1 ? seq_uni(u / x.np) : 0;
+  auto place = [&](int i, const SeqWork& w) {
+    Place x;
+    const int u = i - w.item;
+    x.np = w.cut.parts * a.kv_heads;
+    const int tile = w.cut.tiles > 1 ? seq_uni(u / x.np) : 0;
     x.pair = u - tile * x.np;
     const int p = seq_uni(seq_div(x.pair, a.by_kv_heads));
     x.hk = x.pair - p * a.kv_heads;
-    x.j0 = p * x.w.cut.part_keys;
-    x.j1 = p + 1 < x.w.cut.parts ? x.j0 + x.w.cut.part_keys : 0x7fffffff;
-    x.r0 = tile * x.w.cut.tile_rows;
-    return true;
+    x.j0 = p * w.cut.part_keys;
+    x.j1 = p + 1 < w.cut.parts ? x.j0 + w.cut.part_keys : 0x7fffffff;
+    x.r0 = tile * w.cut.tile_rows;
+    return x;
   };
-  // 8-bit rows of few-row items: the first block of the next item is loaded within this one.
-  typename std::conditional<MX, SqAhead8<T, HD>, SqNoAhead>::type ahead;
-  Item x, y;
-  bool have = find(blockIdx.x, x);
-  if constexpr (MX && FEW_ONLY) {
-    if (have) ahead.start(a, sq_keys<K>(a, x.w, x.hk, x.r0, x.j0, x.j1), threadIdx.x & 63, wave);
-  }
-  for (int i = blockIdx.x; have;) {
-    i += gridDim.x;
-    SqKeys next{x.w.b, x.hk, 0, 1, x.w.q0, x.r0, 1};  // none: the sequence's first key
-    bool have_next = false;
-    if constexpr (MX && FEW_ONLY) {
-      have_next = find(i, y);
-      if (have_next) next = sq_keys<K>(a, y.w, y.hk, y.r0, y.j0, y.j1);
-    }
-    const SeqWork& w = x.w;
-    // An item's lane constants are formed within it: held across the items
-    // they cost the registers that its loads need (56 spills).
-    int lane = threadIdx.x & 63;
-    asm volatile("" : "+v"(lane));
-    // Partial results of a sequence: by tile, part, K/V head, row of the tile.
-    float *part = nullptr, *ml = nullptr;
+  // Partial results of a sequence: by tile, part, K/V head, row of the tile.
+  auto partial = [&](const SeqWork& w, const Place& x, float*& part, float*& ml) {
+    part = ml = nullptr;
     if (w.cut.parts > 1) {
       const int64_t at = w.partial + x.r0 * x.np + x.pair * min(w.qn * a.group - x.r0, w.cut.tile_rows);
       part = a.ws + at * HD;
       ml = a.ws_ml + at * 2;
     }
-    if constexpr (FEW_ONLY) {
-      sq_few_item<T, HD, K>(a, w, x.hk, x.r0, x.j0, x.j1, part, ml, lds, stat, bad, lane, wave, ahead, next);
-    } else if (w.cut.few) {
-      if constexpr (MX) ahead.start(a, sq_keys<K>(a, w, x.hk, x.r0, x.j0, x.j1), lane, wave);
-      sq_few_item<T, HD, K>(a, w, x.hk, x.r0, x.j0, x.j1, part, ml, lds, stat, bad, lane, wave, ahead, next);
-    } else {
-      sq_tile_item<T, HD, K>(a, w.b, w.q0, w.qn, w.kvn, x.hk, x.r0, x.j0, x.j1, part, ml, lds, bad, lane, wave);
-    }
-    // LDS belongs to the next item.
-    if constexpr (MX && FEW_ONLY) {
-      lds_barrier();
+  };
+  if constexpr (MX && FEW_ONLY) {
+    // The first block of the next item is loaded within this one.
+    struct Item {
+      SeqWork w;
+      Place at;
+    };
+    auto find = [&](int i, Item& x) {
+      if (!walk.find(a.s, sh, false, i, x.w)) return false;
+      x.at = place(i, x.w);
+      return true;
+    };
+    SqAhead8<T, HD> ahead;
+    Item x, y;
+    bool have = find(blockIdx.x, x);
+    if (have) ahead.start(a, sq_keys<K>(a, x.w, x.at.hk, x.at.r0, x.at.j0, x.at.j1), threadIdx.x & 63, wave);
+    for (int i = blockIdx.x; have;) {
+      i += gridDim.x;
+      SqKeys next{x.w.b, x.at.hk, 0, 1, x.w.q0, x.at.r0, 1};  // none: the sequence's first key
+      const bool have_next = find(i, y);
+      if (have_next) next = sq_keys<K>(a, y.w, y.at.hk, y.at.r0, y.at.j0, y.at.j1);
+      int lane = threadIdx.x & 63;
+      asm volatile("" : "+v"(lane));  // as below
+      float *part, *ml;
+      partial(x.w, x.at, part, ml);
+      sq_few_item<T, HD, K>(a, x.w, x.at.hk, x.at.r0, x.at.j0, x.at.j1, part, ml, lds, stat, bad, lane, wave, ahead, next);
+      lds_barrier();  // LDS belongs to the next item
       x = y;
       have = have_next;
-    } else {
-      __syncthreads();
-      have = find(i, x);
+    }
+  } else {
+    SeqWork w;
+    for (int i = blockIdx.x; walk.find(a.s, sh, false, i, w); i += gridDim.x) {
+      // An item's lane constants are formed within it: held across the items
+      // they cost the registers that its loads need (56 spills).
+      int lane = threadIdx.x & 63;
+      asm volatile("" : "+v"(lane));
+      const Place x = place(i, w);
+      float *part, *ml;
+      partial(w, x, part, ml);
+      typename std::conditional<MX, SqAhead8<T, HD>, SqNoAhead>::type ahead;
+      const SqKeys next{w.b, x.hk, 0, 1, w.q0, x.r0, 1};
+      if constexpr (FEW_ONLY) {
+        sq_few_item<T, HD, K>(a, w, x.hk, x.r0, x.j0, x.j1, part, ml, lds, stat, bad, lane, wave, ahead, next);
+      } else if (w.cut.few) {
+        if constexpr (MX) ahead.start(a, sq_keys<K>(a, w, x.hk, x.r0, x.j0, x.j1), lane, wave);
+        sq_few_item<T, HD, K>(a, w, x.hk, x.r0, x.j0, x.j1, part, ml, lds, stat, bad, lane, wave, ahead, next);
+      } else {
+        sq_tile_item<T, HD, K>(a, w.b, w.q0, w.qn, w.kvn, x.hk, x.r0, x.j0, x.j1, part, ml, lds, bad, lane, wave);
+      }
+      __syncthreads();  // LDS belongs to the next item
     }
   }
 }

@@ -6,6 +6,10 @@
 // moves need no order between threads; a path ascends, path[i] >= i, so a slot
 // that a move writes is read by no later one, and AC_AT_ONCE rows are read before
 // the first of them is written.
+//
+// Measured: one path of 5 over 8 heads 3.3 us, a launch and the chain; 64 paths of
+// up to 8 over 96 heads of 128 and 8 bits (12 layers that share pages) 7.1, 0.9
+// TB/s of rows that lie 2 KB apart.  A row after another took 12.5.
 #include "seq_common.hpp"
 
 namespace tx {
