@@ -15,6 +15,7 @@ Tolerances, per element, from the roundings alone (eps = finfo(dtype).eps, half 
 
 import math
 import shutil
+from fractions import Fraction
 
 import pytest
 import torch
@@ -1266,3 +1267,43 @@ def test_nothing_to_do(cuda):
                            **sc).tolist() == [0, 9]
     assert _C.cache_accept(kc, vc, table[:0], _cu([], cuda), kvl[:0], torch.zeros(0, 1, dtype=torch.int32, device=cuda), kvl[:0],
                            **sc).shape == (0,)
+
+
+@gpu
+def test_numbers_of_any_kind_and_axes_that_are_not_there(cuda):
+    dtype, hd = torch.float16, 64
+    _, _, kc, vc, sc, table = _cache([70], 2, 16, hd, dtype, cuda, 260, True)
+    q = _randn((3, 4, hd), dtype, cuda, 261)
+    args = (table, _cu([3], cuda), _i32([70], cuda))
+    mask = _C.tree_masks([[-1, 0, 0]], device=cuda)
+    for one in (torch.tensor(0.125), Fraction(1, 8)):
+        assert torch.equal(_mx8(q, kc, vc, sc, *args, one), _mx8(q, kc, vc, sc, *args, 0.125))
+        assert torch.equal(_C.flash_attn_tree(q, kc, vc, *args, mask, one, **sc), _C.flash_attn_tree(q, kc, vc, *args, mask, 0.125, **sc))
+    steps, _ = _C.rotary_steps(hd, device=cuda)
+    pos = torch.tensor([[5, 6, 7], [100, 2, 9]], dtype=torch.int64, device=cuda)
+
+    def turned(axes, **kw):
+        return _C.norm_rotary_append(q, q[:, :2], None, steps, _cu([3], cuda), positions=pos, pair_axis=_i32(axes, cuda), **kw)
+
+    want = turned([0] * 16 + [1] * 16, eps=0.5, amplitude=0.25)
+    for kw in (dict(eps=torch.tensor(0.5), amplitude=torch.tensor(0.25)), dict(eps=Fraction(1, 2), amplitude=Fraction(1, 4))):
+        got = turned([-7] * 15 + [-(2**31), 2**31 - 1] + [2] * 15, **kw)  # cut to the axes that there are
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
+@pytest.mark.parametrize("mx", [False, True])
+def test_an_accepted_token_named_twice(cuda, mx):
+    """Slots that no move has written yet may be read again: both places get it."""
+    dtype, hd, n, last = torch.bfloat16, 64, 12, 40
+    _, _, kc, vc, sc, table = _cache([last], 2, 16, hd, dtype, cuda, 270, mx)
+    at = lambda c, j: c.view(torch.uint8)[int(table[0, j // 16]), :, j % 16].clone()  # noqa: E731
+    path = [3, 3, 9, 9, 9, 5, 6, 7, 11, 11]
+    held = [kc, vc, *sc.values()]
+    old = [[at(c, j) for j in range(last)] for c in held]
+    lens = _C.cache_accept(kc, vc, table, _cu([n], cuda), _i32([last], cuda), _i32([path], cuda), _i32([len(path)], cuda), **sc)
+    assert lens.tolist() == [last - n + len(path)]
+    for c, was in zip(held, old):
+        for j in range(last):
+            i = j - (last - n)
+            assert torch.equal(at(c, j), was[last - n + path[i]] if 0 <= i < len(path) else was[j]), j
