@@ -1556,6 +1556,7 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
   const int sees = max(!TREE && a.causal ? w.kvn - w.qn + i + 1 : w.kvn, 0);
   int parts = w.cut.parts;  // those the row sees
   while (parts > 0 && (parts - 1) * w.cut.part_keys >= sees) --parts;
+  if (TREE) parts = seq_uni(parts);
   const uint32_t po = (uint32_t)(tid % LPR) * 16u;
   auto ml_at = [&](uint32_t off, float& pm, float& pl) {
     const u32x2 x = ld64(ml + off);
@@ -1608,6 +1609,7 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
     if (b > 0) fetch(b);
 #pragma unroll
     for (int x = 0; x < NP; ++x) {
+      if (TREE && b + GRP * x >= parts) break;  // (many rows of few parts)
       const float f = ldexpf(weight(om[x], ol[x]), scale);
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] += f * o[x][e];
@@ -1631,7 +1633,7 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
   }
   if (tid < LPR) {
     bool some = sees > 0;
-    if constexpr (TREE) {
+    if (TREE && L == 0.f) {
       SqTreeRow tr;
       tr.init(a, w.q0 + i, w.kvn - w.qn);
       some = tr.any(w.qn);
