@@ -725,7 +725,7 @@ __device__ __forceinline__ void sq_odd_rows(int b, int q0, int hk, int base, int
   for (int k0 = j0; k0 < lim; k0 += 32) {
     if ((k0 - j0) % 64 == 0) {  // look through 64 keys
       uint32_t any = 0;
-#pragma unroll(MX ? 1 : HD / 8)  // (of codes: the kernels' registers again)
+#pragma unroll MX ? 1 : HD / 8  // (of codes: the kernels' registers again)
       for (int i = 0; i < HD / 8; ++i) {
         const Elem *kr, *vr;
         const int x = 64 * i + lane;
