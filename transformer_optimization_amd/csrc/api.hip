@@ -806,6 +806,8 @@ int tx_norm_rotary_append(const void* q, const int64_t q_strides[2], void* q_out
   if (axes > 1 << 16 || positions_ld < 0 || positions_ld > (int64_t)1 << 40) return TX_EUNSUPPORTED;
   if (((uintptr_t)steps & 7u) || ((uintptr_t)positions & 7u) || ((uintptr_t)kv_lens & 3u) || ((uintptr_t)pair_axis & 3u))
     return TX_EUNSUPPORTED;
+  // Without pair_axis every pair goes by axis 0; without positions there is one axis, the key index.
+  if (!pair_axis || !positions) axes = 1;
   // Rows of one workgroup's tokens are counted in 32 bits.
   if ((q_heads + 2 * kv_heads) * head_dim > (int64_t)1 << 26) return TX_EUNSUPPORTED;
   if (q && (rc = check_rows(q, q_strides, tokens, q_heads, head_dim, false)) != TX_OK) return rc;
