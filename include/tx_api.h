@@ -328,7 +328,8 @@ int tx_flash_attn_paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads
  * norm: TX_NORM_NONE, or with the head's mean square (TX_NORM_RMS) or variance (TX_NORM_LAYER, the mean taken off)
  * m: x / sqrt(m + eps) * weight + bias.  Weights (each nullable: 1) and biases (nullable: 0; TX_NORM_LAYER only) have
  * head_dim values, per_head != 0: as many for each head; of param_dt, dt or TX_F32, 16-byte aligned.
- * positions (int64, nullable as there): of axis x at positions[x * positions_ld + t]; pair i goes by axis pair_axis[i]
+ * positions (int64, nullable as there): of axis x at positions[x * positions_ld + t], positions_ld at least tokens, or
+ * 0 where the axes share one row; pair i goes by axis pair_axis[i]
  * (int32 [rotary_dim / 2]; NULL: axis 0; cut to [0, axes)), without positions by the key index.
  * All of it in fp32, rounded once: the turned q and k to dt (q_out, k_out, a 16-bit cache) or to codes.  With scales
  * (both or neither) the caches are 8-bit (head_dim a multiple of 32).  Otherwise as tx_rotary_append; outputs may

@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from transformer_optimization_amd import _C
-from test_seq_ops import _cu, _randn
+from test_cache8_tree_ops import _Abi
+from test_seq_ops import E, FAKE, U, _cu, _randn
 
 gpu = pytest.mark.gpu
 
@@ -60,3 +61,36 @@ def test_without_positions_there_is_one_axis(cuda):
         code, got = _append_c(q, k, steps, cu, None, 0, 3, pair_axis)
         assert code == 0
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# The call with one row of positions for all axes goes on to a later refusal (steps that are not aligned).
+@pytest.mark.parametrize("change,code", [(dict(pld=0), U), (dict(pld=64), U), (dict(pld=63), E), (dict(pld=1), E),
+                                         (dict(pld=-1), E), (dict(pld=0, t=1), U)])
+def test_rows_of_positions_are_apart_or_one(change, code):
+    call = dict(axes=3, pos=1 << 39, axis=1 << 40, steps=FAKE + 4, ld=8)
+    assert _Abi().append(**call, **change) == code
+
+
+def test_the_wrapper_names_rows_of_positions_that_overlap():
+    q = torch.zeros(6, 4, 64, dtype=torch.bfloat16)
+    args = q, q, None, torch.zeros(32, dtype=torch.int64), _cu((6,), "cpu")
+    axis = torch.zeros(32, dtype=torch.int32)
+    some = torch.zeros(20, dtype=torch.int64)
+    with pytest.raises(ValueError, match="rows of positions"):
+        _C.norm_rotary_append(*args, positions=some.as_strided((3, 6), (5, 1)), pair_axis=axis)
+    for positions in (some[:6].expand(3, 6), some[:18].view(3, 6), some.as_strided((1, 6), (5, 1))):
+        with pytest.raises(ValueError, match="GPU tensors"):
+            _C.norm_rotary_append(*args, positions=positions, pair_axis=axis)
+
+
+@gpu
+@pytest.mark.parametrize("lens", [(5, 1, 14), (1,)])
+def test_one_row_of_positions_for_all_axes(cuda, lens):
+    q, k, steps, cu, positions = _turn_inputs(cuda, lens)
+    axis = (torch.arange(32, dtype=torch.int32) % 3).to(cuda)
+    rows = positions[0].expand(3, q.shape[0])
+    got = _C.norm_rotary_append(q, k, None, steps, cu, positions=rows, pair_axis=axis)
+    want = _C.norm_rotary_append(q, k, None, steps, cu, positions=rows.contiguous(), pair_axis=axis)
+    one = _C.norm_rotary_append(q, k, None, steps, cu, positions=positions[0])
+    for g, w, o in zip(got, want, one):
+        assert torch.equal(g, w) and torch.equal(g, o)

@@ -1095,8 +1095,8 @@ def norm_rotary_append(
     without a norm).  Weights and, for ``"layer"``, biases are ``[hd]``, or ``[heads, hd]`` where each head has its own
     (then all of them), in the tensors' dtype or fp32.
 
-    ``positions``: int64 ``[T]``, or ``[axes, T]`` with ``pair_axis`` (int32 ``[rotary_dim / 2]``), the axis that each
-    pair goes by (time, height, width).  Frequencies that start anew on each axis are ``steps`` joined of several
+    ``positions``: int64 ``[T]``, or ``[axes, T]`` (one row expanded over the axes too) with ``pair_axis`` (int32
+    ``[rotary_dim / 2]``), the axis that each pair goes by (time, height, width).  Frequencies that start anew on each axis are ``steps`` joined of several
     :func:`rotary_steps`.  ``k_scales``, ``v_scales``: with them the caches are 8-bit (:func:`mx8_cache`).  All else as
     :func:`rotary_append`; the result is rounded once."""
     t, kvh, hd = _dims3("k", k)
@@ -1157,6 +1157,8 @@ def norm_rotary_append(
             raise ValueError(f"positions must be int64 [{t}] or [axes, {t}] with contiguous rows")
         if len(shape) == 2:
             axes, positions_ld = shape[0], positions.stride(0)
+            if axes > 1 and 0 < positions_ld < t:
+                raise ValueError("the rows of positions must be apart, or one row for all axes (stride 0)")
         tensors.append(positions)
     if pair_axis is not None:
         _int_vector("pair_axis", pair_axis, half)

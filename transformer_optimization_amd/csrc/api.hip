@@ -802,7 +802,8 @@ int tx_norm_rotary_append(const void* q, const int64_t q_strides[2], void* q_out
     if (!aligned16(p)) return TX_EUNSUPPORTED;
   }
   if (any_param && param_dt != dt && param_dt != TX_F32) return TX_EUNSUPPORTED;
-  if (axes <= 0 || (positions && axes > 1 && positions_ld < tokens)) return TX_EINVAL;
+  // (axes may share one row of positions, but not parts of rows)
+  if (axes <= 0 || (positions && axes > 1 && positions_ld != 0 && positions_ld < tokens)) return TX_EINVAL;
   if (axes > 1 << 16 || positions_ld < 0 || positions_ld > (int64_t)1 << 40) return TX_EUNSUPPORTED;
   if (((uintptr_t)steps & 7u) || ((uintptr_t)positions & 7u) || ((uintptr_t)kv_lens & 3u) || ((uintptr_t)pair_axis & 3u))
     return TX_EUNSUPPORTED;
