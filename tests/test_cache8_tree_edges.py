@@ -2,6 +2,7 @@
 unusual arguments, may make: what each reads and gives, and what is refused."""
 
 import ctypes
+import struct
 
 import pytest
 import torch
@@ -94,3 +95,41 @@ def test_one_row_of_positions_for_all_axes(cuda, lens):
     one = _C.norm_rotary_append(q, k, None, steps, cu, positions=positions[0])
     for g, w, o in zip(got, want, one):
         assert torch.equal(g, w) and torch.equal(g, o)
+
+
+def _kernels(path):
+    """What the compiler wrote beside each kernel of a built library: {name: metadata}."""
+    msgpack = pytest.importorskip("msgpack")
+    data, found, at = path.read_bytes(), {}, -1
+    while (at := data.find(b"__CLANG_OFFLOAD_BUNDLE__", at + 1)) >= 0:
+        entry = at + 32
+        for _ in range(struct.unpack_from("<Q", data, at + 24)[0]):
+            start, size, n = struct.unpack_from("<QQQ", data, entry)
+            target, entry = data[entry + 24:entry + 24 + n], entry + 24 + n
+            elf = data[at + start:at + start + size]
+            if b"amdgcn" not in target or elf[:4] != b"\x7fELF":
+                continue
+            sections, = struct.unpack_from("<Q", elf, 40)
+            each, count = struct.unpack_from("<HH", elf, 58)
+            for i in range(count):
+                kind, = struct.unpack_from("<I", elf, sections + i * each + 4)
+                note, = struct.unpack_from("<Q", elf, sections + i * each + 24)
+                if kind != 7:  # notes
+                    continue
+                name_len, len_, type_ = struct.unpack_from("<III", elf, note)
+                if type_ == 32 and elf[note + 12:note + 18] == b"AMDGPU":
+                    note += 12 + (name_len + 3) // 4 * 4
+                    for k in msgpack.unpackb(elf[note:note + len_], strict_map_key=False)["amdhsa.kernels"]:
+                        found[k[".name"]] = k
+    return found
+
+
+def test_attention_over_16_bits_keeps_its_registers():
+    """The kernels of calls over a 16-bit cache share their source with those over 8 bits and of trees; what only these
+    need costs them no scratch memory (bytes a lane: none, and 48 and 52 for tiles at head dim 128, as before)."""
+    kernels = {n: k for n, k in _kernels(_C.LIB_PATH).items() if "seq_attn_" in n}
+    of16 = {n: k for n, k in kernels.items() if n.endswith("ELi1EEEvNS_11SeqAttnArgsE")}
+    assert len(of16) == 8 and len(kernels) > len(of16)
+    for name, k in of16.items():
+        tiles128 = "Li128ELb0E" in name
+        assert k[".private_segment_fixed_size"] <= (64 if tiles128 else 0), name

@@ -1421,8 +1421,18 @@ __device__ __forceinline__ void sq_few_item(const SeqAttnArgs& a, const SeqWork&
 }
 
 // ---------------------------------------------------------------- paged calls
+// CALL: the call's totals may cut the keys of tiles (seq_call_parts).  Known when
+// compiling: the divisions of that rule took registers of the kernels of 16-bit
+// caches, which never form it (up to 116 bytes a lane of scratch memory; 40 calls
+// of 6 to 110 us took 1.6% longer, the shortest 5%).
+template <bool CALL>
 __host__ __device__ inline SeqShape sq_shape(const SeqAttnArgs& a) {
-  return SeqShape{a.group, a.kv_heads, a.cus, a.head_dim == 128 ? 2 : 1, a.few_parts, a.few, a.call_items};
+  return SeqShape{a.group, a.kv_heads, a.cus, a.head_dim == 128 ? 2 : 1, a.few_parts, a.few, CALL ? a.call_items : 0};
+}
+// Calls over an 8-bit cache or of a draft tree.
+template <int K>
+constexpr bool sq_call() {
+  return (K & (SQ_MX8 | SQ_TREE)) != 0;
 }
 
 // Workgroups of a call that are resident on a CU.
@@ -1443,7 +1453,7 @@ __global__ __launch_bounds__(SQ_THREADS, (sq_resident<HD, FEW_ONLY, K>())) void 
   __shared__ int bad[4];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   constexpr bool MX = (K & SQ_MX8) != 0;
-  const SeqShape sh = sq_shape(a);
+  const SeqShape sh = sq_shape<sq_call<K>()>(a);
   __shared__ int seqs[SeqWalk::LDS_INTS];
   SeqWalk walk;
   walk.init(a.s, sh, false, seqs);
@@ -1645,10 +1655,10 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
   }
 }
 
-template <typename T, int HD, bool TREE>
+template <typename T, int HD, bool CALL, bool TREE>
 __global__ __launch_bounds__(256, 4) void seq_attn_join_kernel(SeqAttnArgs a) {
   __shared__ __attribute__((aligned(16))) float red[256][4];
-  const SeqShape sh = sq_shape(a);
+  const SeqShape sh = sq_shape<CALL>(a);
   __shared__ int seqs[SeqWalk::LDS_INTS];
   SeqWalk walk;
   walk.init(a.s, sh, true, seqs);
@@ -1670,7 +1680,7 @@ __global__ __launch_bounds__(256, 4) void seq_attn_join_kernel(SeqAttnArgs a) {
 
 // ------------------------------------------------------------------- launch
 inline SeqBounds sq_bounds(const SeqAttnArgs& a) {
-  return seq_bounds(sq_shape(a), a.s.tokens, a.s.batch, (int64_t)a.s.max_pages << a.s.page_log2);
+  return seq_bounds(sq_shape<true>(a), a.s.tokens, a.s.batch, (int64_t)a.s.max_pages << a.s.page_log2);
 }
 template <int K>
 void sq_finish(SeqAttnArgs& a) {
@@ -1679,7 +1689,7 @@ void sq_finish(SeqAttnArgs& a) {
   a.cus = s.cus;
   a.few_parts = s.few_parts;
   a.few = s.few;
-  a.call_items = (K & (SQ_MX8 | SQ_TREE)) ? (int)seq_call_items(a.s.tokens, a.s.batch, a.group, a.kv_heads, a.max_q_len) : 0;
+  a.call_items = sq_call<K>() ? (int)seq_call_items(a.s.tokens, a.s.batch, a.group, a.kv_heads, a.max_q_len) : 0;
   a.by_group = seq_div_by(a.group);
   a.by_kv_heads = seq_div_by(a.kv_heads);
 }
@@ -1695,7 +1705,7 @@ int sq_launch_paged(SeqAttnArgs a, hipStream_t st) {
   else seq_attn_paged_kernel<T, HD, false, K><<<grid(b.items, sq_resident<HD, false, K>() * a.cus), block, 0, st>>>(a);
   if (hipGetLastError() != hipSuccess) return TX_EHIP;
   if (b.partials > 0) {
-    seq_attn_join_kernel<T, HD, (K & SQ_TREE) != 0><<<grid(b.join_rows, 4 * a.cus), block, 0, st>>>(a);
+    seq_attn_join_kernel<T, HD, sq_call<K>(), (K & SQ_TREE) != 0><<<grid(b.join_rows, 4 * a.cus), block, 0, st>>>(a);
     if (hipGetLastError() != hipSuccess) return TX_EHIP;
   }
   return TX_OK;
