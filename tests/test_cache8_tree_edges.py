@@ -97,6 +97,15 @@ def test_one_row_of_positions_for_all_axes(cuda, lens):
         assert torch.equal(g, w) and torch.equal(g, o)
 
 
+def test_spans_of_far_rows_are_not_lost():
+    """Strides whose spans pass 63 bits: memory that is two arguments' at once is still seen."""
+    far = dict(t=1 << 22, mld=1 << 40, mask=1 << 50)
+    assert _Abi().paged(tree=True, o=1 << 50, **far) == E
+    assert _Abi().paged(tree=True, o=(1 << 50) + (1 << 43) * 5, **far) == E
+    # rows of the output far apart, the workspace over the first of them
+    assert _Abi().paged(t=1 << 22, o=1 << 50, os=(1 << 40, 64), ws=1 << 50, mp=512, ld=512) == E
+
+
 def _kernels(path):
     """What the compiler wrote beside each kernel of a built library: {name: metadata}."""
     msgpack = pytest.importorskip("msgpack")

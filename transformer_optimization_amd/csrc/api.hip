@@ -705,7 +705,7 @@ static int paged_attention(const void* q, const int64_t q_strides[2], const void
     if (!disjoint(out, m)) return TX_EINVAL;
   const Mem small[] = {mem_span(cu_seqlens, (batch + 1) * 4), mem_span(kv_lens, batch * 4),
                        mem_span(block_table, ((batch - 1) * table_ld + max_pages) * 4),
-                       mem_span(tree ? x.tree : nullptr, tree ? ((tokens - 1) * x.tree_ld + x.tree_words) * 8 : 0),
+                       tree ? Mem{(uintptr_t)x.tree, (__int128)x.tree_ld * 8, (__int128)x.tree_words * 8, tokens} : Mem{},
                        mx ? mem_pages(x.k_scales, x.k_scales_strides, num_pages, kv_heads, page_size, blocks, 1) : Mem{},
                        mx ? mem_pages(x.v_scales, x.v_scales_strides, num_pages, kv_heads, page_size, blocks, 1) : Mem{}};
   if (mx || tree)
@@ -713,9 +713,7 @@ static int paged_attention(const void* q, const int64_t q_strides[2], const void
       if (!disjoint(out, m)) return TX_EINVAL;
   if (need > 0) {
     const uintptr_t ws = (uintptr_t)workspace;
-    if (spans_overlap(ws, need * 4, (uintptr_t)o,
-                      ((tokens - 1) * o_strides[0] + (q_heads - 1) * o_strides[1] + head_dim) * 2))
-      return TX_EINVAL;
+    if (span_meets_byte_blocks(ws, need * 4, out.p, out.stride, out.extent, out.count)) return TX_EINVAL;
     for (const Mem& m : in)
       if (span_meets_byte_blocks(ws, need * 4, m.p, m.stride, m.extent, m.count)) return TX_EINVAL;
     for (const Mem& m : small)
