@@ -5,9 +5,11 @@
 // A sequence of at most SEQ_FEW rows (query heads of one K/V head x new
 // tokens) is bound by reading its keys: one item per K/V head and part of the
 // keys, every row in it.  More rows: tiles of 128 rows, their keys in parts
-// where the tiles alone leave the card idle.  The cut of a sequence depends on
-// nothing but its own rows, keys and head counts (and the card), so that its
-// result does not change with the batch around it.
+// where the tiles alone leave the card idle.  The cut of a sequence of few rows,
+// and over a 16-bit cache of any, depends on nothing but its own rows, keys and
+// head counts (and the card), so that its result does not change with the batch
+// around it.  Tiles over an 8-bit cache or of a draft tree are cut by the call's
+// totals (seq_call_parts).
 #pragma once
 
 #include <stdint.h>
