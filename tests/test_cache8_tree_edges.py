@@ -2,6 +2,7 @@
 unusual arguments, may make: what each reads and gives, and what is refused."""
 
 import ctypes
+import shutil
 import struct
 
 import pytest
@@ -9,6 +10,7 @@ import torch
 
 from transformer_optimization_amd import _C
 from test_cache8_tree_ops import _Abi
+from test_limits import _run_check
 from test_seq_ops import E, FAKE, U, _cu, _randn
 
 gpu = pytest.mark.gpu
@@ -104,6 +106,11 @@ def test_spans_of_far_rows_are_not_lost():
     assert _Abi().paged(tree=True, o=(1 << 50) + (1 << 43) * 5, **far) == E
     # rows of the output far apart, the workspace over the first of them
     assert _Abi().paged(t=1 << 22, o=1 << 50, os=(1 << 40, 64), ws=1 << 50, mp=512, ld=512) == E
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs the host C++ compiler")
+def test_offsets_of_a_row_s_parts_fit_32_bits(tmp_path):
+    _run_check(tmp_path, "cache_join_check")
 
 
 def _kernels(path):

@@ -1558,8 +1558,9 @@ __device__ __forceinline__ void sq_join_row(const SeqAttnArgs& a, const SeqWork&
   const int tile = w.cut.tiles == 1 ? 0 : (w.cut.few ? seq_uni(r / tr) : r / SQ_ROWS), r0 = tile * tr;
   const int n = min(w.qn * a.group - r0, tr);
   const int64_t at = w.partial + r0 * w.cut.parts * a.kv_heads + hk * n + r - r0;  // of part 0
-  // Byte offsets from there to a part's: at most (2 CUs + kv_heads) times a
-  // tile's rows, below 2^32.
+  // Byte offsets from there to a part's: parts times kv_heads are at most 4 CUs
+  // where a sequence's own tiles cut its keys and 8 where the call's totals do
+  // (four parts of 2 CUs' items), times a tile's rows: below 2^32.
   const char *first = (const char*)(a.ws + at * HD), *ml = (const char*)(a.ws_ml + at * 2);
   const uint32_t step = (uint32_t)(a.kv_heads * n) * 8u, step_o = step * (HD / 2);
   const int i = seq_uni(seq_div(r, a.by_group));
