@@ -564,8 +564,7 @@ struct SqTile {
     f32x16 sa[2];
     if constexpr (LEAD) {
       f32x16 sb[2];
-      if constexpr (MX) lds_barrier();
-      else ring_barrier<LPW * (NST - 1)>();  // K of the first tile
+      ring_barrier<LPW * (NST - 1)>();  // K of the first tile
       zero(sa);
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) qk(lds + (kt0 % NST) * L::ELEMS, ks, sa);
@@ -962,8 +961,9 @@ __global__ __launch_bounds__(SQ_THREADS, HD == 64 ? 4 : 2) void seq_attn_packed_
 // if V's rows are taken in that order.  The waves' results meet in LDS at the
 // end.
 //
-// 8-bit rows come through registers instead, a block before their use, and are converted into the same layout of one LDS block, K's first, V's in its
-// place once the scores are formed.
+// 8-bit rows come through registers instead, a block before their use, and are
+// converted into the same layout of one LDS block, K's first, V's in its place
+// once the scores are formed.
 template <typename T, int HD, bool MX>
 struct SqFew {
   typedef typename Mfma16<T>::vec vec;
