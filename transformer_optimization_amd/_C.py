@@ -784,7 +784,7 @@ def _one_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> int:
 
 def _launch_on(at: int, fn: str, args: tuple, keep: tuple, info) -> None:
     """``_launch`` on the current stream of device ``at``; ``info`` is called when a recording is active."""
-    if at != torch._C._cuda_getDevice():  # (initialised: the tensors are on a device)
+    if at != torch.cuda.current_device():
         with torch.cuda.device(at):
             _launch_on(at, fn, args, keep, info)
         return
