@@ -356,9 +356,11 @@ int tx_norm_rotary_append(const void* q, const int64_t q_strides[2], void* q_out
                           float amplitude, int interleaved, int dt, void* stream);
 
 /*
- * tx_flash_attn_paged over an 8-bit cache: the same arguments and results for the values that codes and scales stand
- * for, which are exact in dt (beyond fp16's range: infinite).  Scales' pointers and strides are multiples of head_dim
- * / 32.  o and the workspace (tx_flash_attn_cache_workspace gives its floats, for trees too) may share no memory with
+ * tx_flash_attn_paged over an 8-bit cache (head_dim 64 or 128): the same arguments and results for the values that
+ * codes and scales stand for, each rounded to dt.  Those that an append of the same dt wrote are exact in it; a cache
+ * carries no type, and of other scales (below 112 read as fp16, below 10 as bf16) the smallest values lie between dt's
+ * subnormal ones (bf16's subnormal ones may count as 0), and what is beyond dt's range is infinite.  Scales' pointers
+ * and strides are multiples of head_dim / 32.  o and the workspace (tx_flash_attn_cache_workspace gives its floats, for trees too) may share no memory with
  * any input.  Where a sequence brings more than 16 rows a K/V head, how its keys are cut into parts, and with it the
  * rounding of its result, goes by the call's tokens, batch and max_q_len; the same call gives the same bits.
  */

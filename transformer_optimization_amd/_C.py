@@ -1014,7 +1014,9 @@ def mx8_cache(pages: int, kv_heads: int, page_size: int, head_dim: int, *,
               device: Optional[torch.device] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)`` of one side of an 8-bit cache: e4m3 codes ``[pages, kv_heads, page_size, head_dim]`` and a
     power of two (e8m0) for every 32 elements, ``[pages, kv_heads, page_size, head_dim / 32]``, both all zero bits.
-    Of any other strides they can be views of the caller's own; scales may be uint8 too (2^(byte - 127), 255: NaN)."""
+    Of any other strides they can be views of the caller's own; scales may be uint8 too (2^(byte - 127), 255: NaN).
+    :func:`norm_rotary_append` and :func:`cache_accept` take any such head_dim up to 256, the attention of
+    :func:`flash_attn_paged_mx8` and :func:`flash_attn_tree` 64 and 128."""
     if head_dim <= 0 or head_dim % MX_BLOCK:
         raise ValueError(f"an 8-bit cache needs a head_dim that is a multiple of {MX_BLOCK}")
     codes = torch.zeros((pages, kv_heads, page_size, head_dim), dtype=torch.uint8, device=device)
@@ -1244,8 +1246,9 @@ def flash_attn_paged_mx8(
     workspace: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """:func:`flash_attn_paged` over an 8-bit cache (``tx_flash_attn_paged_mx8``): caches ``[pages, kv_heads,
-    page_size, hd]`` of float8_e4m3fn and their scales, as :func:`norm_rotary_append` writes them.  The result is that
-    of the values that codes and scales stand for.  Workspace: :func:`flash_attn_cache_workspace`."""
+    page_size, hd]`` of float8_e4m3fn and their scales, as :func:`norm_rotary_append` writes them, hd 64 or 128.  The
+    result is that of the values that codes and scales stand for, rounded to q's dtype (exact in it where the append's
+    tensors had the same).  Workspace: :func:`flash_attn_cache_workspace`."""
     t, heads, hd = _dims3("q", q)
     dtype = q.dtype
     qs = _heads3("q", q, t, heads, hd, dtype)
