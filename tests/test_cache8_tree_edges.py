@@ -127,6 +127,30 @@ def test_scales_that_the_append_of_the_type_does_not_write(cuda, dtype, hd, h):
     assert torch.equal(got.cpu().double()[torch.isinf(want)], want[torch.isinf(want)])
 
 
+@gpu
+@pytest.mark.parametrize("tree", [False, True])
+def test_a_bound_in_a_tensor_that_changes(cuda, tree):
+    """max_q_len may be any whole number, also one that the caller writes again between calls."""
+    t, hd = 64, 64
+    q = _randn((t, 8, hd), torch.bfloat16, cuda, 73)
+    (kc, ks), (vc, vs) = (_C.mx8_cache(64, 2, 16, hd, device=cuda) for _ in "kv")
+    seqs = torch.arange(64, dtype=torch.int32, device=cuda)[None], _cu((t,), cuda), _i32([1000], cuda)
+    mask = torch.full((t, 1), -1, dtype=torch.int64, device=cuda)
+    kc.view(torch.uint8).random_(0, 127)
+    vc.view(torch.uint8).random_(0, 127)
+
+    def call(bound):
+        if tree:
+            return _C.flash_attn_tree(q, kc, vc, *seqs, mask, 0.125, k_scales=ks, v_scales=vs, max_q_len=bound)
+        return _C.flash_attn_paged_mx8(q, kc, ks, vc, vs, *seqs, 0.125, max_q_len=bound)
+
+    bound = torch.tensor(1)
+    for n in (1, 8, 64, 1):
+        assert torch.equal(call(bound.fill_(n)), call(n)), n
+    with pytest.raises(TypeError):
+        call(2.5)
+
+
 def test_spans_of_far_rows_are_not_lost():
     """Strides whose spans pass 63 bits: memory that is two arguments' at once is still seen."""
     far = dict(t=1 << 22, mld=1 << 40, mask=1 << 50)

@@ -16,6 +16,7 @@ import contextlib
 import ctypes
 import functools
 import math
+import operator
 import os
 import threading
 from pathlib import Path
@@ -1249,6 +1250,7 @@ def flash_attn_paged_mx8(
     page_size, hd]`` of float8_e4m3fn and their scales, as :func:`norm_rotary_append` writes them, hd 64 or 128.  The
     result is that of the values that codes and scales stand for, rounded to q's dtype (exact in it where the append's
     tensors had the same).  Workspace: :func:`flash_attn_cache_workspace`."""
+    max_q_len = operator.index(max_q_len)  # (a tensor may change later)
     t, heads, hd = _dims3("q", q)
     dtype = q.dtype
     qs = _heads3("q", q, t, heads, hd, dtype)
@@ -1309,6 +1311,7 @@ def flash_attn_tree(
     set in its row of ``tree_mask`` (int64 ``[T, words]``: new token x is bit ``x % 64`` of word ``x // 64``), itself
     included only by its own bit.  :func:`tree_masks` makes the rows from each token's parent.  All else as
     :func:`flash_attn_paged`; workspace: :func:`flash_attn_cache_workspace`."""
+    max_q_len = operator.index(max_q_len)  # (a tensor may change later)
     t, heads, hd = _dims3("q", q)
     dtype = q.dtype
     qs = _heads3("q", q, t, heads, hd, dtype)
