@@ -4,8 +4,8 @@
 // not name.
 //
 // What an 8-bit cache changes is the bytes of few rows (64 streams of 3000 to 30000
-// keys: 245 us for 379 of 16 bits) and, in tiles, the way into LDS (512 tokens over
-// 32768 keys: 170 us for 156 by DMA).  A tree costs a compare more for keys before
+// keys: 245 us for 381 of 16 bits) and, in tiles, the way into LDS (512 tokens over
+// 32768 keys: 170 us for 160 by DMA, beside which the next scores are formed).  A tree costs a compare more for keys before
 // the drafts, which no mask touches, and a window of 64 mask bits for a lane's keys
 // behind them.
 #include "attention_seq.hpp"

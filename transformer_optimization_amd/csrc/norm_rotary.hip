@@ -14,11 +14,11 @@
 // row is read by another wave, so rows may be turned in place.
 //
 // Measured: 19162 tokens of 16 + 4 heads of 128 in 7 prompts, rms norms, three
-// axes, 8-bit cache, 64 us with inputs from memory (3.4 TB/s), 52 with those of the
-// call before still in the memory-side cache; 96 tokens 6.1, one token 3.5 (loads
-// one after another: starts, rows and page, angles' positions).  With rows of q, k
-// and v mixed in a wave, sums by shuffles and angles at a stride of 64 floats the
-// prompts took 96.
+// axes, 8-bit cache, 63 us with inputs from memory (3.4 TB/s), 48 with those of the
+// call before still in the memory-side cache (a 16-bit cache: 64 and 47); 96 tokens
+// 6.1, one token 3.5 (loads one after another: starts, rows and page, angles'
+// positions).  With rows of q, k and v mixed in a wave, sums by shuffles and angles
+// at a stride of 64 floats the prompts took 96.
 #include "mx8.hpp"
 #include "seq_common.hpp"
 
