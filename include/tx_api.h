@@ -333,7 +333,9 @@ int tx_flash_attn_paged_workspace(int64_t tokens, int64_t batch, int64_t q_heads
  * (int32 [rotary_dim / 2]; NULL: axis 0; cut to [0, axes)), without positions by the key index.
  * All of it in fp32, rounded once: the turned q and k to dt (q_out, k_out, a 16-bit cache) or to codes.  With scales
  * (both or neither) the caches are 8-bit (head_dim a multiple of 32).  Otherwise as tx_rotary_append; outputs may
- * share no memory with any input either, but for q_out and k_out that are q and k themselves.
+ * share no memory with any input either, but for q_out and k_out that are q and k themselves.  (Told apart are views
+ * that lie apart, or side by side within pages or rows of one stride; others, as keys and values that alternate slot by
+ * slot, are taken to share memory and refused.  So too in tx_cache_accept.)
  */
 #define TX_NORM_NONE 0
 #define TX_NORM_RMS 1

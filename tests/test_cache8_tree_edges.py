@@ -151,6 +151,13 @@ def test_a_bound_in_a_tensor_that_changes(cuda, tree):
         call(2.5)
 
 
+def test_views_that_alternate_within_a_page_are_refused():
+    """Keys and values in turn, slot by slot: no memory is shared, but only pages and rows are told apart."""
+    st = dict(kcs=(4096, 128, 256), vcs=(4096, 128, 256))
+    for call in (_Abi().append, _Abi().accept):
+        assert call(kc=1 << 33, vc=(1 << 33) + 64 * 2, **st) == E
+
+
 def test_spans_of_far_rows_are_not_lost():
     """Strides whose spans pass 63 bits: memory that is two arguments' at once is still seen."""
     far = dict(t=1 << 22, mld=1 << 40, mask=1 << 50)
